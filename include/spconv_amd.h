@@ -149,6 +149,58 @@ int spc_convnext_mlp(const void* h, const void* x, const void* gamma, const void
                      const void* b1, const void* w2, const void* b2, int dtype, int param_dtype, int64_t N, int C,
                      void* y);
 
+/* ---- Microscaled rows -------------------------------------------------------------------------------------------
+ * 32 consecutive values of a row share the scale 2^(b - 127) of one byte b (255: the block reads as NaN); their elements
+ * are e4m3 (8 bits, largest 448) or e2m1 (4 bits, largest 6, two per byte, the even one in the low half). Row-major:
+ * codes [N, K] or [N, K/2] bytes, scales [N, 16 * ceil(K/512)] bytes, of which a row's first K/32 are in use (the
+ * others are written as zeros and never read). K is a multiple of 32, at most 2^20; all buffers 16-byte aligned.
+ * No counterpart in the reference, whose linears run in fp16 (src/gemm.cu:24-63). */
+enum { SPC_MX_E4M3 = 1, SPC_MX_E2M1 = 2 };
+enum { SPC_NORM_RMS = 0, SPC_NORM_LAYER = 1 };
+
+/* Bytes of the codes and scales of [rows, cols]. Host only; either out-pointer may be NULL. */
+int spc_mx_sizes(int64_t rows, int64_t cols, int fmt, int64_t* code_bytes, int64_t* scale_bytes);
+
+/* Rows x [N,K] (SPC_F32/F16/BF16) into codes and scales: a block's scale is the least power of two for which its largest
+ * magnitude over it rounds to at most the largest element (e4m3: amax / s <= 464; e2m1: < 7); elements round to nearest,
+ * halves to even. A block with an infinity or NaN gets scale 255 and zero elements. spc_mx_dequantize gives the values
+ * back, exact in fp32, rounded once in fp16 / bf16. */
+int spc_mx_quantize(const void* x, int dtype, int64_t N, int64_t K, int fmt, void* codes, void* scales);
+int spc_mx_dequantize(const void* codes, const void* scales, int64_t N, int64_t K, int fmt, int dtype, void* y);
+
+/* sum = x + residual, rounded once to `dtype` (SPC_F16/SPC_BF16), and codes/scales = the quantised norm of sum's rows
+ * [N,C] times gamma plus beta: SPC_NORM_RMS t / sqrt(mean(t^2) + eps), SPC_NORM_LAYER (t - mean(t)) / sqrt(var(t) + eps),
+ * fp32 statistics (|t| below 2^60). residual may be NULL: then x's rows are normalised, and sum may be NULL. sum may be x
+ * or residual. gamma, beta [C] of `param_dtype` or NULL (1, 0). C a multiple of 32, at most 16384.
+ * Beside spc_gather_ln_act: the norm ahead of a microscaled product, with a transformer block's residual addition. */
+int spc_add_norm_mx(const void* x, const void* residual, const void* gamma, const void* beta, int param_dtype,
+                    float eps, int kind, int dtype, int64_t N, int64_t C, int fmt, void* sum, void* codes,
+                    void* scales);
+
+/* out [N,Co] = act(x w^T + bias) + residual, fp32 sums. w [Co,K]: e2m1 codes and scales, Co a multiple of 32. x: codes of
+ * x_fmt with x_scales, or, with x_scales NULL, values of x_dtype that the call quantises to x_fmt. out: values of
+ * out_type (SPC_F32/F16/BF16) with out_scales NULL, one rounding, residual [N,Co] of the same type or NULL (out may be the
+ * residual); else codes of format out_type with out_scales, without a residual. bias [Co] of b_dtype or NULL. out
+ * overlaps no other operand. workspace: spc_mx_linear_workspace's bytes on the device, 16-byte aligned, in use until
+ * the call's work is done, for x that the call quantises; NULL: the library's own, refused while the stream is being captured into a
+ * graph (a captured call needs a workspace of its own for as long as the graph lives). */
+int spc_mx_linear_workspace(int64_t N, int64_t K, int64_t Co, int x_fmt, int64_t* bytes);
+int spc_mx_linear(const void* x, const void* x_scales, int x_dtype, int x_fmt, const void* w_codes,
+                  const void* w_scales, const void* bias, int b_dtype, const void* residual, int act, int64_t N,
+                  int64_t K, int64_t Co, int out_type, void* out, void* out_scales, void* workspace,
+                  int64_t workspace_bytes);
+
+/* ConvNeXt tail with microscaled products: y = x + W2 q(silu(W1 q(LayerNorm(h) * gamma + beta) + b1)) + b2 per row, q the
+ * quantisation to fmt; w1 [4C,C] and w2 [C,4C] e2m1. h, x, y [N,C] of `dtype` (SPC_F16/SPC_BF16), y may be h or x; gamma,
+ * beta, b2 [C] and b1 [4C] of `param_dtype` or NULL; C a multiple of 32, at most 4096. workspace as above, of
+ * spc_convnext_mlp_mx_workspace's bytes.
+ * Beside spc_convnext_mlp (the tail of SDecoder::convnext, src/sdec.cu:60-66), with weights of 4 bits. */
+int spc_convnext_mlp_mx_workspace(int64_t N, int64_t C, int fmt, int64_t* bytes);
+int spc_convnext_mlp_mx(const void* h, const void* x, const void* gamma, const void* beta, float eps,
+                        const void* w1_codes, const void* w1_scales, const void* b1, const void* w2_codes,
+                        const void* w2_scales, const void* b2, int dtype, int param_dtype, int fmt, int64_t N,
+                        int64_t C, void* y, void* workspace, int64_t workspace_bytes);
+
 /* Conv and the upsample block's skip connection in one pass: out = act(conv(x, w) + b) + skip with skip[i,c] =
  * x_skip[src[i] >> 3, (src[i] & 7) * Cin/8 + c / rep], rep = Co / (Cin/8) a power of two; fp32 sum, one rounding.
  * x [N,Ci], w [Co,27,Ci], x_skip [n_skip,Cin] (Cin % 64 == 0), out [N,Co]: one 16-bit `dtype`; src int32 [N] (the

@@ -1,0 +1,442 @@
+"""Microscaled operators on the GPU against their definitions in 64 bits (mx_reference).
+
+Quantisation is exact arithmetic (a power-of-two scale, one rounding), so codes and scales have to be equal. A norm's
+fp32 result is off by at most TOL = 2^-15 of the magnitudes that enter it: up to 16384 / 256 = 64 additions in a lane, 8
+across lanes and 4 across wavefronts for a sum, twice for a LayerNorm, at 2^-24 each, give 2^-16; the reciprocal root,
+its three multiplications and the fused additions a few 2^-23 more. Its elements are then off by that and half an
+element's step. Products: operands with few bits whose sums all fit in 24 are compared bit for bit; others by the
+worst case of K additions of 2^-23 each, and the output's rounding of finfo.eps / 2. Of eight neighbouring e4m3 products,
+which the matrix unit adds at once, it drops what is below 2^-13 of the largest: at most 7 * 2^-13 of it for each group (256 * 1
+keeps 2^-5 * 1 beside it and loses 2^-6 * 1; e2m1 products all lie within 13 bits).
+"""
+import pytest
+import torch
+
+import mx_reference as R
+import spconv_amd as sp
+
+pytestmark = pytest.mark.gpu
+TOL = 2.0 ** -15
+F = {sp.MX_E4M3: "e4m3", sp.MX_E2M1: "e2m1"}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def features(n, k, dt, seed):
+    g = gen(seed)
+    spread = torch.exp(torch.randn(k, generator=g)) * torch.where(torch.rand(k, generator=g) < 0.05, 20.0, 1.0)
+    return (torch.randn((n, k), generator=g) * spread).to(dt)
+
+
+def ragged(q):
+    """q's used scale bytes (int64)."""
+    return q.scales[:, :q.shape[1] // 32].long()
+
+
+def same(q, x, fmt):
+    el, byte = R.quantize(x, fmt)
+    assert torch.equal(ragged(q), byte)
+    assert torch.equal(R.elements(q.codes, fmt), el)
+    assert int(q.scales[:, q.shape[1] // 32:].sum()) == 0
+
+
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,k", [(1, 32), (3, 96), (1, 4096), (257, 512), (1000, 544), (33, 2080)])
+def test_quantize(gpu, fmt, dt, n, k):
+    x = features(n, k, dt, n + k).to(gpu)
+    q = sp.mx_quantize(x, fmt)
+    assert q.shape == (n, k) and q.fmt == fmt
+    same(q, x, fmt)
+    v = R.values(*R.quantize(x, fmt))
+    for odt in (torch.float32, torch.bfloat16, torch.float16):
+        assert torch.equal(sp.mx_dequantize(q, odt), v.to(odt))
+
+
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+def test_quantize_borders(gpu, fmt):
+    """Halves between elements, the border between two scales, the smallest and largest floats, signed zeros, blocks of zeros."""
+    one = torch.linspace(0, 8, 1025, dtype=torch.float64)[:1024]
+    rows = [one, -one, one * 2.0 ** -126, one * 2.0 ** -149, one * 2.0 ** 120, torch.zeros(1024, dtype=torch.float64)]
+    tops = []
+    for m in (255, 256, 447, 448, 449, 463, 464, 464.0001, 465, 511, 5.99, 6, 6.0001, 6.999999, 7, 7.5, 3.4e38, 1e-45):
+        r = torch.zeros(32, dtype=torch.float64)
+        r[:] = torch.linspace(-1, 1, 32, dtype=torch.float64) * m
+        r[7] = m
+        tops.append(r)
+    rows.append(torch.cat(tops + [torch.zeros(1024 - 32 * len(tops), dtype=torch.float64)]))
+    x = torch.stack(rows).float().to(gpu)
+    q = sp.mx_quantize(x, fmt)
+    same(q, x, fmt)
+    assert torch.equal(sp.mx_dequantize(q, torch.float32), R.values(*R.quantize(x, fmt)).float())
+
+
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+def test_quantize_not_finite(gpu, fmt, dt):
+    """A block with an infinity or NaN has scale 255, zero elements and reads as NaN; its neighbours are untouched."""
+    x = features(5, 160, dt, 3)
+    x[1, 40] = float("inf")
+    x[2, 0] = float("-inf")
+    x[3, 159] = float("nan")
+    q = sp.mx_quantize(x.to(gpu), fmt)
+    same(q, x.to(gpu), fmt)
+    bad = torch.zeros((5, 5), dtype=torch.bool)
+    bad[1, 1] = bad[2, 0] = bad[3, 4] = True
+    v = sp.mx_dequantize(q, torch.float32).cpu().view(5, 5, 32)
+    assert torch.equal(v.isnan().all(2), bad) and torch.equal(v.isnan().any(2), bad)
+    assert int(q.codes.view(5, 5, -1)[bad.to(gpu)].sum()) == 0
+
+
+def test_quantize_into_given_buffers(gpu):
+    """Rows behind the given ones stay as they were; a view of later rows is a valid buffer."""
+    x = features(11, 96, torch.float16, 1).to(gpu)
+    codes = torch.full((16, 48), 9, dtype=torch.uint8, device=gpu)
+    scales = torch.full((16, 16), 9, dtype=torch.uint8, device=gpu)
+    q = sp.MxTensor(codes[2:13], scales[2:13], 96, sp.MX_E2M1)
+    assert sp.mx_quantize(x, sp.MX_E2M1, out=q) is q
+    same(q, x, sp.MX_E2M1)
+    for t in (codes, scales):
+        assert bool((t[:2] == 9).all()) and bool((t[13:] == 9).all())
+
+
+def norm64(t, kind, gamma, beta, eps):
+    """The norm of float64 rows, and what its fp32 computation may be off by."""
+    mean = t.mean(1, keepdim=True) if kind == sp.NORM_LAYER else torch.zeros_like(t[:, :1])
+    rstd = 1 / torch.sqrt((t - mean).square().mean(1, keepdim=True) + eps)
+    g = 1.0 if gamma is None else gamma.double()
+    y = (t - mean) * rstd * g
+    off = TOL * (t.abs() + (t.abs().mean(1, keepdim=True) if kind == sp.NORM_LAYER else 0)) * rstd * (1.0 if gamma is None else g.abs())
+    if beta is not None:
+        y = y + beta.double()
+        off = off + 2.0 ** -22 * beta.double().abs()
+    return y, off
+
+
+def near(q, y, off, fmt):
+    """q holds y, computed within off and then quantised."""
+    n, k = y.shape
+    byte = ragged(q)
+    top, slack = y.view(n, -1, 32).abs().amax(2), off.view(n, -1, 32).amax(2)
+    assert bool((byte >= R.scale_bytes((top - slack).clamp(min=0), fmt)).all()) and bool((byte <= R.scale_bytes(top + slack, fmt)).all())
+    s = R.scale_values(byte).repeat_interleave(32, 1)
+    err = (R.values(R.elements(q.codes, fmt), byte) - y).abs()
+    allowed = R.half_step(y.abs() + off, s, fmt) + off
+    assert bool((err <= allowed).all()), float((err / allowed).max())
+
+
+NORM_C = [32, 64, 96, 128, 160, 256, 352, 512, 544, 1024, 1056, 2048, 2080, 4096, 4128, 8192, 16384]
+
+
+@pytest.mark.parametrize("C", NORM_C)
+@pytest.mark.parametrize("kind", [sp.NORM_RMS, sp.NORM_LAYER])
+def test_add_norm(gpu, C, kind):
+    for n, dt, fmt, affine, residual in ((1, torch.bfloat16, sp.MX_E4M3, True, True), (37, torch.float16, sp.MX_E4M3, True, False),
+                                         (130, torch.bfloat16, sp.MX_E2M1, False, True)):
+        g = gen(C + n)
+        x = features(n, C, dt, C + n)
+        x[n // 2] = 0.25  # a constant row: no variance
+        r = (torch.randn((n, C), generator=g) * 3 + 1).to(dt) if residual else None
+        gamma = (torch.rand(C, generator=g) + 0.5).to(dt if n == 37 else torch.float32) if affine else None
+        beta = torch.randn(C, generator=g).to(gamma.dtype) if affine and kind == sp.NORM_LAYER else None
+        dev = [None if a is None else a.to(gpu) for a in (x, r, gamma, beta)]
+        t, q = sp.add_norm_mx(*dev, eps=1e-5, kind=kind, fmt=fmt)
+        if residual:
+            want = (dev[0].double() + dev[1].double()).to(dt)
+            assert torch.equal(t, want)
+        else:
+            assert t is dev[0] and torch.equal(t.cpu(), x)
+        near(q, *norm64(t.double(), kind, dev[2], dev[3], 1e-5), fmt)
+        assert int(q.scales[:, C // 32:].sum()) == 0
+
+
+@pytest.mark.parametrize("C,n", [(64, 70001), (256, 40003), (1024, 9001), (4096, 5003)])
+def test_add_norm_many_rows(gpu, C, n):
+    """More rows than a launch's workgroups hold at once; the sum over the residual, then over x, gives the same bits."""
+    x, r = features(n, C, torch.bfloat16, 1).to(gpu), features(n, C, torch.bfloat16, 2).to(gpu)
+    t, q = sp.add_norm_mx(x, r)
+    near(q, *norm64(t.double(), sp.NORM_RMS, None, None, 1e-6), sp.MX_E4M3)
+    for over in (1, 0):
+        a = [x.clone(), r.clone()]
+        t2, q2 = sp.add_norm_mx(*a, sum=a[over])
+        assert t2.data_ptr() == a[over].data_ptr() and torch.equal(t2, t)
+        assert torch.equal(q2.codes, q.codes) and torch.equal(q2.scales, q.scales)
+
+
+def test_add_norm_edges(gpu):
+    """Zero rows, rows whose sum overflows fp16, infinities and NaN. A NaN, or infinities alone, make the row NaN; beside one
+    infinity the formula gives t / sqrt(inf) = 0 for the finite values and NaN for it, so its block alone reads as NaN."""
+    x = torch.ones((6, 128), dtype=torch.float16)
+    x[1] = 0
+    x[2] = 60000
+    x[3, 5] = float("nan")
+    x[4, 70] = float("-inf")
+    r = x.clone()
+    t, q = sp.add_norm_mx(x.to(gpu), r.to(gpu))
+    v = sp.mx_dequantize(q, torch.float32).cpu()
+    assert torch.equal(v[0], torch.ones(128)) and torch.equal(v[5], torch.ones(128)) and torch.equal(v[1], torch.zeros(128))
+    assert bool(v[2:4].isnan().all())
+    assert bool(v[4, 64:96].isnan().all()) and torch.equal(v[4, :64], torch.zeros(64)) and torch.equal(v[4, 96:], torch.zeros(32))
+
+
+# ---- product ----------------------------------------------------------------------------------------------------
+
+
+def small_ints(rows, k, fmt, seed, lo, hi):
+    """Rows whose elements are integers in [lo, hi] (times 1/2 for e2m1 below 2) and whose scales are 1/2, 1 or 2."""
+    g = gen(seed)
+    if fmt == sp.MX_E4M3:
+        el = torch.randint(lo, hi + 1, (rows, k), generator=g).float()
+        codes = el.to(torch.float8_e4m3fn).view(torch.uint8)
+    else:
+        c = torch.randint(0, 16, (rows, k // 2, 2), generator=g, dtype=torch.uint8)
+        codes = c[:, :, 0] | c[:, :, 1] << 4
+    scales = torch.full((rows, (k + 511) // 512 * 16), 255, dtype=torch.uint8)  # the padding is not to be read
+    scales[:, :k // 32] = torch.randint(126, 129, (rows, k // 32), generator=g, dtype=torch.uint8)
+    return codes, scales
+
+
+def mx(codes, scales, k, fmt, dev):
+    return sp.MxTensor(codes.to(dev), scales.to(dev), k, fmt)
+
+
+def matrix(q):
+    return R.values(R.elements(q.codes, q.fmt), ragged(q))
+
+
+SHAPES = [(1, 32, 32), (1, 4096, 96), (2, 64, 32), (5, 160, 288), (15, 512, 128), (16, 544, 4128), (17, 128, 64), (31, 96, 1056),
+          (33, 1024, 256), (63, 288, 160), (65, 2080, 96), (77, 4096, 512), (127, 256, 256), (129, 480, 384), (255, 640, 288),
+          (257, 1024, 1024), (300, 96, 32), (1803, 1024, 544), (2500, 128, 4096), (5000, 224, 3520)]
+
+
+@pytest.mark.parametrize("n,k,o", SHAPES)
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+def test_linear_bits(gpu, n, k, o, fmt):
+    """Sums of few bits come out exactly, whatever their order: at most 8 * 6 * 4 K in units of 1/8 (e4m3: integers, halves,
+    scales from 1/4) or 6 * 6 * 4 K in units of 1/16 (e2m1) stay below 2^24 units for K <= 4096."""
+    x = mx(*small_ints(n, k, fmt, n + k, -8, 8), k, fmt, gpu)
+    w = mx(*small_ints(o, k, sp.MX_E2M1, o + k, 0, 0), k, sp.MX_E2M1, gpu)
+    want = matrix(x) @ matrix(w).T
+    got = sp.mx_linear(x, w, out_dtype=torch.float32)
+    assert torch.equal(got.double(), want)
+    g = gen(o)
+    bias = torch.randint(-64, 65, (o,), generator=g).to(torch.float16).to(gpu)
+    res = torch.randint(-64, 65, (n, o), generator=g)
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        r = res.to(dt).to(gpu)
+        full = want + bias.double() + r.double()
+        buf = torch.full((n + 3, o), 7.0, dtype=dt, device=gpu)
+        got = sp.mx_linear(x, w, bias, residual=r, out=buf[:n])
+        assert torch.equal(got, full.float().to(dt)) and bool((buf[n:] == 7).all())
+        got = sp.mx_linear(x, w, bias, residual=r, out=r)  # over the residual
+        assert got is r and torch.equal(got, full.float().to(dt))
+
+
+def eights(X, W):
+    """Sum over groups of 8 consecutive columns of the group's largest |x w|, [n,o]."""
+    s = torch.zeros((X.shape[0], W.shape[0]), dtype=torch.float64, device=X.device)
+    for c in range(0, X.shape[1], 8):
+        s += (X[:, None, c:c + 8].abs() * W[None, :, c:c + 8].abs()).amax(2)
+    return s
+
+
+@pytest.mark.parametrize("n,k,o", [(1, 256, 256), (3, 4096, 128), (16, 1024, 96), (40, 96, 512), (200, 512, 1024), (1500, 352, 800)])
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16, torch.float32])
+def test_linear_of_values(gpu, n, k, o, fmt, dt):
+    """x quantised by the call, SiLU, residual; values or microscaled rows out. The call's quantisation is mx_quantize's."""
+    g = gen(n + k + o)
+    x = features(n, k, dt, n + k).to(gpu)
+    w = sp.mx_quantize((torch.randn((o, k), generator=g) / k ** 0.5).to(gpu), sp.MX_E2M1)
+    bias = torch.randn(o, generator=g).to(gpu)
+    q = sp.mx_quantize(x, fmt)
+    X, W = matrix(q), matrix(w)
+    acc = X @ W.T + bias.double()
+    off = (2.0 ** -23 * (k + 2)) * (X.abs() @ W.abs().T + bias.double().abs())  # of the sum before the activation
+    if fmt == sp.MX_E4M3:
+        off = off + 7 * 2.0 ** -13 * eights(X, W)
+    # silu(v): |silu'| <= 1.1; its exp and reciprocal are off by (|v| + 4) 2^-23 relative
+    y = acc * torch.sigmoid(acc)
+    yoff = 1.1 * off + (acc.abs() + 4) * 2.0 ** -23 * y.abs() + 1e-37
+    res = torch.randn((n, o), generator=g).to(dt).to(gpu)
+    for act, ref, roff in ((sp.ACT_NONE, acc, off), (sp.ACT_SILU, y, yoff)):
+        for r in (None, res):
+            got = sp.mx_linear(x, w, bias, residual=r, act=act, fmt=fmt)
+            assert got.dtype == dt
+            want = ref if r is None else ref + r.double()
+            allowed = roff + 2.0 ** -22 * want.abs() + (torch.finfo(dt).eps / 2) * (want.abs() + roff) + torch.finfo(dt).tiny
+            err = (got.double() - want).abs()
+            assert bool((err <= allowed).all()), (act, float((err / allowed).max()))
+            assert torch.equal(got, sp.mx_linear(q, w, bias, residual=r, act=act, out_dtype=dt))
+        for ofmt in (sp.MX_E4M3, sp.MX_E2M1):
+            got = sp.mx_linear(x, w, bias, act=act, fmt=fmt, out_fmt=ofmt)
+            assert got.fmt == ofmt and int(got.scales[:, o // 32:].sum()) == 0
+            near(got, ref, roff, ofmt)
+
+
+def test_linear_not_finite(gpu):
+    """A row with an infinity or NaN is NaN throughout; a weight row whose block is NaN is a NaN channel; nothing else is."""
+    x = features(70, 256, torch.bfloat16, 5)
+    x[3, 100] = float("inf")
+    x[66, 0] = float("nan")
+    w = sp.mx_quantize(features(96, 256, torch.float32, 6).to(gpu), sp.MX_E2M1)
+    w.scales[50, 7] = 255
+    for rows in (70, 4):  # both forms of the product
+        for fmt in (sp.MX_E4M3, sp.MX_E2M1):
+            y = sp.mx_linear(x[:rows].contiguous().to(gpu), w, fmt=fmt, out_dtype=torch.float32).cpu()
+            bad = torch.zeros((rows, 96), dtype=torch.bool)
+            bad[3] = True
+            bad[:, 50] = True
+            if rows > 66:
+                bad[66] = True
+            assert torch.equal(y.isnan(), bad)
+
+
+def test_linear_scales_at_their_ends(gpu):
+    """Scale bytes 0 and 254 are 2^-127 and 2^127: their product with the other operand's 2^127 and 2^-127 is 1."""
+    k = 128
+    one = torch.full((20, k), 0x38, dtype=torch.uint8)  # e4m3 1.0
+    two = torch.full((32, k // 2), 0x44, dtype=torch.uint8)  # e2m1 2.0
+    for bx, bw in ((0, 254), (254, 0), (127, 127)):
+        sx, sw = torch.full((20, 16), bx, dtype=torch.uint8), torch.full((32, 16), bw, dtype=torch.uint8)
+        y = sp.mx_linear(mx(one, sx, k, sp.MX_E4M3, gpu), mx(two, sw, k, sp.MX_E2M1, gpu), out_dtype=torch.float32)
+        assert torch.equal(y, torch.full((20, 32), 2.0 * k, device=gpu)), (bx, bw)
+
+
+def test_empty(gpu):
+    w = sp.mx_quantize(torch.ones((64, 32), device=gpu), sp.MX_E2M1)
+    x = torch.empty((0, 32), dtype=torch.bfloat16, device=gpu)
+    assert sp.mx_quantize(x, sp.MX_E4M3).shape == (0, 32)
+    assert sp.mx_dequantize(sp.mx_quantize(x, sp.MX_E4M3)).shape == (0, 32)
+    assert sp.mx_linear(x, w).shape == (0, 64) and sp.mx_linear(x, w, out_fmt=sp.MX_E4M3).shape == (0, 64)
+    t, q = sp.add_norm_mx(x, x)
+    assert t.shape == (0, 32) and q.shape == (0, 32)
+    w1 = sp.mx_quantize(torch.ones((128, 32), device=gpu), sp.MX_E2M1)
+    w2 = sp.mx_quantize(torch.ones((32, 128), device=gpu), sp.MX_E2M1)
+    assert sp.convnext_mlp_mx(x, x, None, None, w1, None, w2, None).shape == (0, 32)
+
+
+# ---- the operators together ----------------------------------------------------------------------------------------
+
+
+def tail(n, c, dt, seed, dev, pdt=torch.float32):
+    g = gen(seed)
+    h, x = (features(n, c, dt, seed) + 1).to(dt), torch.randn((n, c), generator=g).to(dt)
+    gamma, beta = (torch.rand(c, generator=g) + 0.5).to(pdt), (torch.randn(c, generator=g) * 0.2).to(pdt)
+    w1 = sp.mx_quantize((torch.randn((4 * c, c), generator=g) / c ** 0.5).to(dev), sp.MX_E2M1)
+    w2 = sp.mx_quantize((torch.randn((c, 4 * c), generator=g) / (4 * c) ** 0.5).to(dev), sp.MX_E2M1)
+    b1, b2 = (torch.randn(4 * c, generator=g) * 0.1).to(pdt), (torch.randn(c, generator=g) * 0.1).to(pdt)
+    return h.to(dev), x.to(dev), gamma.to(dev), beta.to(dev), w1, b1.to(dev), w2, b2.to(dev)
+
+
+@pytest.mark.parametrize("c,n", [(32, 1), (96, 77), (256, 1), (256, 4099), (512, 300), (544, 1000), (1024, 1803), (256, 140001)])
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+def test_tail(gpu, c, n, fmt):
+    """The tail is its parts: norm, product with SiLU into microscaled rows, product with the residual, also with many rows
+    in parts, over h and over x; and without the parameters."""
+    dt = torch.float16 if c % 64 else torch.bfloat16
+    a = tail(n, c, dt, c + n, gpu, torch.float32 if n > 1 else dt)
+    h, x, gamma, beta, w1, b1, w2, b2 = a
+    _, q = sp.add_norm_mx(h, None, gamma, beta, kind=sp.NORM_LAYER, fmt=fmt)
+    want = sp.mx_linear(sp.mx_linear(q, w1, b1, act=sp.ACT_SILU, out_fmt=fmt), w2, b2, residual=x, out_dtype=dt)
+    y = sp.convnext_mlp_mx(*a, fmt=fmt)
+    assert y.dtype == dt and bool(torch.isfinite(y).all()) and torch.equal(y, want)
+    for over in (0, 1):
+        b = [t.clone() if isinstance(t, torch.Tensor) else t for t in a]
+        assert torch.equal(sp.convnext_mlp_mx(*b, fmt=fmt, out=b[over]), want)
+    bare = sp.convnext_mlp_mx(h, x, None, None, w1, None, w2, None, fmt=fmt)
+    ones, zeros = torch.ones(c, device=gpu), torch.zeros(4 * c, device=gpu)
+    assert torch.equal(bare, sp.convnext_mlp_mx(h, x, ones, zeros[:c].contiguous(), w1, zeros, w2, zeros[:c].contiguous(), fmt=fmt))
+
+
+def test_block(gpu):
+    """A ConvNeXt block as a decoder runs it: conv on a kernel map, then the tail with 4-bit weights, beside the tail in
+    16 bits. The difference is what quantising costs: e2m1 weights are off by 11%, e4m3 activations by 2.7% (2-norm), so
+    each product by about 12% of its size, and the MLP's part of y by about twice that."""
+    from spconv_amd import workloads as W
+    c = 64
+    coords = torch.from_numpy(W.shell_coords(W.CONFIGS["c1"])).to(gpu)
+    cache, n = sp.build_neighbors(coords), coords.shape[0]
+    g = gen(9)
+    x = torch.randn((n, c), generator=g).to(torch.float16).to(gpu)
+    cw = (torch.randn((c, 27, c), generator=g) / (14 * c) ** 0.5).to(torch.float16).to(gpu)
+    h = sp.subm_conv_fused(x, cw, None, cache)
+    w1 = (torch.randn((4 * c, c), generator=g) / c ** 0.5).to(torch.float16).to(gpu)
+    w2 = (torch.randn((c, 4 * c), generator=g) / (4 * c) ** 0.5).to(torch.float16).to(gpu)
+    full = sp.convnext_mlp(h, x, None, None, w1, None, w2, None)
+    mx_y = sp.convnext_mlp_mx(h, x, None, None, sp.mx_quantize(w1), None, sp.mx_quantize(w2), None)
+    part = (full.double() - x.double()).norm()
+    assert float((mx_y.double() - full.double()).norm() / part) < 0.3
+    assert float((mx_y.double() - full.double()).norm() / part) > 0.02  # the weights do have 4 bits
+
+
+def test_graph_replays(gpu):
+    """Two captured calls (each with its own workspace, taken at capture), replayed in turn with eager work between, on a stream
+    of their own, give the eager results on every replay."""
+    a, b = tail(700, 256, torch.bfloat16, 1, gpu), tail(9, 256, torch.bfloat16, 2, gpu)
+    x = features(40, 512, torch.float16, 3).to(gpu)
+    w = sp.mx_quantize(features(96, 512, torch.float32, 4).to(gpu), sp.MX_E2M1)
+    want = [sp.convnext_mlp_mx(*a), sp.convnext_mlp_mx(*b), sp.mx_linear(x, w)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    try:
+        for call in (lambda: sp.convnext_mlp_mx(*a), lambda: sp.convnext_mlp_mx(*b), lambda: sp.mx_linear(x, w)):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                sp.set_stream(torch.cuda.current_stream())
+                outs.append(call())
+            graphs.append(graph)
+    finally:
+        torch.cuda.synchronize()
+        sp.set_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for out in outs:
+            out.fill_(3.0)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for out, ref in zip(outs, want):
+            assert torch.equal(out, ref)
+        assert torch.equal(sp.convnext_mlp_mx(*a), want[0])
+
+
+def test_other_stream(gpu):
+    """Calls on a stream that the library was given, ordered after work on it."""
+    x = features(300, 256, torch.bfloat16, 3).to(gpu)
+    w = sp.mx_quantize(features(128, 256, torch.float32, 4).to(gpu), sp.MX_E2M1)
+    want = sp.mx_linear(x * 2, w)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    try:
+        with torch.cuda.stream(s):
+            sp.set_stream(s)
+            got = sp.mx_linear(x * 2, w)
+        s.synchronize()
+    finally:
+        sp.set_stream(torch.cuda.current_stream())
+    assert torch.equal(got, want)
+
+
+def test_refusals(gpu):
+    """Calls that the binding or the library refuses before anything runs."""
+    x = features(8, 64, torch.bfloat16, 1).to(gpu)
+    w = sp.mx_quantize(features(32, 64, torch.float32, 1).to(gpu), sp.MX_E2M1)
+    big = torch.zeros((16, 64), dtype=torch.bfloat16, device=gpu)
+    for call in (lambda: sp.mx_quantize(x[:, :48].contiguous()), lambda: sp.mx_quantize(x.t()), lambda: sp.mx_quantize(x, 3),
+                 lambda: sp.mx_linear(x, sp.mx_quantize(x, sp.MX_E4M3)), lambda: sp.mx_linear(x[:, :32].contiguous(), w),
+                 lambda: sp.mx_linear(x, sp.mx_quantize(x[:5].contiguous(), sp.MX_E2M1)),
+                 lambda: sp.mx_linear(x, w, residual=x), lambda: sp.mx_linear(x, w, act=2), lambda: sp.mx_linear(x.cpu(), w),
+                 lambda: sp.mx_linear(x, w, torch.zeros(31, device=gpu)),
+                 lambda: sp.mx_linear(x, w, out_fmt=sp.MX_E4M3, residual=torch.zeros((8, 32), device=gpu)),
+                 lambda: sp.add_norm_mx(big[:8], big[4:12], sum=big[1:9]), lambda: sp.add_norm_mx(x, x.float()),
+                 lambda: sp.add_norm_mx(x.float()), lambda: sp.add_norm_mx(x, kind=2),
+                 lambda: sp.add_norm_mx(torch.zeros((2, 16416), dtype=torch.float16, device=gpu))):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+    n64 = sp.mx_quantize(torch.ones((64, 64), device=gpu), sp.MX_E2M1)
+    sq = features(64, 64, torch.bfloat16, 2).to(gpu)
+    with pytest.raises(RuntimeError, match="overlap"):
+        sp.mx_linear(sq, n64, out=sq)

@@ -386,3 +386,108 @@ SPC_API int spc_subdivide_noalloc(const int32_t* coords, const uint16_t* logits_
                                   int32_t* src, int64_t* m_dev) {
   return guarded([&] { subdivide_noalloc(coords, logits_f16, n, child_coords, src, m_dev); });
 }
+
+namespace {
+MxTensor mx_rows(const void* codes, const void* scales, int fmt, i64 rows, i64 cols) {
+  REQ(fmt == SPC_MX_E4M3 || fmt == SPC_MX_E2M1, "format %d", fmt);
+  REQ(rows >= 0 && cols > 0, "rows=%lld cols=%lld", (long long)rows, (long long)cols);
+  MxTensor q;
+  q.fmt = fmt;
+  q.rows = rows;
+  q.cols = cols;
+  q.codes = borrow(codes, {rows * mx_row_bytes(fmt, cols)}, U8);
+  q.scales = borrow(scales, {rows * mx_scale_bytes(cols)}, U8);
+  return q;
+}
+}  // namespace
+
+SPC_API int spc_mx_sizes(int64_t rows, int64_t cols, int fmt, int64_t* code_bytes, int64_t* scale_bytes) {
+  return guarded([&] {
+    REQ(rows >= 0 && cols > 0 && cols % 32 == 0 && (fmt == SPC_MX_E4M3 || fmt == SPC_MX_E2M1), "rows=%lld cols=%lld format %d",
+        (long long)rows, (long long)cols, fmt);
+    if (code_bytes) *code_bytes = rows * mx_row_bytes(fmt, cols);
+    if (scale_bytes) *scale_bytes = rows * mx_scale_bytes(cols);
+  });
+}
+
+SPC_API int spc_mx_quantize(const void* x, int dtype, int64_t N, int64_t K, int fmt, void* codes, void* scales) {
+  return guarded([&] {
+    MxTensor q = mx_rows(codes, scales, fmt, N, K);
+    mx_quantize(borrow(x, {N, K}, float_dt(dtype, "x")), q);
+  });
+}
+
+SPC_API int spc_mx_dequantize(const void* codes, const void* scales, int64_t N, int64_t K, int fmt, int dtype, void* y) {
+  return guarded([&] {
+    Tensor ty = borrow(y, {N, K}, float_dt(dtype, "y"));
+    mx_dequantize(mx_rows(codes, scales, fmt, N, K), ty);
+  });
+}
+
+SPC_API int spc_add_norm_mx(const void* x, const void* residual, const void* gamma, const void* beta, int param_dtype,
+                            float eps, int kind, int dtype, int64_t N, int64_t C, int fmt, void* sum, void* codes,
+                            void* scales) {
+  return guarded([&] {
+    const DT dt = float_dt(dtype, "x"), pdt = float_dt(param_dtype, "gamma/beta");
+    MxTensor q = mx_rows(codes, scales, fmt, N, C);
+    Tensor tx = borrow(x, {N, C}, dt), tr = borrow(residual, {N, C}, dt), ts = borrow(sum, {N, C}, dt);
+    Tensor tg = borrow(gamma, {C}, pdt), tb = borrow(beta, {C}, pdt);
+    add_norm_mx(tx, residual ? &tr : nullptr, gamma ? &tg : nullptr, beta ? &tb : nullptr, eps, kind, sum ? &ts : nullptr, q);
+  });
+}
+
+SPC_API int spc_mx_linear_workspace(int64_t N, int64_t K, int64_t Co, int x_fmt, int64_t* bytes) {
+  return guarded([&] {
+    REQ(bytes && N >= 0 && K > 0 && Co > 0 && (x_fmt == SPC_MX_E4M3 || x_fmt == SPC_MX_E2M1), "arguments");
+    *bytes = mx_linear_workspace(N, K, x_fmt, Co);
+  });
+}
+
+SPC_API int spc_mx_linear(const void* x, const void* x_scales, int x_dtype, int x_fmt, const void* w_codes,
+                          const void* w_scales, const void* bias, int b_dtype, const void* residual, int act, int64_t N,
+                          int64_t K, int64_t Co, int out_type, void* out, void* out_scales, void* workspace,
+                          int64_t workspace_bytes) {
+  return guarded([&] {
+    REQ(N >= 0 && K > 0 && Co > 0, "N=%lld K=%lld Co=%lld", (long long)N, (long long)K, (long long)Co);
+    const MxTensor w = mx_rows(w_codes, w_scales, SPC_MX_E2M1, Co, K);
+    Tensor tb, tr, to;
+    MxTensor qo;
+    if (bias) tb = borrow(bias, {Co}, float_dt(b_dtype, "bias"));
+    if (out_scales) {
+      qo = mx_rows(out, out_scales, out_type, N, Co);
+    } else {
+      to = borrow(out, {N, Co}, float_dt(out_type, "out"));
+    }
+    if (residual) tr = borrow(residual, {N, Co}, out_scales ? F32 : to.dt);
+    const Tensor *pb = bias ? &tb : nullptr, *pr = residual ? &tr : nullptr;
+    Tensor* py = out_scales ? nullptr : &to;
+    MxTensor* pq = out_scales ? &qo : nullptr;
+    if (x_scales) mx_linear(mx_rows(x, x_scales, x_fmt, N, K), w, pb, pr, act, py, pq);
+    else mx_linear(borrow(x, {N, K}, float_dt(x_dtype, "x")), x_fmt, w, pb, pr, act, py, pq, workspace, workspace_bytes);
+  });
+}
+
+SPC_API int spc_convnext_mlp_mx_workspace(int64_t N, int64_t C, int fmt, int64_t* bytes) {
+  return guarded([&] {
+    REQ(bytes && N >= 0 && C > 0 && (fmt == SPC_MX_E4M3 || fmt == SPC_MX_E2M1), "arguments");
+    *bytes = convnext_mlp_mx_workspace(N, C, fmt);
+  });
+}
+
+SPC_API int spc_convnext_mlp_mx(const void* h, const void* x, const void* gamma, const void* beta, float eps,
+                                const void* w1_codes, const void* w1_scales, const void* b1, const void* w2_codes,
+                                const void* w2_scales, const void* b2, int dtype, int param_dtype, int fmt, int64_t N,
+                                int64_t C, void* y, void* workspace, int64_t workspace_bytes) {
+  return guarded([&] {
+    REQ(N >= 0 && C > 0, "N=%lld C=%lld", (long long)N, (long long)C);
+    const DT dt = float_dt(dtype, "h/x"), pdt = float_dt(param_dtype, "gamma/beta/b1/b2");
+    const MxTensor w1 = mx_rows(w1_codes, w1_scales, SPC_MX_E2M1, 4 * C, C), w2 = mx_rows(w2_codes, w2_scales, SPC_MX_E2M1, C, 4 * C);
+    Tensor th = borrow(h, {N, C}, dt), tx = borrow(x, {N, C}, dt), ty = borrow(y, {N, C}, dt), tg, tb, tb1, tb2;
+    if (gamma) tg = borrow(gamma, {C}, pdt);
+    if (beta) tb = borrow(beta, {C}, pdt);
+    if (b1) tb1 = borrow(b1, {4 * C}, pdt);
+    if (b2) tb2 = borrow(b2, {C}, pdt);
+    convnext_mlp_mx(th, tx, gamma ? &tg : nullptr, beta ? &tb : nullptr, eps, w1, b1 ? &tb1 : nullptr, w2, b2 ? &tb2 : nullptr,
+                    fmt, ty, workspace, workspace_bytes);
+  });
+}

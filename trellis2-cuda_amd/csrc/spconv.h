@@ -165,6 +165,50 @@ void gather_ln_act(const Tensor& x_src, const Tensor* row_map, int shift, const 
 void convnext_mlp(const Tensor& h, const Tensor& x, const Tensor* gamma, const Tensor* beta, float eps, const Tensor& w1,
                   const Tensor* b1, const Tensor& w2, const Tensor* b2, Tensor& y);
 
+// Microscaled rows: 32 consecutive values of a row share the scale 2^(b - 127) of one byte b (255: the block reads as
+// NaN), their elements are e4m3 (8 bits) or e2m1 (4 bits, two per byte, the even one in the low half). codes:
+// [rows, mx_row_bytes] and scales: [rows, mx_scale_bytes] of U8, contiguous and 16-byte aligned; the first cols / 32
+// scale bytes of a row are in use, the rest are written as zeros and never read. cols is a multiple of 32. A block with
+// an infinity or NaN among its values gets scale 255 and zero elements.
+enum MxFormat : int { MX_E4M3 = 1, MX_E2M1 = 2 };
+struct MxTensor {
+  Tensor codes, scales;
+  int fmt = MX_E4M3;
+  i64 rows = 0, cols = 0;
+};
+i64 mx_row_bytes(int fmt, i64 cols);
+i64 mx_scale_bytes(i64 cols);  // 16 * ceil(cols / 512)
+// x fp32/fp16/bf16 [rows, cols] into q's buffers: per block the least power of two for which the largest magnitude over
+// it rounds to at most the largest element, elements rounded to nearest, halves to even. And q's values into y
+// (fp32: exact; fp16/bf16: rounded once).
+void mx_quantize(const Tensor& x, MxTensor& q);
+void mx_dequantize(const MxTensor& q, Tensor& y);
+
+// t = x + residual (one rounding; without a residual t = x) into sum, which may be x or residual (or null without a
+// residual), and q = the quantised norm of t's rows times gamma plus beta: MX_NORM_RMS t / sqrt(mean(t^2) + eps),
+// MX_NORM_LAYER (t - mean(t)) / sqrt(var(t) + eps); fp32 statistics (|t| below 2^60). x, residual, sum fp16 or bf16
+// [N,C], C a multiple of 32 up to 16384; gamma, beta of any float type or null (1, 0).
+enum MxNorm : int { MX_NORM_RMS = 0, MX_NORM_LAYER = 1 };
+void add_norm_mx(const Tensor& x, const Tensor* residual, const Tensor* gamma, const Tensor* beta, float eps, int kind,
+                 Tensor* sum, MxTensor& q);
+
+// act(x w^T + bias) + residual with fp32 sums: x [N,K] microscaled (either format), w [O,K] e2m1, O a multiple of 32, into
+// y (fp32/fp16/bf16 [N,O], one rounding; residual of y's type, which y may be) or, without a residual, quantised into
+// yq. bias of any float type or null. The second form quantises x (fp32/fp16/bf16) to x_fmt first, in a workspace of
+// mx_linear_workspace() bytes (16-byte aligned; null: one of the library's own, refused while the stream is captured).
+void mx_linear(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y, MxTensor* yq);
+void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y,
+               MxTensor* yq, void* workspace = nullptr, i64 workspace_bytes = 0);
+i64 mx_linear_workspace(i64 N, i64 K, int x_fmt, i64 O);
+
+// convnext_mlp with microscaled products: y = x + W2 mx(silu(W1 mx(LayerNorm(h) * gamma + beta) + b1)) + b2, w1 [4C,C]
+// and w2 [C,4C] e2m1, both activations quantised to fmt; any C that is a multiple of 32 up to 4096. h, x, y of one 16-bit type;
+// y may be h or x. workspace as above, of convnext_mlp_mx_workspace() bytes.
+void convnext_mlp_mx(const Tensor& h, const Tensor& x, const Tensor* gamma, const Tensor* beta, float eps, const MxTensor& w1,
+                     const Tensor* b1, const MxTensor& w2, const Tensor* b2, int fmt, Tensor& y, void* workspace = nullptr,
+                     i64 workspace_bytes = 0);
+i64 convnext_mlp_mx_workspace(i64 N, i64 C, int fmt);
+
 // Conv plus the upsample block's skip connection in one pass: out = act(conv(x) + b) + skip, skip[i, c] =
 // x_skip[src[i] >> 3, (src[i] & 7) * Cin/8 + c / rep], rep = Co / (Cin/8) a power of two, one rounding (reference:
 // subm_conv then k_add_skip, src/sdec.cu:38-43, 82-84). Fused into the 64 -> 64 halo kernel; other shapes run the

@@ -23,6 +23,8 @@ F32, F16, BF16 = 0, 1, 2
 ACT_NONE, ACT_SILU = 0, 1
 EPI_F16_COMPAT = 256  # or'ed into act: the reference's fp16 epilogue rounding sequence
 EMPTY = 0xFFFFFFFF
+MX_E4M3, MX_E2M1 = 1, 2  # element formats of microscaled rows (MxTensor)
+NORM_RMS, NORM_LAYER = 0, 1
 
 # the C ABI's exported symbols (every declaration of include/spconv_amd.h)
 SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_build_neighbors", "spc_build_neighbors_ex", "spc_cache_lookup",
@@ -31,7 +33,9 @@ SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_build_neighbors", "spc_build
            "spc_gather_ln_act", "spc_add_skip", "spc_convnext_mlp", "spc_subm_conv_skip",
            "spc_subdivide", "spc_subdivide_noalloc", "spc_subm_conv_replay", "spc_grid_sample_map",
            "spc_grid_sample_sum", "spc_subdivide_build", "spc_subm_conv_preln", "spc_alloc_counts", "spc_kernel_timing",
-           "spc_kernel_times", "spc_release_cached_memory")
+           "spc_kernel_times", "spc_release_cached_memory", "spc_mx_sizes", "spc_mx_quantize", "spc_mx_dequantize",
+           "spc_add_norm_mx", "spc_mx_linear_workspace", "spc_mx_linear", "spc_convnext_mlp_mx_workspace",
+           "spc_convnext_mlp_mx")
 
 _lib = None
 
@@ -81,6 +85,15 @@ def load_library():
     L.spc_kernel_timing.argtypes = [I]
     L.spc_release_cached_memory.argtypes = [ctypes.POINTER(I64)]
     L.spc_kernel_times.argtypes = [ctypes.POINTER(ctypes.c_float), I, ctypes.POINTER(I)]
+    PI64 = ctypes.POINTER(I64)
+    L.spc_mx_sizes.argtypes = [I64, I64, I, PI64, PI64]
+    L.spc_mx_quantize.argtypes = [P, I, I64, I64, I, P, P]
+    L.spc_mx_dequantize.argtypes = [P, P, I64, I64, I, I, P]
+    L.spc_add_norm_mx.argtypes = [P, P, P, P, I, ctypes.c_float, I, I, I64, I64, I, P, P, P]
+    L.spc_mx_linear_workspace.argtypes = [I64, I64, I64, I, PI64]
+    L.spc_mx_linear.argtypes = [P, P, I, I, P, P, P, I, P, I, I64, I64, I64, I, P, P, P, I64]
+    L.spc_convnext_mlp_mx_workspace.argtypes = [I64, I64, I, PI64]
+    L.spc_convnext_mlp_mx.argtypes = [P, P, P, P, ctypes.c_float, P, P, P, P, P, P, I, I, I, I64, I64, P, P, I64]
     for name in SYMBOLS:
         if name != "spc_last_error":
             getattr(L, name).restype = I
@@ -333,6 +346,203 @@ def convnext_mlp(h, x, gamma, beta, w1, b1, w2, b2, eps: float = 1e-6, out=None)
     _check(load_library().spc_convnext_mlp(_ptr(h), _ptr(x), _ptr(gamma), _ptr(beta), eps, _ptr(w1), _ptr(b1),
                                            _ptr(w2), _ptr(b2), _dt(h), _dt(ps[0]) if ps else F32, N, C,
                                            _ptr(out)))
+    return out
+
+
+class MxTensor:
+    """Microscaled rows [N, K]: 32 consecutive values share the scale 2^(b - 127) of one byte b (255: they read as NaN),
+    their elements are e4m3 (fmt MX_E4M3) or e2m1 (MX_E2M1, two per byte, the even one in the low half). codes uint8
+    [N, K] or [N, K/2], scales uint8 [N, 16 * ceil(K/512)], of which a row's first K/32 are in use."""
+
+    __slots__ = ("codes", "scales", "fmt", "shape")
+
+    def __init__(self, codes, scales, cols: int, fmt: int):
+        torch = _torch()
+        if fmt not in (MX_E4M3, MX_E2M1):
+            raise ValueError(f"unknown format {fmt}")
+        if cols <= 0 or cols % 32:
+            raise ValueError(f"{cols} columns: a positive multiple of 32")
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
+            raise ValueError("codes and scales must be uint8 matrices")
+        rows = codes.shape[0]
+        if codes.shape[1] != (cols // 2 if fmt == MX_E2M1 else cols) or tuple(scales.shape) != (rows, (cols + 511) // 512 * 16):
+            raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not those of {cols} columns")
+        self.codes, self.scales, self.fmt, self.shape = codes, scales, fmt, (rows, cols)
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, fmt: int, device):
+        torch = _torch()
+        codes = torch.empty((rows, cols // 2 if fmt == MX_E2M1 else cols), dtype=torch.uint8, device=device)
+        return cls(codes, torch.empty((rows, (cols + 511) // 512 * 16), dtype=torch.uint8, device=device), cols, fmt)
+
+    def dequantize(self, dtype=None):
+        return mx_dequantize(self, dtype)
+
+
+def _here(*tensors):
+    """The tensors' one device, which has to be the current one (the library launches there)."""
+    torch = _torch()
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if isinstance(t, MxTensor):
+            if t.codes.device != t.scales.device:
+                raise ValueError("codes and scales on different devices")
+            t = t.codes
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise ValueError("tensor must be on the GPU")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    return dev
+
+
+def _matrix(t, name, shape=None, dtype=None):
+    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        raise ValueError(f"{name} must be {list(shape) if shape is not None else 'a matrix'}, got {list(t.shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _vector(t, name, n):
+    if t is not None and t.numel() != n:
+        raise ValueError(f"{name} must have {n} elements")
+
+
+def mx_quantize(x, fmt: int = MX_E2M1, out: MxTensor = None) -> MxTensor:
+    """x (float32, float16 or bfloat16 [N, K], K a multiple of 32) in blocks of 32 values. A block's scale is the least
+    power of two for which its largest magnitude over it rounds to at most the largest element; elements round to
+    nearest, halves to even. A block with an infinity or NaN reads as NaN."""
+    _matrix(x, "x")
+    dev = _here(x, out)
+    if out is None:
+        out = MxTensor.empty(x.shape[0], x.shape[1], fmt, dev)
+    elif out.shape != tuple(x.shape) or out.fmt != fmt:
+        raise ValueError(f"out must be of x's shape {list(x.shape)} and format {fmt}")
+    _check(load_library().spc_mx_quantize(_ptr(x), _dt(x), x.shape[0], x.shape[1], fmt, _ptr(out.codes), _ptr(out.scales)))
+    return out
+
+
+def mx_dequantize(q: MxTensor, dtype=None, out=None):
+    """q's values [N, K] in dtype (default bfloat16; float32 holds every one of them exactly)."""
+    torch = _torch()
+    dev = _here(q, out)
+    if out is None:
+        out = torch.empty(q.shape, dtype=dtype or torch.bfloat16, device=dev)
+    _matrix(out, "out", q.shape, dtype)
+    _check(load_library().spc_mx_dequantize(_ptr(q.codes), _ptr(q.scales), q.shape[0], q.shape[1], q.fmt, _dt(out), _ptr(out)))
+    return out
+
+
+def add_norm_mx(x, residual=None, gamma=None, beta=None, eps: float = 1e-6, kind: int = NORM_RMS, fmt: int = MX_E4M3, sum=None,
+                out: MxTensor = None):
+    """(t, q): t = x + residual, rounded to x's type (x itself without a residual), and q = norm(t) * gamma + beta
+    quantised to fmt; NORM_RMS: t / sqrt(mean(t^2) + eps), NORM_LAYER: (t - mean(t)) / sqrt(var(t) + eps). x, residual
+    float16 or bfloat16 [N, C], C a multiple of 32 up to 16384; sum, the buffer for t, may be x or residual."""
+    torch = _torch()
+    _matrix(x, "x")
+    N, C = x.shape
+    dev = _here(x, residual, gamma, beta, sum, out)
+    if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
+        raise ValueError("gamma and beta must share one dtype")
+    _vector(gamma, "gamma", C)
+    _vector(beta, "beta", C)
+    if residual is not None:
+        _matrix(residual, "residual", x.shape, x.dtype)
+        if sum is None:
+            sum = torch.empty_like(x)
+    if sum is not None:
+        _matrix(sum, "sum", x.shape, x.dtype)
+    if out is None:
+        out = MxTensor.empty(N, C, fmt, dev)
+    elif out.shape != (N, C) or out.fmt != fmt:
+        raise ValueError(f"out must be [{N}, {C}] of format {fmt}")
+    p = gamma if gamma is not None else beta
+    _check(load_library().spc_add_norm_mx(_ptr(x), _ptr(residual), _ptr(gamma), _ptr(beta), _dt(p) if p is not None else F32,
+                                          eps, kind, _dt(x), N, C, fmt, _ptr(sum), _ptr(out.codes), _ptr(out.scales)))
+    return (x if sum is None else sum), out
+
+
+def _workspace(query, device, *sizes):
+    torch = _torch()
+    n = ctypes.c_int64()
+    _check(query(*sizes, ctypes.byref(n)))
+    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+
+
+def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt: int = MX_E4M3, out_dtype=None, out_fmt=None,
+              out=None):
+    """act(x w^T + bias) + residual with fp32 sums: w an MxTensor [Co, K] of format MX_E2M1 (mx_quantize of a torch Linear's
+    weight), Co a multiple of 32; x an MxTensor [N, K] of either format, or a float matrix, which the call quantises to
+    fmt. The result is of out_dtype (default: x's type; bfloat16 for an MxTensor), as residual has to be; out may be the
+    residual. With out_fmt (and no residual) it is an MxTensor of that format."""
+    torch = _torch()
+    quantized = isinstance(x, MxTensor)
+    if not isinstance(w, MxTensor) or w.fmt != MX_E2M1:
+        raise ValueError("w must be an MxTensor of format MX_E2M1")
+    if not quantized:
+        _matrix(x, "x")
+    N, K = x.shape
+    Co = w.shape[0]
+    if w.shape[1] != K:
+        raise ValueError(f"w has {w.shape[1]} columns, x {K}")
+    dev = _here(x, w, bias, residual, out)
+    _vector(bias, "bias", Co)
+    mx_out = out_fmt is not None or isinstance(out, MxTensor)
+    if mx_out:
+        if residual is not None or out_dtype is not None:
+            raise ValueError("a microscaled result takes no residual and no out_dtype")
+        if out is None:
+            out = MxTensor.empty(N, Co, out_fmt, dev)
+        elif not isinstance(out, MxTensor) or out.shape != (N, Co) or out_fmt not in (None, out.fmt):
+            raise ValueError(f"out must be an MxTensor [{N}, {Co}] of format {out_fmt}")
+    else:
+        if out is None:
+            out = torch.empty((N, Co), dtype=out_dtype or (torch.bfloat16 if quantized else x.dtype), device=dev)
+        _matrix(out, "out", (N, Co), out_dtype)
+        if residual is not None:
+            _matrix(residual, "residual", (N, Co), out.dtype)
+    L = load_library()
+    fmt = x.fmt if quantized else fmt
+    ws = None if quantized else _workspace(L.spc_mx_linear_workspace, dev, N, K, Co, fmt)
+    _check(L.spc_mx_linear(
+        _ptr(x.codes if quantized else x), _ptr(x.scales) if quantized else None, F32 if quantized else _dt(x), fmt,
+        _ptr(w.codes), _ptr(w.scales), _ptr(bias), _dt(bias) if bias is not None else F32, _ptr(residual), act, N, K, Co,
+        out.fmt if mx_out else _dt(out), _ptr(out.codes if mx_out else out), _ptr(out.scales) if mx_out else None, _ptr(ws),
+        ws.numel() if ws is not None else 0))
+    return out
+
+
+def convnext_mlp_mx(h, x, gamma, beta, w1: MxTensor, b1, w2: MxTensor, b2, eps: float = 1e-6, fmt: int = MX_E4M3, out=None):
+    """convnext_mlp with 4-bit weights: x + W2 q(silu(W1 q(LayerNorm(h) * gamma + beta) + b1)) + b2, q the quantisation
+    of the activations to fmt. w1 [4C, C], w2 [C, 4C] MxTensors of format MX_E2M1; C a multiple of 32 up to 4096; gamma, beta,
+    b1, b2 share one float dtype (or are None). out may be h or x."""
+    torch = _torch()
+    _matrix(h, "h")
+    N, C = h.shape
+    _matrix(x, "x", h.shape, h.dtype)
+    ps = [p for p in (gamma, beta, b1, b2) if p is not None]
+    if any(p.dtype != ps[0].dtype for p in ps):
+        raise ValueError("gamma, beta, b1, b2 must share one dtype")
+    for name, t, n in (("gamma", gamma, C), ("beta", beta, C), ("b1", b1, 4 * C), ("b2", b2, C)):
+        _vector(t, name, n)
+    for name, w, shape in (("w1", w1, (4 * C, C)), ("w2", w2, (C, 4 * C))):
+        if not isinstance(w, MxTensor) or w.fmt != MX_E2M1 or w.shape != shape:
+            raise ValueError(f"{name} must be an MxTensor {list(shape)} of format MX_E2M1")
+    dev = _here(h, x, gamma, beta, w1, b1, w2, b2, out)
+    if out is None:
+        out = torch.empty_like(h)
+    _matrix(out, "out", h.shape, h.dtype)
+    L = load_library()
+    ws = _workspace(L.spc_convnext_mlp_mx_workspace, dev, N, C, fmt)
+    _check(L.spc_convnext_mlp_mx(
+        _ptr(h), _ptr(x), _ptr(gamma), _ptr(beta), eps, _ptr(w1.codes), _ptr(w1.scales), _ptr(b1), _ptr(w2.codes),
+        _ptr(w2.scales), _ptr(b2), _dt(h), _dt(ps[0]) if ps else F32, fmt, N, C, _ptr(out), _ptr(ws),
+        ws.numel() if ws is not None else 0))
     return out
 
 
