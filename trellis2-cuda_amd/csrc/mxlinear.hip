@@ -27,7 +27,7 @@ struct LinArgs {
   i64 N;
   int K, O, bias_dt, act, f16;
   int xrow, wrow, srow, osrow;  // bytes of a row: X's and W's codes, their scales, out's scales
-  int tiles_n, tiles_o, per, o_major;
+  int tiles_n, tiles_o, per, band;
 };
 
 __device__ __forceinline__ i32x4 rsrc4(const void* p, uint32_t bytes) {  // a raw buffer's descriptor, in SGPRs
@@ -54,22 +54,40 @@ __device__ __forceinline__ void bare_barrier() {
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
 
 template <int XB>
-__device__ __forceinline__ f32x4 mfma(mx_u32x4 w, const mx_u32x4 (&x)[XB / 4], f32x4 c, int sw, int sx) {
+struct XFrag {  // 16 rows of X by 128 columns, this lane's part
+  mx_u32x4 q[XB / 4];
+};
+template <>
+struct XFrag<4> {
+  mx_u32x4 q[1];
+};
+// The scales are byte I of sw and sx
+template <int XB, int I>
+__device__ __forceinline__ f32x4 mfma(mx_u32x4 w, const XFrag<XB>& x, f32x4 c, int sw, int sx) {
   const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
   if constexpr (XB == 8) {
-    const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], (int)x[1][0], (int)x[1][1], (int)x[1][2], (int)x[1][3]};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, 0, sw, 0, sx);
+    const i32x8 b = {(int)x.q[0][0], (int)x.q[0][1], (int)x.q[0][2], (int)x.q[0][3],
+                     (int)x.q[1][0], (int)x.q[1][1], (int)x.q[1][2], (int)x.q[1][3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, I, sw, I, sx);
   } else {
-    const i32x8 b = {(int)x[0][0], (int)x[0][1], (int)x[0][2], (int)x[0][3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, 0, sw, 0, sx);
+    const i32x8 b = {(int)x.q[0][0], (int)x.q[0][1], (int)x.q[0][2], (int)x.q[0][3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, I, sw, I, sx);
   }
+}
+// Of four e4m3 elements those of magnitude 4 and more (codes from 0x48), zeros for the others: a byte's low seven bits plus
+// 0x38 carry into bit 7, which a byte permute spreads (selectors 8 and 9 repeat bits 15 and 31 of its second operand,
+// 10 and 11 those of its first).
+__device__ __forceinline__ uint32_t e4m3_large(uint32_t v) {
+  const uint32_t t = (v & 0x7f7f7f7fu) + 0x38383838u;
+  return v & __builtin_amdgcn_perm(t, t << 8, 0x0b090a08u);
 }
 template <int OUT, int TO>
 constexpr int run_tiles() {  // G above
   return OUT == OUT_F32 ? 1 : OUT == OUT_16 ? 2 : 4 < TO ? 4 : TO;
 }
 
-// Epilogue of 4 G consecutive channels o .. of row n in v: bias, activation, residual, store
+// Epilogue of NV consecutive channels o .. of row n in v: bias, activation, residual, store. Lanes l, l + 16, l + 32, l + 48
+// hold neighbouring runs of one row; ok is the same for all lanes of a block of 32 channels.
 template <int OUT, int NV>
 __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v)[NV], const float (&bias)[NV], bool ok, int g) {
 #pragma unroll
@@ -88,32 +106,46 @@ __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v
     }
     *(f32x4*)((float*)a.out + n * a.O + o) = f32x4{v[0], v[1], v[2], v[3]};
   } else if constexpr (OUT == OUT_16) {
-    static_assert(NV == 8, "one 16-byte piece");
+    static_assert(NV == 8 || NV == 4, "one 16-byte piece, or half of one");
     if (!ok) return;
+    uint32_t q[NV / 2];
     if (a.res) {
-      const mx_u32x4 q = *(const mx_u32x4*)((const uint16_t*)a.res + n * a.O + o);
-      float r[8];
-      if (a.f16) mx_unpack8<true>(q, r);
-      else mx_unpack8<false>(q, r);
+      const uint32_t* r = (const uint32_t*)((const uint16_t*)a.res + n * a.O + o);
+      if constexpr (NV == 8) *(mx_u32x4*)q = *(const mx_u32x4*)r;
+      else *(mx_u32x2*)q = *(const mx_u32x2*)r;
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] += r[j];
+      for (int j = 0; j < NV / 2; j++) {
+        v[2 * j] += a.f16 ? mx_lo<true>(q[j]) : mx_lo<false>(q[j]);
+        v[2 * j + 1] += a.f16 ? mx_hi<true>(q[j]) : mx_hi<false>(q[j]);
+      }
     }
-    *(mx_u32x4*)((uint16_t*)a.out + n * a.O + o) = a.f16 ? mx_pack8<true>(v) : mx_pack8<false>(v);
+#pragma unroll
+    for (int j = 0; j < NV / 2; j++) q[j] = a.f16 ? mx_pack2<true>(v[2 * j], v[2 * j + 1]) : mx_pack2<false>(v[2 * j], v[2 * j + 1]);
+    uint32_t* y = (uint32_t*)((uint16_t*)a.out + n * a.O + o);
+    if constexpr (NV == 8) *(mx_u32x4*)y = *(mx_u32x4*)q;
+    else *(mx_u32x2*)y = *(mx_u32x2*)q;
   } else {
-    // 16 channels a lane, two lanes (g and g ^ 1) a block; both are inside or outside together
-    static_assert(NV == 16, "half a block");
+    static_assert(NV == 16 || NV == 8, "a half or a quarter of a block");
     constexpr int FMT = OUT == OUT_MX8 ? MX_E4M3 : MX_E2M1;
-    float(&lo)[8] = *(float(*)[8])&v[0];
-    float(&hi)[8] = *(float(*)[8])&v[8];
-    uint32_t top = max(mx_top8(lo), mx_top8(hi));
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < NV; j += 8) top = max(top, mx_top8(*(float(*)[8])&v[j]));
     top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    if constexpr (NV == 8) top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
     const uint32_t byte = mx_scale_byte<FMT>(top);
     const float inv = mx_inverse(byte);
-    const mx_u32x2 p = mx_encode8<FMT>(lo, inv), q = mx_encode8<FMT>(hi, inv);
-    if (!ok) return;
-    if constexpr (FMT == MX_E4M3) *(mx_u32x4*)((uint8_t*)a.out + n * a.O + o) = mx_u32x4{p[0], p[1], q[0], q[1]};
-    else *(mx_u32x2*)((uint8_t*)a.out + (n * a.O + o) / 2) = mx_u32x2{p[0], q[0]};
-    if ((g & 1) == 0) {
+    const mx_u32x2 p = mx_encode8<FMT>(*(float(*)[8])&v[0], inv);
+    if constexpr (NV == 16) {
+      const mx_u32x2 q = mx_encode8<FMT>(*(float(*)[8])&v[8], inv);
+      if (!ok) return;
+      if constexpr (FMT == MX_E4M3) *(mx_u32x4*)((uint8_t*)a.out + n * a.O + o) = mx_u32x4{p[0], p[1], q[0], q[1]};
+      else *(mx_u32x2*)((uint8_t*)a.out + (n * a.O + o) / 2) = mx_u32x2{p[0], q[0]};
+    } else {
+      if (!ok) return;
+      if constexpr (FMT == MX_E4M3) *(mx_u32x2*)((uint8_t*)a.out + n * a.O + o) = p;
+      else *(uint32_t*)((uint8_t*)a.out + (n * a.O + o) / 2) = p[0];
+    }
+    if (o % 32 == 0) {
       uint8_t* s = a.outs + n * a.osrow;
       s[o / 32] = (uint8_t)byte;
       if (o / 32 + 1 == a.O / 32)
@@ -122,28 +154,205 @@ __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v
   }
 }
 
+// The parts of e4m3 elements that SPLIT products take apart (see k_mx_gemm)
+__device__ __forceinline__ void split(const XFrag<8>& x, XFrag<8>& small, XFrag<8>& large) {
+#pragma unroll
+  for (int k = 0; k < 2; k++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      large.q[k][j] = e4m3_large(x.q[k][j]);
+      small.q[k][j] = x.q[k][j] ^ large.q[k][j];
+    }
+}
+
+// Few rows: what counts is that all of W is on its way at once. A workgroup of 8 wavefronts has 16 OT channels by 16 NT rows;
+// each wavefront takes a contiguous eighth of K, both operands straight into registers, and the eight sums meet in
+// LDS in a fixed order. XT: x's type (fp32, fp16, bf16), quantised here by every workgroup for itself, which costs less
+// than a launch of its own (NT = 1); or -1: x's codes.
+template <int XB, int OUT, int XT, int OT, int NT>
+__global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
+  constexpr bool SPLIT = XB == 8 && OUT != OUT_16;
+  constexpr int G = OUT == OUT_F32 ? 1 : OT;
+  __shared__ f32x4 part[8][OT * NT][64];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int S = (a.K + 127) / 128, blocks = a.K / 32, per = (S + 7) / 8;
+  const int s0 = wave * per, s1 = min(s0 + per, S);
+  const i64 n0 = (i64)blockIdx.y * (16 * NT);
+  const int o0 = blockIdx.x * (16 * OT);
+  int chan[OT];
+#pragma unroll
+  for (int t = 0; t < OT; t++) chan[t] = o0 + t / G * (16 * G) + r16 / 4 * (4 * G) + t % G * 4 + r16 % 4;
+  f32x4 acc[OT][NT];
+#pragma unroll
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int u = 0; u < NT; u++) acc[t][u] = f32x4{};
+  struct Step {
+    mx_u32x4 w[OT];
+    int sw[OT], sx[NT];
+    XFrag<XB> x[NT];
+  };
+  // O is a multiple of 32, so every channel exists; rows past the last repeat it (their results are not stored)
+  auto load = [&](Step& q, int s) __attribute__((always_inline)) {
+    const bool in = s * 4 + g < blocks;  // columns past the last: zeros and scale 0
+#pragma unroll
+    for (int t = 0; t < OT; t++) {
+      q.w[t] = in ? *(const mx_u32x4*)(a.w + (i64)chan[t] * a.wrow + s * 64 + g * 16) : mx_u32x4{};
+      q.sw[t] = in ? a.ws[(i64)chan[t] * a.srow + s * 4 + g] : 0;
+    }
+    if constexpr (XT < 0) {
+#pragma unroll
+      for (int u = 0; u < NT; u++) {
+        const i64 n = min(n0 + u * 16 + r16, a.N - 1);
+        const uint8_t* x = a.x + n * a.xrow + s * (XB * 16) + g * 16;
+        if constexpr (XB == 8) {  // block g / 2 for the first piece, 2 + g / 2 for the second
+          q.x[u].q[0] = s * 4 + g / 2 < blocks ? *(const mx_u32x4*)x : mx_u32x4{};
+          q.x[u].q[1] = s * 4 + 2 + g / 2 < blocks ? *(const mx_u32x4*)(x + 64) : mx_u32x4{};
+        } else {
+          q.x[u].q[0] = in ? *(const mx_u32x4*)x : mx_u32x4{};
+        }
+        q.sx[u] = in ? a.xs[n * a.srow + s * 4 + g] : 0;
+      }
+    } else {
+      static_assert(NT == 1, "quantised once per workgroup");
+      const bool row = n0 + r16 < a.N;
+      float v[32];  // e2m1: block g; e4m3: halves of blocks g / 2 and 2 + g / 2
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int c = XB == 4 ? g * 32 + k * 8 : k / 2 * 64 + g * 16 + k % 2 * 8;
+        const i64 at = (n0 + r16) * a.K + s * 128 + c;
+        const bool live = row && s * 128 + c < a.K;
+        float(&o)[8] = *(float(*)[8])&v[k * 8];
+        if constexpr (XT == F32) {
+          const f32x4 p = live ? *(const f32x4*)((const float*)a.x + at) : f32x4{}, r = live ? *(const f32x4*)((const float*)a.x + at + 4) : f32x4{};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            o[j] = p[j];
+            o[4 + j] = r[j];
+          }
+        } else {
+          mx_unpack8<XT == F16>(live ? *(const mx_u32x4*)((const uint16_t*)a.x + at) : mx_u32x4{}, o);
+        }
+      }
+      uint32_t top[2];
+#pragma unroll
+      for (int h = 0; h < 2; h++) top[h] = max(mx_top8(*(float(*)[8])&v[h * 16]), mx_top8(*(float(*)[8])&v[h * 16 + 8]));
+      if constexpr (XB == 8) {
+        uint32_t byte[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          top[h] = max(top[h], (uint32_t)__shfl_xor((int)top[h], 16, 64));
+          byte[h] = mx_scale_byte<MX_E4M3>(top[h]);
+          const float inv = mx_inverse(byte[h]);
+          const mx_u32x2 p = mx_encode8<MX_E4M3>(*(float(*)[8])&v[h * 16], inv), r = mx_encode8<MX_E4M3>(*(float(*)[8])&v[h * 16 + 8], inv);
+          q.x[0].q[h] = mx_u32x4{p[0], p[1], r[0], r[1]};
+        }
+        // block g's scale is with lanes 32 (g % 2) + r16 of half g / 2
+        const int from = (g & 1) * 32 + r16, b0 = __shfl((int)byte[0], from, 64), b1 = __shfl((int)byte[1], from, 64);
+        q.sx[0] = g < 2 ? b0 : b1;
+      } else {
+        const uint32_t byte = mx_scale_byte<MX_E2M1>(max(top[0], top[1]));
+        const float inv = mx_inverse(byte);
+#pragma unroll
+        for (int k = 0; k < 4; k++) q.x[0].q[0][k] = mx_encode8<MX_E2M1>(*(float(*)[8])&v[k * 8], inv)[0];
+        q.sx[0] = (int)byte;
+      }
+    }
+  };
+  auto multiply = [&](const Step& q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NT; u++) {
+      if constexpr (SPLIT) {
+        XFrag<8> small, large;
+        split(q.x[u], small, large);
+#pragma unroll
+        for (int t = 0; t < OT; t++) {
+          acc[t][u] = mfma<XB, 0>(q.w[t], small, acc[t][u], q.sw[t], q.sx[u]);
+          acc[t][u] = mfma<XB, 0>(q.w[t], large, acc[t][u], q.sw[t], q.sx[u]);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < OT; t++) acc[t][u] = mfma<XB, 0>(q.w[t], q.x[u], acc[t][u], q.sw[t], q.sx[u]);
+      }
+    }
+  };
+  constexpr int U = NT == 1 ? 4 : NT <= 2 ? 2 : 1;  // steps loaded at once
+  int s = s0;
+  for (; s + U <= s1; s += U) {
+    Step q[U];
+#pragma unroll
+    for (int k = 0; k < U; k++) load(q[k], s + k);
+#pragma unroll
+    for (int k = 0; k < U; k++) multiply(q[k]);
+  }
+  for (; s < s1; s++) {
+    Step q;
+    load(q, s);
+    multiply(q);
+  }
+#pragma unroll
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int u = 0; u < NT; u++) part[wave][t * NT + u][lane] = acc[t][u];
+  __syncthreads();
+  // a wavefront finishes whole runs (G tiles) of the row tiles that fall to it
+  constexpr int RUNS = OT / G * NT;
+  for (int k = wave; k < RUNS; k += 8) {
+    const int t = k / NT * G, u = k % NT;
+    float v[4 * G], bias[4 * G];
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+      f32x4 c = part[0][(t + j) * NT + u][lane];
+#pragma unroll
+      for (int w = 1; w < 8; w++) c += part[w][(t + j) * NT + u][lane];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[j * 4 + i] = c[i];
+    }
+    const i64 n = n0 + u * 16 + r16;
+    const int o = o0 + t / G * (16 * G) + g * (4 * G);
+    mx_params<4 * G>(a.bias, a.bias_dt, o, 0.f, bias);
+    finish<OUT>(a, n, o, v, bias, n < a.N, g);
+  }
+}
+
 // Tiled product. A workgroup of WO x WN wavefronts has BO = 16 TO WO channels by BN = 16 TN WN rows; K goes by steps of
-// 128 through NS slots of LDS, filled by DMA NS - 1 steps ahead, with one barrier a step; the scales go by 512 columns
-// (16 bytes a row), two slots. LDS rows are 64 (e2m1) or 128 bytes (e4m3) of a step, their 16-byte pieces permuted
-// (piece c of row q at c ^ (q >> 2) % 4 or c ^ q % 8), so that eight lanes of neighbouring rows read from distinct banks.
-template <int XB, int OUT, int TO, int TN, int WO, int WN, int NS>
+// 128 through NS slots of LDS, filled by DMA; the scales go by 512 columns (16 bytes a row), two slots. LDS rows are 64
+// (e2m1) or 128 bytes (e4m3) of a step, their 16-byte pieces permuted (piece c of row q at c ^ (q >> 2) % 4 or c ^ q % 8),
+// so that eight lanes of neighbouring rows read from distinct banks.
+//
+// A step's products go in four quarters, halves of W's channel tiles by halves of X's row tiles, in the order (0, f), (0, 1 - f),
+// (1, 1 - f), (1, f) with f = 0, 1 in turn: each quarter changes one operand's half, whose registers were free a quarter
+// earlier, so every LDS read is issued one quarter before its use and a wavefront holds one step's operands only. In the
+// middle all wavefronts meet: by then each has read the whole slot, so it is filled again at once. One barrier a stage,
+// and NS - 1/2 stages for a DMA to land.
+//
+// SPLIT (e4m3): the matrix unit adds eight neighbouring products at a time and drops what is below 2^-13 of the largest.
+// An output of 16 bits does not show it. Where the result keeps more (fp32) or is quantised again (an error that moves a
+// value over a border between elements costs a whole step), each step's products are taken for the elements of magnitude
+// 4 and more and for the smaller ones apart: with e2m1 factors both parts span 13 bits and are exact.
+template <int XB, int OUT, int TO, int TN, int WO, int WN, int KS, int NS>
 __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
-  constexpr int NW = WO * WN, BO = 16 * TO * WO, BN = 16 * TN * WN, D = NS - 1;
-  constexpr int XR = XB == 8 ? 128 : 64;                                       // bytes of a row of X per step
-  constexpr int XI = BN * XR / 1024 / NW, WI = BO * 64 / 1024 / NW, SI = (BO + BN) / 64 / NW;  // DMAs per wavefront
-  static_assert(XI * 1024 * NW == BN * XR && WI * 1024 * NW == BO * 64 && SI * 64 * NW == BO + BN, "whole DMAs");
+  constexpr int NW = WO * WN, BO = 16 * TO * WO, BN = 16 * TN * WN, H = TO / 2, HX = TN / 2;
+  constexpr bool SPLIT = XB == 8 && OUT != OUT_16;
+  constexpr int XR = XB * 16 * KS, WR = 64 * KS;                                // bytes of a row of X and W per stage
+  constexpr int XP = XR / 16, WP = WR / 16;                                     // 16-byte pieces of them
+  constexpr int XI = BN * XR / 1024 / NW, WI = BO * WR / 1024 / NW, SI = (BO + BN) / 64 / NW;  // DMAs per wavefront
+  static_assert(XI * 1024 * NW == BN * XR && WI * 1024 * NW == BO * WR && SI * 64 * NW == BO + BN, "whole DMAs");
+  static_assert((XR == 64 || XR == 128) && (WR == 64 || WR == 128), "swizzles");
   constexpr int G = run_tiles<OUT, TO>();
-  static_assert(TO % G == 0, "whole runs");
-  __shared__ __attribute__((aligned(16))) mx_u32x4 lds[NS * (BN * XR + BO * 64) / 16 + 2 * (BO + BN)];
-  constexpr uint32_t kSlot = BN * XR + BO * 64, kScales = NS * kSlot, kScaleSlot = (BO + BN) * 16;
+  static_assert(TO % G == 0 && TO % 2 == 0 && TN % 2 == 0 && NS >= 2 && NS <= 4, "whole runs, two halves");
+  __shared__ __attribute__((aligned(16))) mx_u32x4 lds[NS * (BN * XR + BO * WR) / 16 + 2 * (BO + BN)];
+  constexpr uint32_t kSlot = BN * XR + BO * WR, kScales = NS * kSlot, kScaleSlot = (BO + BN) * 16;
 
   const int logical = (blockIdx.x % 8) * a.per + blockIdx.x / 8;  // each XCD walks one contiguous range of tiles
   if (logical >= a.tiles_n * a.tiles_o) return;
-  const int tn = a.o_major ? logical % a.tiles_n : logical / a.tiles_o;
-  const int to = a.o_major ? logical / a.tiles_n : logical % a.tiles_o;
+  // tiles in bands of `band` columns, row by row within a band
+  const int first = logical / (a.band * a.tiles_n) * a.band, width = min(a.band, a.tiles_o - first);
+  const int inside = logical - first * a.tiles_n, tn = inside / width, to = first + inside % width;
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wo = wave % WO, wn = wave / WO;
-  const int S = (a.K + 127) / 128;
+  const int S = (a.K + 127) / 128, stages = (S + KS - 1) / KS, blocks = a.K / 32;
   const i64 n0 = (i64)tn * BN;
   const int o0 = to * BO;
   const int rows = (int)min((i64)BN, a.N - n0), chans = min(BO, a.O - o0);
@@ -157,44 +366,67 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
     const int t = p / 16 % TO, r = p % 16;
     return p / (16 * TO) * (16 * TO) + t / G * (16 * G) + r / 4 * (4 * G) + t % G * 4 + r % 4;
   };
+  // where piece c of a row lies in the row's place in LDS, and (an involution) the piece that lies there
+  auto place = [](auto PC, int row, int c) __attribute__((always_inline)) {
+    return decltype(PC)::value == 8 ? c ^ (row & 7) : c ^ (row >> 1 & 3);
+  };
+  constexpr std::integral_constant<int, XP> XPC{};
+  constexpr std::integral_constant<int, WP> WPC{};
   uint32_t xoff[XI], woff[WI], soff[SI];
-  int xc[XI], wc[WI];  // first byte within the step, to cut a last step short
 #pragma unroll
   for (int k = 0; k < XI; k++) {
-    const int p = (wave * XI + k) * 64 + lane, q = p / (XR / 16), c = p % (XR / 16);
-    xc[k] = XB == 8 ? (c ^ (q & 7)) * 16 : (c ^ ((q >> 2) & 3)) * 16;
-    xoff[k] = q < rows ? (uint32_t)(q * a.xrow + xc[k]) : kOOR;
+    const int p = (wave * XI + k) * 64 + lane, q = p / XP;
+    xoff[k] = q < rows ? (uint32_t)(q * a.xrow + place(XPC, q, p % XP) * 16) : kOOR;
   }
 #pragma unroll
   for (int k = 0; k < WI; k++) {
-    const int p = (wave * WI + k) * 64 + lane, q = p / 4, c = p % 4, ch = channel(q);
-    wc[k] = (c ^ ((q >> 2) & 3)) * 16;
-    woff[k] = ch < chans ? (uint32_t)(ch * a.wrow + wc[k]) : kOOR;
+    const int p = (wave * WI + k) * 64 + lane, q = p / WP, ch = channel(q);
+    woff[k] = ch < chans ? (uint32_t)(ch * a.wrow + place(WPC, q, p % WP) * 16) : kOOR;
   }
 #pragma unroll
   for (int k = 0; k < SI; k++) {
     const int p = (wave * SI + k) * 64 + lane, ch = channel(p < BO ? p : 0);
     soff[k] = p < BO ? (ch < chans ? (uint32_t)(ch * a.srow) : kOOR) : p - BO < rows ? (uint32_t)((p - BO) * a.srow) : kOOR;
   }
-  // fills step t's slot; past the last step the DMAs still run (the waits count them) but read nothing
+  // fills stage t's slot; past the last one the DMAs still run (the waits count them) but read nothing
   auto issue = [&](int t, int slot) __attribute__((always_inline)) {
-    const bool live = t < S;
-    if (t % 4 == 0) {
+    const bool live = t < stages;
+    auto of = [&](i32x4 r) __attribute__((always_inline)) {
+      r[2] = live ? r[2] : 0;
+      return r;
+    };
+    if (t * KS % 4 == 0) {
 #pragma unroll
       for (int k = 0; k < SI; k++) {
         const int p0 = (wave * SI + k) * 64;  // BO is a multiple of 64: a DMA's rows are all W's or all X's
-        const bool w = p0 < BO;
-        dma16(w ? rws : rxs, lds0 + kScales + (t / 4 & 1) * kScaleSlot + p0 * 16, live ? soff[k] : kOOR, live ? t * 4 : 0);
+        dma16(of(p0 < BO ? rws : rxs), lds0 + kScales + (t * KS / 4 & 1) * kScaleSlot + p0 * 16, soff[k], live ? t * KS * 4 : 0);
       }
     }
-    const bool cut = live && (t + 1) * 128 > a.K;
-    const int xleft = cut ? a.xrow - t * XR : XR, wleft = cut ? a.wrow - t * 64 : 64;
+    const i32x4 fx = of(rx), fw = of(rw);
+    const int xs = live ? t * XR : 0, ws = live ? t * WR : 0;
+    const uint32_t at = lds0 + slot * kSlot;
+    if (live && (t + 1) * (KS * 128) > a.K) {
+      // the last stage ends inside its columns: pieces past them read as zeros. (Their places are computed here, from a
+      // copy of the lane that the compiler cannot see through: kept in registers over the loop they would spill.)
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      const int xleft = a.xrow - xs, wleft = a.wrow - ws;
 #pragma unroll
-    for (int k = 0; k < XI; k++)
-      dma16(rx, lds0 + slot * kSlot + (wave * XI + k) * 1024, live && xc[k] < xleft ? xoff[k] : kOOR, live ? t * XR : 0);
+      for (int k = 0; k < XI; k++) {
+        const int p = (wave * XI + k) * 64 + l;
+        dma16(fx, at + (wave * XI + k) * 1024, place(XPC, p / XP, p % XP) * 16 < xleft ? xoff[k] : kOOR, xs);
+      }
 #pragma unroll
-    for (int k = 0; k < WI; k++)
-      dma16(rw, lds0 + slot * kSlot + BN * XR + (wave * WI + k) * 1024, live && wc[k] < wleft ? woff[k] : kOOR, live ? t * 64 : 0);
+      for (int k = 0; k < WI; k++) {
+        const int p = (wave * WI + k) * 64 + l;
+        dma16(fw, at + BN * XR + (wave * WI + k) * 1024, place(WPC, p / WP, p % WP) * 16 < wleft ? woff[k] : kOOR, ws);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < XI; k++) dma16(fx, at + (wave * XI + k) * 1024, xoff[k], xs);
+#pragma unroll
+      for (int k = 0; k < WI; k++) dma16(fw, at + BN * XR + (wave * WI + k) * 1024, woff[k], ws);
+    }
   };
 
   f32x4 acc[TO][TN];
@@ -203,46 +435,111 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
 #pragma unroll
     for (int u = 0; u < TN; u++) acc[t][u] = f32x4{};
 
-  // where this lane reads, in 16-byte units of a slot
+  // where this lane reads, in 16-byte units of a slot: pieces of sub-step j
   const int xq = wn * (16 * TN) + r16, wp = wo * (16 * TO) + r16;
-  const int xa0 = XB == 8 ? xq * 8 + (g ^ (r16 & 7)) : xq * 4 + (g ^ (r16 >> 2)), xa1 = xq * 8 + ((g + 4) ^ (r16 & 7));
-  const int wa = BN * XR / 16 + wp * 4 + (g ^ (r16 >> 2));
-  const int blocks = a.K / 32;
-
-  int fill = 0;
+  auto xat = [&](int c) __attribute__((always_inline)) { return xq * XP + place(XPC, r16, c); };
+  auto wat = [&](int c) __attribute__((always_inline)) { return BN * XP + wp * WP + place(WPC, r16, c); };
+  int xa[XB == 8 ? 2 : KS], wa[KS];  // e4m3: its two pieces (KS = 1); e2m1: one per sub-step
 #pragma unroll
-  for (int t = 0; t < D; t++) issue(t, fill++);
-  int cur = 0;
-  auto step = [&](auto I, int s) __attribute__((always_inline)) {
-    constexpr int i = decltype(I)::value;
-    // the D - 1 steps after this one may be in flight, and the scales that come with them
-    constexpr int ahead = (D - 1) * (XI + WI) + SI * ((D > 1 && (i + 1) % 4 == 0) + (D > 2 && (i + 2) % 4 == 0));
-    static_assert(D <= 3, "at most two steps after this one");
-    wait_vm<ahead>();
-    bare_barrier();
-    issue(s + D, fill);
-    fill = fill + 1 == NS ? 0 : fill + 1;
-    const mx_u32x4* slot = lds + cur * (kSlot / 16);
-    const uint8_t* sc = (const uint8_t*)lds + kScales + (s / 4 & 1) * kScaleSlot + i * 4 + g;
-    const bool in = s * 4 + g < blocks;  // the padding behind a row's last scale is not read as a scale
-    mx_u32x4 fx[TN][XB / 4];
-    int sx[TN];
+  for (int j = 0; j < (XB == 8 ? 2 : KS); j++) xa[j] = xat(4 * j + g);
 #pragma unroll
-    for (int u = 0; u < TN; u++) {
-      fx[u][0] = slot[xa0 + u * (XR)];
-      if constexpr (XB == 8) fx[u][1] = slot[xa1 + u * XR];
-      const int b = sc[(BO + xq + u * 16) * 16];
-      sx[u] = in ? b : 0;
+  for (int j = 0; j < KS; j++) wa[j] = wat(4 * j + g);
+  static_assert(XB == 4 || KS == 1, "e4m3 rows are 128 bytes a step");
+  XFrag<XB> fx[2][HX];
+  mx_u32x4 fw[2][H];
+  int sx[TN], sw[TO];  // scales of four steps: byte i is step i's
+  auto read_x = [&](XFrag<XB>(&f)[HX], int slot, int j, int half) __attribute__((always_inline)) {
+    const mx_u32x4* l = lds + slot * (kSlot / 16) + half * (HX * 16 * XP);
+#pragma unroll
+    for (int u = 0; u < HX; u++) {
+      f[u].q[0] = l[xa[XB == 8 ? 0 : j] + u * (16 * XP)];
+      if constexpr (XB == 8) f[u].q[1] = l[xa[1] + u * (16 * XP)];
     }
+  };
+  auto read_w = [&](mx_u32x4(&f)[H], int slot, int j, int half) __attribute__((always_inline)) {
+    const mx_u32x4* l = lds + slot * (kSlot / 16) + wa[j] + half * (H * 16 * WP);
+#pragma unroll
+    for (int t = 0; t < H; t++) f[t] = l[t * (16 * WP)];
+  };
+  const uint32_t pick = (uint32_t)g * 0x0101u + 0x0400u;  // bytes g of two words, the second operand's first
+  auto read_scales = [&](int c) __attribute__((always_inline)) {
+    const mx_u32x4* l = lds + (kScales + (c & 1) * kScaleSlot) / 16;
+    auto gather = [&](mx_u32x4 q) __attribute__((always_inline)) {
+      const uint32_t lo = __builtin_amdgcn_perm(q[1], q[0], pick), hi = __builtin_amdgcn_perm(q[3], q[2], pick);
+      return (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
+    };
 #pragma unroll
     for (int t = 0; t < TO; t++) {
-      const mx_u32x4 fw = slot[wa + t * 64];
-      const int b = sc[(wp + t * 16) * 16];
-      const int sw = in ? b : 0;
-#pragma unroll
-      for (int u = 0; u < TN; u++) acc[t][u] = mfma<XB>(fw, fx[u], acc[t][u], sw, sx[u]);
+      sw[t] = gather(l[wp + t * 16]);
+      if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // few words at a time: the registers are short
     }
-    cur = cur + 1 == NS ? 0 : cur + 1;
+#pragma unroll
+    for (int u = 0; u < TN; u++) {
+      sx[u] = gather(l[BO + xq + u * 16]);
+      if (u % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (c * 16 + 16 > blocks) {  // the padding behind a row's last scale is not read as a scale
+      uint32_t keep = 0;
+#pragma unroll
+      for (int i = 0; i < 4; i++) keep |= c * 16 + i * 4 + g < blocks ? 0xffu << (8 * i) : 0u;
+#pragma unroll
+      for (int t = 0; t < TO; t++) sw[t] &= keep;
+#pragma unroll
+      for (int u = 0; u < TN; u++) sx[u] &= keep;
+    }
+  };
+
+#pragma unroll
+  for (int t = 0; t < NS; t++) issue(t, t);
+  wait_vm<(NS - 1) * (XI + WI)>();
+  bare_barrier();
+  read_x(fx[0], 0, 0, 0);
+  read_w(fw[0], 0, 0, 0);
+  read_scales(0);
+  int cur = 0;
+  auto step = [&](auto IC, int s) __attribute__((always_inline)) {
+    constexpr int I = decltype(IC)::value, J = I % KS, JN = (I + 1) % KS;  // sub-step of this and of the next one
+    constexpr int f = I & 1;
+    auto quarter = [&](auto WC, auto XC) __attribute__((always_inline)) {
+      constexpr int hw = decltype(WC)::value, hx = decltype(XC)::value;
+#pragma unroll
+      for (int u = 0; u < HX; u++) {
+        XFrag<XB> small = fx[hx][u], large = {};
+        if constexpr (SPLIT) split(fx[hx][u], small, large);
+#pragma unroll
+        for (int t = 0; t < H; t++) {
+          f32x4& c = acc[hw * H + t][hx * HX + u];
+          c = mfma<XB, I>(fw[hw][t], small, c, sw[hw * H + t], sx[hx * HX + u]);
+          if constexpr (SPLIT) c = mfma<XB, I>(fw[hw][t], large, c, sw[hw * H + t], sx[hx * HX + u]);
+        }
+      }
+    };
+    constexpr std::integral_constant<int, 0> first{};
+    constexpr std::integral_constant<int, 1> second{};
+    constexpr std::integral_constant<int, f> xf{};
+    constexpr std::integral_constant<int, 1 - f> xo{};
+    read_x(fx[1 - f], cur, J, 1 - f);
+    read_w(fw[1], cur, J, 1);
+    quarter(first, xf);
+    __builtin_amdgcn_sched_barrier(0);
+    quarter(first, xo);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (JN == 0) {
+      // the next stage has landed (up to NS - 2 later ones may be on their way), and this one is in registers
+      constexpr int A = I + 1 - KS;  // first step of this stage, modulo 4
+      wait_vm<(NS - 2) * (XI + WI) + SI * ((NS > 2 && (A + 2 * KS) % 4 == 0) + (NS > 3 && (A + 3 * KS) % 4 == 0))>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      bare_barrier();
+      issue(s / KS + NS, cur);
+      cur = cur + 1 == NS ? 0 : cur + 1;
+    }
+    read_w(fw[0], cur, JN, 0);
+    quarter(second, xo);
+    __builtin_amdgcn_sched_barrier(0);
+    read_x(fx[1 - f], cur, JN, 1 - f);
+    quarter(second, xf);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (I == 3) read_scales(s / 4 + 1);
   };
   for (int s = 0; s < S; s += 4) {
     step(std::integral_constant<int, 0>{}, s);
@@ -270,7 +567,7 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
   }
 }
 
-template <int XB, int OUT, int TO, int TN, int WO, int WN, int NS>
+template <int XB, int OUT, int TO, int TN, int WO, int WN, int KS, int NS>
 void launch(LinArgs a) {
   constexpr int BO = 16 * TO * WO, BN = 16 * TN * WN;
   const i64 tn = (a.N + BN - 1) / BN, to = (a.O + BO - 1) / BO;
@@ -278,17 +575,38 @@ void launch(LinArgs a) {
   a.tiles_n = (int)tn;
   a.tiles_o = (int)to;
   a.per = cdiv(tn * to, 8);
-  a.o_major = (i64)a.O * a.wrow > (2 << 20);
-  k_mx_gemm<XB, OUT, TO, TN, WO, WN, NS><<<a.per * 8, 64 * WO * WN, 0, stream()>>>(a);
+  a.band = (int)std::min<i64>(to, 4);
+  k_mx_gemm<XB, OUT, TO, TN, WO, WN, KS, NS><<<a.per * 8, 64 * WO * WN, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
 
+// Up to kFewRows rows go through k_mx_rows; up to 16 of them may come as values.
+constexpr int kFewRows = 128, kValueRows = 16;
+template <int XB, int OUT, int XT, int NT>
+void launch_rows(const LinArgs& a) {
+  constexpr int OT = OUT == OUT_MX8 || OUT == OUT_MX4 ? 2 : NT == 1 ? 1 : 2;
+  const dim3 grid(a.O / (16 * OT), (unsigned)((a.N + 16 * NT - 1) / (16 * NT)));
+  k_mx_rows<XB, OUT, XT, OT, NT><<<grid, 512, 0, stream()>>>(a);
+  CK(hipGetLastError());
+}
 template <int XB, int OUT>
-void gemm(const LinArgs& a) {
+void gemm(const LinArgs& a, int xt) {
+  if (xt >= 0) {
+    if (xt == F32) launch_rows<XB, OUT, F32, 1>(a);
+    else if (xt == F16) launch_rows<XB, OUT, F16, 1>(a);
+    else launch_rows<XB, OUT, BF16, 1>(a);
+    return;
+  }
+  if (a.N <= 16) return launch_rows<XB, OUT, -1, 1>(a);
+  if (a.N <= 32) return launch_rows<XB, OUT, -1, 2>(a);
+  if (a.N <= 64) return launch_rows<XB, OUT, -1, 4>(a);
+  if (a.N <= kFewRows) return launch_rows<XB, OUT, -1, 5>(a);
   const i64 cus = mx_device_cus();
   const i64 big = (i64)cdiv(a.N, 256) * cdiv(a.O, 256);
-  if (big >= cus) launch<XB, OUT, 8, 4, 2, 4, XB == 8 ? 3 : 4>(a);
-  else launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 3 : 4>(a);
+  if constexpr (XB == 4 || OUT == OUT_16) {
+    if (big >= cus) return launch<XB, OUT, 8, 4, 2, 4, 1, XB == 8 ? 3 : 4>(a);
+  }
+  launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
 }
 }  // namespace
 
@@ -335,10 +653,12 @@ i64 rows_bytes(int fmt, i64 n, i64 cols) {
 }
 
 // shapes and types are checked by the callers
-void product(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* res, int act, Tensor* y, MxTensor* yq) {
+// xv: x's values (at most 16 rows), which the product quantises to x's format itself; else x's codes
+void product(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* res, int act, Tensor* y, MxTensor* yq,
+             const Tensor* xv = nullptr) {
   if (x.rows == 0) return;
   LinArgs a{};
-  a.x = x.codes.ptr<uint8_t>();
+  a.x = xv ? xv->ptr<uint8_t>() : x.codes.ptr<uint8_t>();
   a.xs = x.scales.ptr<uint8_t>();
   a.w = w.codes.ptr<uint8_t>();
   a.ws = w.scales.ptr<uint8_t>();
@@ -362,9 +682,10 @@ void product(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Ten
   }
   auto by_out = [&](auto X) {
     constexpr int XB = decltype(X)::value;
-    if (!y) yq->fmt == MX_E4M3 ? gemm<XB, OUT_MX8>(a) : gemm<XB, OUT_MX4>(a);
-    else if (y->dt == F32) gemm<XB, OUT_F32>(a);
-    else gemm<XB, OUT_16>(a);
+    const int xt = xv ? (int)xv->dt : -1;
+    if (!y) yq->fmt == MX_E4M3 ? gemm<XB, OUT_MX8>(a, xt) : gemm<XB, OUT_MX4>(a, xt);
+    else if (y->dt == F32) gemm<XB, OUT_F32>(a, xt);
+    else gemm<XB, OUT_16>(a, xt);
   };
   x.fmt == MX_E4M3 ? by_out(std::integral_constant<int, 8>{}) : by_out(std::integral_constant<int, 4>{});
 }
@@ -425,13 +746,20 @@ void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias
   if (bias) out_apart(y, yq, *bias, "bias");
   if (n == 0) return;
   Workspace ws(workspace, workspace_bytes, mx_linear_workspace(n, K, x_fmt, w.rows));
+  if (n <= kValueRows) {
+    MxTensor q;
+    q.fmt = x_fmt;
+    q.rows = n;
+    q.cols = K;
+    return product(q, w, bias, residual, act, y, yq, &x);
+  }
   MxTensor q = ws.rows(x_fmt, n, K);
   mx_quantize(x, q);
   product(q, w, bias, residual, act, y, yq);
 }
 
 i64 mx_linear_workspace(i64 n, i64 K, int x_fmt, i64 O) {
-  return n > 0 && K > 0 ? rows_bytes(x_fmt, n, K) : 0;
+  return n > kValueRows && K > 0 ? rows_bytes(x_fmt, n, K) : 0;
 }
 
 // ---- ConvNeXt tail ----------------------------------------------------------------------------------------------

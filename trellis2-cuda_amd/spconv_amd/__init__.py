@@ -14,6 +14,7 @@ Errors raise RuntimeError carrying spc_last_error() (the reference's t2_last_err
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 _PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -357,15 +358,15 @@ class MxTensor:
     __slots__ = ("codes", "scales", "fmt", "shape")
 
     def __init__(self, codes, scales, cols: int, fmt: int):
-        torch = _torch()
-        if fmt not in (MX_E4M3, MX_E2M1):
+        if fmt != MX_E2M1 and fmt != MX_E4M3:
             raise ValueError(f"unknown format {fmt}")
         if cols <= 0 or cols % 32:
             raise ValueError(f"{cols} columns: a positive multiple of 32")
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.dim() != 2 or scales.dim() != 2:
+        u8 = _torch().uint8
+        if codes.dtype != u8 or scales.dtype != u8 or codes.dim() != 2:
             raise ValueError("codes and scales must be uint8 matrices")
-        rows = codes.shape[0]
-        if codes.shape[1] != (cols // 2 if fmt == MX_E2M1 else cols) or tuple(scales.shape) != (rows, (cols + 511) // 512 * 16):
+        rows, width = codes.shape
+        if width != (cols // 2 if fmt == MX_E2M1 else cols) or scales.shape != (rows, (cols + 511) // 512 * 16):
             raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not those of {cols} columns")
         self.codes, self.scales, self.fmt, self.shape = codes, scales, fmt, (rows, cols)
 
@@ -379,30 +380,20 @@ class MxTensor:
         return mx_dequantize(self, dtype)
 
 
-def _here(*tensors):
-    """The tensors' one device, which has to be the current one (the library launches there)."""
-    torch = _torch()
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if isinstance(t, MxTensor):
-            if t.codes.device != t.scales.device:
-                raise ValueError("codes and scales on different devices")
-            t = t.codes
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    if dev.type != "cuda":
-        raise ValueError("tensor must be on the GPU")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
-    return dev
+def _adr(t, dev):
+    """Address of a contiguous tensor on device number dev, the current one (the library launches there); None for None."""
+    if t is None:
+        return None
+    if t.get_device() != dev:
+        raise ValueError("tensor must be on the GPU" if t.get_device() < 0 else
+                         f"tensor on cuda:{t.get_device()}, but the current device is cuda:{dev}")
+    if not t.is_contiguous():
+        raise ValueError("tensor must be contiguous")
+    return t.data_ptr()
 
 
 def _matrix(t, name, shape=None, dtype=None):
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+    if t.dim() != 2 or (shape is not None and t.shape != shape):
         raise ValueError(f"{name} must be {list(shape) if shape is not None else 'a matrix'}, got {list(t.shape)}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
@@ -418,23 +409,26 @@ def mx_quantize(x, fmt: int = MX_E2M1, out: MxTensor = None) -> MxTensor:
     power of two for which its largest magnitude over it rounds to at most the largest element; elements round to
     nearest, halves to even. A block with an infinity or NaN reads as NaN."""
     _matrix(x, "x")
-    dev = _here(x, out)
+    N, K = x.shape
     if out is None:
-        out = MxTensor.empty(x.shape[0], x.shape[1], fmt, dev)
-    elif out.shape != tuple(x.shape) or out.fmt != fmt:
+        out = MxTensor.empty(N, K, fmt, x.device)
+    elif out.shape != (N, K) or out.fmt != fmt:
         raise ValueError(f"out must be of x's shape {list(x.shape)} and format {fmt}")
-    _check(load_library().spc_mx_quantize(_ptr(x), _dt(x), x.shape[0], x.shape[1], fmt, _ptr(out.codes), _ptr(out.scales)))
+    dev = _torch().cuda.current_device()
+    _check(load_library().spc_mx_quantize(_adr(x, dev), _dt(x), N, K, fmt, _adr(out.codes, dev), _adr(out.scales, dev)))
     return out
 
 
 def mx_dequantize(q: MxTensor, dtype=None, out=None):
     """q's values [N, K] in dtype (default bfloat16; float32 holds every one of them exactly)."""
     torch = _torch()
-    dev = _here(q, out)
+    N, K = q.shape
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype or torch.bfloat16, device=dev)
-    _matrix(out, "out", q.shape, dtype)
-    _check(load_library().spc_mx_dequantize(_ptr(q.codes), _ptr(q.scales), q.shape[0], q.shape[1], q.fmt, _dt(out), _ptr(out)))
+        out = torch.empty((N, K), dtype=dtype or torch.bfloat16, device=q.codes.device)
+    else:
+        _matrix(out, "out", q.shape, dtype)
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_mx_dequantize(_adr(q.codes, dev), _adr(q.scales, dev), N, K, q.fmt, _dt(out), _adr(out, dev)))
     return out
 
 
@@ -445,33 +439,34 @@ def add_norm_mx(x, residual=None, gamma=None, beta=None, eps: float = 1e-6, kind
     float16 or bfloat16 [N, C], C a multiple of 32 up to 16384; sum, the buffer for t, may be x or residual."""
     torch = _torch()
     _matrix(x, "x")
-    N, C = x.shape
-    dev = _here(x, residual, gamma, beta, sum, out)
+    N, C = shape = x.shape
     if gamma is not None and beta is not None and gamma.dtype != beta.dtype:
         raise ValueError("gamma and beta must share one dtype")
     _vector(gamma, "gamma", C)
     _vector(beta, "beta", C)
     if residual is not None:
-        _matrix(residual, "residual", x.shape, x.dtype)
+        _matrix(residual, "residual", shape, x.dtype)
         if sum is None:
             sum = torch.empty_like(x)
     if sum is not None:
-        _matrix(sum, "sum", x.shape, x.dtype)
+        _matrix(sum, "sum", shape, x.dtype)
     if out is None:
-        out = MxTensor.empty(N, C, fmt, dev)
+        out = MxTensor.empty(N, C, fmt, x.device)
     elif out.shape != (N, C) or out.fmt != fmt:
         raise ValueError(f"out must be [{N}, {C}] of format {fmt}")
     p = gamma if gamma is not None else beta
-    _check(load_library().spc_add_norm_mx(_ptr(x), _ptr(residual), _ptr(gamma), _ptr(beta), _dt(p) if p is not None else F32,
-                                          eps, kind, _dt(x), N, C, fmt, _ptr(sum), _ptr(out.codes), _ptr(out.scales)))
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_add_norm_mx(
+        _adr(x, dev), _adr(residual, dev), _adr(gamma, dev), _adr(beta, dev), _dt(p) if p is not None else F32, eps, kind, _dt(x),
+        N, C, fmt, _adr(sum, dev), _adr(out.codes, dev), _adr(out.scales, dev)))
     return (x if sum is None else sum), out
 
 
-def _workspace(query, device, *sizes):
-    torch = _torch()
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(name, *sizes):
     n = ctypes.c_int64()
-    _check(query(*sizes, ctypes.byref(n)))
-    return torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None
+    _check(getattr(load_library(), name)(*sizes, ctypes.byref(n)))
+    return n.value
 
 
 def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt: int = MX_E4M3, out_dtype=None, out_fmt=None,
@@ -481,39 +476,43 @@ def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt
     fmt. The result is of out_dtype (default: x's type; bfloat16 for an MxTensor), as residual has to be; out may be the
     residual. With out_fmt (and no residual) it is an MxTensor of that format."""
     torch = _torch()
-    quantized = isinstance(x, MxTensor)
     if not isinstance(w, MxTensor) or w.fmt != MX_E2M1:
         raise ValueError("w must be an MxTensor of format MX_E2M1")
-    if not quantized:
+    quantized = isinstance(x, MxTensor)
+    if quantized:
+        fmt, xv, xs, xdt = x.fmt, x.codes, x.scales, F32
+    else:
         _matrix(x, "x")
+        xv, xs, xdt = x, None, _dt(x)
     N, K = x.shape
-    Co = w.shape[0]
-    if w.shape[1] != K:
-        raise ValueError(f"w has {w.shape[1]} columns, x {K}")
-    dev = _here(x, w, bias, residual, out)
+    Co, wk = w.shape
+    if wk != K:
+        raise ValueError(f"w has {wk} columns, x {K}")
     _vector(bias, "bias", Co)
-    mx_out = out_fmt is not None or isinstance(out, MxTensor)
-    if mx_out:
+    if out_fmt is not None or isinstance(out, MxTensor):
         if residual is not None or out_dtype is not None:
             raise ValueError("a microscaled result takes no residual and no out_dtype")
         if out is None:
-            out = MxTensor.empty(N, Co, out_fmt, dev)
+            out = MxTensor.empty(N, Co, out_fmt, xv.device)
         elif not isinstance(out, MxTensor) or out.shape != (N, Co) or out_fmt not in (None, out.fmt):
             raise ValueError(f"out must be an MxTensor [{N}, {Co}] of format {out_fmt}")
+        y, ys, ot = out.codes, out.scales, out.fmt
     else:
         if out is None:
-            out = torch.empty((N, Co), dtype=out_dtype or (torch.bfloat16 if quantized else x.dtype), device=dev)
-        _matrix(out, "out", (N, Co), out_dtype)
+            out = torch.empty((N, Co), dtype=out_dtype or (torch.bfloat16 if quantized else x.dtype), device=xv.device)
+        else:
+            _matrix(out, "out", (N, Co), out_dtype)
         if residual is not None:
             _matrix(residual, "residual", (N, Co), out.dtype)
-    L = load_library()
-    fmt = x.fmt if quantized else fmt
-    ws = None if quantized else _workspace(L.spc_mx_linear_workspace, dev, N, K, Co, fmt)
-    _check(L.spc_mx_linear(
-        _ptr(x.codes if quantized else x), _ptr(x.scales) if quantized else None, F32 if quantized else _dt(x), fmt,
-        _ptr(w.codes), _ptr(w.scales), _ptr(bias), _dt(bias) if bias is not None else F32, _ptr(residual), act, N, K, Co,
-        out.fmt if mx_out else _dt(out), _ptr(out.codes if mx_out else out), _ptr(out.scales) if mx_out else None, _ptr(ws),
-        ws.numel() if ws is not None else 0))
+        y, ys, ot = out, None, _dt(out)
+    ws, nws = None, 0 if quantized else _workspace_bytes("spc_mx_linear_workspace", N, K, Co, fmt)
+    if nws:
+        ws = torch.empty(nws, dtype=torch.uint8, device=xv.device)
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_mx_linear(
+        _adr(xv, dev), _adr(xs, dev), xdt, fmt, _adr(w.codes, dev), _adr(w.scales, dev), _adr(bias, dev),
+        _dt(bias) if bias is not None else F32, _adr(residual, dev), act, N, K, Co, ot, _adr(y, dev), _adr(ys, dev),
+        _adr(ws, dev), nws))
     return out
 
 
@@ -523,26 +522,27 @@ def convnext_mlp_mx(h, x, gamma, beta, w1: MxTensor, b1, w2: MxTensor, b2, eps: 
     b1, b2 share one float dtype (or are None). out may be h or x."""
     torch = _torch()
     _matrix(h, "h")
-    N, C = h.shape
-    _matrix(x, "x", h.shape, h.dtype)
+    N, C = shape = h.shape
+    _matrix(x, "x", shape, h.dtype)
     ps = [p for p in (gamma, beta, b1, b2) if p is not None]
     if any(p.dtype != ps[0].dtype for p in ps):
         raise ValueError("gamma, beta, b1, b2 must share one dtype")
     for name, t, n in (("gamma", gamma, C), ("beta", beta, C), ("b1", b1, 4 * C), ("b2", b2, C)):
         _vector(t, name, n)
-    for name, w, shape in (("w1", w1, (4 * C, C)), ("w2", w2, (C, 4 * C))):
-        if not isinstance(w, MxTensor) or w.fmt != MX_E2M1 or w.shape != shape:
-            raise ValueError(f"{name} must be an MxTensor {list(shape)} of format MX_E2M1")
-    dev = _here(h, x, gamma, beta, w1, b1, w2, b2, out)
+    for name, w, want in (("w1", w1, (4 * C, C)), ("w2", w2, (C, 4 * C))):
+        if not isinstance(w, MxTensor) or w.fmt != MX_E2M1 or w.shape != want:
+            raise ValueError(f"{name} must be an MxTensor {list(want)} of format MX_E2M1")
     if out is None:
         out = torch.empty_like(h)
-    _matrix(out, "out", h.shape, h.dtype)
-    L = load_library()
-    ws = _workspace(L.spc_convnext_mlp_mx_workspace, dev, N, C, fmt)
-    _check(L.spc_convnext_mlp_mx(
-        _ptr(h), _ptr(x), _ptr(gamma), _ptr(beta), eps, _ptr(w1.codes), _ptr(w1.scales), _ptr(b1), _ptr(w2.codes),
-        _ptr(w2.scales), _ptr(b2), _dt(h), _dt(ps[0]) if ps else F32, fmt, N, C, _ptr(out), _ptr(ws),
-        ws.numel() if ws is not None else 0))
+    else:
+        _matrix(out, "out", shape, h.dtype)
+    nws = _workspace_bytes("spc_convnext_mlp_mx_workspace", N, C, fmt)
+    ws = torch.empty(nws, dtype=torch.uint8, device=h.device) if nws else None
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_convnext_mlp_mx(
+        _adr(h, dev), _adr(x, dev), _adr(gamma, dev), _adr(beta, dev), eps, _adr(w1.codes, dev), _adr(w1.scales, dev),
+        _adr(b1, dev), _adr(w2.codes, dev), _adr(w2.scales, dev), _adr(b2, dev), _dt(h), _dt(ps[0]) if ps else F32, fmt, N, C,
+        _adr(out, dev), _adr(ws, dev), nws))
     return out
 
 
