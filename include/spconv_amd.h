@@ -181,10 +181,10 @@ int spc_add_norm_mx(const void* x, const void* residual, const void* gamma, cons
  * x_fmt with x_scales, or, with x_scales NULL, values of x_dtype that the call quantises to x_fmt. out: values of
  * out_type (SPC_F32/F16/BF16) with out_scales NULL, one rounding, residual [N,Co] of the same type or NULL (out may be the
  * residual); else codes of format out_type with out_scales, without a residual. bias [Co] of b_dtype or NULL. out
- * overlaps no other operand. workspace: spc_mx_linear_workspace's bytes on the device, 16-byte aligned, in use until
- * the call's work is done, for x that the call quantises; NULL: the library's own, refused while the stream is being captured into a
- * graph (a captured call needs a workspace of its own for as long as the graph lives). */
-int spc_mx_linear_workspace(int64_t N, int64_t K, int64_t Co, int x_fmt, int64_t* bytes);
+ * overlaps no other operand. workspace: spc_mx_linear_workspace's bytes on the device for the rows that the call
+ * quantises (0 for few rows), 16-byte aligned, in use until the call's work is done; NULL: the library's own, refused while the stream is
+ * being captured into a graph (a captured call needs a workspace of its own for as long as the graph lives). */
+int spc_mx_linear_workspace(int64_t N, int64_t K, int x_fmt, int64_t* bytes);
 int spc_mx_linear(const void* x, const void* x_scales, int x_dtype, int x_fmt, const void* w_codes,
                   const void* w_scales, const void* bias, int b_dtype, const void* residual, int act, int64_t N,
                   int64_t K, int64_t Co, int out_type, void* out, void* out_scales, void* workspace,

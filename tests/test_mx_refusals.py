@@ -27,9 +27,10 @@ def test_sizes():
     refused(lib.spc_mx_sizes(3, 33, 1, None, None), "cols=33")
     refused(lib.spc_mx_sizes(3, 32, 4, None, None), "format 4")
     n = ctypes.c_int64()
-    assert lib.spc_mx_linear_workspace(10, 64, 32, 2, ctypes.byref(n)) == 0 and n.value >= 10 * 32 + 10 * 16
+    assert lib.spc_mx_linear_workspace(100, 64, 2, ctypes.byref(n)) == 0 and n.value >= 100 * 32 + 100 * 16
     assert lib.spc_convnext_mlp_mx_workspace(10, 64, 1, ctypes.byref(n)) == 0 and n.value >= 10 * (64 + 256) + 20 * 16
-    assert lib.spc_mx_linear_workspace(0, 64, 32, 2, ctypes.byref(n)) == 0 and n.value == 0
+    for rows in (0, 16):  # few rows are quantised on the way
+        assert lib.spc_mx_linear_workspace(rows, 64, 2, ctypes.byref(n)) == 0 and n.value == 0
 
 
 def test_quantize():
@@ -117,7 +118,7 @@ def test_tail():
 
 def test_binding():
     x = torch.zeros((4, 64), dtype=torch.bfloat16)
-    for call in (lambda: sp.mx_quantize(x), lambda: sp.add_norm_mx(x), lambda: sp.mx_quantize(x[0]),
+    for call in (lambda: sp.mx_quantize(x[0]),
                  lambda: sp.MxTensor(x, x, 64, sp.MX_E4M3),
                  lambda: sp.MxTensor(torch.zeros((4, 64), dtype=torch.uint8), torch.zeros((4, 2), dtype=torch.uint8), 64, sp.MX_E4M3),
                  lambda: sp.MxTensor(torch.zeros((4, 64), dtype=torch.uint8), torch.zeros((4, 16), dtype=torch.uint8), 64, 0),

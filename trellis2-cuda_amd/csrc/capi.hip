@@ -436,10 +436,10 @@ SPC_API int spc_add_norm_mx(const void* x, const void* residual, const void* gam
   });
 }
 
-SPC_API int spc_mx_linear_workspace(int64_t N, int64_t K, int64_t Co, int x_fmt, int64_t* bytes) {
+SPC_API int spc_mx_linear_workspace(int64_t N, int64_t K, int x_fmt, int64_t* bytes) {
   return guarded([&] {
-    REQ(bytes && N >= 0 && K > 0 && Co > 0 && (x_fmt == SPC_MX_E4M3 || x_fmt == SPC_MX_E2M1), "arguments");
-    *bytes = mx_linear_workspace(N, K, x_fmt, Co);
+    REQ(bytes && N >= 0 && K > 0 && (x_fmt == SPC_MX_E4M3 || x_fmt == SPC_MX_E2M1), "arguments");
+    *bytes = mx_linear_workspace(N, K, x_fmt);
   });
 }
 

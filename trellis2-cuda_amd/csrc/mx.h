@@ -31,21 +31,20 @@ __device__ __forceinline__ float mx_inverse(uint32_t byte) {
 __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
   return byte == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte ? byte << 23 : 0x00400000u);
 }
-// v * inv, zero where inv is (an infinity or NaN is not to reach the conversion: it would give a NaN element)
-__device__ __forceinline__ float mx_scaled(float v, float inv) { return inv == 0.f ? 0.f : v * inv; }
 
-// 8 values -> their elements, each v * inv rounded to nearest, halves to even: 8 bytes (e4m3) or 4 (e2m1, in [0])
+// 8 values -> their elements, each v * inv rounded to nearest, halves to even: 8 bytes (e4m3) or 4 (e2m1, in [0]). Where
+// inv is 0 (a block with an infinity or NaN) the elements are zeros, whatever the conversion makes of the values.
 template <int FMT>
 __device__ __forceinline__ mx_u32x2 mx_encode8(const float (&v)[8], float inv) {
   mx_u32x2 r = {0, 0};
   float t[8];
 #pragma unroll
-  for (int j = 0; j < 8; j++) t[j] = mx_scaled(v[j], inv);
+  for (int j = 0; j < 8; j++) t[j] = v[j] * inv;
   if constexpr (FMT == MX_E4M3) {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       int q = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * j], t[4 * j + 1], 0, false);
-      r[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[4 * j + 2], t[4 * j + 3], q, true);
+      r[j] = inv == 0.f ? 0u : (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[4 * j + 2], t[4 * j + 3], q, true);
     }
   } else {
     uint32_t q = 0;
@@ -53,7 +52,7 @@ __device__ __forceinline__ mx_u32x2 mx_encode8(const float (&v)[8], float inv) {
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, t[2], t[3], 1.0f, 1);
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, t[4], t[5], 1.0f, 2);
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, t[6], t[7], 1.0f, 3);
-    r[0] = q;
+    r[0] = inv == 0.f ? 0u : q;
   }
   return r;
 }

@@ -27,7 +27,7 @@ struct LinArgs {
   i64 N;
   int K, O, bias_dt, act, f16;
   int xrow, wrow, srow, osrow;  // bytes of a row: X's and W's codes, their scales, out's scales
-  int tiles_n, tiles_o, per, band;
+  int tiles_n, tiles_o, per, per_rest, band;
 };
 
 __device__ __forceinline__ i32x4 rsrc4(const void* p, uint32_t bytes) {  // a raw buffer's descriptor, in SGPRs
@@ -86,10 +86,11 @@ constexpr int run_tiles() {  // G above
   return OUT == OUT_F32 ? 1 : OUT == OUT_16 ? 2 : 4 < TO ? 4 : TO;
 }
 
-// Epilogue of NV consecutive channels o .. of row n in v: bias, activation, residual, store. Lanes l, l + 16, l + 32, l + 48
+// Epilogue of NV consecutive channels o .. of row n in v: bias, activation, residual (its words in r), store. Lanes l, l + 16, l + 32, l + 48
 // hold neighbouring runs of one row; ok is the same for all lanes of a block of 32 channels.
 template <int OUT, int NV>
-__device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v)[NV], const float (&bias)[NV], bool ok, int g) {
+__device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v)[NV], const float (&bias)[NV],
+                                       const uint32_t (&r)[4], bool ok) {
 #pragma unroll
   for (int j = 0; j < NV; j++) v[j] += bias[j];
   if (a.act == ACT_SILU) {
@@ -100,9 +101,8 @@ __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v
     static_assert(NV == 4, "one 16-byte piece");
     if (!ok) return;
     if (a.res) {
-      const f32x4 r = *(const f32x4*)((const float*)a.res + n * a.O + o);
 #pragma unroll
-      for (int j = 0; j < 4; j++) v[j] += r[j];
+      for (int j = 0; j < 4; j++) v[j] += __uint_as_float(r[j]);
     }
     *(f32x4*)((float*)a.out + n * a.O + o) = f32x4{v[0], v[1], v[2], v[3]};
   } else if constexpr (OUT == OUT_16) {
@@ -110,13 +110,10 @@ __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v
     if (!ok) return;
     uint32_t q[NV / 2];
     if (a.res) {
-      const uint32_t* r = (const uint32_t*)((const uint16_t*)a.res + n * a.O + o);
-      if constexpr (NV == 8) *(mx_u32x4*)q = *(const mx_u32x4*)r;
-      else *(mx_u32x2*)q = *(const mx_u32x2*)r;
 #pragma unroll
       for (int j = 0; j < NV / 2; j++) {
-        v[2 * j] += a.f16 ? mx_lo<true>(q[j]) : mx_lo<false>(q[j]);
-        v[2 * j + 1] += a.f16 ? mx_hi<true>(q[j]) : mx_hi<false>(q[j]);
+        v[2 * j] += a.f16 ? mx_lo<true>(r[j]) : mx_lo<false>(r[j]);
+        v[2 * j + 1] += a.f16 ? mx_hi<true>(r[j]) : mx_hi<false>(r[j]);
       }
     }
 #pragma unroll
@@ -154,14 +151,28 @@ __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v
   }
 }
 
+// The residual's words for NV channels of 16 or 32 bits
+template <int OUT, int NV>
+__device__ __forceinline__ void load_residual(const LinArgs& a, i64 n, int o, bool ok, uint32_t (&r)[4]) {
+  if constexpr (OUT == OUT_16 && NV == 4) {
+    const mx_u32x2 q = ok ? *(const mx_u32x2*)((const uint16_t*)a.res + n * a.O + o) : mx_u32x2{};
+    r[0] = q[0];
+    r[1] = q[1];
+  } else if constexpr (OUT == OUT_16 || OUT == OUT_F32) {
+    const mx_u32x4 q = ok ? *(const mx_u32x4*)((const char*)a.res + (n * a.O + o) * (OUT == OUT_16 ? 2 : 4)) : mx_u32x4{};
+#pragma unroll
+    for (int j = 0; j < 4; j++) r[j] = q[j];
+  }
+}
+
 // The parts of e4m3 elements that SPLIT products take apart (see k_mx_gemm)
-__device__ __forceinline__ void split(const XFrag<8>& x, XFrag<8>& small, XFrag<8>& large) {
+__device__ __forceinline__ void split(XFrag<8>& x, XFrag<8>& large) {  // x keeps the small ones
 #pragma unroll
   for (int k = 0; k < 2; k++)
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       large.q[k][j] = e4m3_large(x.q[k][j]);
-      small.q[k][j] = x.q[k][j] ^ large.q[k][j];
+      x.q[k][j] ^= large.q[k][j];
     }
 }
 
@@ -193,46 +204,58 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
     int sw[OT], sx[NT];
     XFrag<XB> x[NT];
   };
-  // O is a multiple of 32, so every channel exists; rows past the last repeat it (their results are not stored)
+  // Every load is a buffer load whose offset is past the end where there is nothing (a row past the last, columns past K): no
+  // branches, so all of a step's loads are on their way together.
+  auto rsrc = [](const void* p, uint32_t bytes) __attribute__((always_inline)) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+  };
+  const int rows = (int)min((i64)(16 * NT), a.N - n0);
+  constexpr int XS = XT == F32 ? 4 : 2;  // bytes of a value
+  const auto rw = rsrc(a.w + (i64)o0 * a.wrow, 16 * OT * a.wrow), rws = rsrc(a.ws + (i64)o0 * a.srow, 16 * OT * a.srow);
+  const auto rx = XT < 0 ? rsrc(a.x + n0 * a.xrow, rows * a.xrow) : rsrc(a.x + n0 * a.K * XS, rows * a.K * XS);
+  const auto rxs = rsrc(XT < 0 ? a.xs + n0 * a.srow : nullptr, XT < 0 ? rows * a.srow : 0);
   auto load = [&](Step& q, int s) __attribute__((always_inline)) {
     const bool in = s * 4 + g < blocks;  // columns past the last: zeros and scale 0
 #pragma unroll
     for (int t = 0; t < OT; t++) {
-      q.w[t] = in ? *(const mx_u32x4*)(a.w + (i64)chan[t] * a.wrow + s * 64 + g * 16) : mx_u32x4{};
-      q.sw[t] = in ? a.ws[(i64)chan[t] * a.srow + s * 4 + g] : 0;
+      q.w[t] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? (uint32_t)((chan[t] - o0) * a.wrow + g * 16) : kOOR, s * 64, 0);
+      q.sw[t] = __builtin_amdgcn_raw_buffer_load_b8(rws, in ? (uint32_t)((chan[t] - o0) * a.srow + g) : kOOR, s * 4, 0);
     }
     if constexpr (XT < 0) {
 #pragma unroll
       for (int u = 0; u < NT; u++) {
-        const i64 n = min(n0 + u * 16 + r16, a.N - 1);
-        const uint8_t* x = a.x + n * a.xrow + s * (XB * 16) + g * 16;
+        const uint32_t x = (uint32_t)((u * 16 + r16) * a.xrow + g * 16);
         if constexpr (XB == 8) {  // block g / 2 for the first piece, 2 + g / 2 for the second
-          q.x[u].q[0] = s * 4 + g / 2 < blocks ? *(const mx_u32x4*)x : mx_u32x4{};
-          q.x[u].q[1] = s * 4 + 2 + g / 2 < blocks ? *(const mx_u32x4*)(x + 64) : mx_u32x4{};
+          q.x[u].q[0] = __builtin_amdgcn_raw_buffer_load_b128(rx, s * 4 + g / 2 < blocks ? x : kOOR, s * 128, 0);
+          q.x[u].q[1] = __builtin_amdgcn_raw_buffer_load_b128(rx, s * 4 + 2 + g / 2 < blocks ? x + 64 : kOOR, s * 128, 0);
         } else {
-          q.x[u].q[0] = in ? *(const mx_u32x4*)x : mx_u32x4{};
+          q.x[u].q[0] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? x : kOOR, s * 64, 0);
         }
-        q.sx[u] = in ? a.xs[n * a.srow + s * 4 + g] : 0;
+        q.sx[u] = __builtin_amdgcn_raw_buffer_load_b8(rxs, in ? (uint32_t)((u * 16 + r16) * a.srow + g) : kOOR, s * 4, 0);
       }
     } else {
       static_assert(NT == 1, "quantised once per workgroup");
-      const bool row = n0 + r16 < a.N;
       float v[32];  // e2m1: block g; e4m3: halves of blocks g / 2 and 2 + g / 2
+      mx_u32x4 raw[XT == F32 ? 8 : 4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const int c = XB == 4 ? g * 32 + k * 8 : k / 2 * 64 + g * 16 + k % 2 * 8;
-        const i64 at = (n0 + r16) * a.K + s * 128 + c;
-        const bool live = row && s * 128 + c < a.K;
+        const uint32_t at = s * 128 + c < a.K ? (uint32_t)((r16 * a.K + c) * XS) : kOOR;
+        if constexpr (XT == F32) {
+          raw[2 * k] = __builtin_amdgcn_raw_buffer_load_b128(rx, at, s * 128 * XS, 0);
+          raw[2 * k + 1] = __builtin_amdgcn_raw_buffer_load_b128(rx, at == kOOR ? kOOR : at + 16, s * 128 * XS, 0);
+        } else {
+          raw[k] = __builtin_amdgcn_raw_buffer_load_b128(rx, at, s * 128 * XS, 0);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
         float(&o)[8] = *(float(*)[8])&v[k * 8];
         if constexpr (XT == F32) {
-          const f32x4 p = live ? *(const f32x4*)((const float*)a.x + at) : f32x4{}, r = live ? *(const f32x4*)((const float*)a.x + at + 4) : f32x4{};
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            o[j] = p[j];
-            o[4 + j] = r[j];
-          }
+          for (int j = 0; j < 8; j++) o[j] = __uint_as_float(raw[2 * k + j / 4][j % 4]);
         } else {
-          mx_unpack8<XT == F16>(live ? *(const mx_u32x4*)((const uint16_t*)a.x + at) : mx_u32x4{}, o);
+          mx_unpack8<XT == F16>(raw[k], o);
         }
       }
       uint32_t top[2];
@@ -264,8 +287,8 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
 #pragma unroll
     for (int u = 0; u < NT; u++) {
       if constexpr (SPLIT) {
-        XFrag<8> small, large;
-        split(q.x[u], small, large);
+        XFrag<8> small = q.x[u], large;
+        split(small, large);
 #pragma unroll
         for (int t = 0; t < OT; t++) {
           acc[t][u] = mfma<XB, 0>(q.w[t], small, acc[t][u], q.sw[t], q.sx[u]);
@@ -277,7 +300,7 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
       }
     }
   };
-  constexpr int U = NT == 1 ? 4 : NT <= 2 ? 2 : 1;  // steps loaded at once
+  constexpr int U = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // steps loaded at once
   int s = s0;
   for (; s + U <= s1; s += U) {
     Step q[U];
@@ -312,12 +335,14 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
     const i64 n = n0 + u * 16 + r16;
     const int o = o0 + t / G * (16 * G) + g * (4 * G);
     mx_params<4 * G>(a.bias, a.bias_dt, o, 0.f, bias);
-    finish<OUT>(a, n, o, v, bias, n < a.N, g);
+    uint32_t r[4] = {};
+    if (a.res) load_residual<OUT, 4 * G>(a, n, o, n < a.N, r);
+    finish<OUT>(a, n, o, v, bias, r, n < a.N);
   }
 }
 
 // Tiled product. A workgroup of WO x WN wavefronts has BO = 16 TO WO channels by BN = 16 TN WN rows; K goes by steps of
-// 128 through NS slots of LDS, filled by DMA; the scales go by 512 columns (16 bytes a row), two slots. LDS rows are 64
+// 128, KS of them a stage, through NS slots of LDS, filled by DMA; the scales go by 512 columns (16 bytes a row), one slot. LDS rows are 64
 // (e2m1) or 128 bytes (e4m3) of a step, their 16-byte pieces permuted (piece c of row q at c ^ (q >> 2) % 4 or c ^ q % 8),
 // so that eight lanes of neighbouring rows read from distinct banks.
 //
@@ -332,24 +357,35 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
 // value over a border between elements costs a whole step), each step's products are taken for the elements of magnitude
 // 4 and more and for the smaller ones apart: with e2m1 factors both parts span 13 bits and are exact.
 template <int XB, int OUT, int TO, int TN, int WO, int WN, int KS, int NS>
-__global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
+__global__ void __launch_bounds__(64 * WO * WN, 2) k_mx_gemm(LinArgs a) {
   constexpr int NW = WO * WN, BO = 16 * TO * WO, BN = 16 * TN * WN, H = TO / 2, HX = TN / 2;
   constexpr bool SPLIT = XB == 8 && OUT != OUT_16;
   constexpr int XR = XB * 16 * KS, WR = 64 * KS;                                // bytes of a row of X and W per stage
   constexpr int XP = XR / 16, WP = WR / 16;                                     // 16-byte pieces of them
-  constexpr int XI = BN * XR / 1024 / NW, WI = BO * WR / 1024 / NW, SI = (BO + BN) / 64 / NW;  // DMAs per wavefront
-  static_assert(XI * 1024 * NW == BN * XR && WI * 1024 * NW == BO * WR && SI * 64 * NW == BO + BN, "whole DMAs");
+  constexpr int XI = BN * XR / 1024 / NW, WI = BO * WR / 1024 / NW, ST = (BO + BN) / 64, SI = (ST + NW - 1) / NW;  // DMAs per wavefront
+  static_assert(XI * 1024 * NW == BN * XR && WI * 1024 * NW == BO * WR && BO % 64 == 0 && BN % 64 == 0 && ST >= NW, "whole DMAs");
   static_assert((XR == 64 || XR == 128) && (WR == 64 || WR == 128), "swizzles");
   constexpr int G = run_tiles<OUT, TO>();
   static_assert(TO % G == 0 && TO % 2 == 0 && TN % 2 == 0 && NS >= 2 && NS <= 4, "whole runs, two halves");
-  __shared__ __attribute__((aligned(16))) mx_u32x4 lds[NS * (BN * XR + BO * WR) / 16 + 2 * (BO + BN)];
-  constexpr uint32_t kSlot = BN * XR + BO * WR, kScales = NS * kSlot, kScaleSlot = (BO + BN) * 16;
+  __shared__ __attribute__((aligned(16))) mx_u32x4 lds[NS * (BN * XR + BO * WR) / 16 + (BO + BN)];
+  constexpr uint32_t kSlot = BN * XR + BO * WR, kScales = NS * kSlot;
 
-  const int logical = (blockIdx.x % 8) * a.per + blockIdx.x / 8;  // each XCD walks one contiguous range of tiles
-  if (logical >= a.tiles_n * a.tiles_o) return;
-  // tiles in bands of `band` columns, row by row within a band
-  const int first = logical / (a.band * a.tiles_n) * a.band, width = min(a.band, a.tiles_o - first);
-  const int inside = logical - first * a.tiles_n, tn = inside / width, to = first + inside % width;
+  // Whole tiles first, then those that the last rows or channels end in (they skip the products of what they lack): each
+  // XCD takes a contiguous range of either, whole tiles in bands of `band` columns, row by row within a band.
+  const int fn = (int)(a.N / BN), fo = a.O / BO, xcd = blockIdx.x % 8, k = blockIdx.x / 8;
+  int tn, to;
+  if (k < a.per) {
+    const int l = xcd * a.per + k;
+    if (l >= fn * fo) return;
+    const int first = l / (a.band * fn) * a.band, width = min(a.band, fo - first), inside = l - first * fn;
+    tn = inside / width;
+    to = first + inside % width;
+  } else {
+    const int l = xcd * a.per_rest + k - a.per, below = (a.tiles_n - fn) * a.tiles_o;
+    if (l >= below + (a.tiles_o - fo) * fn) return;
+    tn = l < below ? fn : l - below;
+    to = l < below ? l : fo;
+  }
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wo = wave % WO, wn = wave / WO;
   const int S = (a.K + 127) / 128, stages = (S + KS - 1) / KS, blocks = a.K / 32;
@@ -385,24 +421,26 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
   }
 #pragma unroll
   for (int k = 0; k < SI; k++) {
-    const int p = (wave * SI + k) * 64 + lane, ch = channel(p < BO ? p : 0);
+    const int p = (k * NW + wave) * 64 + lane, ch = channel(p < BO ? p : 0);
     soff[k] = p < BO ? (ch < chans ? (uint32_t)(ch * a.srow) : kOOR) : p - BO < rows ? (uint32_t)((p - BO) * a.srow) : kOOR;
   }
+  auto none_unless = [](i32x4 r, bool live) __attribute__((always_inline)) {
+    r[2] = live ? r[2] : 0;
+    return r;
+  };
+  auto issue_scales = [&](int c) __attribute__((always_inline)) {  // of columns 512 c .., past the last one nothing
+    const bool live = c * 4 < S;
+#pragma unroll
+    for (int k = 0; k < SI; k++) {
+      const int p0 = (k * NW + wave) * 64;  // BO is a multiple of 64: a DMA's rows are all W's or all X's
+      if (p0 >= BO + BN) break;             // (the waits count ST / NW of them, which every wavefront has)
+      dma16(none_unless(p0 < BO ? rws : rxs, live), lds0 + kScales + p0 * 16, soff[k], live ? c * 16 : 0);
+    }
+  };
   // fills stage t's slot; past the last one the DMAs still run (the waits count them) but read nothing
   auto issue = [&](int t, int slot) __attribute__((always_inline)) {
     const bool live = t < stages;
-    auto of = [&](i32x4 r) __attribute__((always_inline)) {
-      r[2] = live ? r[2] : 0;
-      return r;
-    };
-    if (t * KS % 4 == 0) {
-#pragma unroll
-      for (int k = 0; k < SI; k++) {
-        const int p0 = (wave * SI + k) * 64;  // BO is a multiple of 64: a DMA's rows are all W's or all X's
-        dma16(of(p0 < BO ? rws : rxs), lds0 + kScales + (t * KS / 4 & 1) * kScaleSlot + p0 * 16, soff[k], live ? t * KS * 4 : 0);
-      }
-    }
-    const i32x4 fx = of(rx), fw = of(rw);
+    const i32x4 fx = none_unless(rx, live), fw = none_unless(rw, live);
     const int xs = live ? t * XR : 0, ws = live ? t * WR : 0;
     const uint32_t at = lds0 + slot * kSlot;
     if (live && (t + 1) * (KS * 128) > a.K) {
@@ -463,7 +501,7 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
   };
   const uint32_t pick = (uint32_t)g * 0x0101u + 0x0400u;  // bytes g of two words, the second operand's first
   auto read_scales = [&](int c) __attribute__((always_inline)) {
-    const mx_u32x4* l = lds + (kScales + (c & 1) * kScaleSlot) / 16;
+    const mx_u32x4* l = lds + kScales / 16;
     auto gather = [&](mx_u32x4 q) __attribute__((always_inline)) {
       const uint32_t lo = __builtin_amdgcn_perm(q[1], q[0], pick), hi = __builtin_amdgcn_perm(q[3], q[2], pick);
       return (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
@@ -489,6 +527,7 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
     }
   };
 
+  issue_scales(0);
 #pragma unroll
   for (int t = 0; t < NS; t++) issue(t, t);
   wait_vm<(NS - 1) * (XI + WI)>();
@@ -496,23 +535,32 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
   read_x(fx[0], 0, 0, 0);
   read_w(fw[0], 0, 0, 0);
   read_scales(0);
+  // which halves of this wavefront's part hold anything (a run of channels may lie across W's halves: then both or none)
+  const bool xl[2] = {wn * (16 * TN) < rows, wn * (16 * TN) + 16 * HX < rows};
+  const bool wl[2] = {wo * (16 * TO) < chans, wo * (16 * TO) + (H % G == 0 ? 16 * H : 0) < chans};
   int cur = 0;
   auto step = [&](auto IC, int s) __attribute__((always_inline)) {
     constexpr int I = decltype(IC)::value, J = I % KS, JN = (I + 1) % KS;  // sub-step of this and of the next one
     constexpr int f = I & 1;
+    XFrag<XB> large[SPLIT ? 2 : 1][SPLIT ? HX : 1];
+    auto take_apart = [&](auto XC) __attribute__((always_inline)) {
+      constexpr int hx = decltype(XC)::value;
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int u = 0; u < HX; u++) split(fx[hx][u], large[hx][u]);
+      }
+    };
     auto quarter = [&](auto WC, auto XC) __attribute__((always_inline)) {
       constexpr int hw = decltype(WC)::value, hx = decltype(XC)::value;
+      if (!(xl[hx] && wl[hw])) return;
 #pragma unroll
-      for (int u = 0; u < HX; u++) {
-        XFrag<XB> small = fx[hx][u], large = {};
-        if constexpr (SPLIT) split(fx[hx][u], small, large);
+      for (int u = 0; u < HX; u++)
 #pragma unroll
         for (int t = 0; t < H; t++) {
           f32x4& c = acc[hw * H + t][hx * HX + u];
-          c = mfma<XB, I>(fw[hw][t], small, c, sw[hw * H + t], sx[hx * HX + u]);
-          if constexpr (SPLIT) c = mfma<XB, I>(fw[hw][t], large, c, sw[hw * H + t], sx[hx * HX + u]);
+          c = mfma<XB, I>(fw[hw][t], fx[hx][u], c, sw[hw * H + t], sx[hx * HX + u]);
+          if constexpr (SPLIT) c = mfma<XB, I>(fw[hw][t], large[hx][u], c, sw[hw * H + t], sx[hx * HX + u]);
         }
-      }
     };
     constexpr std::integral_constant<int, 0> first{};
     constexpr std::integral_constant<int, 1> second{};
@@ -520,16 +568,21 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
     constexpr std::integral_constant<int, 1 - f> xo{};
     read_x(fx[1 - f], cur, J, 1 - f);
     read_w(fw[1], cur, J, 1);
+    take_apart(xf);
     quarter(first, xf);
     __builtin_amdgcn_sched_barrier(0);
+    take_apart(xo);
     quarter(first, xo);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (JN == 0) {
-      // the next stage has landed (up to NS - 2 later ones may be on their way), and this one is in registers
-      constexpr int A = I + 1 - KS;  // first step of this stage, modulo 4
-      wait_vm<(NS - 2) * (XI + WI) + SI * ((NS > 2 && (A + 2 * KS) % 4 == 0) + (NS > 3 && (A + 3 * KS) % 4 == 0))>();
+      // The next stage has landed (the NS - 2 after it may be on their way, and scales issued with them), and this one is
+      // in registers. The scales of the next four steps are asked for at the first meeting after all have read those of
+      // these four; they are older than the stage that the last meeting of the four waits for.
+      constexpr auto with_scales = [](int back) { return ((I - back * KS) & 3) == KS - 1; };
+      wait_vm<(NS - 2) * (XI + WI) + ST / NW * ((NS > 2 && with_scales(1)) + (NS > 3 && with_scales(2)))>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       bare_barrier();
+      if constexpr (I == KS - 1) issue_scales(s / 4 + 1);
       issue(s / KS + NS, cur);
       cur = cur + 1 == NS ? 0 : cur + 1;
     }
@@ -549,9 +602,31 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
   }
   wait_vm<0>();  // nothing lands in LDS after the workgroup has gone
 
+  // The residual's loads go out together (a wavefront that waited for each in turn would spend the epilogue on latency):
+  // of all runs for 16 bits, whose words fit where the operands were, else of one run's rows.
+  constexpr bool RES = OUT == OUT_16 || OUT == OUT_F32;
+  constexpr int RUNS = TO / G, AHEAD = OUT == OUT_16 ? RUNS : 1;
+  uint32_t res[RES ? AHEAD : 1][RES ? TN : 1][4];
+  auto channel_of = [&](int run) __attribute__((always_inline)) { return o0 + wo * (16 * TO) + run * (16 * G) + g * (4 * G); };
+  auto load_run = [&](uint32_t(&r)[RES ? TN : 1][4], int run) __attribute__((always_inline)) {
 #pragma unroll
-  for (int t = 0; t < TO; t += G) {
-    const int o = o0 + wo * (16 * TO) + t / G * (16 * G) + g * (4 * G);
+    for (int u = 0; u < TN; u++) {
+      const i64 n = n0 + xq + u * 16;
+      load_residual<OUT, 4 * G>(a, n, channel_of(run), n < a.N && channel_of(run) < a.O, r[u]);
+    }
+  };
+  if constexpr (RES && AHEAD > 1) {
+    if (a.res) {
+#pragma unroll
+      for (int run = 0; run < RUNS; run++) load_run(res[run], run);
+    }
+  }
+#pragma unroll
+  for (int run = 0; run < RUNS; run++) {
+    const int o = channel_of(run);
+    if constexpr (RES && AHEAD == 1) {
+      if (a.res) load_run(res[0], run);
+    }
     float bias[4 * G];
     mx_params<4 * G>(o < a.O ? a.bias : nullptr, a.bias_dt, o, 0.f, bias);
 #pragma unroll
@@ -561,8 +636,10 @@ __global__ void __launch_bounds__(64 * WO * WN) k_mx_gemm(LinArgs a) {
 #pragma unroll
       for (int j = 0; j < G; j++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[j * 4 + i] = acc[t + j][u][i];
-      finish<OUT>(a, n, o, v, bias, n < a.N && o < a.O, g);
+        for (int i = 0; i < 4; i++) v[j * 4 + i] = acc[run * G + j][u][i];
+      uint32_t none[4] = {};
+      if constexpr (RES) finish<OUT>(a, n, o, v, bias, res[AHEAD > 1 ? run : 0][u], n < a.N && o < a.O);
+      else finish<OUT>(a, n, o, v, bias, none, n < a.N && o < a.O);
     }
   }
 }
@@ -574,13 +651,17 @@ void launch(LinArgs a) {
   REQ(tn * to < (1ll << 30), "%lld rows by %d channels: too many tiles", (long long)a.N, a.O);
   a.tiles_n = (int)tn;
   a.tiles_o = (int)to;
-  a.per = cdiv(tn * to, 8);
-  a.band = (int)std::min<i64>(to, 4);
-  k_mx_gemm<XB, OUT, TO, TN, WO, WN, KS, NS><<<a.per * 8, 64 * WO * WN, 0, stream()>>>(a);
+  const i64 whole = a.N / BN * (a.O / BO);
+  a.per = cdiv(whole, 8);
+  a.per_rest = cdiv(tn * to - whole, 8);
+  a.band = 4;
+  k_mx_gemm<XB, OUT, TO, TN, WO, WN, KS, NS><<<(a.per + a.per_rest) * 8, 64 * WO * WN, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
 
-// Up to kFewRows rows go through k_mx_rows; up to 16 of them may come as values.
+// Up to kFewRows rows go through k_mx_rows; up to kValueRows of them may come as values. (Tiles whose K goes in pieces over more
+// workgroups, with the partial sums added by a second launch, were slower from 17 rows on: us with 4 pieces / k_mx_rows,
+// [77, 4096, 8192] 18.5 / 21 without SPLIT and 23 with, [33, 4096, 4096] 12 / 9, [20, 1024, 4096] 14 / 7.)
 constexpr int kFewRows = 128, kValueRows = 16;
 template <int XB, int OUT, int XT, int NT>
 void launch_rows(const LinArgs& a) {
@@ -601,12 +682,12 @@ void gemm(const LinArgs& a, int xt) {
   if (a.N <= 32) return launch_rows<XB, OUT, -1, 2>(a);
   if (a.N <= 64) return launch_rows<XB, OUT, -1, 4>(a);
   if (a.N <= kFewRows) return launch_rows<XB, OUT, -1, 5>(a);
-  const i64 cus = mx_device_cus();
-  const i64 big = (i64)cdiv(a.N, 256) * cdiv(a.O, 256);
-  if constexpr (XB == 4 || OUT == OUT_16) {
-    if (big >= cus) return launch<XB, OUT, 8, 4, 2, 4, 1, XB == 8 ? 3 : 4>(a);
-  }
-  launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
+  // Tiles of 256 channels by 128 rows read fewer operand bytes per product than 128 by 128, but there are half as many: where
+  // they do not fill most of the slots (two workgroups per CU), the smaller ones do. us at 256 / 128, [N, K, O]:
+  // e4m3 [16411, 4096, 4096] 278 / 314, [8209, 2080, 4128] 102 / 108, [58321, 1024, 256] 32 / 34, [11467, 2048, 512] 29 / 24,
+  // [2048, 4096, 4096] 45 / 40, [1803, 4096, 1024] 41 / 26; e2m1 [16411, 4096, 4096] 237 / 250.
+  if ((i64)cdiv(a.N, 128) * cdiv(a.O, 256) * 2 >= 3 * (i64)mx_device_cus()) launch<XB, OUT, 8, 4, 2, 2, 1, XB == 8 ? 2 : 3>(a);
+  else launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
 }
 }  // namespace
 
@@ -725,6 +806,8 @@ void out_apart(const Tensor* y, const MxTensor* yq, const Tensor& t, const char*
 }
 }  // namespace
 
+i64 mx_linear_workspace(i64 n, i64 K, int x_fmt) { return n > kValueRows && K > 0 ? rows_bytes(x_fmt, n, K) : 0; }
+
 void mx_linear(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y, MxTensor* yq) {
   mx_check(x, "x");
   check_linear(x.rows, x.cols, w, bias, residual, act, y, yq);
@@ -745,7 +828,7 @@ void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias
   for (const Tensor* t : {&w.codes, &w.scales}) out_apart(y, yq, *t, "w");
   if (bias) out_apart(y, yq, *bias, "bias");
   if (n == 0) return;
-  Workspace ws(workspace, workspace_bytes, mx_linear_workspace(n, K, x_fmt, w.rows));
+  Workspace ws(workspace, workspace_bytes, mx_linear_workspace(n, K, x_fmt));
   if (n <= kValueRows) {
     MxTensor q;
     q.fmt = x_fmt;
@@ -756,10 +839,6 @@ void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias
   MxTensor q = ws.rows(x_fmt, n, K);
   mx_quantize(x, q);
   product(q, w, bias, residual, act, y, yq);
-}
-
-i64 mx_linear_workspace(i64 n, i64 K, int x_fmt, i64 O) {
-  return n > kValueRows && K > 0 ? rows_bytes(x_fmt, n, K) : 0;
 }
 
 // ---- ConvNeXt tail ----------------------------------------------------------------------------------------------

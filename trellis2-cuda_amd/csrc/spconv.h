@@ -195,11 +195,12 @@ void add_norm_mx(const Tensor& x, const Tensor* residual, const Tensor* gamma, c
 // act(x w^T + bias) + residual with fp32 sums: x [N,K] microscaled (either format), w [O,K] e2m1, O a multiple of 32, into
 // y (fp32/fp16/bf16 [N,O], one rounding; residual of y's type, which y may be) or, without a residual, quantised into
 // yq. bias of any float type or null. The second form quantises x (fp32/fp16/bf16) to x_fmt first, in a workspace of
-// mx_linear_workspace() bytes (16-byte aligned; null: one of the library's own, refused while the stream is captured).
+// mx_linear_workspace() bytes (0 for few rows; 16-byte aligned; null: one of the library's own, refused while the stream is
+// captured if any is needed).
 void mx_linear(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y, MxTensor* yq);
 void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y,
                MxTensor* yq, void* workspace = nullptr, i64 workspace_bytes = 0);
-i64 mx_linear_workspace(i64 N, i64 K, int x_fmt, i64 O);
+i64 mx_linear_workspace(i64 N, i64 K, int x_fmt);
 
 // convnext_mlp with microscaled products: y = x + W2 mx(silu(W1 mx(LayerNorm(h) * gamma + beta) + b1)) + b2, w1 [4C,C]
 // and w2 [C,4C] e2m1, both activations quantised to fmt; any C that is a multiple of 32 up to 4096. h, x, y of one 16-bit type;

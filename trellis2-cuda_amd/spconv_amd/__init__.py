@@ -91,7 +91,7 @@ def load_library():
     L.spc_mx_quantize.argtypes = [P, I, I64, I64, I, P, P]
     L.spc_mx_dequantize.argtypes = [P, P, I64, I64, I, I, P]
     L.spc_add_norm_mx.argtypes = [P, P, P, P, I, ctypes.c_float, I, I, I64, I64, I, P, P, P]
-    L.spc_mx_linear_workspace.argtypes = [I64, I64, I64, I, PI64]
+    L.spc_mx_linear_workspace.argtypes = [I64, I64, I, PI64]
     L.spc_mx_linear.argtypes = [P, P, I, I, P, P, P, I, P, I, I64, I64, I64, I, P, P, P, I64]
     L.spc_convnext_mlp_mx_workspace.argtypes = [I64, I64, I, PI64]
     L.spc_convnext_mlp_mx.argtypes = [P, P, P, P, ctypes.c_float, P, P, P, P, P, P, I, I, I, I64, I64, P, P, I64]
@@ -505,7 +505,7 @@ def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt
         if residual is not None:
             _matrix(residual, "residual", (N, Co), out.dtype)
         y, ys, ot = out, None, _dt(out)
-    ws, nws = None, 0 if quantized else _workspace_bytes("spc_mx_linear_workspace", N, K, Co, fmt)
+    ws, nws = None, 0 if quantized else _workspace_bytes("spc_mx_linear_workspace", N, K, fmt)
     if nws:
         ws = torch.empty(nws, dtype=torch.uint8, device=xv.device)
     dev = torch.cuda.current_device()
