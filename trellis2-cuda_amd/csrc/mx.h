@@ -37,6 +37,7 @@ __device__ __forceinline__ float mx_scale_value(uint32_t byte) {
 template <int FMT>
 __device__ __forceinline__ mx_u32x2 mx_encode8(const float (&v)[8], float inv) {
   mx_u32x2 r = {0, 0};
+  const uint32_t keep = inv == 0.f ? 0u : ~0u;
   float t[8];
 #pragma unroll
   for (int j = 0; j < 8; j++) t[j] = v[j] * inv;
@@ -44,7 +45,7 @@ __device__ __forceinline__ mx_u32x2 mx_encode8(const float (&v)[8], float inv) {
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       int q = __builtin_amdgcn_cvt_pk_fp8_f32(t[4 * j], t[4 * j + 1], 0, false);
-      r[j] = inv == 0.f ? 0u : (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[4 * j + 2], t[4 * j + 3], q, true);
+      r[j] = keep & (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(t[4 * j + 2], t[4 * j + 3], q, true);
     }
   } else {
     uint32_t q = 0;
@@ -52,7 +53,7 @@ __device__ __forceinline__ mx_u32x2 mx_encode8(const float (&v)[8], float inv) {
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, t[2], t[3], 1.0f, 1);
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, t[4], t[5], 1.0f, 2);
     q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, t[6], t[7], 1.0f, 3);
-    r[0] = inv == 0.f ? 0u : q;
+    r[0] = keep & q;
   }
   return r;
 }
@@ -119,6 +120,52 @@ __device__ __forceinline__ void mx_params(const void* p, int dt, i64 i, float no
   }
 }
 
+// mean and 1 / sqrt(variance + eps) of a row held by LPR lanes (this one has units sub, sub + LPR, ... below `units`, zeros
+// else), or, without the mean, 1 / sqrt(mean square + eps); across: adds the lanes' sums over what LPR does not reach.
+template <int LPR, int CH, class F>
+__device__ __forceinline__ void mx_row_stats(const float (&v)[CH][8], int sub, int units, float inv_c, float eps, bool layer,
+                                             float& mean, float& rstd, F&& across) {
+  auto total = [&](float s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 1; d < (LPR < 64 ? LPR : 64); d <<= 1) s += __shfl_xor(s, d, 64);
+    return across(s);
+  };
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < CH; k++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) s += layer ? v[k][j] : v[k][j] * v[k][j];
+  s = total(s);
+  mean = 0.f;
+  if (layer) {
+    mean = s * inv_c;
+    s = 0.f;
+#pragma unroll
+    for (int k = 0; k < CH; k++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const float d = k * LPR + sub < units ? v[k][j] - mean : 0.f;
+        s += d * d;
+      }
+    s = total(s);
+  }
+  rstd = rsqrtf(s * inv_c + eps);
+}
+__device__ __forceinline__ void mx_norm8(const float (&v)[8], float mean, float rstd, const float (&g)[8], const float (&b)[8],
+                                         float (&o)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) o[j] = (v[j] - mean) * rstd * g[j] + b[j];
+}
+// f(integral_constant 0), f(1), ... f(N - 1)
+template <class F, int... I>
+__device__ __forceinline__ void mx_unroll_impl(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void mx_unroll(F&& f) {
+  mx_unroll_impl(f, std::make_integer_sequence<int, N>{});
+}
+
 // Host side, shared by the operators: argument checks
 void mx_check(const MxTensor& q, const char* what);
 // Whether [a, a + na) and [b, b + nb) share a byte
@@ -127,3 +174,57 @@ inline bool mx_overlap(const void* a, size_t na, const void* b, size_t nb) {
   return a && b && na && nb && x < y + nb && y < x + na;
 }
 int mx_device_cus();
+
+// The caller's workspace, or one of the library's own. The latter is refused while the stream is being captured: the graph
+// would keep the address of a block that the library hands to other calls.
+struct MxWorkspace {
+  Tensor own;
+  char* p;
+  MxWorkspace(void* ws, i64 bytes, i64 need) {
+    if (ws) {
+      REQ((uintptr_t)ws % 16 == 0 && bytes >= need, "workspace of %lld bytes: %lld needed, 16-byte aligned", (long long)bytes,
+          (long long)need);
+      p = (char*)ws;
+    } else if (need) {
+      hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+      CK(hipStreamIsCapturing(stream(), &st));
+      REQ(st == hipStreamCaptureStatusNone, "a captured call needs a workspace of its caller (%lld bytes)", (long long)need);
+      own = empty({need}, U8);
+      p = (char*)own.p;
+    } else {
+      p = nullptr;
+    }
+  }
+  Tensor take(i64 bytes) {
+    Tensor t = borrow(p, {bytes}, U8);
+    p += (bytes + 255) / 256 * 256;
+    return t;
+  }
+  MxTensor rows(int fmt, i64 n, i64 cols) {
+    MxTensor q;
+    q.fmt = fmt;
+    q.rows = n;
+    q.cols = cols;
+    q.codes = take(n * mx_row_bytes(fmt, cols));
+    q.scales = take(n * mx_scale_bytes(cols));
+    return q;
+  }
+};
+inline i64 mx_rows_bytes(int fmt, i64 n, i64 cols) {
+  return (n * mx_row_bytes(fmt, cols) + 255) / 256 * 256 + (n * mx_scale_bytes(cols) + 255) / 256 * 256;
+}
+
+inline void mx_apart(const void* a, size_t na, const void* b, size_t nb, const char* what) {
+  REQ(!mx_overlap(a, na, b, nb), "out must not overlap %s", what);
+}
+inline void mx_out_apart(const Tensor* y, const MxTensor* yq, const Tensor& t, const char* what) {
+  if (y) mx_apart(y->p, y->bytes(), t.p, t.bytes(), what);
+  if (yq) {
+    mx_apart(yq->codes.p, yq->codes.bytes(), t.p, t.bytes(), what);
+    mx_apart(yq->scales.p, yq->scales.bytes(), t.p, t.bytes(), what);
+  }
+}
+
+// mx_linear without its checks. xv: x's values (at most 16 rows), which the product quantises to x's format itself; else x's codes
+void mx_product(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* res, int act, Tensor* y, MxTensor* yq,
+                const Tensor* xv = nullptr);

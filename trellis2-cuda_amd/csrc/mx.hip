@@ -199,24 +199,10 @@ struct NormArgs {
   uint32_t stride;
 };
 
-template <int LPR>
-__device__ __forceinline__ float row_sum(float s, float (*part)[4], int& slot) {
-#pragma unroll
-  for (int d = 1; d < (LPR < 64 ? LPR : 64); d <<= 1) s += __shfl_xor(s, d, 64);
-  if constexpr (LPR == 256) {  // three slots in turn: a slot is written again only after two more barriers
-    float* p = part[slot];
-    slot = slot == 2 ? 0 : slot + 1;
-    if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = (p[0] + p[1]) + (p[2] + p[3]);
-  }
-  return s;
-}
-
 template <bool F16, int FMT, int LPR, int CH>
 __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
   constexpr int RPB = 256 / LPR;  // rows of a workgroup at a time
-  __shared__ float part[3][4];
+  __shared__ float part[2][4];
   int slot = 0;
   const int sub = threadIdx.x % LPR, units = a.C / 8;
   float g[CH][8], b[CH][8];
@@ -241,7 +227,6 @@ __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
       r[k] = a.r && u < units ? ((const mx_u32x4*)a.r)[base + u] : mx_u32x4{};
     }
     float v[CH][8];
-    float s = 0.f;
 #pragma unroll
     for (int k = 0; k < CH; k++) {
       mx_unpack8<F16>(q[k], v[k]);
@@ -253,30 +238,22 @@ __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
         q[k] = mx_pack8<F16>(v[k]);
         mx_unpack8<F16>(q[k], v[k]);
       }
-#pragma unroll
-      for (int j = 0; j < 8; j++) s += a.kind == MX_NORM_LAYER ? v[k][j] : v[k][j] * v[k][j];
     }
-    s = row_sum<LPR>(s, part, slot);
-    float mean = 0.f;
-    if (a.kind == MX_NORM_LAYER) {
-      mean = s * inv_c;
-      s = 0.f;
-#pragma unroll
-      for (int k = 0; k < CH; k++)
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-          const float d = k * LPR + sub < units ? v[k][j] - mean : 0.f;
-          s += d * d;
-        }
-      s = row_sum<LPR>(s, part, slot);
-    }
-    const float rstd = rsqrtf(s * inv_c + a.eps);
+    float mean, rstd;
+    mx_row_stats<LPR, CH>(v, sub, units, inv_c, a.eps, a.kind == MX_NORM_LAYER, mean, rstd, [&](float s) __attribute__((always_inline)) {
+      if constexpr (LPR == 256) {  // two slots in turn: one is written again only past another barrier
+        float* p = part[slot ^= 1];
+        if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = s;
+        __syncthreads();
+        s = (p[0] + p[1]) + (p[2] + p[3]);
+      }
+      return s;
+    });
 #pragma unroll
     for (int k = 0; k < CH; k++) {
       const int u = k * LPR + sub;
       float o[8];
-#pragma unroll
-      for (int j = 0; j < 8; j++) o[j] = (v[k][j] - mean) * rstd * g[k][j] + b[k][j];
+      mx_norm8(v[k], mean, rstd, g[k], b[k], o);
       const uint32_t byte = mx_scale_byte<FMT>(mx_quad_max(mx_top8(o)));
       const mx_u32x2 e = mx_encode8<FMT>(o, mx_inverse(byte));
       if (!live || u >= units) continue;

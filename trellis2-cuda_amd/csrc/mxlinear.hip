@@ -1,35 +1,9 @@
 // Linear layers of microscaled rows (mx.h):  y = act(X . W^T + b) + r,  X [N,K] e4m3 or e2m1, W [O,K] e2m1, fp32 sums.
-//
-// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 16 x 128 by 128 x 16 elements and their scales, one scale byte per row
-// and 32 columns. Lane l supplies row l % 16 of either operand. With g = l / 16 it holds, of 4-bit elements, columns
-// 32 g .. 32 g + 31 (16 bytes), of 8-bit ones 16 g .. and 64 + 16 g .. (two times 16 bytes), and in both cases the
-// scale of columns 32 g .. 32 g + 31. The result gives lane l column l % 16 and rows 4 g + i. W is the first operand, so
-// a lane holds 4 channels of one row of X per product, and the channel that each of W's 16 rows stands for is free:
-// channel(tile t, g, i) = (t / G) * 16 G + g * 4 G + (t % G) * 4 + i gives a lane 4 G consecutive channels over G tiles, so
-// its stores are whole 16-byte pieces.
-#include "mx.h"
+#include "mxgemm.h"
 
 #include <algorithm>
 
 namespace {
-typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-typedef int32_t i32x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-constexpr uint32_t kOOR = 0x80000000u;  // past every buffer below (at most 2^28 bytes), also with a step's offset added: reads as zeros
-
-enum { OUT_16 = 0, OUT_F32 = 1, OUT_MX8 = 2, OUT_MX4 = 3 };
-
-struct LinArgs {
-  const uint8_t *x, *xs, *w, *ws;  // codes and scales
-  const void *bias, *res;          // res: of out's type
-  void* out;
-  uint8_t* outs;
-  i64 N;
-  int K, O, bias_dt, act, f16;
-  int xrow, wrow, srow, osrow;  // bytes of a row: X's and W's codes, their scales, out's scales
-  int tiles_n, tiles_o, per, per_rest, band;
-};
-
 __device__ __forceinline__ i32x4 rsrc4(const void* p, uint32_t bytes) {  // a raw buffer's descriptor, in SGPRs
   const uint64_t b = (uint64_t)(uintptr_t)p;
   return i32x4{(int32_t)__builtin_amdgcn_readfirstlane((uint32_t)b), (int32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32)),
@@ -51,129 +25,9 @@ __device__ __forceinline__ void bare_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-__device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
-
-template <int XB>
-struct XFrag {  // 16 rows of X by 128 columns, this lane's part
-  mx_u32x4 q[XB / 4];
-};
-template <>
-struct XFrag<4> {
-  mx_u32x4 q[1];
-};
-// The scales are byte I of sw and sx
-template <int XB, int I>
-__device__ __forceinline__ f32x4 mfma(mx_u32x4 w, const XFrag<XB>& x, f32x4 c, int sw, int sx) {
-  const i32x8 a = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-  if constexpr (XB == 8) {
-    const i32x8 b = {(int)x.q[0][0], (int)x.q[0][1], (int)x.q[0][2], (int)x.q[0][3],
-                     (int)x.q[1][0], (int)x.q[1][1], (int)x.q[1][2], (int)x.q[1][3]};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, I, sw, I, sx);
-  } else {
-    const i32x8 b = {(int)x.q[0][0], (int)x.q[0][1], (int)x.q[0][2], (int)x.q[0][3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 4, I, sw, I, sx);
-  }
-}
-// Of four e4m3 elements those of magnitude 4 and more (codes from 0x48), zeros for the others: a byte's low seven bits plus
-// 0x38 carry into bit 7, which a byte permute spreads (selectors 8 and 9 repeat bits 15 and 31 of its second operand,
-// 10 and 11 those of its first).
-__device__ __forceinline__ uint32_t e4m3_large(uint32_t v) {
-  const uint32_t t = (v & 0x7f7f7f7fu) + 0x38383838u;
-  return v & __builtin_amdgcn_perm(t, t << 8, 0x0b090a08u);
-}
 template <int OUT, int TO>
 constexpr int run_tiles() {  // G above
   return OUT == OUT_F32 ? 1 : OUT == OUT_16 ? 2 : 4 < TO ? 4 : TO;
-}
-
-// Epilogue of NV consecutive channels o .. of row n in v: bias, activation, residual (its words in r), store. Lanes l, l + 16, l + 32, l + 48
-// hold neighbouring runs of one row; ok is the same for all lanes of a block of 32 channels.
-template <int OUT, int NV>
-__device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v)[NV], const float (&bias)[NV],
-                                       const uint32_t (&r)[4], bool ok) {
-#pragma unroll
-  for (int j = 0; j < NV; j++) v[j] += bias[j];
-  if (a.act == ACT_SILU) {
-#pragma unroll
-    for (int j = 0; j < NV; j++) v[j] = silu(v[j]);
-  }
-  if constexpr (OUT == OUT_F32) {
-    static_assert(NV == 4, "one 16-byte piece");
-    if (!ok) return;
-    if (a.res) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) v[j] += __uint_as_float(r[j]);
-    }
-    *(f32x4*)((float*)a.out + n * a.O + o) = f32x4{v[0], v[1], v[2], v[3]};
-  } else if constexpr (OUT == OUT_16) {
-    static_assert(NV == 8 || NV == 4, "one 16-byte piece, or half of one");
-    if (!ok) return;
-    uint32_t q[NV / 2];
-    if (a.res) {
-#pragma unroll
-      for (int j = 0; j < NV / 2; j++) {
-        v[2 * j] += a.f16 ? mx_lo<true>(r[j]) : mx_lo<false>(r[j]);
-        v[2 * j + 1] += a.f16 ? mx_hi<true>(r[j]) : mx_hi<false>(r[j]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < NV / 2; j++) q[j] = a.f16 ? mx_pack2<true>(v[2 * j], v[2 * j + 1]) : mx_pack2<false>(v[2 * j], v[2 * j + 1]);
-    uint32_t* y = (uint32_t*)((uint16_t*)a.out + n * a.O + o);
-    if constexpr (NV == 8) *(mx_u32x4*)y = *(mx_u32x4*)q;
-    else *(mx_u32x2*)y = *(mx_u32x2*)q;
-  } else {
-    static_assert(NV == 16 || NV == 8, "a half or a quarter of a block");
-    constexpr int FMT = OUT == OUT_MX8 ? MX_E4M3 : MX_E2M1;
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < NV; j += 8) top = max(top, mx_top8(*(float(*)[8])&v[j]));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-    if constexpr (NV == 8) top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    const uint32_t byte = mx_scale_byte<FMT>(top);
-    const float inv = mx_inverse(byte);
-    const mx_u32x2 p = mx_encode8<FMT>(*(float(*)[8])&v[0], inv);
-    if constexpr (NV == 16) {
-      const mx_u32x2 q = mx_encode8<FMT>(*(float(*)[8])&v[8], inv);
-      if (!ok) return;
-      if constexpr (FMT == MX_E4M3) *(mx_u32x4*)((uint8_t*)a.out + n * a.O + o) = mx_u32x4{p[0], p[1], q[0], q[1]};
-      else *(mx_u32x2*)((uint8_t*)a.out + (n * a.O + o) / 2) = mx_u32x2{p[0], q[0]};
-    } else {
-      if (!ok) return;
-      if constexpr (FMT == MX_E4M3) *(mx_u32x2*)((uint8_t*)a.out + n * a.O + o) = p;
-      else *(uint32_t*)((uint8_t*)a.out + (n * a.O + o) / 2) = p[0];
-    }
-    if (o % 32 == 0) {
-      uint8_t* s = a.outs + n * a.osrow;
-      s[o / 32] = (uint8_t)byte;
-      if (o / 32 + 1 == a.O / 32)
-        for (int k = a.O / 32; k < a.osrow; k++) s[k] = 0;
-    }
-  }
-}
-
-// The residual's words for NV channels of 16 or 32 bits
-template <int OUT, int NV>
-__device__ __forceinline__ void load_residual(const LinArgs& a, i64 n, int o, bool ok, uint32_t (&r)[4]) {
-  if constexpr (OUT == OUT_16 && NV == 4) {
-    const mx_u32x2 q = ok ? *(const mx_u32x2*)((const uint16_t*)a.res + n * a.O + o) : mx_u32x2{};
-    r[0] = q[0];
-    r[1] = q[1];
-  } else if constexpr (OUT == OUT_16 || OUT == OUT_F32) {
-    const mx_u32x4 q = ok ? *(const mx_u32x4*)((const char*)a.res + (n * a.O + o) * (OUT == OUT_16 ? 2 : 4)) : mx_u32x4{};
-#pragma unroll
-    for (int j = 0; j < 4; j++) r[j] = q[j];
-  }
-}
-
-// The parts of e4m3 elements that SPLIT products take apart (see k_mx_gemm)
-__device__ __forceinline__ void split(XFrag<8>& x, XFrag<8>& large) {  // x keeps the small ones
-#pragma unroll
-  for (int k = 0; k < 2; k++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      large.q[k][j] = e4m3_large(x.q[k][j]);
-      x.q[k][j] ^= large.q[k][j];
-    }
 }
 
 // Few rows: what counts is that all of W is on its way at once. A workgroup of 8 wavefronts has 16 OT channels by 16 NT rows;
@@ -291,12 +145,12 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
         split(small, large);
 #pragma unroll
         for (int t = 0; t < OT; t++) {
-          acc[t][u] = mfma<XB, 0>(q.w[t], small, acc[t][u], q.sw[t], q.sx[u]);
-          acc[t][u] = mfma<XB, 0>(q.w[t], large, acc[t][u], q.sw[t], q.sx[u]);
+          acc[t][u] = mfma<XB, 0, 0>(q.w[t], small, acc[t][u], q.sw[t], q.sx[u]);
+          acc[t][u] = mfma<XB, 0, 0>(q.w[t], large, acc[t][u], q.sw[t], q.sx[u]);
         }
       } else {
 #pragma unroll
-        for (int t = 0; t < OT; t++) acc[t][u] = mfma<XB, 0>(q.w[t], q.x[u], acc[t][u], q.sw[t], q.sx[u]);
+        for (int t = 0; t < OT; t++) acc[t][u] = mfma<XB, 0, 0>(q.w[t], q.x[u], acc[t][u], q.sw[t], q.sx[u]);
       }
     }
   };
@@ -558,8 +412,8 @@ __global__ void __launch_bounds__(64 * WO * WN, 2) k_mx_gemm(LinArgs a) {
 #pragma unroll
         for (int t = 0; t < H; t++) {
           f32x4& c = acc[hw * H + t][hx * HX + u];
-          c = mfma<XB, I>(fw[hw][t], fx[hx][u], c, sw[hw * H + t], sx[hx * HX + u]);
-          if constexpr (SPLIT) c = mfma<XB, I>(fw[hw][t], large[hx][u], c, sw[hw * H + t], sx[hx * HX + u]);
+          c = mfma<XB, I, I>(fw[hw][t], fx[hx][u], c, sw[hw * H + t], sx[hx * HX + u]);
+          if constexpr (SPLIT) c = mfma<XB, I, I>(fw[hw][t], large[hx][u], c, sw[hw * H + t], sx[hx * HX + u]);
         }
     };
     constexpr std::integral_constant<int, 0> first{};
@@ -691,52 +545,9 @@ void gemm(const LinArgs& a, int xt) {
 }
 }  // namespace
 
-namespace {
-// The caller's workspace, or one of the library's own. The latter is refused while the stream is being captured: the graph
-// would keep the address of a block that the library hands to other calls.
-struct Workspace {
-  Tensor own;
-  char* p;
-  i64 left;
-  Workspace(void* ws, i64 bytes, i64 need) {
-    if (ws) {
-      REQ((uintptr_t)ws % 16 == 0 && bytes >= need, "workspace of %lld bytes: %lld needed, 16-byte aligned", (long long)bytes,
-          (long long)need);
-      p = (char*)ws;
-    } else if (need) {
-      hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-      CK(hipStreamIsCapturing(stream(), &st));
-      REQ(st == hipStreamCaptureStatusNone, "a captured call needs a workspace of its caller (%lld bytes)", (long long)need);
-      own = empty({need}, U8);
-      p = (char*)own.p;
-    } else {
-      p = nullptr;
-    }
-    left = need;
-  }
-  Tensor take(i64 bytes) {
-    Tensor t = borrow(p, {bytes}, U8);
-    p += (bytes + 255) / 256 * 256;
-    return t;
-  }
-  MxTensor rows(int fmt, i64 n, i64 cols) {
-    MxTensor q;
-    q.fmt = fmt;
-    q.rows = n;
-    q.cols = cols;
-    q.codes = take(n * mx_row_bytes(fmt, cols));
-    q.scales = take(n * mx_scale_bytes(cols));
-    return q;
-  }
-};
-i64 rows_bytes(int fmt, i64 n, i64 cols) {
-  return (n * mx_row_bytes(fmt, cols) + 255) / 256 * 256 + (n * mx_scale_bytes(cols) + 255) / 256 * 256;
-}
-
-// shapes and types are checked by the callers
 // xv: x's values (at most 16 rows), which the product quantises to x's format itself; else x's codes
-void product(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* res, int act, Tensor* y, MxTensor* yq,
-             const Tensor* xv = nullptr) {
+void mx_product(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* res, int act, Tensor* y, MxTensor* yq,
+                const Tensor* xv) {
   if (x.rows == 0) return;
   LinArgs a{};
   a.x = xv ? xv->ptr<uint8_t>() : x.codes.ptr<uint8_t>();
@@ -771,6 +582,7 @@ void product(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Ten
   x.fmt == MX_E4M3 ? by_out(std::integral_constant<int, 8>{}) : by_out(std::integral_constant<int, 4>{});
 }
 
+namespace {
 void check_linear(i64 n, i64 K, const MxTensor& w, const Tensor* bias, const Tensor* res, int act, const Tensor* y, const MxTensor* yq) {
   mx_check(w, "w");
   REQ(w.fmt == MX_E2M1, "w must be e2m1 (format %d)", w.fmt);
@@ -794,26 +606,16 @@ void check_linear(i64 n, i64 K, const MxTensor& w, const Tensor* bias, const Ten
     REQ(!res, "a microscaled output takes no residual");
   }
 }
-void apart(const void* a, size_t na, const void* b, size_t nb, const char* what) {
-  REQ(!mx_overlap(a, na, b, nb), "out must not overlap %s", what);
-}
-void out_apart(const Tensor* y, const MxTensor* yq, const Tensor& t, const char* what) {
-  if (y) apart(y->p, y->bytes(), t.p, t.bytes(), what);
-  if (yq) {
-    apart(yq->codes.p, yq->codes.bytes(), t.p, t.bytes(), what);
-    apart(yq->scales.p, yq->scales.bytes(), t.p, t.bytes(), what);
-  }
-}
 }  // namespace
 
-i64 mx_linear_workspace(i64 n, i64 K, int x_fmt) { return n > kValueRows && K > 0 ? rows_bytes(x_fmt, n, K) : 0; }
+i64 mx_linear_workspace(i64 n, i64 K, int x_fmt) { return n > kValueRows && K > 0 ? mx_rows_bytes(x_fmt, n, K) : 0; }
 
 void mx_linear(const MxTensor& x, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y, MxTensor* yq) {
   mx_check(x, "x");
   check_linear(x.rows, x.cols, w, bias, residual, act, y, yq);
-  for (const Tensor* t : {&x.codes, &x.scales, &w.codes, &w.scales}) out_apart(y, yq, *t, "x or w");
-  if (bias) out_apart(y, yq, *bias, "bias");
-  product(x, w, bias, residual, act, y, yq);
+  for (const Tensor* t : {&x.codes, &x.scales, &w.codes, &w.scales}) mx_out_apart(y, yq, *t, "x or w");
+  if (bias) mx_out_apart(y, yq, *bias, "bias");
+  mx_product(x, w, bias, residual, act, y, yq);
 }
 
 void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y,
@@ -824,86 +626,19 @@ void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias
   check_linear(n, K, w, bias, residual, act, y, yq);
   REQ(n < (1ll << 31), "%lld rows", (long long)n);
   REQ((uintptr_t)x.p % 16 == 0 && (x.p || n == 0), "x must be 16-byte aligned and not null");
-  out_apart(y, yq, x, "x");
-  for (const Tensor* t : {&w.codes, &w.scales}) out_apart(y, yq, *t, "w");
-  if (bias) out_apart(y, yq, *bias, "bias");
+  mx_out_apart(y, yq, x, "x");
+  for (const Tensor* t : {&w.codes, &w.scales}) mx_out_apart(y, yq, *t, "w");
+  if (bias) mx_out_apart(y, yq, *bias, "bias");
   if (n == 0) return;
-  Workspace ws(workspace, workspace_bytes, mx_linear_workspace(n, K, x_fmt));
+  MxWorkspace ws(workspace, workspace_bytes, mx_linear_workspace(n, K, x_fmt));
   if (n <= kValueRows) {
     MxTensor q;
     q.fmt = x_fmt;
     q.rows = n;
     q.cols = K;
-    return product(q, w, bias, residual, act, y, yq, &x);
+    return mx_product(q, w, bias, residual, act, y, yq, &x);
   }
   MxTensor q = ws.rows(x_fmt, n, K);
   mx_quantize(x, q);
-  product(q, w, bias, residual, act, y, yq);
-}
-
-// ---- ConvNeXt tail ----------------------------------------------------------------------------------------------
-//   y = x + W2 mx(silu(W1 mx(LayerNorm(h) * gamma + beta) + b1)) + b2
-// norm pass, product with the SiLU and the quantisation in its epilogue, product with the residual. Many rows go in
-// equal parts whose hidden units stay below kHidBytes, so that they are read back from the 256 MB cache.
-namespace {
-constexpr i64 kHidBytes = 128ll << 20;
-i64 tail_rows(i64 n, i64 C, int fmt) {
-  const i64 parts = (n * mx_row_bytes(fmt, 4 * C) + kHidBytes - 1) / kHidBytes;
-  return n == 0 ? 0 : std::min(n, ((n + parts - 1) / parts + 255) / 256 * 256);
-}
-}  // namespace
-
-i64 convnext_mlp_mx_workspace(i64 n, i64 C, int fmt) {
-  if (n <= 0 || C <= 0) return 0;
-  const i64 m = tail_rows(n, C, fmt);
-  return rows_bytes(fmt, m, C) + rows_bytes(fmt, m, 4 * C);
-}
-
-void convnext_mlp_mx(const Tensor& h, const Tensor& x, const Tensor* gamma, const Tensor* beta, float eps, const MxTensor& w1,
-                     const Tensor* b1, const MxTensor& w2, const Tensor* b2, int fmt, Tensor& y, void* workspace,
-                     i64 workspace_bytes) {
-  REQ(h.dim() == 2 && (h.dt == BF16 || h.dt == F16), "h must be bf16/fp16 [N,C]");
-  const i64 n = h.size(0), C = h.size(1);
-  REQ(C > 0 && C % 32 == 0 && C <= 4096, "C=%lld: a multiple of 32, at most 4096", (long long)C);
-  REQ(n < (1ll << 31), "%lld rows", (long long)n);
-  REQ(fmt == MX_E4M3 || fmt == MX_E2M1, "fmt=%d", fmt);
-  mx_check(w1, "w1");
-  mx_check(w2, "w2");
-  REQ(w1.fmt == MX_E2M1 && w2.fmt == MX_E2M1, "w1 and w2 must be e2m1");
-  REQ(w1.rows == 4 * C && w1.cols == C, "w1 must be [4C, C]");
-  REQ(w2.rows == C && w2.cols == 4 * C, "w2 must be [C, 4C]");
-  REQ(x.dt == h.dt && x.dim() == 2 && x.size(0) == n && x.size(1) == C, "x must match h");
-  REQ(y.dt == h.dt && y.dim() == 2 && y.size(0) == n && y.size(1) == C, "y must match h");
-  const Tensor* params[4] = {gamma, beta, b1, b2};
-  for (int k = 0; k < 4; k++) {
-    const Tensor* t = params[k];
-    REQ(!t || (t->numel() == (k == 2 ? 4 * C : C) && (t->dt == F32 || t->dt == F16 || t->dt == BF16)), "gamma/beta/b2 must have C elements, b1 4C");
-    if (t) out_apart(&y, nullptr, *t, "the parameters");
-  }
-  if (n == 0) return;
-  REQ(h.p && x.p && y.p && ((uintptr_t)h.p | (uintptr_t)x.p | (uintptr_t)y.p) % 16 == 0, "h, x, y must be 16-byte aligned and not null");
-  for (const Tensor* t : {&h, &x}) REQ(t->p == y.p || !mx_overlap(t->p, t->bytes(), y.p, y.bytes()), "y must be h, x or apart from both");
-  for (const MxTensor* w : {&w1, &w2}) {
-    out_apart(&y, nullptr, w->codes, "the weights");
-    out_apart(&y, nullptr, w->scales, "the weights");
-  }
-  const i64 step = tail_rows(n, C, fmt);
-  Workspace ws(workspace, workspace_bytes, convnext_mlp_mx_workspace(n, C, fmt));
-  const MxTensor a = ws.rows(fmt, step, C), hid = ws.rows(fmt, step, 4 * C);
-  auto first = [](const MxTensor& q, i64 m) {
-    MxTensor r = q;
-    r.rows = m;
-    r.codes = borrow(q.codes.p, {m * mx_row_bytes(q.fmt, q.cols)}, U8);
-    r.scales = borrow(q.scales.p, {m * mx_scale_bytes(q.cols)}, U8);
-    return r;
-  };
-  for (i64 r0 = 0; r0 < n; r0 += step) {
-    const i64 m = std::min(step, n - r0);
-    MxTensor am = first(a, m), hm = first(hid, m);
-    Tensor ym = y.slice0(r0, r0 + m);
-    const Tensor xm = x.slice0(r0, r0 + m);
-    add_norm_mx(h.slice0(r0, r0 + m), nullptr, gamma, beta, eps, MX_NORM_LAYER, nullptr, am);
-    product(am, w1, b1, nullptr, ACT_SILU, nullptr, &hm);
-    product(hm, w2, b2, &xm, ACT_NONE, &ym, nullptr);
-  }
+  mx_product(q, w, bias, residual, act, y, yq);
 }
