@@ -71,6 +71,16 @@ __device__ __forceinline__ uint32_t mx_quad_max(uint32_t m) {
   return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));  // lanes 2, 3, 0, 1
 }
 
+// The maximum over lanes l and l ^ 16, and over l and l ^ 32: the swaps give every lane of a pair both values
+__device__ __forceinline__ uint32_t mx_max_across16(uint32_t m) {
+  const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+__device__ __forceinline__ uint32_t mx_max_across32(uint32_t m) {
+  const auto r = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+
 // 16-bit storage <-> fp32, two values a word
 typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 mx_f16x2 __attribute__((ext_vector_type(2)));

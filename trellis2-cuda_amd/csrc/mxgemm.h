@@ -100,8 +100,8 @@ __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < NV; j += 8) top = max(top, mx_top8(*(float(*)[8])&v[j]));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-    if constexpr (NV == 8) top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+    top = mx_max_across16(top);
+    if constexpr (NV == 8) top = mx_max_across32(top);
     const uint32_t byte = mx_scale_byte<FMT>(top);
     const float inv = mx_inverse(byte);
     const mx_u32x2 p = mx_encode8<FMT>(*(float(*)[8])&v[0], inv);

@@ -68,12 +68,25 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
   const auto rw = rsrc(a.w + (i64)o0 * a.wrow, 16 * OT * a.wrow), rws = rsrc(a.ws + (i64)o0 * a.srow, 16 * OT * a.srow);
   const auto rx = XT < 0 ? rsrc(a.x + n0 * a.xrow, rows * a.xrow) : rsrc(a.x + n0 * a.K * XS, rows * a.K * XS);
   const auto rxs = rsrc(XT < 0 ? a.xs + n0 * a.srow : nullptr, XT < 0 ? rows * a.srow : 0);
+  // More row tiles: a load for every scale byte would be a third of the loads, so the scales of four steps come together
+  mx_u32x4 cw[OT], cx[NT];
+  auto load_scales = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < OT; t++) cw[t] = __builtin_amdgcn_raw_buffer_load_b128(rws, (uint32_t)((chan[t] - o0) * a.srow), c * 16, 0);
+#pragma unroll
+    for (int u = 0; u < NT; u++) cx[u] = __builtin_amdgcn_raw_buffer_load_b128(rxs, (uint32_t)((u * 16 + r16) * a.srow), c * 16, 0);
+  };
+  auto scale_of = [&](mx_u32x4 q, int s) __attribute__((always_inline)) {  // block 4 s + g's, in byte 0
+    const uint32_t w = s % 4 == 0 ? q[0] : s % 4 == 1 ? q[1] : s % 4 == 2 ? q[2] : q[3];
+    return (int)(w >> (8 * g));
+  };
   auto load = [&](Step& q, int s) __attribute__((always_inline)) {
     const bool in = s * 4 + g < blocks;  // columns past the last: zeros and scale 0
 #pragma unroll
     for (int t = 0; t < OT; t++) {
       q.w[t] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? (uint32_t)((chan[t] - o0) * a.wrow + g * 16) : kOOR, s * 64, 0);
-      q.sw[t] = __builtin_amdgcn_raw_buffer_load_b8(rws, in ? (uint32_t)((chan[t] - o0) * a.srow + g) : kOOR, s * 4, 0);
+      if constexpr (NT == 1) q.sw[t] = __builtin_amdgcn_raw_buffer_load_b8(rws, in ? (uint32_t)((chan[t] - o0) * a.srow + g) : kOOR, s * 4, 0);
+      else q.sw[t] = in ? scale_of(cw[t], s) : 0;
     }
     if constexpr (XT < 0) {
 #pragma unroll
@@ -85,7 +98,8 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
         } else {
           q.x[u].q[0] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? x : kOOR, s * 64, 0);
         }
-        q.sx[u] = __builtin_amdgcn_raw_buffer_load_b8(rxs, in ? (uint32_t)((u * 16 + r16) * a.srow + g) : kOOR, s * 4, 0);
+        if constexpr (NT == 1) q.sx[u] = __builtin_amdgcn_raw_buffer_load_b8(rxs, in ? (uint32_t)((u * 16 + r16) * a.srow + g) : kOOR, s * 4, 0);
+        else q.sx[u] = in ? scale_of(cx[u], s) : 0;
       }
     } else {
       static_assert(NT == 1, "quantised once per workgroup");
@@ -119,8 +133,7 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
         uint32_t byte[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          top[h] = max(top[h], (uint32_t)__shfl_xor((int)top[h], 16, 64));
-          byte[h] = mx_scale_byte<MX_E4M3>(top[h]);
+          byte[h] = mx_scale_byte<MX_E4M3>(mx_max_across16(top[h]));
           const float inv = mx_inverse(byte[h]);
           const mx_u32x2 p = mx_encode8<MX_E4M3>(*(float(*)[8])&v[h * 16], inv), r = mx_encode8<MX_E4M3>(*(float(*)[8])&v[h * 16 + 8], inv);
           q.x[0].q[h] = mx_u32x4{p[0], p[1], r[0], r[1]};
@@ -154,19 +167,28 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
       }
     }
   };
-  constexpr int U = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // steps loaded at once
-  int s = s0;
-  for (; s + U <= s1; s += U) {
-    Step q[U];
+  if constexpr (NT == 1) {
+    constexpr int U = 4;  // steps loaded at once
+    int s = s0;
+    for (; s + U <= s1; s += U) {
+      Step q[U];
 #pragma unroll
-    for (int k = 0; k < U; k++) load(q[k], s + k);
+      for (int k = 0; k < U; k++) load(q[k], s + k);
 #pragma unroll
-    for (int k = 0; k < U; k++) multiply(q[k]);
-  }
-  for (; s < s1; s++) {
-    Step q;
-    load(q, s);
-    multiply(q);
+      for (int k = 0; k < U; k++) multiply(q[k]);
+    }
+    for (; s < s1; s++) {
+      Step q;
+      load(q, s);
+      multiply(q);
+    }
+  } else {
+    for (int s = s0; s < s1; s++) {
+      if (s == s0 || s % 4 == 0) load_scales(s / 4);
+      Step q;
+      load(q, s);
+      multiply(q);
+    }
   }
 #pragma unroll
   for (int t = 0; t < OT; t++)

@@ -28,7 +28,7 @@ constexpr int kTailRows = 64;  // rows of a workgroup
 template <bool F16, int C>
 __global__ void __launch_bounds__(512, 4) k_mx_tail(TailArgs a) {
   constexpr int BN = kTailRows, S1 = C / 128, ROUNDS = C / 64, OT = C / 128, G = OT == 1 ? 1 : 2;
-  constexpr int T = C == 256 ? 1 : 2, U = BN / 16, R1 = C / 2, R2 = 2 * C;         // row tiles; bytes of W1's and W2's rows
+  constexpr int U = BN / 16, R1 = C / 2, R2 = 2 * C;         // row tiles; bytes of W1's and W2's rows
   constexpr int SR2 = C / 8;                                 // of W2's scale rows (W1's: 16)
   constexpr int LPR = C / 8, PASS = 512 / LPR;               // lanes of a row, rows of a pass
   __shared__ __attribute__((aligned(16))) mx_u32x4 xl[2][S1][BN * 8], hid[2][2][BN * 8];  // small, large; slots, steps
@@ -120,39 +120,37 @@ __global__ void __launch_bounds__(512, 4) k_mx_tail(TailArgs a) {
 #pragma unroll 1
   for (int round = 0; round < ROUNDS; round++) {
     const int slot = round & 1;
-    mx_unroll<U / T>([&](auto HC) __attribute__((always_inline)) {  // T row tiles at a time
-      constexpr int u0 = decltype(HC)::value * T;
-      f32x4 hacc[2][T] = {};
-      // fragments one ahead of their products; the scheduling barriers keep the compiler from reading all of them first
-      auto read_x = [&](int i) __attribute__((always_inline)) {  // i = (step, part, row tile)
-        const mx_u32x4* l = xl[i / T & 1][i / (2 * T)] + (u0 + i % T) * 128;
-        return XFrag<8>{{l[p0], l[p1]}};
-      };
-      XFrag<8> xf[2] = {read_x(0), {}};
-      mx_unroll<S1 * 2 * T>([&](auto IC) __attribute__((always_inline)) {
-        constexpr int i = decltype(IC)::value, s = i / (2 * T), u = i % T;
-        if constexpr (i + 1 < S1 * 2 * T) xf[(i + 1) & 1] = read_x(i + 1);
-        hacc[0][u] = mfma<8, 0, s>(w1[0][s], xf[i & 1], hacc[0][u], (int)(s1[0][s] >> (8 * g)), sx[u0 + u]);
-        hacc[1][u] = mfma<8, 0, s>(w1[1][s], xf[i & 1], hacc[1][u], (int)(s1[1][s] >> (8 * g)), sx[u0 + u]);
-        __builtin_amdgcn_sched_barrier(0);
+    // Row tile u + 1's products are issued beside row tile u's SiLU and quantisation.
+    f32x4 hacc[2][2];
+    auto product1 = [&](auto UC) __attribute__((always_inline)) {
+      constexpr int u = decltype(UC)::value;
+      f32x4(&c)[2] = hacc[u & 1];
+      c[0] = c[1] = f32x4{};
+      mx_unroll<S1 * 2>([&](auto IC) __attribute__((always_inline)) {
+        constexpr int i = decltype(IC)::value, s = i / 2, part = i % 2;
+        const mx_u32x4* l = xl[part][s] + u * 128;
+        const XFrag<8> x = {{l[p0], l[p1]}};
+        c[0] = mfma<8, 0, s>(w1[0][s], x, c[0], (int)(s1[0][s] >> (8 * g)), sx[u]);
+        c[1] = mfma<8, 0, s>(w1[1][s], x, c[1], (int)(s1[1][s] >> (8 * g)), sx[u]);
       });
-      if constexpr (u0 + T == U) load2(round);
-      float bias[8];
+    };
+    float bias[8];
 #pragma unroll
-      for (int j = 0; j < 2; j++) *(f32x4*)&bias[4 * j] = *(const f32x4*)&b1l[round * 256 + wave * 32 + g * 8 + 4 * j];
+    for (int j = 0; j < 2; j++) *(f32x4*)&bias[4 * j] = *(const f32x4*)&b1l[round * 256 + wave * 32 + g * 8 + 4 * j];
+    product1(std::integral_constant<int, 0>{});
+    __builtin_amdgcn_sched_barrier(0);
+    mx_unroll<U>([&](auto UC) __attribute__((always_inline)) {
+      constexpr int u = decltype(UC)::value;
+      if constexpr (u + 1 < U) product1(std::integral_constant<int, u + 1>{});
+      else load2(round);
+      float v[8];
 #pragma unroll
-      for (int u = 0; u < T; u++) {
-        float v[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = silu(hacc[j / 4][u][j % 4] + bias[j]);
-        uint32_t top = mx_top8(v);
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        const uint32_t byte = mx_scale_byte<MX_E4M3>(top);
-        const int row = (u0 + u) * 16 + r16;
-        ((mx_u32x2*)hid[slot][wave / 4])[(row * 8 + ((wave % 4 * 2 + g / 2) ^ (row & 7))) * 2 + g % 2] = mx_encode8<MX_E4M3>(v, mx_inverse(byte));
-        if (g == 0) hsc[slot][row * 8 + wave] = (uint8_t)byte;
-      }
+      for (int j = 0; j < 8; j++) v[j] = silu(hacc[u & 1][j / 4][j % 4] + bias[j]);
+      const uint32_t byte = mx_scale_byte<MX_E4M3>(mx_max_across32(mx_max_across16(mx_top8(v))));
+      const int row = u * 16 + r16;
+      ((mx_u32x2*)hid[slot][wave / 4])[(row * 8 + ((wave % 4 * 2 + g / 2) ^ (row & 7))) * 2 + g % 2] = mx_encode8<MX_E4M3>(v, mx_inverse(byte));
+      if (g == 0) hsc[slot][row * 8 + wave] = (uint8_t)byte;
+      __builtin_amdgcn_sched_barrier(0);
     });
     // The hidden units are written. (A slot is written again two rounds on, past the next round's barrier, which no
     // wavefront reaches before it has read this one's.) The weights' loads stay on their way.

@@ -112,12 +112,17 @@ def _torch():
     return torch
 
 
+_DTYPES = {}
+
+
 def _dt(t) -> int:
-    torch = _torch()
-    m = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if t.dtype not in m:
+    if not _DTYPES:
+        torch = _torch()
+        _DTYPES.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         raise TypeError(f"unsupported dtype {t.dtype}")
-    return m[t.dtype]
+    return code
 
 
 def _ptr(t):
@@ -372,12 +377,24 @@ class MxTensor:
 
     @classmethod
     def empty(cls, rows: int, cols: int, fmt: int, device):
-        torch = _torch()
-        codes = torch.empty((rows, cols // 2 if fmt == MX_E2M1 else cols), dtype=torch.uint8, device=device)
-        return cls(codes, torch.empty((rows, (cols + 511) // 512 * 16), dtype=torch.uint8, device=device), cols, fmt)
+        return _new_rows(_torch().empty(0, device=device), rows, cols, fmt)
 
     def dequantize(self, dtype=None):
         return mx_dequantize(self, dtype)
+
+
+def _new_rows(like, rows, cols, fmt):
+    """An MxTensor with buffers of its own beside the tensor `like`."""
+    if fmt != MX_E2M1 and fmt != MX_E4M3:
+        raise ValueError(f"unknown format {fmt}")
+    if cols <= 0 or cols % 32:
+        raise ValueError(f"{cols} columns: a positive multiple of 32")
+    u8 = _torch().uint8
+    q = MxTensor.__new__(MxTensor)
+    q.codes = like.new_empty((rows, cols >> 1 if fmt == MX_E2M1 else cols), dtype=u8)
+    q.scales = like.new_empty((rows, (cols + 511) // 512 * 16), dtype=u8)
+    q.fmt, q.shape = fmt, (rows, cols)
+    return q
 
 
 def _adr(t, dev):
@@ -411,7 +428,7 @@ def mx_quantize(x, fmt: int = MX_E2M1, out: MxTensor = None) -> MxTensor:
     _matrix(x, "x")
     N, K = x.shape
     if out is None:
-        out = MxTensor.empty(N, K, fmt, x.device)
+        out = _new_rows(x, N, K, fmt)
     elif out.shape != (N, K) or out.fmt != fmt:
         raise ValueError(f"out must be of x's shape {list(x.shape)} and format {fmt}")
     dev = _torch().cuda.current_device()
@@ -424,7 +441,7 @@ def mx_dequantize(q: MxTensor, dtype=None, out=None):
     torch = _torch()
     N, K = q.shape
     if out is None:
-        out = torch.empty((N, K), dtype=dtype or torch.bfloat16, device=q.codes.device)
+        out = q.codes.new_empty((N, K), dtype=dtype or torch.bfloat16)
     else:
         _matrix(out, "out", q.shape, dtype)
     dev = torch.cuda.current_device()
@@ -451,7 +468,7 @@ def add_norm_mx(x, residual=None, gamma=None, beta=None, eps: float = 1e-6, kind
     if sum is not None:
         _matrix(sum, "sum", shape, x.dtype)
     if out is None:
-        out = MxTensor.empty(N, C, fmt, x.device)
+        out = _new_rows(x, N, C, fmt)
     elif out.shape != (N, C) or out.fmt != fmt:
         raise ValueError(f"out must be [{N}, {C}] of format {fmt}")
     p = gamma if gamma is not None else beta
@@ -493,13 +510,13 @@ def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt
         if residual is not None or out_dtype is not None:
             raise ValueError("a microscaled result takes no residual and no out_dtype")
         if out is None:
-            out = MxTensor.empty(N, Co, out_fmt, xv.device)
+            out = _new_rows(xv, N, Co, out_fmt)
         elif not isinstance(out, MxTensor) or out.shape != (N, Co) or out_fmt not in (None, out.fmt):
             raise ValueError(f"out must be an MxTensor [{N}, {Co}] of format {out_fmt}")
         y, ys, ot = out.codes, out.scales, out.fmt
     else:
         if out is None:
-            out = torch.empty((N, Co), dtype=out_dtype or (torch.bfloat16 if quantized else x.dtype), device=xv.device)
+            out = xv.new_empty((N, Co), dtype=out_dtype or (torch.bfloat16 if quantized else x.dtype))
         else:
             _matrix(out, "out", (N, Co), out_dtype)
         if residual is not None:
