@@ -71,6 +71,12 @@ __device__ __forceinline__ uint32_t mx_quad_max(uint32_t m) {
   return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, true));  // lanes 2, 3, 0, 1
 }
 
+// In lanes that are multiples of 16: the bytes of lanes l, l + 4, l + 8, l + 12, lowest first (elsewhere: of no use)
+__device__ __forceinline__ uint32_t mx_four_bytes(uint32_t b) {
+  uint32_t w = b | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, 0x104, 0xf, 0xf, true) << 8;  // of four lanes on
+  return w | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x108, 0xf, 0xf, true) << 16;
+}
+
 // The maximum over lanes l and l ^ 16, and over l and l ^ 32: the swaps give every lane of a pair both values
 __device__ __forceinline__ uint32_t mx_max_across16(uint32_t m) {
   const auto r = __builtin_amdgcn_permlane16_swap(m, m, false, false);

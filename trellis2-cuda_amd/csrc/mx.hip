@@ -69,12 +69,20 @@ __global__ void __launch_bounds__(256) k_mx_quantize(const void* __restrict__ x,
     const i64 u = u0 + k * 256;
     const uint32_t byte = mx_scale_byte<FMT>(mx_quad_max(mx_top8(v[k])));
     const mx_u32x2 q = mx_encode8<FMT>(v[k], mx_inverse(byte));
-    if (u >= units) break;  // a quad's four units are inside or outside together
+    if (u >= units) break;  // a quad's four units are inside or outside together, and 16 lanes' where per % 4 == 0
     if constexpr (FMT == MX_E4M3) ((mx_u32x2*)codes)[u] = q;
     else ((uint32_t*)codes)[u] = q[0];
-    if ((threadIdx.x & 3) == 0) {
-      const uint32_t b = (uint32_t)(u >> 2), row = b / per;
-      put_scale(scales, row, b - row * per, per, stride, byte);
+    const uint32_t b = (uint32_t)(u >> 2), row = b / per, col = b - row * per;
+    if (per % 4 == 0) {  // four blocks' bytes are a word of one row
+      const uint32_t w = mx_four_bytes(byte);
+      if ((threadIdx.x & 15) == 0) {
+        uint32_t* s = (uint32_t*)(scales + (i64)row * stride + col);
+        *s = w;
+        if (col + 4 == per)
+          for (uint32_t k = 1; k < (stride - col) / 4; k++) s[k] = 0;
+      }
+    } else if ((threadIdx.x & 3) == 0) {
+      put_scale(scales, row, col, per, stride, byte);
     }
   }
 }
@@ -256,11 +264,19 @@ __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
       mx_norm8(v[k], mean, rstd, g[k], b[k], o);
       const uint32_t byte = mx_scale_byte<FMT>(mx_quad_max(mx_top8(o)));
       const mx_u32x2 e = mx_encode8<FMT>(o, mx_inverse(byte));
-      if (!live || u >= units) continue;
+      // scales, and zeros behind a row's last: 16 lanes' blocks are a word, a row of up to 256 channels fills 16 bytes by itself
+      const uint32_t w = mx_four_bytes(u < units ? byte : 0u);
+      const uint32_t w1 = LPR == 32 ? (uint32_t)__shfl_down((int)w, 16, 64) : 0u;
+      if (!live) continue;
+      if constexpr (LPR >= 64) {
+        if (sub % 16 == 0 && u / 4 < (int)a.stride) *(uint32_t*)(a.scales + row * a.stride + u / 4) = w;
+      } else {
+        if (sub == 0) *(mx_u32x4*)(a.scales + row * a.stride) = mx_u32x4{LPR == 8 ? w & 0xffffu : w, w1, 0, 0};
+      }
+      if (u >= units) continue;
       if (a.sum) ((mx_u32x4*)a.sum)[base + u] = q[k];
       if constexpr (FMT == MX_E4M3) ((mx_u32x2*)a.codes)[base + u] = e;
       else ((uint32_t*)a.codes)[base + u] = e[0];
-      if ((sub & 3) == 0) put_scale(a.scales, row, (uint32_t)u >> 2, (uint32_t)units >> 2, a.stride, byte);
     }
   }
 }
@@ -286,6 +302,8 @@ void add_norm_mx(const Tensor& x, const Tensor* residual, const Tensor* gamma, c
     REQ(!mx_overlap(t->p, t->bytes(), q.codes.p, q.codes.bytes()) && !mx_overlap(t->p, t->bytes(), q.scales.p, q.scales.bytes()),
         "codes and scales must not overlap x, residual or sum");
   }
+  for (const Tensor* t : {gamma, beta})
+    if (t) mx_out_apart(sum, &q, *t, "gamma or beta");
   for (const Tensor* t : {&x, residual})  // in place is fine: a lane reads what it then writes
     REQ(!t || !sum || sum->p == t->p || !mx_overlap(t->p, t->bytes(), sum->p, sum->bytes()), "sum must be x, residual or apart from both");
   NormArgs a{};
