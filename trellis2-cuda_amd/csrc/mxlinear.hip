@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(64 * WO * WN, 2) k_mx_gemm(LinArgs a) {
   constexpr int XR = XB * 16 * KS, WR = 64 * KS;                                // bytes of a row of X and W per stage
   constexpr int XP = XR / 16, WP = WR / 16;                                     // 16-byte pieces of them
   constexpr int XI = BN * XR / 1024 / NW, WI = BO * WR / 1024 / NW, ST = (BO + BN) / 64, SI = (ST + NW - 1) / NW;  // DMAs per wavefront
-  static_assert(XI * 1024 * NW == BN * XR && WI * 1024 * NW == BO * WR && BO % 64 == 0 && BN % 64 == 0 && ST >= NW, "whole DMAs");
+  static_assert(XI * 1024 * NW == BN * XR && WI * 1024 * NW == BO * WR && BO % 64 == 0 && BN % 64 == 0, "whole DMAs");
   static_assert((XR == 64 || XR == 128) && (WR == 64 || WR == 128), "swizzles");
   constexpr int G = run_tiles<OUT, TO>();
   static_assert(TO % G == 0 && TO % 2 == 0 && TN % 2 == 0 && NS >= 2 && NS <= 4, "whole runs, two halves");
@@ -558,12 +558,15 @@ void gemm(const LinArgs& a, int xt) {
   if (a.N <= 32) return launch_rows<XB, OUT, -1, 2>(a);
   if (a.N <= 64) return launch_rows<XB, OUT, -1, 4>(a);
   if (a.N <= kFewRows) return launch_rows<XB, OUT, -1, 5>(a);
-  // Tiles of 256 channels by 128 rows read fewer operand bytes per product than 128 by 128, but there are half as many: where
-  // they do not fill most of the slots (two workgroups per CU), the smaller ones do. us at 256 / 128, [N, K, O]:
-  // e4m3 [16411, 4096, 4096] 278 / 314, [8209, 2080, 4128] 102 / 108, [58321, 1024, 256] 32 / 34, [11467, 2048, 512] 29 / 24,
-  // [2048, 4096, 4096] 45 / 40, [1803, 4096, 1024] 41 / 26; e2m1 [16411, 4096, 4096] 237 / 250.
-  if ((i64)cdiv(a.N, 128) * cdiv(a.O, 256) * 2 >= 3 * (i64)mx_device_cus()) launch<XB, OUT, 8, 4, 2, 2, 1, XB == 8 ? 2 : 3>(a);
-  else launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
+  // Larger tiles read fewer operand bytes per product, smaller ones are more. Two workgroups of 256 channels by 128 rows fit a
+  // CU: they are taken where they fill most of these slots; 128 by 64 where 128 by 128 would leave a quarter of them free.
+  // us at 256 x 128 / 128 x 128 / 128 x 64, [N, K, O]: e4m3 [16411, 4096, 4096] 278 / 314 / -, [8209, 2080, 4128] 102 / 108 / -,
+  // [58321, 1024, 256] 32 / 34 / -, [2048, 4096, 4096] 45 / 42 / 52, [1803, 4096, 1024] 41 / 27 / 19, [11467, 2048, 512] 29 / 24 / 22,
+  // [300, 1024, 1024] - / 13 / 9; e2m1 [16411, 4096, 4096] 237 / 250 / -, [600, 2048, 2048] - / 14 / 11.
+  const i64 n128 = cdiv(a.N, 128), cus = mx_device_cus();
+  if (n128 * cdiv(a.O, 256) * 2 >= 3 * cus) launch<XB, OUT, 8, 4, 2, 2, 1, XB == 8 ? 2 : 3>(a);
+  else if (n128 * cdiv(a.O, 128) * 2 > 3 * cus) launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
+  else launch<XB, OUT, 4, 2, 2, 2, 1, 3>(a);
 }
 }  // namespace
 
