@@ -165,6 +165,45 @@ def test_add_norm_many_rows(gpu, C, n):
         assert torch.equal(q2.codes, q.codes) and torch.equal(q2.scales, q.scales)
 
 
+@pytest.mark.parametrize("C", [32, 96, 160, 544, 2080])
+def test_add_norm_writes_its_rows_only(gpu, C):
+    """Rows before and behind stay as they were; the sum alone (no residual) is a copy of x."""
+    x = features(5, C, torch.float16, C).to(gpu)
+    buf = sp.MxTensor.empty(9, C, sp.MX_E4M3, gpu)
+    buf.codes.fill_(9)
+    buf.scales.fill_(9)
+    sums = torch.full((9, C), 9.0, dtype=torch.float16, device=gpu)
+    q = sp.MxTensor(buf.codes[2:7], buf.scales[2:7], C, sp.MX_E4M3)
+    t, got = sp.add_norm_mx(x, sum=sums[2:7], out=q)
+    assert got is q and torch.equal(sums[2:7], x) and torch.equal(t, x)
+    near(q, *norm64(x.double(), sp.NORM_RMS, None, None, 1e-6), sp.MX_E4M3)
+    for b in (buf.codes, buf.scales, sums):
+        assert bool((b[:2] == 9).all()) and bool((b[7:] == 9).all())
+
+
+def test_past_four_gigabytes(gpu):
+    """Rows whose offsets pass 32 bits, in and out: the last ones are right."""
+    n, k, o = 1100000, 64, 2080
+    x = torch.full((n, 2048), 0.5, dtype=torch.bfloat16, device=gpu)  # 4.5 GB
+    x[-3:] = features(3, 2048, torch.bfloat16, 1).to(gpu)
+    t, q = sp.add_norm_mx(x, x, sum=x)
+    assert bool((t[:-3] == 1).all())
+    tail = sp.MxTensor(q.codes[-3:], q.scales[-3:], 2048, sp.MX_E4M3)
+    near(tail, *norm64(t[-3:].double(), sp.NORM_RMS, None, None, 1e-6), sp.MX_E4M3)
+    assert bool((q.codes[:-3] == q.codes[0]).all()) and bool((q.scales[:-3] == q.scales[0]).all())
+    q = sp.mx_quantize(x, sp.MX_E2M1)
+    want = sp.mx_quantize(x[-5:].contiguous(), sp.MX_E2M1)
+    assert torch.equal(q.codes[-5:], want.codes) and torch.equal(q.scales[-5:], want.scales)
+    assert torch.equal(sp.mx_dequantize(q)[-5:], sp.mx_dequantize(want))
+    del x, t, q, tail
+    x = mx(*small_ints(4, k, sp.MX_E2M1, 1, 0, 0), k, sp.MX_E2M1, gpu)
+    big = sp.MxTensor(x.codes.repeat(n // 4, 1), x.scales.repeat(n // 4, 1), k, sp.MX_E2M1)
+    w = mx(*small_ints(o, k, sp.MX_E2M1, 2, 0, 0), k, sp.MX_E2M1, gpu)
+    y = sp.mx_linear(big, w)  # 4.6 GB
+    want = (matrix(x) @ matrix(w).T).to(torch.bfloat16)
+    assert bool((y.view(n // 4, 4, o) == want).all())
+
+
 def test_add_norm_edges(gpu):
     """Zero rows, rows whose sum overflows fp16, infinities and NaN. A NaN, or infinities alone, make the row NaN; beside one
     infinity the formula gives t / sqrt(inf) = 0 for the finite values and NaN for it, so its block alone reads as NaN."""
@@ -349,6 +388,31 @@ def test_tail(gpu, c, n, fmt):
     bare = sp.convnext_mlp_mx(h, x, None, None, w1, None, w2, None, fmt=fmt)
     ones, zeros = torch.ones(c, device=gpu), torch.zeros(4 * c, device=gpu)
     assert torch.equal(bare, sp.convnext_mlp_mx(h, x, ones, zeros[:c].contiguous(), w1, zeros, w2, zeros[:c].contiguous(), fmt=fmt))
+
+
+@pytest.mark.parametrize("c,n", [(128, 131), (256, 129), (256, 65 * 7 + 1), (512, 140)])
+def test_tail_writes_its_rows_only(gpu, c, n):
+    a = tail(n, c, torch.bfloat16, c, gpu)
+    buf = torch.full((n + 8, c), 7.0, dtype=torch.bfloat16, device=gpu)
+    y = sp.convnext_mlp_mx(*a, out=buf[4:n + 4])
+    assert torch.equal(y, sp.convnext_mlp_mx(*a)) and bool((buf[:4] == 7).all()) and bool((buf[n + 4:] == 7).all())
+
+
+@pytest.mark.parametrize("c,n", [(128, 200), (256, 300), (512, 300)])
+def test_tail_not_finite(gpu, c, n):
+    """A row of h with an infinity or NaN gives a NaN row, an infinite x passes through, no other row changes."""
+    a = list(tail(n, c, torch.float16, c, gpu))
+    want = sp.convnext_mlp_mx(*a)
+    a[0], a[1] = a[0].clone(), a[1].clone()
+    a[0][5, 3] = float("nan")
+    a[0][70, c - 1] = float("inf")
+    a[1][9, 0] = float("inf")
+    y = sp.convnext_mlp_mx(*a)
+    assert bool(y[5].isnan().all()) and bool(y[70].isnan().all()) and float(y[9, 0]) == float("inf")
+    same = torch.ones((n, c), dtype=torch.bool, device=gpu)
+    same[5] = same[70] = False
+    same[9, 0] = False
+    assert torch.equal(y[same], want[same])
 
 
 def test_block(gpu):

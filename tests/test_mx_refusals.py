@@ -94,6 +94,8 @@ def test_linear():
     refused(call(xs=None, xdt=2, y=A), "overlap")
     refused(call(xs=None, xdt=2, n=1000, work=9 * A, nwork=1), "workspace of 1 bytes")
     refused(call(xs=None, xdt=2, n=1000, y=16 * A, work=9 * A + 8, nwork=1 << 30), "16-byte aligned")
+    refused(call(xs=None, xdt=2, n=1000, y=16 * A, work=16 * A, nwork=1 << 30), "overlap the workspace")
+    refused(call(xs=None, xdt=2, n=1000, x=20 * A, y=16 * A, work=20 * A, nwork=1 << 30), "overlap the workspace")
     assert call(n=0, x=None, xs=None, y=None) == 0
 
 
@@ -113,6 +115,7 @@ def test_tail():
     refused(call(g=7 * A), "overlap")
     refused(call(h=None), "null")
     refused(call(work=9 * A, nwork=16), "workspace of 16 bytes")
+    refused(call(work=7 * A, nwork=1 << 30), "overlap the workspace")
     assert call(n=0) == 0
 
 

@@ -231,7 +231,7 @@ inline i64 mx_rows_bytes(int fmt, i64 n, i64 cols) {
 }
 
 inline void mx_apart(const void* a, size_t na, const void* b, size_t nb, const char* what) {
-  REQ(!mx_overlap(a, na, b, nb), "out must not overlap %s", what);
+  REQ(!mx_overlap(a, na, b, nb), "operands must not overlap %s", what);
 }
 inline void mx_out_apart(const Tensor* y, const MxTensor* yq, const Tensor& t, const char* what) {
   if (y) mx_apart(y->p, y->bytes(), t.p, t.bytes(), what);

@@ -655,7 +655,14 @@ void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias
   for (const Tensor* t : {&w.codes, &w.scales}) mx_out_apart(y, yq, *t, "w");
   if (bias) mx_out_apart(y, yq, *bias, "bias");
   if (n == 0) return;
-  MxWorkspace ws(workspace, workspace_bytes, mx_linear_workspace(n, K, x_fmt));
+  const i64 need = mx_linear_workspace(n, K, x_fmt);
+  if (workspace) {
+    const Tensor room = borrow(workspace, {need}, U8);
+    mx_out_apart(y, yq, room, "the workspace");
+    for (const Tensor* t : {&x, &w.codes, &w.scales, bias, residual})
+      if (t) mx_apart(t->p, t->bytes(), room.p, room.bytes(), "the workspace");
+  }
+  MxWorkspace ws(workspace, workspace_bytes, need);
   if (n <= kValueRows) {
     MxTensor q;
     q.fmt = x_fmt;

@@ -135,11 +135,16 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr())
 
 
+_stream = None  # what set_stream was last given
+
+
 def set_stream(stream=None) -> None:
     """Run later calls on a torch.cuda.Stream (None = torch's current stream)."""
+    global _stream
     torch = _torch()
     s = torch.cuda.current_stream() if stream is None else stream
     _check(load_library().spc_set_stream(ctypes.c_void_p(s.cuda_stream)))
+    _stream = s
 
 
 class SpConvCache:
@@ -486,6 +491,15 @@ def _workspace_bytes(name, *sizes):
     return n.value
 
 
+def _workspace(nbytes, like):
+    """A call's workspace beside the tensor `like`. It is let go when the call returns: torch must not hand it to work on its
+    own stream before the library's is done with it."""
+    ws = like.new_empty(nbytes, dtype=_torch().uint8)
+    if _stream is not None:
+        ws.record_stream(_stream)
+    return ws
+
+
 def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt: int = MX_E4M3, out_dtype=None, out_fmt=None,
               out=None):
     """act(x w^T + bias) + residual with fp32 sums: w an MxTensor [Co, K] of format MX_E2M1 (mx_quantize of a torch Linear's
@@ -524,7 +538,7 @@ def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt
         y, ys, ot = out, None, _dt(out)
     ws, nws = None, 0 if quantized else _workspace_bytes("spc_mx_linear_workspace", N, K, fmt)
     if nws:
-        ws = torch.empty(nws, dtype=torch.uint8, device=xv.device)
+        ws = _workspace(nws, xv)
     dev = torch.cuda.current_device()
     _check(load_library().spc_mx_linear(
         _adr(xv, dev), _adr(xs, dev), xdt, fmt, _adr(w.codes, dev), _adr(w.scales, dev), _adr(bias, dev),
@@ -554,7 +568,7 @@ def convnext_mlp_mx(h, x, gamma, beta, w1: MxTensor, b1, w2: MxTensor, b2, eps: 
     else:
         _matrix(out, "out", shape, h.dtype)
     nws = _workspace_bytes("spc_convnext_mlp_mx_workspace", N, C, fmt)
-    ws = torch.empty(nws, dtype=torch.uint8, device=h.device) if nws else None
+    ws = _workspace(nws, h) if nws else None
     dev = torch.cuda.current_device()
     _check(load_library().spc_convnext_mlp_mx(
         _adr(h, dev), _adr(x, dev), _adr(gamma, dev), _adr(beta, dev), eps, _adr(w1.codes, dev), _adr(w1.scales, dev),
