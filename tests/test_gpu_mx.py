@@ -315,6 +315,46 @@ def test_linear_of_values(gpu, n, k, o, fmt, dt):
             near(got, ref, roff, ofmt)
 
 
+@pytest.mark.parametrize("n,k,o", [(5, 160, 288), (77, 1024, 96), (300, 1024, 1024), (1803, 1024, 544), (2500, 128, 4096), (7001, 224, 2080)])
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+def test_linear_microscaled_bits(gpu, n, k, o, fmt):
+    """Of exact sums (test_linear_bits) the epilogue's quantisation is mx_quantize's, and rows behind the last stay."""
+    x = mx(*small_ints(n, k, fmt, n + k, -8, 8), k, fmt, gpu)
+    w = mx(*small_ints(o, k, sp.MX_E2M1, o + k, 0, 0), k, sp.MX_E2M1, gpu)
+    bias = torch.randint(-64, 65, (o,), generator=gen(o)).float().to(gpu)
+    exact = (matrix(x) @ matrix(w).T + bias.double()).float()
+    for ofmt in (sp.MX_E4M3, sp.MX_E2M1):
+        want = sp.mx_quantize(exact, ofmt)
+        buf = sp.MxTensor.empty(n + 2, o, ofmt, gpu)
+        buf.codes.fill_(9)
+        buf.scales.fill_(9)
+        out = sp.MxTensor(buf.codes[:n], buf.scales[:n], o, ofmt)
+        assert sp.mx_linear(x, w, bias, out=out) is out
+        # (zeros keep a sign that the sum of opposite terms need not share)
+        assert torch.equal(out.scales, want.scales)
+        assert torch.equal(sp.mx_dequantize(out, torch.float32), sp.mx_dequantize(want, torch.float32))
+        assert bool((buf.codes[n:] == 9).all()) and bool((buf.scales[n:] == 9).all())
+
+
+@pytest.mark.parametrize("n,o", [(300, 96), (2500, 4096), (7001, 2080)])
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+def test_linear_not_finite_in_tiles(gpu, n, o, fmt):
+    """A row with a NaN block and a channel with one are NaN throughout in each size of tile; the rest is as without them."""
+    x = mx(*small_ints(n, 160, fmt, n, -8, 8), 160, fmt, gpu)
+    w = mx(*small_ints(o, 160, sp.MX_E2M1, o, 0, 0), 160, sp.MX_E2M1, gpu)
+    for kw in ({"out_dtype": torch.float32}, {"out_dtype": torch.float16}):
+        x.scales[n - 2, 3] = w.scales[33, 4] = 127
+        want = sp.mx_linear(x, w, **kw)
+        want[n - 2], want[:, 33] = float("nan"), float("nan")
+        x.scales[n - 2, 3] = w.scales[33, 4] = 255
+        assert torch.equal(sp.mx_linear(x, w, **kw).nan_to_num(1e4), want.nan_to_num(1e4))
+    got = sp.mx_dequantize(sp.mx_linear(x, w, out_fmt=sp.MX_E4M3), torch.float32).isnan()
+    blocks = torch.zeros((n, o), dtype=torch.bool, device=gpu)
+    blocks[n - 2] = True
+    blocks[:, 32:64] = True  # a block with a NaN reads as NaN
+    assert torch.equal(got, blocks)
+
+
 def test_linear_not_finite(gpu):
     """A row with an infinity or NaN is NaN throughout; a weight row whose block is NaN is a NaN channel; nothing else is."""
     x = features(70, 256, torch.bfloat16, 5)
@@ -482,6 +522,26 @@ def test_other_stream(gpu):
     finally:
         sp.set_stream(torch.cuda.current_stream())
     assert torch.equal(got, want)
+
+
+def test_library_on_another_stream_than_torch(gpu):
+    """Workspaces follow the library's stream, not torch's: work on torch's own meanwhile does not reach them."""
+    x = features(4000, 1024, torch.bfloat16, 3).to(gpu)
+    w = sp.mx_quantize(features(1024, 1024, torch.float32, 4).to(gpu), sp.MX_E2M1)
+    want = sp.mx_linear(x, w)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    outs, junk = [], []
+    try:
+        sp.set_stream(s)
+        for _ in range(8):
+            outs.append(sp.mx_linear(x, w, out=torch.empty_like(want)))
+            junk.append(torch.full((4000, 1056), 255, dtype=torch.uint8, device=gpu))  # on torch's stream
+        s.synchronize()
+    finally:
+        sp.set_stream(torch.cuda.current_stream())
+    for got in outs:
+        assert torch.equal(got, want)
 
 
 def test_refusals(gpu):

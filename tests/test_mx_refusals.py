@@ -26,6 +26,7 @@ def test_sizes():
         assert lib.spc_mx_sizes(rows, cols, fmt, ctypes.byref(c), ctypes.byref(s)) == 0 and (c.value, s.value) == want
     refused(lib.spc_mx_sizes(3, 33, 1, None, None), "cols=33")
     refused(lib.spc_mx_sizes(3, 32, 4, None, None), "format 4")
+    refused(lib.spc_mx_sizes(1 << 31, 32, 1, None, None), "rows=2147483648")
     n = ctypes.c_int64()
     assert lib.spc_mx_linear_workspace(100, 64, 2, ctypes.byref(n)) == 0 and n.value >= 100 * 32 + 100 * 16
     assert lib.spc_convnext_mlp_mx_workspace(10, 64, 1, ctypes.byref(n)) == 0 and n.value >= 10 * (64 + 256) + 20 * 16

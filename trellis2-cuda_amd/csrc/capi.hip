@@ -403,8 +403,8 @@ MxTensor mx_rows(const void* codes, const void* scales, int fmt, i64 rows, i64 c
 
 SPC_API int spc_mx_sizes(int64_t rows, int64_t cols, int fmt, int64_t* code_bytes, int64_t* scale_bytes) {
   return guarded([&] {
-    REQ(rows >= 0 && cols > 0 && cols % 32 == 0 && (fmt == SPC_MX_E4M3 || fmt == SPC_MX_E2M1), "rows=%lld cols=%lld format %d",
-        (long long)rows, (long long)cols, fmt);
+    REQ(rows >= 0 && rows < (1ll << 31) && cols > 0 && cols % 32 == 0 && cols <= (1 << 20) && (fmt == SPC_MX_E4M3 || fmt == SPC_MX_E2M1),
+        "rows=%lld cols=%lld format %d", (long long)rows, (long long)cols, fmt);
     if (code_bytes) *code_bytes = rows * mx_row_bytes(fmt, cols);
     if (scale_bytes) *scale_bytes = rows * mx_scale_bytes(cols);
   });
@@ -438,7 +438,7 @@ SPC_API int spc_add_norm_mx(const void* x, const void* residual, const void* gam
 
 SPC_API int spc_mx_linear_workspace(int64_t N, int64_t K, int x_fmt, int64_t* bytes) {
   return guarded([&] {
-    REQ(bytes && N >= 0 && K > 0 && (x_fmt == SPC_MX_E4M3 || x_fmt == SPC_MX_E2M1), "arguments");
+    REQ(bytes && N >= 0 && N < (1ll << 31) && K > 0 && K <= (1 << 20) && (x_fmt == SPC_MX_E4M3 || x_fmt == SPC_MX_E2M1), "arguments");
     *bytes = mx_linear_workspace(N, K, x_fmt);
   });
 }
@@ -469,7 +469,7 @@ SPC_API int spc_mx_linear(const void* x, const void* x_scales, int x_dtype, int 
 
 SPC_API int spc_convnext_mlp_mx_workspace(int64_t N, int64_t C, int fmt, int64_t* bytes) {
   return guarded([&] {
-    REQ(bytes && N >= 0 && C > 0 && (fmt == SPC_MX_E4M3 || fmt == SPC_MX_E2M1), "arguments");
+    REQ(bytes && N >= 0 && N < (1ll << 31) && C > 0 && C <= 4096 && (fmt == SPC_MX_E4M3 || fmt == SPC_MX_E2M1), "arguments");
     *bytes = convnext_mlp_mx_workspace(N, C, fmt);
   });
 }

@@ -492,12 +492,14 @@ def _workspace_bytes(name, *sizes):
 
 
 def _workspace(nbytes, like):
-    """A call's workspace beside the tensor `like`. It is let go when the call returns: torch must not hand it to work on its
-    own stream before the library's is done with it."""
-    ws = like.new_empty(nbytes, dtype=_torch().uint8)
-    if _stream is not None:
-        ws.record_stream(_stream)
-    return ws
+    """A call's workspace beside the tensor `like`. It is let go when the call returns, so it is taken on the library's stream:
+    torch hands it on only to work behind the call's, and never while earlier work on it is under way."""
+    torch = _torch()
+    lib = torch.cuda.default_stream() if _stream is None else _stream
+    if torch.cuda.current_stream() == lib:
+        return like.new_empty(nbytes, dtype=torch.uint8)
+    with torch.cuda.stream(lib):
+        return like.new_empty(nbytes, dtype=torch.uint8)
 
 
 def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt: int = MX_E4M3, out_dtype=None, out_fmt=None,
