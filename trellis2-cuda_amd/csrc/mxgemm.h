@@ -60,7 +60,10 @@ __device__ __forceinline__ uint32_t e4m3_large(uint32_t v) {
   return v & __builtin_amdgcn_perm(t, t << 8, 0x0b090a08u);
 }
 // Epilogue of NV consecutive channels o .. of row n in v: bias, activation, residual (its words in r), store. Lanes l, l + 16, l + 32, l + 48
-// hold neighbouring runs of one row; ok is the same for all lanes of a block of 32 channels.
+// hold neighbouring runs of one row; ok is the same for all lanes of a block of 32 channels. Runs of 64 bytes of a row are
+// stored past the caches, which keep the operands ([8209, 2080] by [4128, 2080] 102 -> 94 us, [11467, 2048] by [512, 2048]
+// 20.9 -> 20.2; fp32 level). Runs of 32 bytes are not (tail of 391007 rows, 128 channels: 193 us, 203 past the caches), nor are
+// microscaled rows, which the next product reads at once (tail of 11467 rows, 512 channels: 63 us, 69 past the caches).
 template <int OUT, int NV>
 __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v)[NV], const float (&bias)[NV],
                                        const uint32_t (&r)[4], bool ok) {
@@ -92,7 +95,7 @@ __device__ __forceinline__ void finish(const LinArgs& a, i64 n, int o, float (&v
 #pragma unroll
     for (int j = 0; j < NV / 2; j++) q[j] = a.f16 ? mx_pack2<true>(v[2 * j], v[2 * j + 1]) : mx_pack2<false>(v[2 * j], v[2 * j + 1]);
     uint32_t* y = (uint32_t*)((uint16_t*)a.out + n * a.O + o);
-    if constexpr (NV == 8) *(mx_u32x4*)y = *(mx_u32x4*)q;
+    if constexpr (NV == 8) __builtin_nontemporal_store(*(mx_u32x4*)q, (mx_u32x4*)y);
     else *(mx_u32x2*)y = *(mx_u32x2*)q;
   } else {
     static_assert(NV == 16 || NV == 8, "a half or a quarter of a block");

@@ -24,6 +24,10 @@ struct TailArgs {
 // is two lane exchanges away), SiLU, quantises them into LDS, and after a barrier multiplies all 256 into its C / 8
 // channels of y. The weights go from L2 straight into registers, each to the one wavefront that needs it, read while
 // the other product runs. Two slots of hidden units make it one barrier a round.
+// us, this kernel / three passes (the 16-bit tail): [58321, 256] 80 / 104 (112), [15000, 256] 27 (40), [391007, 128] 193 (202). 61 GFLOP at
+// the first size: about 20 us are norm, residual and stores, 27 the two products, 12 waits for weights, 6 SiLU and quantisation,
+// which follow each other in every wavefront. At 512 channels the sums of y leave room for 32 rows only, and each workgroup
+// reads all weights for them: [11467, 512] 84 us with 8 wavefronts, 128 with 4, against 63 in three passes.
 constexpr int kTailRows = 64;  // rows of a workgroup
 template <bool F16, int C>
 __global__ void __launch_bounds__(512, 4) k_mx_tail(TailArgs a) {

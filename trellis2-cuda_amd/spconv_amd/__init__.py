@@ -396,8 +396,8 @@ def _new_rows(like, rows, cols, fmt):
         raise ValueError(f"{cols} columns: a positive multiple of 32")
     u8 = _torch().uint8
     q = MxTensor.__new__(MxTensor)
-    q.codes = like.new_empty((rows, cols >> 1 if fmt == MX_E2M1 else cols), dtype=u8)
-    q.scales = like.new_empty((rows, (cols + 511) // 512 * 16), dtype=u8)
+    q.codes = like.new_empty(rows, cols >> 1 if fmt == MX_E2M1 else cols, dtype=u8)
+    q.scales = like.new_empty(rows, (cols + 511) // 512 * 16, dtype=u8)
     q.fmt, q.shape = fmt, (rows, cols)
     return q
 
@@ -446,7 +446,7 @@ def mx_dequantize(q: MxTensor, dtype=None, out=None):
     torch = _torch()
     N, K = q.shape
     if out is None:
-        out = q.codes.new_empty((N, K), dtype=dtype or torch.bfloat16)
+        out = q.codes.new_empty(N, K, dtype=dtype or torch.bfloat16)
     else:
         _matrix(out, "out", q.shape, dtype)
     dev = torch.cuda.current_device()
@@ -532,7 +532,7 @@ def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt
         y, ys, ot = out.codes, out.scales, out.fmt
     else:
         if out is None:
-            out = xv.new_empty((N, Co), dtype=out_dtype or (torch.bfloat16 if quantized else x.dtype))
+            out = xv.new_empty(N, Co, dtype=out_dtype or (torch.bfloat16 if quantized else x.dtype))
         else:
             _matrix(out, "out", (N, Co), out_dtype)
         if residual is not None:
