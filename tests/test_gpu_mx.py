@@ -507,6 +507,37 @@ def test_graph_replays(gpu):
         assert torch.equal(sp.convnext_mlp_mx(*a), want[0])
 
 
+def test_captured_call_without_a_workspace(gpu):
+    """The C entries' own workspace is not for a graph: refused before anything is recorded, and the capture goes on."""
+    lib, P = sp.load_library(), lambda t: t.data_ptr()
+    x = features(40, 64, torch.float16, 3).to(gpu)
+    w = sp.mx_quantize(features(32, 64, torch.float32, 4).to(gpu), sp.MX_E2M1)
+    y = torch.empty((40, 32), dtype=torch.float16, device=gpu)
+
+    def call():
+        return lib.spc_mx_linear(P(x), None, sp.F16, sp.MX_E4M3, P(w.codes), P(w.scales), None, 0, None, 0, 40, 64, 32, sp.F16, P(y),
+                                 None, None, 0)
+
+    assert call() == 0
+    want = y.clone()
+    assert torch.equal(want, sp.mx_linear(x, w))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, stream=s):
+            sp.set_stream(torch.cuda.current_stream())
+            y.fill_(2.0)
+            rc = call()
+    finally:
+        torch.cuda.synchronize()
+        sp.set_stream(torch.cuda.current_stream())
+    assert rc == -1 and "workspace" in lib.spc_last_error().decode()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((y == 2).all()) and call() == 0 and torch.equal(y, want)
+
+
 def test_other_stream(gpu):
     """Calls on a stream that the library was given, ordered after work on it."""
     x = features(300, 256, torch.bfloat16, 3).to(gpu)
