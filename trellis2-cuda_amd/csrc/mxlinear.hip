@@ -34,7 +34,7 @@ constexpr int run_tiles() {  // G above
 // each wavefront takes a contiguous eighth of K, both operands straight into registers, and the eight sums meet in
 // LDS in a fixed order. XT: x's type (fp32, fp16, bf16), quantised here by every workgroup for itself, which costs less
 // than a launch of its own (NT = 1); or -1: x's codes.
-// Bound by the latency of the weights: [1, 4096] by [4096, 4096] (8.9 MB) 7.9 us a call, 2 of them at the copy rate;
+// Bound by the latency of the weights: [1, 4096] by [4096, 4096] (8.9 MB) 7.2 us, 2 of them at the copy rate;
 // [77, 4096] by [8192, 4096] (17.8 MB) 15.5 us, where each wavefront also reads all rows of X for 32 channels.
 template <int XB, int OUT, int XT, int OT, int NT>
 __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
@@ -230,9 +230,9 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
 // middle all wavefronts meet: by then each has read the whole slot, so it is filled again at once. One barrier a stage,
 // and NS - 1/2 stages for a DMA to land.
 //
-// Measured: [16411, 4096] by [4096, 4096], 551 GFLOP, e4m3 245 us quantisation included (2.2 PFLOP/s); e2m1
-// 237. The DMA path bounds both (35 to 43 KB/us into a CU while products run; 125 alone, in segments of 128 bytes: the
-// reason for two steps a stage where a step of e2m1 has 64), and the epilogue's stores are not hidden behind another tile.
+// Measured: [16411, 4096] by [4096, 4096] with a residual, 551 GFLOP, e2m1 235 us (2.3 PFLOP/s), e4m3 272. The DMA path bounds
+// both (44 KB/us into a CU beside the products of e4m3, 53 of e2m1; alone 60 to 80 in segments of 64 bytes and 125 of 128, the
+// reason for two steps of e2m1 a stage at 128 x 128), then the residual and the stores, which add their time at the copy rate.
 //
 // SPLIT (e4m3): the matrix unit adds eight neighbouring products at a time and drops what is below 2^-13 of the largest.
 // An output of 16 bits does not show it. Where the result keeps more (fp32) or is quantised again (an error that moves a
@@ -567,9 +567,9 @@ void gemm(const LinArgs& a, int xt) {
   if (a.N <= kFewRows) return launch_rows<XB, OUT, -1, 5>(a);
   // Larger tiles read fewer operand bytes per product, smaller ones are more. Two workgroups of 256 channels by 128 rows fit a
   // CU: they are taken where they fill most of these slots; 128 by 64 where 128 by 128 would leave a quarter of them free.
-  // us at 256 x 128 / 128 x 128 / 128 x 64, [N, K, O]: e4m3 [16411, 4096, 4096] 278 / 314 / -, [8209, 2080, 4128] 102 / 108 / -,
-  // [58321, 1024, 256] 32 / 34 / -, [2048, 4096, 4096] 45 / 42 / 52, [1803, 4096, 1024] 41 / 27 / 19, [11467, 2048, 512] 29 / 24 / 22,
-  // [300, 1024, 1024] - / 13 / 9; e2m1 [16411, 4096, 4096] 237 / 250 / -, [600, 2048, 2048] - / 14 / 11.
+  // us at 256 x 128 / 128 x 128 / 128 x 64, [N, K, O]: e4m3 [16411, 4096, 4096] 272 / 314 / 365, [8209, 2080, 4128] 94 / 103 / 114,
+  // [58321, 1024, 256] 29 / 32 / 32, [2048, 4096, 4096] 44 / 41 / 46, [1803, 4096, 1024] 41 / 26 / 18, [11467, 2048, 512] 28 / 23 / 21,
+  // [300, 1024, 1024] 20 / 12 / 9; e2m1 [16411, 4096, 4096] 236 / 242 / 306, [600, 2048, 2048] 23 / 15 / 12.
   const i64 n128 = cdiv(a.N, 128), cus = mx_device_cus();
   if (n128 * cdiv(a.O, 256) * 2 >= 3 * cus) launch<XB, OUT, 8, 4, 2, 2, 1, XB == 8 ? 2 : 3>(a);
   else if (n128 * cdiv(a.O, 128) * 2 > 3 * cus) launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
