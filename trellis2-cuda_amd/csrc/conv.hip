@@ -1811,7 +1811,8 @@ __global__ void __launch_bounds__(256, 1) k_conv_w256(ConvArgs a) {
     };
     auto dma = [&](int slot, int k) __attribute__((always_inline)) {
       const uint32_t m0 = __builtin_amdgcn_readfirstlane(dma_lds + (uint32_t)slot * (SU * 16) + (uint32_t)k * 1024u);
-      asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+      // (one wait state between the scalar write of M0 and the load that reads it: the compiler inserts none in here)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                    :: "s"(m0), "v"(off[k]), "s"(rx), "s"(ka) : "memory", "m0");
     };
     u32x4 rb[2][4];  // weights of the stage being computed: column block t, K step j

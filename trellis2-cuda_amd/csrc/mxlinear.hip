@@ -10,9 +10,10 @@ __device__ __forceinline__ i32x4 rsrc4(const void* p, uint32_t bytes) {  // a ra
                (int32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000};
 }
 // 16 bytes per lane, global -> LDS: lane l's land at dst + 16 l. Inline assembly, so that the compiler does not put a
-// wait for it before every LDS read; the loop below counts them.
+// wait for it before every LDS read; the loop below counts them. M0 (dst) needs one wait state between its scalar write
+// and the load that reads it, which the compiler does not insert in here.
 __device__ __forceinline__ void dma16(i32x4 r, uint32_t lds, uint32_t off, int soff) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                ::"s"(lds), "v"(off), "s"(r), "s"(soff) : "memory", "m0");
 }
 template <int N>
