@@ -120,6 +120,20 @@ def test_tail():
     assert call(n=0) == 0
 
 
+@pytest.mark.parametrize("operand", range(8))
+def test_tail_workspace_apart_from_weights_and_parameters(operand):
+    """The three-pass tail writes its workspace while it still reads these."""
+    lib, room = sp.load_library(), 1 << 24
+    work = 16 * room
+    for at in (work, work + 512):  # the same address, and one inside (200 rows of 64 and 256 columns take 64 KB and more)
+        # gamma, beta, w1, s1, b1, w2, s2, b2
+        ops = [(k + 1) * room for k in range(8)]
+        ops[operand] = at
+        g, b, w1, s1, b1, w2, s2, b2 = (p(v) for v in ops)
+        refused(lib.spc_convnext_mlp_mx(p(9 * room), p(10 * room), g, b, 1e-6, w1, s1, b1, w2, s2, b2, 2, 0, 1, 200, 64, p(11 * room),
+                                        p(work), room), "overlap the workspace")
+
+
 def test_binding():
     x = torch.zeros((4, 64), dtype=torch.bfloat16)
     for call in (lambda: sp.mx_quantize(x[0]),

@@ -289,7 +289,8 @@ void convnext_mlp_mx(const Tensor& h, const Tensor& x, const Tensor* gamma, cons
   }
   const i64 step = tail_rows(n, C, fmt);
   if (workspace)
-    for (const Tensor* t : {&h, &x, (const Tensor*)&y}) mx_apart(t->p, t->bytes(), workspace, (size_t)convnext_mlp_mx_workspace(n, C, fmt), "the workspace");
+    for (const Tensor* t : {&h, &x, (const Tensor*)&y, &w1.codes, &w1.scales, &w2.codes, &w2.scales, gamma, beta, b1, b2})
+      if (t) mx_apart(t->p, t->bytes(), workspace, (size_t)convnext_mlp_mx_workspace(n, C, fmt), "the workspace");
   MxWorkspace ws(workspace, workspace_bytes, convnext_mlp_mx_workspace(n, C, fmt));
   const MxTensor a = ws.rows(fmt, step, C), hid = ws.rows(fmt, step, 4 * C);
   auto first = [](const MxTensor& q, i64 m) {
