@@ -134,6 +134,16 @@ def test_tail_workspace_apart_from_weights_and_parameters(operand):
                                         p(work), room), "overlap the workspace")
 
 
+@pytest.mark.parametrize("scales", [2 * A, 2 * A + 64, 2 * A - 16])
+def test_codes_and_scales_apart(scales):
+    """A call that writes both refuses buffers that share a byte (4 rows of 64 columns: 256 bytes of codes, 64 of scales)."""
+    lib, c, s = sp.load_library(), p(2 * A), p(scales)
+    refused(lib.spc_mx_quantize(p(A), 2, 4, 64, 1, c, s), "codes and scales must not overlap")
+    refused(lib.spc_add_norm_mx(p(A), None, None, None, 0, 1e-6, 0, 2, 4, 64, 1, None, c, s), "codes and scales must not overlap")
+    refused(lib.spc_mx_linear(p(4 * A), p(5 * A), 0, 1, p(6 * A), p(7 * A), None, 0, None, 0, 4, 64, 64, 1, c, s, None, 0),
+            "codes and scales must not overlap")
+
+
 def test_binding():
     x = torch.zeros((4, 64), dtype=torch.bfloat16)
     for call in (lambda: sp.mx_quantize(x[0]),

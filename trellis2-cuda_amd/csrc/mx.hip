@@ -29,6 +29,10 @@ void mx_check(const MxTensor& q, const char* what) {
   REQ(q.rows == 0 || (q.codes.p && q.scales.p), "%s: null codes or scales", what);
   REQ(((uintptr_t)q.codes.p | (uintptr_t)q.scales.p) % 16 == 0, "%s: codes and scales must be 16-byte aligned", what);
 }
+void mx_check_out(const MxTensor& q, const char* what) {
+  mx_check(q, what);
+  REQ(!mx_overlap(q.codes.p, q.codes.bytes(), q.scales.p, q.scales.bytes()), "%s: codes and scales must not overlap", what);
+}
 
 namespace {
 // 8 consecutive values of unit u
@@ -154,7 +158,7 @@ bool is_float(DT dt) { return dt == F32 || dt == F16 || dt == BF16; }
 }  // namespace
 
 void mx_quantize(const Tensor& x, MxTensor& q) {
-  mx_check(q, "q");
+  mx_check_out(q, "q");
   REQ(is_float(x.dt) && x.dim() == 2 && x.size(0) == q.rows && x.size(1) == q.cols, "x must be fp32/fp16/bf16 [%lld,%lld]",
       (long long)q.rows, (long long)q.cols);
   REQ((uintptr_t)x.p % 16 == 0 && (x.p || q.rows == 0), "x must be 16-byte aligned and not null");
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
 
 void add_norm_mx(const Tensor& x, const Tensor* residual, const Tensor* gamma, const Tensor* beta, float eps, int kind,
                  Tensor* sum, MxTensor& q) {
-  mx_check(q, "q");
+  mx_check_out(q, "q");
   REQ(x.dim() == 2 && (x.dt == BF16 || x.dt == F16), "x must be bf16/fp16 [N,C]");
   const i64 n = x.size(0), C = x.size(1);
   REQ(C > 0 && C % 32 == 0 && C <= 16384, "C=%lld: a multiple of 32, at most 16384", (long long)C);
