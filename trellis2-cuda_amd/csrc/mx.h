@@ -184,7 +184,7 @@ __device__ __forceinline__ void mx_unroll(F&& f) {
 
 // Host side, shared by the operators: argument checks
 void mx_check(const MxTensor& q, const char* what);
-void mx_check_out(const MxTensor& q, const char* what);  // and that codes and scales, both written, share no byte
+void mx_check_apart(const MxTensor& q, const char* what);  // of a result: codes and scales share no byte
 // Whether [a, a + na) and [b, b + nb) share a byte
 inline bool mx_overlap(const void* a, size_t na, const void* b, size_t nb) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;

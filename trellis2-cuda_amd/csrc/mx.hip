@@ -29,8 +29,7 @@ void mx_check(const MxTensor& q, const char* what) {
   REQ(q.rows == 0 || (q.codes.p && q.scales.p), "%s: null codes or scales", what);
   REQ(((uintptr_t)q.codes.p | (uintptr_t)q.scales.p) % 16 == 0, "%s: codes and scales must be 16-byte aligned", what);
 }
-void mx_check_out(const MxTensor& q, const char* what) {
-  mx_check(q, what);
+void mx_check_apart(const MxTensor& q, const char* what) {
   REQ(!mx_overlap(q.codes.p, q.codes.bytes(), q.scales.p, q.scales.bytes()), "%s: codes and scales must not overlap", what);
 }
 
@@ -158,7 +157,8 @@ bool is_float(DT dt) { return dt == F32 || dt == F16 || dt == BF16; }
 }  // namespace
 
 void mx_quantize(const Tensor& x, MxTensor& q) {
-  mx_check_out(q, "q");
+  mx_check(q, "q");
+  mx_check_apart(q, "q");
   REQ(is_float(x.dt) && x.dim() == 2 && x.size(0) == q.rows && x.size(1) == q.cols, "x must be fp32/fp16/bf16 [%lld,%lld]",
       (long long)q.rows, (long long)q.cols);
   REQ((uintptr_t)x.p % 16 == 0 && (x.p || q.rows == 0), "x must be 16-byte aligned and not null");
@@ -294,11 +294,12 @@ __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
 
 void add_norm_mx(const Tensor& x, const Tensor* residual, const Tensor* gamma, const Tensor* beta, float eps, int kind,
                  Tensor* sum, MxTensor& q) {
-  mx_check_out(q, "q");
+  mx_check(q, "q");
   REQ(x.dim() == 2 && (x.dt == BF16 || x.dt == F16), "x must be bf16/fp16 [N,C]");
   const i64 n = x.size(0), C = x.size(1);
   REQ(C > 0 && C % 32 == 0 && C <= 16384, "C=%lld: a multiple of 32, at most 16384", (long long)C);
   REQ(q.rows == n && q.cols == C, "q must be [%lld,%lld]", (long long)n, (long long)C);
+  mx_check_apart(q, "q");
   REQ(kind == MX_NORM_RMS || kind == MX_NORM_LAYER, "kind=%d", kind);
   if (residual) REQ(residual->dt == x.dt && residual->dim() == 2 && residual->size(0) == n && residual->size(1) == C, "residual must match x");
   if (sum) REQ(sum->dt == x.dt && sum->dim() == 2 && sum->size(0) == n && sum->size(1) == C, "sum must match x");

@@ -634,7 +634,8 @@ void check_linear(i64 n, i64 K, const MxTensor& w, const Tensor* bias, const Ten
       REQ(res->p == y->p || !mx_overlap(res->p, res->bytes(), y->p, y->bytes()), "out must be the residual or apart from it");
     }
   } else {
-    mx_check_out(*yq, "out");
+    mx_check(*yq, "out");
+    mx_check_apart(*yq, "out");
     REQ(yq->rows == n && yq->cols == w.rows, "out must be [%lld,%lld]", (long long)n, (long long)w.rows);
     REQ(!res, "a microscaled output takes no residual");
   }
