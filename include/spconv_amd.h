@@ -34,6 +34,8 @@ const char* spc_last_error(void);
 /* Make `hip_stream` (a hipStream_t, or NULL for the null stream) the stream every later call runs on.
  * Reference: the single global stream of src/core.cu:20-28. */
 int spc_set_stream(void* hip_stream);
+/* The stream that later calls run on (NULL: the null stream): where a caller's own allocator has to order a workspace. Host only. */
+int spc_get_stream(void** hip_stream);
 
 /* Build the hash table and 27-offset neighbour map of `coords` (int32 [n,4] = (b,x,y,z), unique rows) in a
  * W x H x D grid, plus the gray-code sorted row order.

@@ -45,6 +45,20 @@ def test_error_convention_without_gpu():
     assert spconv_amd.spconv_cfg(1000, 32, 64)[1] == 32
 
 
+def test_stream_as_set_by_any_caller():
+    """The library says which stream it has; the binding asks it, also where a C caller set the stream."""
+    lib, s = spconv_amd.load_library(), ctypes.c_void_p(1)
+    assert lib.spc_get_stream(None) == -1
+    try:
+        assert lib.spc_set_stream(ctypes.c_void_p(0x1230)) == 0  # (an address only: nothing runs here)
+        assert lib.spc_get_stream(ctypes.byref(s)) == 0 and s.value == 0x1230
+        assert spconv_amd._library_stream() == 0x1230
+    finally:
+        lib.spc_set_stream(None)
+    assert lib.spc_get_stream(ctypes.byref(s)) == 0 and s.value is None
+    assert spconv_amd._library_stream() == 0
+
+
 def test_no_oracle_in_product():
     """The product library and binding never reference the oracle."""
     pkg = os.path.join(ROOT, "trellis2-cuda_amd")

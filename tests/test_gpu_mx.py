@@ -575,6 +575,28 @@ def test_library_on_another_stream_than_torch(gpu):
         assert torch.equal(got, want)
 
 
+def test_stream_set_through_the_c_entry(gpu):
+    """As above where the stream was set behind the binding's back: workspaces still follow it."""
+    lib = sp.load_library()
+    x = features(4000, 1024, torch.bfloat16, 3).to(gpu)
+    w = sp.mx_quantize(features(1024, 1024, torch.float32, 4).to(gpu), sp.MX_E2M1)
+    want = sp.mx_linear(x, w)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    outs, junk = [torch.empty_like(want) for _ in range(8)], []
+    try:
+        assert lib.spc_set_stream(s.cuda_stream) == 0
+        assert sp._library_stream() == s.cuda_stream
+        for out in outs:
+            sp.mx_linear(x, w, out=out)
+            junk.append(torch.full((4000, 1056), 255, dtype=torch.uint8, device=gpu))  # on torch's stream
+        s.synchronize()
+    finally:
+        sp.set_stream(torch.cuda.current_stream())
+    for got in outs:
+        assert torch.equal(got, want)
+
+
 def test_refusals(gpu):
     """Calls that the binding or the library refuses before anything runs."""
     x = features(8, 64, torch.bfloat16, 1).to(gpu)

@@ -42,6 +42,13 @@ SPC_API int spc_set_stream(void* s) {
   return guarded([&] { set_stream((hipStream_t)s); });
 }
 
+SPC_API int spc_get_stream(void** s) {
+  return guarded([&] {
+    REQ(s, "hip_stream is null");
+    *s = (void*)stream();
+  });
+}
+
 SPC_API int spc_build_neighbors(const int32_t* coords, int64_t n, int W, int H, int D, spc_cache** out) {
   return guarded([&] {
     REQ(out, "out is null");

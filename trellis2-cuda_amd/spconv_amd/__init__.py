@@ -28,7 +28,7 @@ MX_E4M3, MX_E2M1 = 1, 2  # element formats of microscaled rows (MxTensor)
 NORM_RMS, NORM_LAYER = 0, 1
 
 # the C ABI's exported symbols (every declaration of include/spconv_amd.h)
-SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_build_neighbors", "spc_build_neighbors_ex", "spc_cache_lookup",
+SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_get_stream", "spc_build_neighbors", "spc_build_neighbors_ex", "spc_cache_lookup",
            "spc_fdg_quads", "spc_fdg_quads_filled", "spc_cache_free", "spc_cache_info", "spc_cache_valid", "spc_conv_cfg",
            "spc_conv_cfg_autotune", "spc_conv_cfg_autotune_strict", "spc_subm_conv", "spc_subm_conv_fused", "spc_subm_conv_gathered",
            "spc_gather_ln_act", "spc_add_skip", "spc_convnext_mlp", "spc_subm_conv_skip",
@@ -53,6 +53,7 @@ def load_library():
     PP = ctypes.POINTER(ctypes.c_void_p)
     L.spc_last_error.restype = ctypes.c_char_p
     L.spc_last_error.argtypes = []
+    L.spc_get_stream.argtypes = [ctypes.POINTER(P)]
     L.spc_set_stream.argtypes = [P]
     L.spc_build_neighbors.argtypes = [P, I64, I, I, I, PP]
     L.spc_build_neighbors_ex.argtypes = [P, I64, I, I, I, I, PP]
@@ -135,16 +136,11 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr())
 
 
-_stream = None  # what set_stream was last given
-
-
 def set_stream(stream=None) -> None:
     """Run later calls on a torch.cuda.Stream (None = torch's current stream)."""
-    global _stream
     torch = _torch()
     s = torch.cuda.current_stream() if stream is None else stream
     _check(load_library().spc_set_stream(ctypes.c_void_p(s.cuda_stream)))
-    _stream = s
 
 
 class SpConvCache:
@@ -491,14 +487,21 @@ def _workspace_bytes(name, *sizes):
     return n.value
 
 
+def _library_stream() -> int:
+    """Address of the stream that the library's calls run on (0: the null stream), whoever set it."""
+    s = ctypes.c_void_p()
+    _check(load_library().spc_get_stream(ctypes.byref(s)))
+    return s.value or 0
+
+
 def _workspace(nbytes, like):
     """A call's workspace beside the tensor `like`. It is let go when the call returns, so it is taken on the library's stream:
     torch hands it on only to work behind the call's, and never while earlier work on it is under way."""
     torch = _torch()
-    lib = torch.cuda.default_stream() if _stream is None else _stream
-    if torch.cuda.current_stream() == lib:
+    lib = _library_stream()
+    if torch.cuda.current_stream().cuda_stream == lib:
         return like.new_empty(nbytes, dtype=torch.uint8)
-    with torch.cuda.stream(lib):
+    with torch.cuda.stream(torch.cuda.ExternalStream(lib, like.device) if lib else torch.cuda.default_stream(like.device)):
         return like.new_empty(nbytes, dtype=torch.uint8)
 
 
