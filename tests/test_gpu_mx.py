@@ -181,6 +181,18 @@ def test_add_norm_writes_its_rows_only(gpu, C):
         assert bool((b[:2] == 9).all()) and bool((b[7:] == 9).all())
 
 
+@pytest.mark.parametrize("C", [32, 96, 224, 416, 480, 832, 1984, 3936, 7872, 16320])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_layer_norm_of_constant_rows(gpu, C, dt):
+    """Every value is the mean, so the norm is beta, whatever the row's size: the sums fit in 24 bits (11 of the value, at most 11 of the
+    count of eights), and their quotient by C is the value itself."""
+    v = torch.tensor([65504.0, -65504.0, 60000.0, 1000.5, -333.25, 2.0 ** -14, 0.0]).to(dt)
+    x = v[:, None].expand(-1, C).contiguous().to(gpu)
+    for beta in (None, torch.full((C,), -1.5, device=gpu)):
+        _, q = sp.add_norm_mx(x, None, torch.full((C,), 2.0, device=gpu), beta, kind=sp.NORM_LAYER)
+        assert torch.equal(sp.mx_dequantize(q, torch.float32), torch.full((len(v), C), 0.0 if beta is None else -1.5, device=gpu))
+
+
 def test_past_four_gigabytes(gpu):
     """Rows whose offsets pass 32 bits, in and out: the last ones are right."""
     n, k, o = 1100000, 64, 2080
