@@ -138,10 +138,11 @@ __device__ __forceinline__ void mx_params(const void* p, int dt, i64 i, float no
 
 // mean and 1 / sqrt(variance + eps) of a row held by LPR lanes (this one has units sub, sub + LPR, ... below `units`, zeros
 // else), or, without the mean, 1 / sqrt(mean square + eps); across: adds the lanes' sums over what LPR does not reach.
-// The mean is divided, not multiplied by 1 / c: that is off by an ulp for a third of all c, and a row of one large value, whose
-// variance is 0, then has elements of that ulp, which 1 / sqrt(their square + eps) makes as large as 1.
+// s * (1 / c) is an ulp off s / c for a third of all c; a row of one large value, whose variance is 0, then has elements of that
+// ulp, which 1 / sqrt(their square + eps) makes as large as 1. The mean gets the remainder's quotient (a division proper: [58321,
+// 256] 12.8 -> 13.6 us).
 template <int LPR, int CH, class F>
-__device__ __forceinline__ void mx_row_stats(const float (&v)[CH][8], int sub, int units, float c, float eps, bool layer,
+__device__ __forceinline__ void mx_row_stats(const float (&v)[CH][8], int sub, int units, float c, float inv_c, float eps, bool layer,
                                              float& mean, float& rstd, F&& across) {
   auto total = [&](float s) __attribute__((always_inline)) {
 #pragma unroll
@@ -156,7 +157,8 @@ __device__ __forceinline__ void mx_row_stats(const float (&v)[CH][8], int sub, i
   s = total(s);
   mean = 0.f;
   if (layer) {
-    mean = s / c;
+    mean = s * inv_c;
+    mean = fmaf(fmaf(-mean, c, s), inv_c, mean);
     s = 0.f;
 #pragma unroll
     for (int k = 0; k < CH; k++)
@@ -167,7 +169,7 @@ __device__ __forceinline__ void mx_row_stats(const float (&v)[CH][8], int sub, i
       }
     s = total(s);
   }
-  rstd = rsqrtf(s / c + eps);
+  rstd = rsqrtf(s * inv_c + eps);
 }
 __device__ __forceinline__ void mx_norm8(const float (&v)[8], float mean, float rstd, const float (&g)[8], const float (&b)[8],
                                          float (&o)[8]) {

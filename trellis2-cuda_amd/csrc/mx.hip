@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
     mx_params<8>(u < units ? a.gamma : nullptr, a.gdt, u * 8, 1.f, g[k]);
     mx_params<8>(u < units ? a.beta : nullptr, a.bdt, u * 8, 0.f, b[k]);
   }
-  const float c = (float)a.C;
+  const float c = (float)a.C, inv_c = 1.f / c;
   const i64 step = (i64)gridDim.x * RPB;
   // whole workgroups go round together (the reductions below need every lane): rows past the last repeat it
   for (i64 row0 = (i64)blockIdx.x * RPB; row0 < a.n; row0 += step) {
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(256) k_add_norm_mx(NormArgs a) {
       }
     }
     float mean, rstd;
-    mx_row_stats<LPR, CH>(v, sub, units, c, a.eps, a.kind == MX_NORM_LAYER, mean, rstd, [&](float s) __attribute__((always_inline)) {
+    mx_row_stats<LPR, CH>(v, sub, units, c, inv_c, a.eps, a.kind == MX_NORM_LAYER, mean, rstd, [&](float s) __attribute__((always_inline)) {
       if constexpr (LPR == 256) {  // two slots in turn: one is written again only past another barrier
         float* p = part[slot ^= 1];
         if ((threadIdx.x & 63) == 0) p[threadIdx.x >> 6] = s;

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(512, 4) k_mx_tail(TailArgs a) {
       float v[1][8], o[8];
       mx_unpack8<F16>(q[p], v[0]);
       float mean, rstd;
-      mx_row_stats<LPR, 1>(v, sub, LPR, (float)C, a.eps, true, mean, rstd, [](float s) { return s; });
+      mx_row_stats<LPR, 1>(v, sub, LPR, (float)C, 1.f / (float)C, a.eps, true, mean, rstd, [](float s) { return s; });
       mx_norm8(v[0], mean, rstd, gam, bet, o);
       const uint32_t byte = mx_scale_byte<MX_E4M3>(mx_quad_max(mx_top8(o)));
       const mx_u32x2 e = mx_encode8<MX_E4M3>(o, mx_inverse(byte)), large = {e4m3_large(e[0]), e4m3_large(e[1])};
