@@ -172,8 +172,9 @@ int spc_mx_dequantize(const void* codes, const void* scales, int64_t N, int64_t 
 
 /* sum = x + residual, rounded once to `dtype` (SPC_F16/SPC_BF16), and codes/scales = the quantised norm of sum's rows
  * [N,C] times gamma plus beta: SPC_NORM_RMS t / sqrt(mean(t^2) + eps), SPC_NORM_LAYER (t - mean(t)) / sqrt(var(t) + eps),
- * fp32 statistics (|t| below 2^60). residual may be NULL: then x's rows are normalised, and sum may be NULL. sum may be x
- * or residual. gamma, beta [C] of `param_dtype` or NULL (1, 0). C a multiple of 32, at most 16384.
+ * fp32 statistics (|t| below 2^57: the sum of C squares is to stay finite). residual may be NULL: then x's rows are
+ * normalised, and sum may be NULL. sum may be x or residual. gamma, beta [C] of `param_dtype` or NULL (1, 0). C a
+ * multiple of 32, at most 16384.
  * Beside spc_gather_ln_act: the norm ahead of a microscaled product, with a transformer block's residual addition. */
 int spc_add_norm_mx(const void* x, const void* residual, const void* gamma, const void* beta, int param_dtype,
                     float eps, int kind, int dtype, int64_t N, int64_t C, int fmt, void* sum, void* codes,

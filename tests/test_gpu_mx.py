@@ -193,6 +193,19 @@ def test_layer_norm_of_constant_rows(gpu, C, dt):
         assert torch.equal(sp.mx_dequantize(q, torch.float32), torch.full((len(v), C), 0.0 if beta is None else -1.5, device=gpu))
 
 
+@pytest.mark.parametrize("C", [32, 512, 4096, 16384])
+@pytest.mark.parametrize("kind", [sp.NORM_RMS, sp.NORM_LAYER])
+def test_add_norm_of_the_largest_values(gpu, C, kind):
+    """Up to the documented 2^57 the sum of squares stays below 2^128: 2^14 * (2^57 (1 - 2^-8))^2."""
+    top = 2.0 ** 57 * (1 - 2.0 ** -8)
+    x = torch.full((3, C), top)
+    x[1, ::2] = -top
+    x[2] = torch.linspace(-top, top, C)
+    x = x.to(torch.bfloat16).to(gpu)
+    t, q = sp.add_norm_mx(x, None, kind=kind)
+    near(q, *norm64(x.double(), kind, None, None, 1e-6), sp.MX_E4M3)
+
+
 def test_past_four_gigabytes(gpu):
     """Rows whose offsets pass 32 bits, in and out: the last ones are right."""
     n, k, o = 1100000, 64, 2080

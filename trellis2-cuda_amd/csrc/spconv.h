@@ -186,7 +186,7 @@ void mx_dequantize(const MxTensor& q, Tensor& y);
 
 // t = x + residual (one rounding; without a residual t = x) into sum, which may be x or residual (or null without a
 // residual), and q = the quantised norm of t's rows times gamma plus beta: MX_NORM_RMS t / sqrt(mean(t^2) + eps),
-// MX_NORM_LAYER (t - mean(t)) / sqrt(var(t) + eps); fp32 statistics (|t| below 2^60). x, residual, sum fp16 or bf16
+// MX_NORM_LAYER (t - mean(t)) / sqrt(var(t) + eps); fp32 statistics (|t| below 2^57). x, residual, sum fp16 or bf16
 // [N,C], C a multiple of 32 up to 16384; gamma, beta of any float type or null (1, 0).
 enum MxNorm : int { MX_NORM_RMS = 0, MX_NORM_LAYER = 1 };
 void add_norm_mx(const Tensor& x, const Tensor* residual, const Tensor* gamma, const Tensor* beta, float eps, int kind,

@@ -454,7 +454,7 @@ def add_norm_mx(x, residual=None, gamma=None, beta=None, eps: float = 1e-6, kind
                 out: MxTensor = None):
     """(t, q): t = x + residual, rounded to x's type (x itself without a residual), and q = norm(t) * gamma + beta
     quantised to fmt; NORM_RMS: t / sqrt(mean(t^2) + eps), NORM_LAYER: (t - mean(t)) / sqrt(var(t) + eps). x, residual
-    float16 or bfloat16 [N, C], C a multiple of 32 up to 16384; sum, the buffer for t, may be x or residual."""
+    float16 or bfloat16 [N, C], C a multiple of 32 up to 16384, |t| below 2^57; sum, the buffer for t, may be x or residual."""
     torch = _torch()
     _matrix(x, "x")
     N, C = shape = x.shape
