@@ -361,6 +361,58 @@ def test_linear_microscaled_bits(gpu, n, k, o, fmt):
         assert bool((buf.codes[n:] == 9).all()) and bool((buf.scales[n:] == 9).all())
 
 
+SMALL = torch.tensor([2.0 ** -9, 3 * 2.0 ** -9, 2.0 ** -6, 1.875 * 2.0 ** -6, 2.0 ** -3, 0.5, 1.125, 1.875, 2.25, 3.5, 3.75])
+LARGE = torch.tensor([256.0, 288.0, 320.0, 416.0, 448.0])
+
+
+def both_ends(n, k, o, cancel, seed, dev):
+    """e4m3 rows (as values) and e2m1 weights with both ends of the elements in one group of eight neighbours: cancel: every block
+    of 32 has a large element and its opposite beside it, under equal weights; else four blocks of a row have a single large one, or
+    one from 4 up. All sums are multiples of 2^-10 below 2^14: exact in fp32, whatever their order."""
+    g = gen(seed)
+    pick = lambda t, *shape: t[torch.randint(0, len(t), shape, generator=g)]
+    sign = lambda *shape: 1.0 - 2.0 * torch.randint(0, 2, shape, generator=g)
+    x = pick(SMALL, n, k) * sign(n, k) * (torch.rand((n, k), generator=g) < 0.2)
+    if cancel:
+        at = torch.arange(0, k, 32) + 2 * torch.randint(0, 16, (n, k // 32), generator=g)
+        v = pick(LARGE, n, k // 32) * sign(n, k // 32)
+        x.scatter_(1, at, v).scatter_(1, at + 1, -v)
+    else:
+        at = 32 * torch.rand((n, k // 32), generator=g).argsort(1)[:, :4] + torch.randint(0, 32, (n, 4), generator=g)
+        x.scatter_(1, at, pick(torch.cat((LARGE, torch.tensor([4.0, 4.5, 7.5]))), n, 4) * sign(n, 4))
+    c = torch.randint(0, 16, (o, k // 2), generator=g, dtype=torch.uint8)
+    c = c | c << 4 if cancel else c | torch.randint(0, 16, (o, k // 2), generator=g, dtype=torch.uint8) << 4
+    one = lambda rows: torch.full((rows, (k + 511) // 512 * 16), 127, dtype=torch.uint8)
+    w = mx(c, one(o), k, sp.MX_E2M1, dev)
+    q = mx(x.to(torch.float8_e4m3fn).view(torch.uint8), one(n), k, sp.MX_E4M3, dev)
+    X, W = matrix(q), matrix(w)
+    assert torch.equal(X.cpu().float(), x) and float((X.abs() @ W.abs().T).max()) < (2 ** 19 if cancel else 2 ** 14)
+    full = X @ W.T
+    assert float(full.abs().max()) < 2 ** 14
+    return x.to(dev), q, w, full
+
+
+@pytest.mark.parametrize("n,o", [(1, 32), (5, 96), (16, 64), (30, 64), (70, 4096), (100, 4096), (70, 8192), (90, 8192), (128, 8192),
+                                 (300, 1024), (2500, 4096), (5000, 3520)])
+@pytest.mark.parametrize("cancel", [False, True])
+def test_linear_both_ends_of_e4m3(gpu, n, o, cancel):
+    """Nothing of a small element is lost beside a large one: fp32 and microscaled results, and 16-bit ones of up to 32 rows."""
+    x, q, w, full = both_ends(n, 640, o, cancel, n + o, gpu)
+    exact = full.float()
+    assert torch.equal(sp.mx_linear(q, w, out_dtype=torch.float32), exact)
+    for ofmt in (sp.MX_E4M3, sp.MX_E2M1):
+        got, want = sp.mx_linear(q, w, out_fmt=ofmt), sp.mx_quantize(exact, ofmt)
+        assert torch.equal(got.scales, want.scales)
+        assert torch.equal(sp.mx_dequantize(got, torch.float32), sp.mx_dequantize(want, torch.float32))
+    if n <= 32:
+        for dt in (torch.float16, torch.bfloat16):
+            assert torch.equal(sp.mx_linear(q, w, out_dtype=dt), exact.to(dt))
+    if cancel and n <= 16:  # as values: each block's largest element makes its scale 1
+        for dt in (torch.float32, torch.float16, torch.bfloat16):
+            assert torch.equal(sp.mx_linear(x.to(dt), w, out_dtype=dt), exact.to(dt))
+            assert torch.equal(sp.mx_linear(x.to(dt), w, out_dtype=torch.float32), exact)
+
+
 @pytest.mark.parametrize("n,o", [(300, 96), (2500, 4096), (7001, 2080)])
 @pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
 def test_linear_not_finite_in_tiles(gpu, n, o, fmt):
