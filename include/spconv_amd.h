@@ -189,6 +189,9 @@ int spc_add_norm_mx(const void* x, const void* residual, const void* gamma, cons
  * quantises (0 for few rows), 16-byte aligned, in use until the call's work is done; NULL: the library's own, refused while the stream is
  * being captured into a graph (a captured call needs a workspace of its own for as long as the graph lives). */
 int spc_mx_linear_workspace(int64_t N, int64_t K, int x_fmt, int64_t* bytes);
+/* Rows and channels of a workgroup of that product on the current device (out_type with out_scales NULL: microscaled 0; else 1).
+ * Up to 32 channels: its wavefronts share out K; more: tiles. Host only. Beside spc_spconv_cfg. */
+int spc_mx_linear_tile(int64_t N, int64_t Co, int x_fmt, int out_type, int microscaled, int* rows, int* channels);
 int spc_mx_linear(const void* x, const void* x_scales, int x_dtype, int x_fmt, const void* w_codes,
                   const void* w_scales, const void* bias, int b_dtype, const void* residual, int act, int64_t N,
                   int64_t K, int64_t Co, int out_type, void* out, void* out_scales, void* workspace,

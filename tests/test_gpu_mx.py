@@ -298,6 +298,39 @@ def test_linear_bits(gpu, n, k, o, fmt):
         assert got is r and torch.equal(got, full.float().to(dt))
 
 
+def tile_is(cus, n, o, fmt, want, **out):
+    """The shape runs in this tile: checked on the part whose number of CUs the shapes below are chosen for."""
+    if cus == 256:
+        assert sp.mx_linear_tile(n, o, fmt, **out) == want
+
+
+# (n, k, o), the tile (rows, channels) for e2m1, and of e4m3 for 16-bit results (else as e2m1)
+FEW = [(24, 160, 16384, (32, 32), None), (60, 1184, 4096, (32, 32), None), (70, 1184, 4096, (48, 32), None),
+       (113, 1184, 4096, (64, 32), None), (70, 1184, 8192, (80, 32), None), (90, 1184, 8192, (96, 32), (64, 128)),
+       (128, 2080, 8192, (128, 32), (64, 128)), (101, 608, 6144, (128, 32), (64, 128)), (40, 160, 16384, (64, 128), (64, 128))]
+
+
+@pytest.mark.parametrize("n,k,o,tile,tile16", FEW)
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+def test_linear_bits_of_few_rows(gpu, n, k, o, tile, tile16, fmt):
+    """test_linear_bits in every number of row tiles."""
+    cus = torch.cuda.get_device_properties(gpu).multi_processor_count
+    x = mx(*small_ints(n, k, fmt, n + k, -8, 8), k, fmt, gpu)
+    w = mx(*small_ints(o, k, sp.MX_E2M1, o + k, 0, 0), k, sp.MX_E2M1, gpu)
+    exact = (matrix(x) @ matrix(w).T).float()
+    tile16 = tile16 if tile16 and fmt == sp.MX_E4M3 else tile
+    for dt in (torch.float32, torch.bfloat16):
+        tile_is(cus, n, o, fmt, tile if dt == torch.float32 else tile16, out_dtype=dt)
+        buf = torch.full((n + 3, o), 7.0, dtype=dt, device=gpu)
+        got = sp.mx_linear(x, w, out=buf[:n])
+        assert torch.equal(got, exact.to(dt)) and bool((buf[n:] == 7).all())
+    for ofmt in (sp.MX_E4M3, sp.MX_E2M1):
+        tile_is(cus, n, o, fmt, tile, out_fmt=ofmt)
+        got, want = sp.mx_linear(x, w, out_fmt=ofmt), sp.mx_quantize(exact, ofmt)
+        assert torch.equal(got.scales, want.scales)
+        assert torch.equal(sp.mx_dequantize(got, torch.float32), sp.mx_dequantize(want, torch.float32))
+
+
 def eights(X, W):
     """Sum over groups of 8 consecutive columns of the group's largest |x w|, [n,o]."""
     s = torch.zeros((X.shape[0], W.shape[0]), dtype=torch.float64, device=X.device)

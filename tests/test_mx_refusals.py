@@ -100,6 +100,14 @@ def test_linear():
     assert call(n=0, x=None, xs=None, y=None) == 0
 
 
+def test_linear_tile():
+    lib, r, c = sp.load_library(), ctypes.c_int(), ctypes.c_int()
+    refused(lib.spc_mx_linear_tile(1, 48, 1, 2, 0, ctypes.byref(r), ctypes.byref(c)), "arguments")
+    refused(lib.spc_mx_linear_tile(1, 64, 3, 2, 0, ctypes.byref(r), ctypes.byref(c)), "arguments")
+    refused(lib.spc_mx_linear_tile(1, 64, 1, 2, 0, None, ctypes.byref(c)), "arguments")
+    refused(lib.spc_mx_linear_tile(1, 64, 1, 9, 0, ctypes.byref(r), ctypes.byref(c)), "dtype code 9")
+
+
 def test_tail():
     lib = sp.load_library()
 

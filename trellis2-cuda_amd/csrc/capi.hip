@@ -450,6 +450,16 @@ SPC_API int spc_mx_linear_workspace(int64_t N, int64_t K, int x_fmt, int64_t* by
   });
 }
 
+SPC_API int spc_mx_linear_tile(int64_t N, int64_t Co, int x_fmt, int out_type, int microscaled, int* rows, int* channels) {
+  return guarded([&] {
+    REQ(rows && channels && N >= 0 && N < (1ll << 31) && Co > 0 && Co % 32 == 0 && Co <= (1 << 20) &&
+            (x_fmt == SPC_MX_E4M3 || x_fmt == SPC_MX_E2M1), "arguments");
+    const MxTile t = mx_linear_tile(N, Co, x_fmt, !microscaled && float_dt(out_type, "out") != F32);
+    *rows = t.rows;
+    *channels = t.channels;
+  });
+}
+
 SPC_API int spc_mx_linear(const void* x, const void* x_scales, int x_dtype, int x_fmt, const void* w_codes,
                           const void* w_scales, const void* bias, int b_dtype, const void* residual, int act, int64_t N,
                           int64_t K, int64_t Co, int out_type, void* out, void* out_scales, void* workspace,

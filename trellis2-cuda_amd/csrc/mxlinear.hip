@@ -546,11 +546,40 @@ void launch(LinArgs a) {
   CK(hipGetLastError());
 }
 
-// Up to kFewRows rows go through k_mx_rows; up to kValueRows of them may come as values. (Tiles whose K goes in pieces over more
-// workgroups, with the partial sums added by a second launch, were slower from 17 rows on: us with 4 pieces / k_mx_rows,
-// [33, 4096, 4096] 12 / 9, [20, 1024, 4096] 14 / 7. Whole tiles of 128 x 64 / k_mx_rows: [128, 4096, 8192] 17.1 / 15.5,
-// [77, 4096, 8192] 17.3 / 15.5, [33, 4096, 4096] 16.2 / 10.2, [20, 1024, 4096] 9.3 / 6.6.)
-constexpr int kFewRows = 128, kValueRows = 16;
+constexpr int kValueRows = 16, kFewRows = 128;  // rows that may come as values; rows up to which k_mx_rows is looked at
+}  // namespace
+
+// Few rows: k_mx_rows, 32 channels a workgroup (16 of values of up to 16 rows), in groups of the fewest row tiles whose
+// workgroups are one round of the CUs: a workgroup's time grows with its row tiles, a second round doubles it. us with 2 / 3 / 4 /
+// 5 / 6 / 8 row tiles / whole tiles of 128 x 64, e4m3 to 16 bits, [N, K, O]: [64, 4096, 4096] 10.0 / 12.0 / 13.8 / - / - / - / 16.6,
+// [80, 4096, 4096] 15.1 / 12.0 / 14.1 / 16.1 / - / - / 16.3, [128, 4096, 4096] 16.9 / 19.2 / 14.2 / 16.4 / 18.4 / 22.8 / 16.8,
+// [40, 4096, 8192] 14.5 / 11.5 / 12.3 / - / - / - / 16.3, [80, 4096, 8192] 21.6 / 19.2 / 21.3 / 16.1 / 17.3 / - / 16.5, [96, 4096, 8192]
+// 22.9 / 20.5 / 22.3 / 25.6 / 18.6 / - / 16.5: more than 5 row tiles are the tiled kernel's. With e2m1, and where that kernel takes
+// its products twice (SPLIT), they are not: e2m1 [128, 4096, 8192] 22.1 / 19.9 / 17.2 / 18.1 / 20.0 / 15.3 / 16.0, e4m3 to e4m3
+// 30.1 / 27.9 / 25.4 / 27.5 / 29.4 / 23.8 / 25.3. Two rounds only with up to 32 rows: [24, 4096, 16384] 15.8 / 17.6 / - / - / - / - /
+// 16.9, but [40, 4096, 16384] 25.8 / 19.8 / 21.7 / - / - / - / 16.7. (K in pieces over more workgroups, whose sums a second launch adds:
+// [33, 4096, 4096] 12 us, [20, 1024, 4096] 14, against 9.6 and 4.6.)
+// More rows: larger tiles read fewer operand bytes per product, smaller ones are more. Two workgroups of 256 channels by 128 rows
+// fit a CU: they are taken where they fill most of these slots; 128 by 64 where 128 by 128 would leave a quarter of them free.
+// us at 256 x 128 / 128 x 128 / 128 x 64, [N, K, O]: e4m3 [16411, 4096, 4096] 272 / 314 / 365, [8209, 2080, 4128] 94 / 103 / 114,
+// [58321, 1024, 256] 29 / 32 / 32, [2048, 4096, 4096] 44 / 41 / 46, [1803, 4096, 1024] 41 / 26 / 18, [11467, 2048, 512] 28 / 23 / 21,
+// [300, 1024, 1024] 20 / 12 / 9; e2m1 [16411, 4096, 4096] 236 / 242 / 306, [600, 2048, 2048] 23 / 15 / 12.
+MxTile mx_linear_tile(i64 n, i64 o, int x_fmt, bool out16) {
+  const i64 cus = mx_device_cus();
+  if (n <= 16) return {16, 32};
+  if (n <= kFewRows) {
+    for (int t : {2, 3, 4, 5, 6, 8}) {
+      if (t > 5 && x_fmt == MX_E4M3 && out16) break;
+      if (cdiv(n, 16 * t) * (o / 32) <= cus || (n <= 32 && o / 32 <= 2 * cus)) return {16 * t, 32};
+    }
+  }
+  const i64 n128 = cdiv(n, 128);
+  if (n128 * cdiv(o, 256) * 2 >= 3 * cus) return {128, 256};
+  if (n128 * cdiv(o, 128) * 2 > 3 * cus) return {128, 128};
+  return {64, 128};
+}
+
+namespace {
 template <int XB, int OUT, int XT, int NT>
 void launch_rows(const LinArgs& a) {
   constexpr int OT = OUT == OUT_MX8 || OUT == OUT_MX4 ? 2 : NT == 1 ? 1 : 2;
@@ -566,18 +595,23 @@ void gemm(const LinArgs& a, int xt) {
     else launch_rows<XB, OUT, BF16, 1>(a);
     return;
   }
-  if (a.N <= 16) return launch_rows<XB, OUT, -1, 1>(a);
-  if (a.N <= 32) return launch_rows<XB, OUT, -1, 2>(a);
-  if (a.N <= 64) return launch_rows<XB, OUT, -1, 4>(a);
-  if (a.N <= kFewRows) return launch_rows<XB, OUT, -1, 5>(a);
-  // Larger tiles read fewer operand bytes per product, smaller ones are more. Two workgroups of 256 channels by 128 rows fit a
-  // CU: they are taken where they fill most of these slots; 128 by 64 where 128 by 128 would leave a quarter of them free.
-  // us at 256 x 128 / 128 x 128 / 128 x 64, [N, K, O]: e4m3 [16411, 4096, 4096] 272 / 314 / 365, [8209, 2080, 4128] 94 / 103 / 114,
-  // [58321, 1024, 256] 29 / 32 / 32, [2048, 4096, 4096] 44 / 41 / 46, [1803, 4096, 1024] 41 / 26 / 18, [11467, 2048, 512] 28 / 23 / 21,
-  // [300, 1024, 1024] 20 / 12 / 9; e2m1 [16411, 4096, 4096] 236 / 242 / 306, [600, 2048, 2048] 23 / 15 / 12.
-  const i64 n128 = cdiv(a.N, 128), cus = mx_device_cus();
-  if (n128 * cdiv(a.O, 256) * 2 >= 3 * cus) launch<XB, OUT, 8, 4, 2, 2, 1, XB == 8 ? 2 : 3>(a);
-  else if (n128 * cdiv(a.O, 128) * 2 > 3 * cus) launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
+  const MxTile t = mx_linear_tile(a.N, a.O, XB == 8 ? MX_E4M3 : MX_E2M1, OUT == OUT_16);
+  if (t.channels <= 32) {
+    switch (t.rows / 16) {
+      case 1: return launch_rows<XB, OUT, -1, 1>(a);
+      case 2: return launch_rows<XB, OUT, -1, 2>(a);
+      case 3: return launch_rows<XB, OUT, -1, 3>(a);
+      case 4: return launch_rows<XB, OUT, -1, 4>(a);
+      case 5: return launch_rows<XB, OUT, -1, 5>(a);
+    }
+    if constexpr (XB == 4 || OUT != OUT_16) {
+      if (t.rows == 96) return launch_rows<XB, OUT, -1, 6>(a);
+      if (t.rows == 128) return launch_rows<XB, OUT, -1, 8>(a);
+    }
+    spc_fail("no kernel for %d rows", t.rows);
+  }
+  if (t.channels == 256) launch<XB, OUT, 8, 4, 2, 2, 1, XB == 8 ? 2 : 3>(a);
+  else if (t.rows == 128) launch<XB, OUT, 4, 4, 2, 2, XB == 8 ? 1 : 2, XB == 8 ? 3 : 2>(a);
   else launch<XB, OUT, 4, 2, 2, 2, 1, 3>(a);
 }
 }  // namespace

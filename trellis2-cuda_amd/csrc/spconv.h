@@ -201,6 +201,12 @@ void mx_linear(const MxTensor& x, const MxTensor& w, const Tensor* bias, const T
 void mx_linear(const Tensor& x, int x_fmt, const MxTensor& w, const Tensor* bias, const Tensor* residual, int act, Tensor* y,
                MxTensor* yq, void* workspace = nullptr, i64 workspace_bytes = 0);
 i64 mx_linear_workspace(i64 N, i64 K, int x_fmt);
+// Rows and channels of a workgroup of the product on the current device (out16: into fp16 or bf16). Up to 32 channels: K is shared
+// out among its wavefronts, operands straight into registers; more: tiles in LDS.
+struct MxTile {
+  int rows, channels;
+};
+MxTile mx_linear_tile(i64 N, i64 O, int x_fmt, bool out16);
 
 // convnext_mlp with microscaled products: y = x + W2 mx(silu(W1 mx(LayerNorm(h) * gamma + beta) + b1)) + b2, w1 [4C,C]
 // and w2 [C,4C] e2m1, both activations quantised to fmt; any C that is a multiple of 32 up to 4096. h, x, y of one 16-bit type;

@@ -35,7 +35,8 @@ SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_get_stream", "spc_build_neig
            "spc_subdivide", "spc_subdivide_noalloc", "spc_subm_conv_replay", "spc_grid_sample_map",
            "spc_grid_sample_sum", "spc_subdivide_build", "spc_subm_conv_preln", "spc_alloc_counts", "spc_kernel_timing",
            "spc_kernel_times", "spc_release_cached_memory", "spc_mx_sizes", "spc_mx_quantize", "spc_mx_dequantize",
-           "spc_add_norm_mx", "spc_mx_linear_workspace", "spc_mx_linear", "spc_convnext_mlp_mx_workspace",
+           "spc_add_norm_mx", "spc_mx_linear_workspace", "spc_mx_linear_tile",
+           "spc_mx_linear", "spc_convnext_mlp_mx_workspace",
            "spc_convnext_mlp_mx")
 
 _lib = None
@@ -93,6 +94,7 @@ def load_library():
     L.spc_mx_dequantize.argtypes = [P, P, I64, I64, I, I, P]
     L.spc_add_norm_mx.argtypes = [P, P, P, P, I, ctypes.c_float, I, I, I64, I64, I, P, P, P]
     L.spc_mx_linear_workspace.argtypes = [I64, I64, I, PI64]
+    L.spc_mx_linear_tile.argtypes = [I64, I64, I, I, I, ctypes.POINTER(I), ctypes.POINTER(I)]
     L.spc_mx_linear.argtypes = [P, P, I, I, P, P, P, I, P, I, I64, I64, I64, I, P, P, P, I64]
     L.spc_convnext_mlp_mx_workspace.argtypes = [I64, I64, I, PI64]
     L.spc_convnext_mlp_mx.argtypes = [P, P, P, P, ctypes.c_float, P, P, P, P, P, P, I, I, I, I64, I64, P, P, I64]
@@ -550,6 +552,15 @@ def mx_linear(x, w: MxTensor, bias=None, residual=None, act: int = ACT_NONE, fmt
         _dt(bias) if bias is not None else F32, _adr(residual, dev), act, N, K, Co, ot, _adr(y, dev), _adr(ys, dev),
         _adr(ws, dev), nws))
     return out
+
+
+def mx_linear_tile(N: int, Co: int, fmt: int = MX_E4M3, out_dtype=None, out_fmt=None):
+    """(rows, channels) of a workgroup of mx_linear's product: up to 32 channels, its wavefronts share out K; more, tiles. fmt: x's;
+    out_dtype (default: 16 bits) or out_fmt: the result's."""
+    r, c = ctypes.c_int(), ctypes.c_int()
+    f32 = out_dtype is not None and out_dtype == _torch().float32
+    _check(load_library().spc_mx_linear_tile(N, Co, fmt, F32 if f32 else BF16, out_fmt is not None, ctypes.byref(r), ctypes.byref(c)))
+    return r.value, c.value
 
 
 def convnext_mlp_mx(h, x, gamma, beta, w1: MxTensor, b1, w2: MxTensor, b2, eps: float = 1e-6, fmt: int = MX_E4M3, out=None):
