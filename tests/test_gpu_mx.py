@@ -331,6 +331,34 @@ def test_linear_bits_of_few_rows(gpu, n, k, o, tile, tile16, fmt):
         assert torch.equal(sp.mx_dequantize(got, torch.float32), sp.mx_dequantize(want, torch.float32))
 
 
+# 64, 128 and 256 channels' tiles with K of several times 512, in even and odd numbers of steps, and a remainder
+DEEP = [(300, 1184, 1056, (64, 128)), (300, 2080, 1024, (64, 128)), (2500, 1184, 4096, (128, 128)), (2500, 2080, 4096, (128, 128)),
+        (2450, 1632, 4128, (128, 128)), (5000, 1184, 3520, (128, 256)), (5000, 2080, 3520, (128, 256)), (5050, 1632, 3552, (128, 256))]
+
+
+@pytest.mark.parametrize("n,k,o,tile", DEEP)
+@pytest.mark.parametrize("fmt", [sp.MX_E4M3, sp.MX_E2M1])
+def test_linear_bits_in_deep_tiles(gpu, n, k, o, tile, fmt):
+    """test_linear_bits where every slot of a tile's pipeline is filled again and all four of a word's scales are used."""
+    cus = torch.cuda.get_device_properties(gpu).multi_processor_count
+    x = mx(*small_ints(n, k, fmt, n + k, -8, 8), k, fmt, gpu)
+    w = mx(*small_ints(o, k, sp.MX_E2M1, o + k, 0, 0), k, sp.MX_E2M1, gpu)
+    exact = matrix(x) @ matrix(w).T
+    g = gen(o)
+    bias = torch.randint(-64, 65, (o,), generator=g).float().to(gpu)
+    res = torch.randint(-64, 65, (n, o), generator=g).to(gpu)
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        tile_is(cus, n, o, fmt, tile, out_dtype=dt)
+        assert torch.equal(sp.mx_linear(x, w, out_dtype=dt), exact.float().to(dt))
+        r = res.to(dt)
+        assert torch.equal(sp.mx_linear(x, w, bias, residual=r, out=r), (exact + bias.double() + res.to(dt).double()).float().to(dt))
+    for ofmt in (sp.MX_E4M3, sp.MX_E2M1):
+        tile_is(cus, n, o, fmt, tile, out_fmt=ofmt)
+        got, want = sp.mx_linear(x, w, bias, out_fmt=ofmt), sp.mx_quantize((exact + bias.double()).float(), ofmt)
+        assert torch.equal(got.scales, want.scales)
+        assert torch.equal(sp.mx_dequantize(got, torch.float32), sp.mx_dequantize(want, torch.float32))
+
+
 def eights(X, W):
     """Sum over groups of 8 consecutive columns of the group's largest |x w|, [n,o]."""
     s = torch.zeros((X.shape[0], W.shape[0]), dtype=torch.float64, device=X.device)
@@ -538,6 +566,57 @@ def test_tail(gpu, c, n, fmt):
     bare = sp.convnext_mlp_mx(h, x, None, None, w1, None, w2, None, fmt=fmt)
     ones, zeros = torch.ones(c, device=gpu), torch.zeros(4 * c, device=gpu)
     assert torch.equal(bare, sp.convnext_mlp_mx(h, x, ones, zeros[:c].contiguous(), w1, zeros, w2, zeros[:c].contiguous(), fmt=fmt))
+
+
+@pytest.mark.parametrize("c,n", [(128, 129), (128, 4099), (128, 70001), (256, 129), (256, 2051), (256, 58321)])
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+def test_tail_in_one_kernel(gpu, c, n, dt):
+    """Where the tail is one kernel (it asks for no workspace) its bits are its parts'."""
+    assert sp._workspace_bytes("spc_convnext_mlp_mx_workspace", n, c, sp.MX_E4M3) == 0
+    h, x, gamma, beta, w1, b1, w2, b2 = a = tail(n, c, dt, c + n, gpu, torch.float32 if n % 2 else dt)
+    _, q = sp.add_norm_mx(h, None, gamma, beta, kind=sp.NORM_LAYER)
+    want = sp.mx_linear(sp.mx_linear(q, w1, b1, act=sp.ACT_SILU, out_fmt=sp.MX_E4M3), w2, b2, residual=x, out_dtype=dt)
+    assert torch.equal(sp.convnext_mlp_mx(*a), want)
+    for over in (0, 1):
+        b = [t.clone() if isinstance(t, torch.Tensor) else t for t in a]
+        assert torch.equal(sp.convnext_mlp_mx(*b, out=b[over]), want)
+    bare = sp.convnext_mlp_mx(h, x, None, None, w1, None, w2, None)
+    _, q = sp.add_norm_mx(h, None, kind=sp.NORM_LAYER)
+    hid = sp.mx_linear(q, w1, act=sp.ACT_SILU, out_fmt=sp.MX_E4M3)
+    assert torch.equal(bare, sp.mx_linear(hid, w2, residual=x, out_dtype=dt))
+
+
+@pytest.mark.parametrize("c", [128, 256])
+def test_tail_in_one_kernel_sums_both_ends(gpu, c):
+    """The first product beside large elements that cancel: gamma = 0 leaves beta, rows of both ends of e4m3, to be multiplied."""
+    x, q, w1, full = both_ends(1, c, 4 * c, True, c, gpu)
+    n = 200
+    h, res = features(n, c, torch.bfloat16, 1).to(gpu), torch.zeros((n, c), dtype=torch.bfloat16, device=gpu)
+    w2 = sp.mx_quantize((torch.randn((c, 4 * c), generator=gen(c)) / c).to(gpu), sp.MX_E2M1)
+    got = sp.convnext_mlp_mx(h, res, torch.zeros(c, device=gpu), x[0].contiguous(), w1, None, w2, None)
+    y = full.expand(n, -1)
+    y = y * torch.sigmoid(y)
+    rows = sp.MxTensor(q.codes.repeat(n, 1), q.scales.repeat(n, 1), c, sp.MX_E4M3)
+    hid = sp.mx_linear(rows, w1, act=sp.ACT_SILU, out_fmt=sp.MX_E4M3)
+    near(hid, y, (full.abs() + 4) * 2.0 ** -23 * y.abs() + 1e-37, sp.MX_E4M3)  # exact sums: what is left is the SiLU's own error
+    assert torch.equal(got, sp.mx_linear(hid, w2, residual=res, out_dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("c,n,fmt", [(512, 140001, sp.MX_E4M3), (256, 300007, sp.MX_E2M1), (1024, 40003, sp.MX_E4M3)])
+def test_tail_in_unequal_parts(gpu, c, n, fmt):
+    """A tail whose hidden units pass the parts' limit, so that its workspace is for some of the rows: every row as in calls of few
+    rows each, also over h and over x."""
+    whole = n * sp._workspace_bytes("spc_convnext_mlp_mx_workspace", 512, c, fmt) // 512
+    assert 0 < sp._workspace_bytes("spc_convnext_mlp_mx_workspace", n, c, fmt) < 0.6 * whole
+    a = tail(n, c, torch.bfloat16, c, gpu)
+    want = torch.empty_like(a[0])
+    step = 20011
+    for i in range(0, n, step):
+        want[i:i + step] = sp.convnext_mlp_mx(a[0][i:i + step], a[1][i:i + step], *a[2:], fmt=fmt)
+    assert torch.equal(sp.convnext_mlp_mx(*a, fmt=fmt), want)
+    for over in (0, 1):
+        b = [t.clone() if k == over else t for k, t in enumerate(a)]
+        assert torch.equal(sp.convnext_mlp_mx(*b, fmt=fmt, out=b[over]), want)
 
 
 @pytest.mark.parametrize("c,n", [(128, 131), (256, 129), (256, 65 * 7 + 1), (512, 140)])
