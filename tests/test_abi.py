@@ -59,6 +59,19 @@ def test_stream_as_set_by_any_caller():
     assert spconv_amd._library_stream() == 0
 
 
+def test_digest_of_the_convolution(tmp_path, monkeypatch):
+    """The digest that stamps the convolution's measured figures changes with its sources and with no other operator's."""
+    import shutil
+    shutil.copytree(os.path.join(ROOT, "trellis2-cuda_amd", "csrc"), tmp_path / "csrc")
+    now = spconv_amd.source_digest()
+    monkeypatch.setattr(spconv_amd, "_PKG", str(tmp_path))
+    assert spconv_amd.source_digest() == now
+    for name, changes in (("mx.hip", False), ("new_operator.hip", False), ("capi.hip", False), ("conv.hip", True)):
+        with open(tmp_path / "csrc" / name, "a") as f:
+            f.write("// more\n")
+        assert (spconv_amd.source_digest() != now) == changes, name
+
+
 def test_no_oracle_in_product():
     """The product library and binding never reference the oracle."""
     pkg = os.path.join(ROOT, "trellis2-cuda_amd")

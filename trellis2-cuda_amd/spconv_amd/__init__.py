@@ -735,15 +735,19 @@ def subdivide_build(coords, logits_f16, W: int = 4096, H: int = 4096, D: int = 4
     return cc[:m.value], src[:m.value], SpConvCache(h, m.value, coords.device)
 
 
+# What a convolution's launches and the kernel map and row order that they read are built from (without spconv.h, which declares
+# every operator, and capi.hip, which checks arguments)
+CONV_SOURCES = ("autotune.hip", "conv.hip", "core.h", "core.hip", "kmap.hip", "lnact.h", "scan.h", "scan.hip", "sort.hip", "splitk.hip")
+
+
 def source_digest() -> str:
-    """sha256 over the HIP/C++ sources of the library (file names and contents, sorted): stamps measured profile
-    figures with the code they were measured on, so a stale figure can be recognised."""
+    """sha256 over the convolution's HIP/C++ sources (file names and contents, sorted): stamps measured profile figures
+    with the code they were measured on, so a stale figure can be recognised, and stays valid beside changes of other operators."""
     import hashlib
     d = os.path.join(_PKG, "csrc")
     h = hashlib.sha256()
-    for name in sorted(os.listdir(d)):
-        if name.endswith((".hip", ".h")):
-            h.update(name.encode())
-            with open(os.path.join(d, name), "rb") as f:
-                h.update(f.read())
+    for name in sorted(CONV_SOURCES):
+        h.update(name.encode())
+        with open(os.path.join(d, name), "rb") as f:
+            h.update(f.read())
     return h.hexdigest()[:16]
