@@ -568,7 +568,7 @@ def test_tail(gpu, c, n, fmt):
     assert torch.equal(bare, sp.convnext_mlp_mx(h, x, ones, zeros[:c].contiguous(), w1, zeros, w2, zeros[:c].contiguous(), fmt=fmt))
 
 
-@pytest.mark.parametrize("c,n", [(128, 129), (128, 4099), (128, 70001), (256, 129), (256, 2051), (256, 58321)])
+@pytest.mark.parametrize("c,n", [(128, 129), (128, 4099), (128, 70001), (256, 6145), (256, 58321)])
 @pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
 def test_tail_in_one_kernel(gpu, c, n, dt):
     """Where the tail is one kernel (it asks for no workspace) its bits are its parts'."""
@@ -590,7 +590,8 @@ def test_tail_in_one_kernel(gpu, c, n, dt):
 def test_tail_in_one_kernel_sums_both_ends(gpu, c):
     """The first product beside large elements that cancel: gamma = 0 leaves beta, rows of both ends of e4m3, to be multiplied."""
     x, q, w1, full = both_ends(1, c, 4 * c, True, c, gpu)
-    n = 200
+    n = 200 if c == 128 else 8200
+    assert sp._workspace_bytes("spc_convnext_mlp_mx_workspace", n, c, sp.MX_E4M3) == 0
     h, res = features(n, c, torch.bfloat16, 1).to(gpu), torch.zeros((n, c), dtype=torch.bfloat16, device=gpu)
     w2 = sp.mx_quantize((torch.randn((c, 4 * c), generator=gen(c)) / c).to(gpu), sp.MX_E2M1)
     got = sp.convnext_mlp_mx(h, res, torch.zeros(c, device=gpu), x[0].contiguous(), w1, None, w2, None)
@@ -625,6 +626,22 @@ def test_tail_writes_its_rows_only(gpu, c, n):
     buf = torch.full((n + 8, c), 7.0, dtype=torch.bfloat16, device=gpu)
     y = sp.convnext_mlp_mx(*a, out=buf[4:n + 4])
     assert torch.equal(y, sp.convnext_mlp_mx(*a)) and bool((buf[:4] == 7).all()) and bool((buf[n + 4:] == 7).all())
+
+
+def test_tail_in_one_kernel_edges(gpu):
+    """At 256 channels: rows before and behind stay, rows that are not finite stay alone (at 128 the tests around this one)."""
+    n, c = 8193 + 64 * 3, 256
+    assert sp._workspace_bytes("spc_convnext_mlp_mx_workspace", n, c, sp.MX_E4M3) == 0
+    a = list(tail(n, c, torch.float16, c, gpu))
+    want = sp.convnext_mlp_mx(*a)
+    a[0], a[1] = a[0].clone(), a[1].clone()
+    a[0][5, 3], a[0][n - 1, c - 1], a[1][9, 0] = float("nan"), float("inf"), float("inf")
+    buf = torch.full((n + 8, c), 7.0, dtype=torch.float16, device=gpu)
+    y = sp.convnext_mlp_mx(*a, out=buf[4:n + 4])
+    assert bool((buf[:4] == 7).all()) and bool((buf[n + 4:] == 7).all())
+    assert bool(y[5].isnan().all()) and bool(y[n - 1].isnan().all()) and float(y[9, 0]) == float("inf")
+    want[5], want[n - 1], want[9, 0] = float("nan"), float("nan"), float("inf")
+    assert torch.equal(y.nan_to_num(5.0), want.nan_to_num(5.0))
 
 
 @pytest.mark.parametrize("c,n", [(128, 200), (256, 300), (512, 300)])

@@ -34,6 +34,14 @@ def test_sizes():
         assert lib.spc_mx_linear_workspace(rows, 64, 2, ctypes.byref(n)) == 0 and n.value == 0
 
 
+def test_tail_in_one_kernel_by_rows():
+    """The tail is one kernel, without a workspace, from the rows on where that is the faster form."""
+    lib, n = sp.load_library(), ctypes.c_int64()
+    for rows, c, fmt, one in ((128, 128, 1, False), (129, 128, 1, True), (129, 128, 2, False), (129, 256, 1, False), (4000, 256, 1, False),
+                              (6145, 256, 1, True), (6145, 256, 2, False), (6145, 512, 1, False)):
+        assert lib.spc_convnext_mlp_mx_workspace(rows, c, fmt, ctypes.byref(n)) == 0 and (n.value == 0) == one, (rows, c, fmt)
+
+
 def test_quantize():
     lib = sp.load_library()
     refused(lib.spc_mx_quantize(p(A), 2, 4, 48, 1, p(2 * A), p(3 * A)), "multiple of 32")

@@ -1,8 +1,8 @@
 // ConvNeXt tail with microscaled products (beside mlp.hip's, whose products are in 16 bits):
 //   y = x + W2 q(silu(W1 q(LayerNorm(h) * gamma + beta) + b1)) + b2,    q: blocks of e4m3 or e2m1 (mx.h), W1, W2 e2m1
 //
-// C = 128 and 256 with e4m3 activations run in one kernel (k_mx_tail): the hidden units, which are what the three-pass
-// form writes and reads most of, stay in LDS. Other widths and formats, and few rows, run as norm pass, product with the
+// C = 128 and 256 with e4m3 activations and enough rows run in one kernel (k_mx_tail): the hidden units, which are what the
+// three-pass form writes and reads most of, stay in LDS. Other widths and formats, and fewer rows, run as norm pass, product with the
 // SiLU and the quantisation in its epilogue, product with the residual. The two forms give the same bits.
 #include <algorithm>
 
@@ -24,10 +24,11 @@ struct TailArgs {
 // is two lane exchanges away), SiLU, quantises them into LDS, and after a barrier multiplies all 256 into its C / 8
 // channels of y. The weights go from L2 straight into registers, each to the one wavefront that needs it, read while
 // the other product runs. Two slots of hidden units make it one barrier a round.
-// us, this kernel / three passes (the 16-bit tail): [58321, 256] 80 / 104 (112), [15000, 256] 27 (40), [391007, 128] 193 (202). 61 GFLOP at
-// the first size: about 20 us are norm, residual and stores, 27 the two products, 12 waits for weights, 6 SiLU and quantisation,
-// which follow each other in every wavefront. At 512 channels the sums of y leave room for 32 rows only, and each workgroup
-// reads all weights for them: [11467, 512] 84 us with 8 wavefronts, 128 with 4, against 63 in three passes.
+// us by graph replays, this kernel / three passes / the 16-bit tail: [15000, 256] 29 / 37 / 47, [58321, 256] 87 / 116 / 126, [391007, 128]
+// 181 / 306 / 218. 61 GFLOP at the second size: with parts left out, about 20 us were norm, residual and stores, 27 the two products,
+// 12 waits for weights, 6 SiLU and quantisation; the rest is their order in every wavefront, one after another. At 512 channels
+// the sums of y leave room for 32 rows only, and each workgroup reads all weights for them: [11467, 512] 84 us with 8 wavefronts,
+// 128 with 4, against 63 in three passes.
 constexpr int kTailRows = 64;  // rows of a workgroup
 template <bool F16, int C>
 __global__ void __launch_bounds__(512, 4) k_mx_tail(TailArgs a) {
@@ -212,8 +213,12 @@ void launch_tail(const TailArgs& a) {
   k_mx_tail<F16, C><<<(unsigned)((a.out.N + kTailRows - 1) / kTailRows), 512, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
-// The widths and rows that k_mx_tail takes (up to 128 rows are k_mx_rows', where K goes over a workgroup's wavefronts)
-bool fused(i64 n, i64 C, int fmt) { return fmt == MX_E4M3 && (C == 128 || C == 256) && n > 128; }
+// The widths and rows that k_mx_tail takes. Up to 128 rows are k_mx_rows', where K goes over a workgroup's wavefronts. A workgroup
+// here takes as long for one row as for 64, and reads all weights: at 256 channels three passes, whose products have more
+// workgroups, are faster until 64 rows each fill three eighths of the CUs. us, one kernel / three passes: 256 channels, 129 rows
+// 25.8 / 16.6, 2000 26.2 / 18.2, 4000 26.2 / 21.4, 6000 26.5 / 25.6, 8000 26.9 / 30.0, 15000 29.1 / 37.3; 128 channels, 129 rows
+// 11.7 / 14.3, 4000 12.1 / 15.2.
+bool fused(i64 n, i64 C, int fmt) { return fmt == MX_E4M3 && ((C == 128 && n > 128) || (C == 256 && n > 6144)); }
 }  // namespace
 
 namespace {
