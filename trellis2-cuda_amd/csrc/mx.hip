@@ -59,7 +59,7 @@ __device__ __forceinline__ void put_scale(uint8_t* scales, i64 row, uint32_t col
 }
 
 // One lane per 8 values, four lanes per block, four blocks' scale bytes a store. HBM-bound: bf16 [390503, 256] (253 MB with
-// e2m1's) 48 us there, 38 back; [65536, 1024] with e4m3 38 and 31. Few values: a launch's latency (3 us).
+// e2m1's) 43 us there, 38 back; [65536, 1024] with e4m3 38 and 31. Few values: a launch's latency (3 us).
 constexpr int kQuantUnits = 4;
 template <int FMT, int T>
 __global__ void __launch_bounds__(256) k_mx_quantize(const void* __restrict__ x, i64 units, uint32_t per, uint32_t stride,
@@ -201,7 +201,8 @@ void mx_dequantize(const MxTensor& q, Tensor& y) {
 // and y's blocks quantised; statistics, norm and amax in fp32 registers, one rounding to the elements. A row is read
 // once: LPR lanes hold it, 8 channels per lane and chunk, so a block of 32 is a quad of lanes (C / 8 is a multiple of 4:
 // a quad has all of a block or nothing). LPR = 256: a workgroup per row, partial sums through LDS; LPR <= 64: a wavefront
-// or part of one. HBM-bound: bf16 with a residual [32771, 4096] 177 us (5.3 TB/s), fp16 [58321, 256] 13 us (3.5), one row 2.9.
+// or part of one. HBM-bound: bf16 with a residual [32771, 4096] 177 us (5.3 TB/s), fp16 [58321, 256] 13 us (3.5;
+// 7291 groups of rows on 4096 workgroups, half of which fit the card: most take two turns), one row 2.9.
 // us with a wavefront / a workgroup per row, [20000, 512] 13.3 / 21.9, [40000, 1024] 52 / 56, [5000, 2048] 14.0 / 12.8,
 // [20000, 2048] 51 / 53, [32771, 4096] 211 / 177, [2000, 4096] 17 / 11: a workgroup from more than 1024 channels on.
 // The sum is stored past the caches (what reads it next is a block away): [32771, 4096] 183 -> 178.

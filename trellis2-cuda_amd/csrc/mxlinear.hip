@@ -31,12 +31,14 @@ constexpr int run_tiles() {  // G above
   return OUT == OUT_F32 ? 1 : OUT == OUT_16 ? 2 : 4 < TO ? 4 : TO;
 }
 
-// Few rows: what counts is that all of W is on its way at once. A workgroup of 8 wavefronts has 16 OT channels by 16 NT rows;
-// each wavefront takes a contiguous eighth of K, both operands straight into registers, and the eight sums meet in
+// Few rows: W's bytes count, and that many of them are on their way at once. A workgroup of 8 wavefronts has 16 OT channels by 16
+// NT rows; each wavefront takes a contiguous eighth of K, both operands straight into registers, and the eight sums meet in
 // LDS in a fixed order. XT: x's type (fp32, fp16, bf16), quantised here by every workgroup for itself, which costs less
 // than a launch of its own (NT = 1); or -1: x's codes.
-// Bound by the latency of the weights: [1, 4096] by [4096, 4096] (8.9 MB) 7.2 us, 2 of them at the copy rate;
-// [77, 4096] by [8192, 4096] (17.8 MB) 15.5 us, where each wavefront also reads all rows of X for 32 channels.
+// Bound by memory's latency, several times in a row: [1, 4096] by [4096, 4096] (8.9 MB: 1.7 us at the copy rate) 7.8 us as values,
+// whose steps wait for their values and quantise them one after another, 5.5 as codes, whose four steps are on their way
+// together; [77, 4096] by [8192, 4096] (17.8 MB) 16.8 us: one step at a time, which waits for its scales before its last codes
+// are asked for (166 registers with 5 row tiles: one workgroup per CU, which could use 256).
 template <int XB, int OUT, int XT, int OT, int NT>
 __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
   constexpr bool SPLIT = XB == 8;
@@ -61,8 +63,7 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
     int sw[OT], sx[NT];
     XFrag<XB> x[NT];
   };
-  // Every load is a buffer load whose offset is past the end where there is nothing (a row past the last, columns past K): no
-  // branches, so all of a step's loads are on their way together.
+  // Every load is a buffer load whose offset is past the end where there is nothing (a row past the last, columns past K).
   auto rsrc = [](const void* p, uint32_t bytes) __attribute__((always_inline)) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
   };
@@ -71,7 +72,8 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
   const auto rw = rsrc(a.w + (i64)o0 * a.wrow, 16 * OT * a.wrow), rws = rsrc(a.ws + (i64)o0 * a.srow, 16 * OT * a.srow);
   const auto rx = XT < 0 ? rsrc(a.x + n0 * a.xrow, rows * a.xrow) : rsrc(a.x + n0 * a.K * XS, rows * a.K * XS);
   const auto rxs = rsrc(XT < 0 ? a.xs + n0 * a.srow : nullptr, XT < 0 ? rows * a.srow : 0);
-  // More row tiles: a load for every scale byte would be a third of the loads, so the scales of four steps come together
+  // More row tiles: a load for every scale byte would be a third of the loads, so the scales of four steps come together. (The
+  // compiler makes branches of the choice between their words, and waits for the scales ahead of each.)
   mx_u32x4 cw[OT], cx[NT];
   auto load_scales = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(512) k_mx_rows(LinArgs a) {
     }
   };
   if constexpr (NT == 1) {
-    constexpr int U = 4;  // steps loaded at once
+    constexpr int U = 4;  // steps loaded at once (codes; the quantisation of values waits within a step)
     int s = s0;
     for (; s + U <= s1; s += U) {
       Step q[U];
