@@ -180,7 +180,7 @@ int spc_add_norm_mx(const void* x, const void* residual, const void* gamma, cons
                     float eps, int kind, int dtype, int64_t N, int64_t C, int fmt, void* sum, void* codes,
                     void* scales);
 
-/* out [N,Co] = act(x w^T + bias) + residual, fp32 sums (of more than 32 rows of e4m3 x, into a 16-bit out, eight neighbouring
+/* out [N,Co] = act(x w^T + bias) + residual, fp32 sums (of more than 16 rows of e4m3 x, into a 16-bit out, eight neighbouring
  * products may be summed to 2^-13 of the largest of them). w [Co,K]: e2m1 codes and scales, Co a multiple of 32. x: codes of
  * x_fmt with x_scales, or, with x_scales NULL, values of x_dtype that the call quantises to x_fmt. out: values of
  * out_type (SPC_F32/F16/BF16) with out_scales NULL, one rounding, residual [N,Co] of the same type or NULL (out may be the

@@ -537,7 +537,7 @@ template <int XB, int OUT, int TO, int TN, int WO, int WN, int KS, int NS>
 void launch(LinArgs a) {
   constexpr int BO = 16 * TO * WO, BN = 16 * TN * WN;
   const i64 tn = (a.N + BN - 1) / BN, to = (a.O + BO - 1) / BO;
-  REQ(tn * to < (1ll << 30), "%lld rows by %d channels: too many tiles", (long long)a.N, a.O);
+  REQ(tn * to <= (1ll << 24) - 16, "%lld rows by %d channels: more than 2^24 tiles", (long long)a.N, a.O);  // 2^32 threads a launch
   a.tiles_n = (int)tn;
   a.tiles_o = (int)to;
   const i64 whole = a.N / BN * (a.O / BO);
