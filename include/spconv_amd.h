@@ -208,6 +208,39 @@ int spc_convnext_mlp_mx(const void* h, const void* x, const void* gamma, const v
                         const void* w2_scales, const void* b2, int dtype, int param_dtype, int fmt, int64_t N,
                         int64_t C, void* y, void* workspace, int64_t workspace_bytes);
 
+/* Linear layers with a weight matrix per group of rows (experts), and their gradients. Rows ends[g-1] .. ends[g] - 1 (ends[-1] is
+ * 0) belong to group g; ends int32 [G] on the device, not falling; values are taken as within [0, N]. Rows from the last end on
+ * belong to no group: they are not read, and their places in y and dx stay as they were. x [N,K], y, dy [N,Co], w [G,Co,K] of
+ * one `dtype` (SPC_F16/SPC_BF16), 16-byte aligned; K and Co multiples of 8, at most 2^20; G at most 2^16. fp32 sums, one rounding.
+ *   spc_group_linear     y = w[g] x + bias[g]; bias [G,Co] of `b_dtype` or NULL
+ *   spc_group_linear_dx  dx = w[g]^T dy
+ *   spc_group_linear_dw  dw[g] = sum of dy x^T over g's rows (zeros where there are none), db[g] = sum of dy unless db is NULL;
+ *                        dw [G,Co,K], db [G,Co] of `out_dtype`: SPC_F32 or `dtype`
+ * Results overlap no input. No counterpart in the reference; beside spc_mx_linear, whose weight all rows share. */
+int spc_group_linear(const void* x, const void* w, const int32_t* ends, const void* bias, int dtype, int b_dtype, int64_t N,
+                     int64_t G, int64_t K, int64_t Co, void* y);
+int spc_group_linear_dx(const void* dy, const void* w, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
+                        int64_t Co, void* dx);
+int spc_group_linear_dw(const void* dy, const void* x, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
+                        int64_t Co, int out_dtype, void* dw, void* db);
+
+/* Low-rank adapters of many requests beside one shared projection. Row n's adapter is s = slots[n] (int32 [N] on the device;
+ * outside [0, L): none), and it gets scale[s] b[s] (a[s] x[n]) added:
+ *   spc_adapter_linear   out = x w^T + bias + that
+ *   spc_adapter_add      out = y + that, for a projection y made elsewhere (spc_mx_linear's); out may be y
+ * x [N,K], w [Co,K], a [L,R,K], b [L,Co,R], y, out [N,Co] of one `dtype` (SPC_F16/SPC_BF16), 16-byte aligned; R a multiple of 8,
+ * at most 256; K and Co multiples of 8, at most 2^20; L at most 2^16; scale float [L] or NULL (1); bias [Co] of `b_dtype` or
+ * NULL. a x is summed in fp32, scaled and held in `dtype`. workspace: device memory of spc_adapter_workspace's bytes, 16-byte
+ * aligned, or NULL (the library's own; refused while the stream is captured, if any is needed).
+ * No counterpart in the reference; beside spc_mx_linear, the shared projection in 4 bits. */
+int spc_adapter_workspace(int64_t N, int64_t K, int64_t R, int64_t* bytes);
+int spc_adapter_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* slots, const float* scale,
+                       const void* bias, int dtype, int b_dtype, int64_t N, int64_t L, int64_t R, int64_t K, int64_t Co,
+                       void* out, void* workspace, int64_t workspace_bytes);
+int spc_adapter_add(const void* y, const void* x, const void* a, const void* b, const int32_t* slots, const float* scale,
+                    int dtype, int64_t N, int64_t L, int64_t R, int64_t K, int64_t Co, void* out, void* workspace,
+                    int64_t workspace_bytes);
+
 /* Conv and the upsample block's skip connection in one pass: out = act(conv(x, w) + b) + skip with skip[i,c] =
  * x_skip[src[i] >> 3, (src[i] & 7) * Cin/8 + c / rep], rep = Co / (Cin/8) a power of two; fp32 sum, one rounding.
  * x [N,Ci], w [Co,27,Ci], x_skip [n_skip,Cin] (Cin % 64 == 0), out [N,Co]: one 16-bit `dtype`; src int32 [N] (the

@@ -1,0 +1,128 @@
+"""Refusals of the entry points of linear layers with many weights that need no device: each is made before any device call."""
+import ctypes
+
+import pytest
+import torch
+
+import spconv_amd as sp
+
+A = 0x100000  # addresses that nothing reads, 1 MB apart
+
+
+def p(v):
+    return ctypes.c_void_p(v)
+
+
+def refused(rc, word):
+    lib = sp.load_library()
+    assert rc == -1
+    assert word in lib.spc_last_error().decode(), lib.spc_last_error()
+
+
+def test_forward():
+    lib = sp.load_library()
+
+    def call(x=A, w=2 * A, ends=3 * A, bias=None, dt=2, bdt=0, n=4, g=3, k=64, o=72, y=4 * A):
+        return lib.spc_group_linear(p(x), p(w), p(ends), p(bias), dt, bdt, n, g, k, o, p(y))
+
+    refused(call(k=60), "multiple of 8")
+    refused(call(o=70), "multiple of 8")
+    refused(call(k=(1 << 20) + 8), "2^20")
+    refused(call(g=0), "G=0")
+    refused(call(g=(1 << 16) + 1), "groups")
+    refused(call(n=-1), "N=-1")
+    refused(call(n=1 << 31), "rows")
+    refused(call(dt=0), "bf16/fp16")
+    refused(call(dt=5), "dtype code 5")
+    refused(call(x=A + 2), "aligned")
+    refused(call(y=4 * A + 8), "aligned")
+    refused(call(x=None), "null")
+    refused(call(w=None), "null")
+    refused(call(ends=None), "null")
+    refused(call(y=None), "null")
+    refused(call(y=A), "overlap")
+    refused(call(y=2 * A + 16), "overlap")
+    refused(call(y=3 * A), "overlap")
+    refused(call(bias=4 * A + 64), "overlap")
+    refused(call(bias=5 * A, bdt=3), "dtype code 3")
+    assert call(n=0, x=None, y=None) == 0
+
+
+def test_gradients():
+    lib = sp.load_library()
+
+    def dx(dy=A, w=2 * A, ends=3 * A, dt=2, n=4, g=3, k=64, o=72, out=4 * A):
+        return lib.spc_group_linear_dx(p(dy), p(w), p(ends), dt, n, g, k, o, p(out))
+
+    def dw(dy=A, x=2 * A, ends=3 * A, dt=2, n=4, g=3, k=64, o=72, odt=0, out=4 * A, db=5 * A):
+        return lib.spc_group_linear_dw(p(dy), p(x), p(ends), dt, n, g, k, o, odt, p(out), p(db))
+
+    refused(dx(k=4), "multiple of 8")
+    refused(dx(dt=0), "bf16/fp16")
+    refused(dx(out=A + 16), "overlap")
+    refused(dx(out=2 * A), "overlap")
+    refused(dx(w=None), "null")
+    refused(dx(ends=None), "null")
+    assert dx(n=0, dy=None, out=None) == 0
+    refused(dw(o=12), "multiple of 8")
+    refused(dw(odt=1), "fp32 or of dy's type")
+    refused(dw(out=None), "null")
+    refused(dw(out=A), "overlap")
+    refused(dw(out=2 * A), "overlap")
+    refused(dw(db=A), "overlap")
+    refused(dw(db=4 * A + 64), "overlap")
+    refused(dw(db=5 * A + 4), "aligned")
+    refused(dw(x=None), "null")
+    refused(dw(n=1 << 31), "rows")
+
+
+def test_adapters():
+    lib, n = sp.load_library(), ctypes.c_int64()
+    refused(lib.spc_adapter_workspace(4, 64, 0, ctypes.byref(n)), "arguments")
+    refused(lib.spc_adapter_workspace(1 << 31, 64, 8, ctypes.byref(n)), "arguments")
+    refused(lib.spc_adapter_workspace(4, 64, 8, None), "arguments")
+    assert lib.spc_adapter_workspace(0, 64, 8, ctypes.byref(n)) == 0 and n.value == 0
+
+    def linear(x=A, w=2 * A, a=3 * A, b=4 * A, slots=5 * A, scale=None, bias=None, dt=2, bdt=0, n=4, l=3, r=16, k=64, o=72, out=6 * A,
+               work=None, nwork=0):
+        return lib.spc_adapter_linear(p(x), p(w), p(a), p(b), p(slots), p(scale), p(bias), dt, bdt, n, l, r, k, o, p(out), p(work), nwork)
+
+    def add(y=2 * A, x=A, a=3 * A, b=4 * A, slots=5 * A, scale=None, dt=2, n=4, l=3, r=16, k=64, o=72, out=6 * A, work=None, nwork=0):
+        return lib.spc_adapter_add(p(y), p(x), p(a), p(b), p(slots), p(scale), dt, n, l, r, k, o, p(out), p(work), nwork)
+
+    for call in (linear, add):
+        refused(call(r=12), "multiple of 8")
+        refused(call(r=264), "at most 256")
+        refused(call(k=12), "multiple of 8")
+        refused(call(o=12), "multiple of 8")
+        refused(call(l=0), "L=0")
+        refused(call(l=(1 << 16) + 1), "adapters")
+        refused(call(dt=0), "bf16/fp16")
+        refused(call(a=None), "null")
+        refused(call(b=4 * A + 4), "aligned")
+        refused(call(slots=None), "null")
+        refused(call(out=None), "null")
+        refused(call(out=A), "overlap")
+        refused(call(out=3 * A), "overlap")
+        refused(call(out=4 * A), "overlap")
+        refused(call(out=5 * A), "overlap")
+        refused(call(scale=6 * A), "overlap")
+        refused(call(n=1 << 31), "rows")
+        assert call(n=0, x=None, slots=None, out=None, **({"y": None} if call is add else {})) == 0
+    refused(linear(out=2 * A), "overlap")
+    refused(linear(bias=6 * A), "overlap")
+    refused(add(out=2 * A + 16), "apart")
+
+
+def test_binding():
+    x, w = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros((3, 72, 64), dtype=torch.bfloat16)
+    ends, a, b = torch.zeros(3, dtype=torch.int32), torch.zeros((2, 8, 64), dtype=torch.bfloat16), torch.zeros((2, 72, 8), dtype=torch.bfloat16)
+    slots, dy = torch.zeros(4, dtype=torch.int32), torch.zeros((4, 72), dtype=torch.bfloat16)
+    for call in (lambda: sp.group_linear(x, w, ends),  # on the CPU
+                 lambda: sp.group_linear(x, w[0], ends), lambda: sp.group_linear(x, w, ends.long()), lambda: sp.group_linear(x.half(), w, ends),
+                 lambda: sp.group_linear(x, w, ends, bias=dy), lambda: sp.group_linear_dx(x, w, ends),
+                 lambda: sp.group_linear_dw(dy, x[:3], ends), lambda: sp.group_linear_dw(dy, x, ends, out=w, out_dtype=torch.float32),
+                 lambda: sp.adapter_linear(x, w[0], a, b, slots.long()), lambda: sp.adapter_linear(x, w[0], a, b[:1], slots),
+                 lambda: sp.adapter_linear(x, w[0], a, b, slots, scale=torch.ones(3)), lambda: sp.adapter_add(x, x, a, b, slots)):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()

@@ -508,3 +508,68 @@ SPC_API int spc_convnext_mlp_mx(const void* h, const void* x, const void* gamma,
                     fmt, ty, workspace, workspace_bytes);
   });
 }
+
+SPC_API int spc_group_linear(const void* x, const void* w, const int32_t* ends, const void* bias, int dtype, int b_dtype, int64_t N,
+                             int64_t G, int64_t K, int64_t Co, void* y) {
+  return guarded([&] {
+    REQ(N >= 0 && G > 0 && K > 0 && Co > 0, "N=%lld G=%lld K=%lld Co=%lld", (long long)N, (long long)G, (long long)K, (long long)Co);
+    const DT dt = float_dt(dtype, "x/w");
+    Tensor tb, ty = borrow(y, {N, Co}, dt);
+    if (bias) tb = borrow(bias, {G, Co}, float_dt(b_dtype, "bias"));
+    group_linear(borrow(x, {N, K}, dt), borrow(w, {G, Co, K}, dt), borrow(ends, {G}, I32), bias ? &tb : nullptr, ty);
+  });
+}
+
+SPC_API int spc_group_linear_dx(const void* dy, const void* w, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
+                                int64_t Co, void* dx) {
+  return guarded([&] {
+    REQ(N >= 0 && G > 0 && K > 0 && Co > 0, "N=%lld G=%lld K=%lld Co=%lld", (long long)N, (long long)G, (long long)K, (long long)Co);
+    const DT dt = float_dt(dtype, "dy/w");
+    Tensor tx = borrow(dx, {N, K}, dt);
+    group_linear_dx(borrow(dy, {N, Co}, dt), borrow(w, {G, Co, K}, dt), borrow(ends, {G}, I32), tx);
+  });
+}
+
+SPC_API int spc_group_linear_dw(const void* dy, const void* x, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
+                                int64_t Co, int out_dtype, void* dw, void* db) {
+  return guarded([&] {
+    REQ(N >= 0 && G > 0 && K > 0 && Co > 0, "N=%lld G=%lld K=%lld Co=%lld", (long long)N, (long long)G, (long long)K, (long long)Co);
+    const DT dt = float_dt(dtype, "dy/x"), odt = float_dt(out_dtype, "out");
+    Tensor tw = borrow(dw, {G, Co, K}, odt), tb = borrow(db, {G, Co}, odt);
+    group_linear_dw(borrow(dy, {N, Co}, dt), borrow(x, {N, K}, dt), borrow(ends, {G}, I32), tw, db ? &tb : nullptr);
+  });
+}
+
+SPC_API int spc_adapter_workspace(int64_t N, int64_t K, int64_t R, int64_t* bytes) {
+  return guarded([&] {
+    REQ(bytes && N >= 0 && N < (1ll << 31) && K > 0 && K <= (1 << 20) && R > 0 && R <= 256, "arguments");
+    *bytes = adapter_workspace(N, K, R);
+  });
+}
+
+SPC_API int spc_adapter_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* slots, const float* scale,
+                               const void* bias, int dtype, int b_dtype, int64_t N, int64_t L, int64_t R, int64_t K, int64_t Co,
+                               void* out, void* workspace, int64_t workspace_bytes) {
+  return guarded([&] {
+    REQ(N >= 0 && L > 0 && R > 0 && K > 0 && Co > 0, "N=%lld L=%lld R=%lld K=%lld Co=%lld", (long long)N, (long long)L, (long long)R,
+        (long long)K, (long long)Co);
+    const DT dt = float_dt(dtype, "x/w/a/b");
+    Tensor ts = borrow(scale, {L}, F32), tb, to = borrow(out, {N, Co}, dt);
+    if (bias) tb = borrow(bias, {Co}, float_dt(b_dtype, "bias"));
+    adapter_linear(borrow(x, {N, K}, dt), borrow(w, {Co, K}, dt), borrow(a, {L, R, K}, dt), borrow(b, {L, Co, R}, dt), borrow(slots, {N}, I32),
+                   scale ? &ts : nullptr, bias ? &tb : nullptr, to, workspace, workspace_bytes);
+  });
+}
+
+SPC_API int spc_adapter_add(const void* y, const void* x, const void* a, const void* b, const int32_t* slots, const float* scale,
+                            int dtype, int64_t N, int64_t L, int64_t R, int64_t K, int64_t Co, void* out, void* workspace,
+                            int64_t workspace_bytes) {
+  return guarded([&] {
+    REQ(N >= 0 && L > 0 && R > 0 && K > 0 && Co > 0, "N=%lld L=%lld R=%lld K=%lld Co=%lld", (long long)N, (long long)L, (long long)R,
+        (long long)K, (long long)Co);
+    const DT dt = float_dt(dtype, "y/x/a/b");
+    Tensor ts = borrow(scale, {L}, F32), to = borrow(out, {N, Co}, dt);
+    adapter_add(borrow(y, {N, Co}, dt), borrow(x, {N, K}, dt), borrow(a, {L, R, K}, dt), borrow(b, {L, Co, R}, dt), borrow(slots, {N}, I32),
+                scale ? &ts : nullptr, to, workspace, workspace_bytes);
+  });
+}

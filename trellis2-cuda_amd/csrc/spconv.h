@@ -216,6 +216,27 @@ void convnext_mlp_mx(const Tensor& h, const Tensor& x, const Tensor* gamma, cons
                      i64 workspace_bytes = 0);
 i64 convnext_mlp_mx_workspace(i64 N, i64 C, int fmt);
 
+// Linear layers with a weight matrix per group of rows (experts), and their gradients: rows ends[g-1] .. ends[g] - 1 (ends[-1] is 0)
+// belong to group g; ends int32 [G] on the device, not falling, taken as within [0, N]. Rows from the last end on belong to no
+// group: they are not read, and their places in y and dx stay as they were. x [N,K], y, dy [N,O], w [G,O,K] of one 16-bit type,
+// K and O multiples of 8 up to 2^20; fp32 sums, one rounding.
+// y = w[g] x + bias[g] (bias [G,O] of any float type or null); dx = w[g]^T dy; dw[g] = sum of dy x^T over g's rows (zeros for
+// an empty group) and, with db, db[g] = sum of dy; dw [G,O,K] and db [G,O] fp32 or of the inputs' type.
+void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Tensor* bias, Tensor& y);
+void group_linear_dx(const Tensor& dy, const Tensor& w, const Tensor& ends, Tensor& dx);
+void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tensor& dw, Tensor* db);
+
+// Low-rank adapters of many requests beside one shared projection: out = x w^T + bias + scale[s] b[s] (a[s] x) per row, s = slots[n]
+// (int32 [N]; outside [0, L): no adapter), or the same added to a projection y made elsewhere (out may be y). x [N,K], w [O,K],
+// a [L,R,K], b [L,O,R], y, out [N,O] of one 16-bit type, R a multiple of 8 up to 256, K and O multiples of 8 up to 2^20;
+// scale fp32 [L] or null (1); bias [O] of any float type or null. a x is summed in fp32 and held in 16 bits. workspace as for mx_linear, of
+// adapter_workspace() bytes.
+void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
+                    const Tensor* bias, Tensor& out, void* workspace = nullptr, i64 workspace_bytes = 0);
+void adapter_add(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale, Tensor& out,
+                 void* workspace = nullptr, i64 workspace_bytes = 0);
+i64 adapter_workspace(i64 N, i64 K, i64 R);
+
 // Conv plus the upsample block's skip connection in one pass: out = act(conv(x) + b) + skip, skip[i, c] =
 // x_skip[src[i] >> 3, (src[i] & 7) * Cin/8 + c / rep], rep = Co / (Cin/8) a power of two, one rounding (reference:
 // subm_conv then k_add_skip, src/sdec.cu:38-43, 82-84). Fused into the 64 -> 64 halo kernel; other shapes run the

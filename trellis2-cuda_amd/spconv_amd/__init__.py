@@ -37,7 +37,8 @@ SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_get_stream", "spc_build_neig
            "spc_kernel_times", "spc_release_cached_memory", "spc_mx_sizes", "spc_mx_quantize", "spc_mx_dequantize",
            "spc_add_norm_mx", "spc_mx_linear_workspace", "spc_mx_linear_tile",
            "spc_mx_linear", "spc_convnext_mlp_mx_workspace",
-           "spc_convnext_mlp_mx")
+           "spc_convnext_mlp_mx", "spc_group_linear", "spc_group_linear_dx", "spc_group_linear_dw", "spc_adapter_workspace",
+           "spc_adapter_linear", "spc_adapter_add")
 
 _lib = None
 
@@ -98,6 +99,12 @@ def load_library():
     L.spc_mx_linear.argtypes = [P, P, I, I, P, P, P, I, P, I, I64, I64, I64, I, P, P, P, I64]
     L.spc_convnext_mlp_mx_workspace.argtypes = [I64, I64, I, PI64]
     L.spc_convnext_mlp_mx.argtypes = [P, P, P, P, ctypes.c_float, P, P, P, P, P, P, I, I, I, I64, I64, P, P, I64]
+    L.spc_group_linear.argtypes = [P, P, P, P, I, I, I64, I64, I64, I64, P]
+    L.spc_group_linear_dx.argtypes = [P, P, P, I, I64, I64, I64, I64, P]
+    L.spc_group_linear_dw.argtypes = [P, P, P, I, I64, I64, I64, I64, I, P, P]
+    L.spc_adapter_workspace.argtypes = [I64, I64, I64, PI64]
+    L.spc_adapter_linear.argtypes = [P, P, P, P, P, P, P, I, I, I64, I64, I64, I64, I64, P, P, I64]
+    L.spc_adapter_add.argtypes = [P, P, P, P, P, P, I, I64, I64, I64, I64, I64, P, P, I64]
     for name in SYMBOLS:
         if name != "spc_last_error":
             getattr(L, name).restype = I
@@ -590,6 +597,139 @@ def convnext_mlp_mx(h, x, gamma, beta, w1: MxTensor, b1, w2: MxTensor, b2, eps: 
         _adr(h, dev), _adr(x, dev), _adr(gamma, dev), _adr(beta, dev), eps, _adr(w1.codes, dev), _adr(w1.scales, dev),
         _adr(b1, dev), _adr(w2.codes, dev), _adr(w2.scales, dev), _adr(b2, dev), _dt(h), _dt(ps[0]) if ps else F32, fmt, N, C,
         _adr(out, dev), _adr(ws, dev), nws))
+    return out
+
+
+def _groups(ends, w, name="w"):
+    """(G, Co, K) of the weights w [G, Co, K], checked against the groups' ends."""
+    if w.dim() != 3:
+        raise ValueError(f"{name} must be [G, Co, K], got {list(w.shape)}")
+    if ends.dtype != _torch().int32 or ends.shape != w.shape[:1]:
+        raise ValueError(f"ends must be int32 [{w.shape[0]}], got {ends.dtype} {list(ends.shape)}")
+    return w.shape
+
+
+def group_linear(x, w, ends, bias=None, out=None):
+    """y = w[g] x + bias[g] per row with fp32 sums: rows ends[g-1] .. ends[g] - 1 of x [N, K] (ends[-1] is 0) belong to group g
+    of the weights w [G, Co, K] of x's 16-bit type. ends int32 [G] on the device, not falling; groups may be empty. Rows from the last
+    end on belong to no group: they are not read and keep what out [N, Co] held. bias [G, Co] of any float type. K and Co
+    multiples of 8."""
+    torch = _torch()
+    _matrix(x, "x")
+    G, Co, K = _groups(ends, w)
+    N = x.shape[0]
+    if x.shape[1] != K or w.dtype != x.dtype:
+        raise ValueError(f"x must be [N, {K}] of w's type, got {list(x.shape)} {x.dtype}")
+    _vector(bias, "bias", G * Co)
+    if out is None:
+        out = x.new_empty(N, Co)
+    else:
+        _matrix(out, "out", (N, Co), x.dtype)
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_group_linear(_adr(x, dev), _adr(w, dev), _adr(ends, dev), _adr(bias, dev), _dt(x),
+                                           _dt(bias) if bias is not None else F32, N, G, K, Co, _adr(out, dev)))
+    return out
+
+
+def group_linear_dx(dy, w, ends, out=None):
+    """group_linear's gradient of x: w[g]^T dy per row, dy [N, Co], w [G, Co, K], ends as there. Rows of no group keep what out
+    [N, K] held."""
+    torch = _torch()
+    _matrix(dy, "dy")
+    G, Co, K = _groups(ends, w)
+    N = dy.shape[0]
+    if dy.shape[1] != Co or w.dtype != dy.dtype:
+        raise ValueError(f"dy must be [N, {Co}] of w's type, got {list(dy.shape)} {dy.dtype}")
+    if out is None:
+        out = dy.new_empty(N, K)
+    else:
+        _matrix(out, "out", (N, K), dy.dtype)
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_group_linear_dx(_adr(dy, dev), _adr(w, dev), _adr(ends, dev), _dt(dy), N, G, K, Co, _adr(out, dev)))
+    return out
+
+
+def group_linear_dw(dy, x, ends, out=None, out_dtype=None, bias: bool = False):
+    """group_linear's gradient of w: the sum of dy x^T over each group's rows [G, Co, K] (zeros for an empty group), in out_dtype
+    (default: dy's type; float32). With bias, the pair of it and the bias' gradient [G, Co], the sum of dy, in the same type.
+    dy [N, Co], x [N, K], ends as for group_linear."""
+    torch = _torch()
+    _matrix(dy, "dy")
+    N, Co = dy.shape
+    _matrix(x, "x", None, dy.dtype)
+    K = x.shape[1]
+    if x.shape[0] != N:
+        raise ValueError(f"x must have dy's {N} rows, got {x.shape[0]}")
+    if ends.dtype != torch.int32 or ends.dim() != 1:
+        raise ValueError(f"ends must be an int32 vector, got {ends.dtype} {list(ends.shape)}")
+    G = ends.shape[0]
+    if out is None:
+        out = dy.new_empty(G, Co, K, dtype=out_dtype)
+    elif out.shape != (G, Co, K) or out_dtype not in (None, out.dtype):
+        raise ValueError(f"out must be [{G}, {Co}, {K}] of {out_dtype or out.dtype}, got {list(out.shape)} {out.dtype}")
+    db = out.new_empty(G, Co) if bias else None
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_group_linear_dw(_adr(dy, dev), _adr(x, dev), _adr(ends, dev), _dt(dy), N, G, K, Co, _dt(out), _adr(out, dev),
+                                              _adr(db, dev)))
+    return (out, db) if bias else out
+
+
+def _adapters(x, a, b, slots, scale):
+    """(N, L, R, K, Co) of a call with adapters a [L, R, K], b [L, Co, R]."""
+    torch = _torch()
+    _matrix(x, "x")
+    N, K = x.shape
+    if a.dim() != 3 or b.dim() != 3 or a.dtype != x.dtype or b.dtype != x.dtype:
+        raise ValueError("a must be [L, R, K] and b [L, Co, R], of x's type")
+    L, R, ak = a.shape
+    Co = b.shape[1]
+    if ak != K or b.shape != (L, Co, R):
+        raise ValueError(f"a {list(a.shape)} and b {list(b.shape)} do not fit x {list(x.shape)}")
+    if slots.dtype != torch.int32 or slots.shape != (N,):
+        raise ValueError(f"slots must be int32 [{N}], got {slots.dtype} {list(slots.shape)}")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (L,)):
+        raise ValueError(f"scale must be float32 [{L}]")
+    return N, L, R, K, Co
+
+
+def adapter_linear(x, w, a, b, slots, scale=None, bias=None, out=None):
+    """x w^T + bias + scale[s] b[s] (a[s] x) per row with fp32 sums, s = slots[n] the row's adapter (int32 [N]; outside [0, L):
+    none): the projection w [Co, K] that all rows share and low-rank adapters a [L, R, K], b [L, Co, R] of many requests, in
+    any order, all of x's 16-bit type. scale float32 [L] (default 1), bias [Co] of any float type. K and Co multiples of 8, R one
+    up to 256. a[s] x, scaled, is held in x's type between its two products."""
+    torch = _torch()
+    N, L, R, K, Co = _adapters(x, a, b, slots, scale)
+    _matrix(w, "w", (Co, K), x.dtype)
+    _vector(bias, "bias", Co)
+    if out is None:
+        out = x.new_empty(N, Co)
+    else:
+        _matrix(out, "out", (N, Co), x.dtype)
+    nws = _workspace_bytes("spc_adapter_workspace", N, K, R)
+    ws = _workspace(nws, x) if nws else None
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_adapter_linear(
+        _adr(x, dev), _adr(w, dev), _adr(a, dev), _adr(b, dev), _adr(slots, dev), _adr(scale, dev), _adr(bias, dev), _dt(x),
+        _dt(bias) if bias is not None else F32, N, L, R, K, Co, _adr(out, dev), _adr(ws, dev), nws))
+    return out
+
+
+def adapter_add(y, x, a, b, slots, scale=None, out=None):
+    """y + scale[s] b[s] (a[s] x) per row: adapter_linear's adapters beside a projection y [N, Co] of x's type made elsewhere, such
+    as mx_linear's. out may be y."""
+    torch = _torch()
+    N, L, R, K, Co = _adapters(x, a, b, slots, scale)
+    _matrix(y, "y", (N, Co), x.dtype)
+    if out is None:
+        out = torch.empty_like(y)
+    else:
+        _matrix(out, "out", (N, Co), x.dtype)
+    nws = _workspace_bytes("spc_adapter_workspace", N, K, R)
+    ws = _workspace(nws, x) if nws else None
+    dev = torch.cuda.current_device()
+    _check(load_library().spc_adapter_add(
+        _adr(y, dev), _adr(x, dev), _adr(a, dev), _adr(b, dev), _adr(slots, dev), _adr(scale, dev), _dt(x), N, L, R, K, Co, _adr(out, dev),
+        _adr(ws, dev), nws))
     return out
 
 
