@@ -1,21 +1,25 @@
 // Products of groups of rows with a weight matrix each, and their gradients. Rows ends[g-1] .. ends[g] - 1 are group g's.
 //   forward  y[n] = W_g x[n] + b_g        dx[n] = W_g^T dy[n]        dW_g = sum over g's rows of dy[n] x[n]^T, db_g = sum of dy[n]
+#include "ldsdma.h"
 #include "mx.h"
 
-#include <algorithm>
+#include <type_traits>
 
 namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 enum { FORWARD = 0, DX = 1, DW = 2 };
+enum { OUT_16 = 0, OUT_F32 = 1 };
 struct GroupArgs {
-  const void *a, *b, *bias;  // forward: x, w; dx: dy, w; dw: dy, x
+  const void *m, *c, *bias;  // operands of the result's rows and columns: x, w (forward); dy, w (dx); dy, x (dw)
   const int32_t* ends;
   void *out, *db;
   i64 N;
-  int G, K, O, bias_dt, out_f32;
+  int G, K, O, bias_dt;
+  int tiles_m, tiles_c, per, band;
 };
 
 template <bool F16>
@@ -30,83 +34,369 @@ __device__ __forceinline__ void rows_of(const GroupArgs& a, int g, i64& first, i
   count = max(e - s, (i64)0);
 }
 
-// 64 x 64 results per workgroup of 4 wavefronts, operands element by element through LDS
-template <int OP, bool F16>
-__global__ void __launch_bounds__(256) k_group(GroupArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t la[64][40], lb[64][40];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int c0 = blockIdx.x * 64;  // first column of the result
-  i64 first, count, m0 = 0;
-  int g = 0, depth = OP == FORWARD ? a.K : a.O;
-  if (OP == DW) {
-    g = blockIdx.z;
-    rows_of(a, g, first, count);
-    m0 = blockIdx.y * 64;
-    depth = 0;
+constexpr uint32_t kOOR = 0x80000000u;  // past every buffer below, also with a step's offset added: reads as zeros
+
+// This workgroup's tile of the rows' products: group, row tile and column tile. The tiles of all groups stand in one list, a group's in
+// bands of `band` columns, row by row within a band; each XCD takes a contiguous eighth of it, so that the tiles that run
+// beside each other on it share operands in its L2. Every wavefront finds it for itself, 64 groups at a time.
+struct TilePlace {
+  i64 first;  // the group's first row
+  int count, g, tm, tc;
+};
+template <int BM>
+__device__ __forceinline__ bool find_tile(const GroupArgs& a, int lane, TilePlace& at) {
+  auto chunk = [&](int g0, int& first, int& count) __attribute__((always_inline)) {  // lane's group, and the tiles up to its end
+    const int g = g0 + lane, N = (int)a.N;
+    const int s = g > 0 && g < a.G ? min(max(a.ends[g - 1], 0), N) : 0, e = g < a.G ? min(max(a.ends[g], 0), N) : 0;
+    first = s;
+    count = max(e - s, 0);
+    int sum = (int)(((i64)count + BM - 1) / BM);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int below = __shfl_up(sum, d, 64);
+      sum += lane >= d ? below : 0;
+    }
+    return sum;
+  };
+  int first, count, upto = chunk(0, first, count), total = __builtin_amdgcn_readlane(upto, 63);
+  if (a.G > 64) {
+    for (int g0 = 64; g0 < a.G; g0 += 64) total += __builtin_amdgcn_readlane(chunk(g0, first, count), 63);
+    upto = chunk(0, first, count);
+  }
+  const int xcd = blockIdx.x % 8, k = blockIdx.x / 8;
+  const i64 all = (i64)total * a.tiles_c, per = (all + 7) / 8, l = xcd * per + k;
+  if (k >= per || l >= all) return false;
+  const int row_tile = (int)(l / a.tiles_c);
+  int before = 0;
+  for (int g0 = 0;; g0 += 64) {
+    if (g0) upto = chunk(g0, first, count);
+    const uint64_t past = __ballot(before + upto > row_tile);
+    if (past) {
+      const int who = __builtin_ctzll(past);
+      at.g = g0 + who;
+      at.first = __builtin_amdgcn_readlane(first, who);
+      at.count = __builtin_amdgcn_readlane(count, who);
+      if (who) before += __builtin_amdgcn_readlane(upto, who - 1);
+      break;
+    }
+    if (g0 + 64 >= a.G) return false;
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  const int tiles = (int)(((i64)at.count + BM - 1) / BM), inside = (int)(l - (i64)before * a.tiles_c);
+  const int band = inside / (a.band * tiles) * a.band, width = min(a.band, a.tiles_c - band), rest = inside - band * tiles;
+  at.tm = rest / width;
+  at.tc = band + rest % width;
+  return inside >= 0 && at.tm < tiles;
+}
+
+// Tiled products of all three kinds. A workgroup of WC x WM wavefronts has BC = 16 TC WC columns of the result by BM = 16 TM WM rows;
+// the depth goes by stages of 64 through two slots of LDS, filled by DMA. An operand whose depth is contiguous (x and w of the
+// forward product, dy of dx) lies there as rows of 64 values, its 16-byte pieces permuted (piece c of row q at c ^ q % 8), so that
+// eight lanes of neighbouring rows read from distinct banks; one whose depth runs over rows (w of dx, dy and x of dw) as 64 rows, and
+// is transposed on its way into registers (ds_read_b64_tr_b16: 16 lanes give the addresses of 4 rows by four pieces of 4 values, lane i gets
+// column i of the four rows); piece c of row q is at c ^ (4 (q % 4) + 2 (q / 8 % 2)) there.
+//
+// The columns' operand is the matrix instruction's first, so a lane has 4 columns of one row of the result per product, and
+// which channel each of its 16 rows stands for is free: RUN tiles give a lane 4 RUN consecutive columns.
+//
+// A step's (32 deep) products go in four quarters, halves of the column tiles by halves of the row tiles, in the order (0, f),
+// (0, 1 - f), (1, 1 - f), (1, f) with f = 0, 1 in turn: each quarter changes one operand's half, whose registers were free a quarter
+// earlier, so every LDS read is issued one quarter before its use and a wavefront holds one step's operands only. In the
+// middle of a stage's second step all wavefronts meet: by then each has read the whole slot, so it is filled again at once.
+template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM>
+__global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
+  constexpr bool MT = OP == DW, CT = OP != FORWARD;  // transposed: the rows' operand, the columns'
+  constexpr int NW = WC * WM, BC = 16 * TC * WC, BM = 16 * TM * WM, HC = TC / 2, HM = TM / 2;
+  constexpr int RUN = OUT == OUT_F32 ? 1 : 2;
+  constexpr int MI = BM / 8 / NW, CI = BC / 8 / NW;  // DMAs per wavefront and stage
+  static_assert(MI * 8 * NW == BM && CI * 8 * NW == BC && TC % 2 == 0 && TM % 2 == 0 && HC % RUN == 0, "whole DMAs, halves of whole runs");
+  constexpr uint32_t kC = BM * 128, kSlot = (BM + BC) * 128;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kSlot];
+
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wc = wave % WC, wm = wave / WC;
+  TilePlace at;
+  if constexpr (OP == DW) {
+    const int b = blockIdx.x;
+    int inside;
+    if (a.per) {  // many tiles a group: each XCD takes a contiguous eighth of every group's
+      at.g = b / 8 / a.per;
+      inside = b % 8 * a.per + b / 8 % a.per;
+      if (inside >= a.tiles_m * a.tiles_c) return;
+    } else {
+      at.g = b / (a.tiles_m * a.tiles_c);
+      inside = b % (a.tiles_m * a.tiles_c);
+    }
+    at.tm = inside / a.tiles_c;
+    at.tc = inside % a.tiles_c;
+    i64 count;
+    rows_of(a, at.g, at.first, count);
+    at.count = (int)count;
   } else {
-    i64 t = blockIdx.y;
-    for (; g < a.G; g++) {
-      rows_of(a, g, first, count);
-      const i64 tiles = (count + 63) / 64;
-      if (t < tiles) break;
-      t -= tiles;
-    }
-    if (g == a.G) return;
-    m0 = t * 64;
+    if (!find_tile<BM>(a, lane, at)) return;
   }
-  const i64 inner = OP == DW ? count : depth, rows = OP == DW ? a.O : count;
-  const int cols = OP == FORWARD ? a.O : a.K;
-  const uint16_t *pa = (const uint16_t*)a.a, *pb = (const uint16_t*)a.b;
-  const i64 wbase = (i64)g * a.O * a.K;
-  f32x4 acc[4] = {};
-  float sum = 0.f;
-  for (i64 k0 = 0; k0 < inner; k0 += 32) {
-    for (int i = tid; i < 64 * 32; i += 256) {
-      const int r = OP == DW ? i % 64 : i / 32, k = OP == DW ? i / 64 : i % 32;
-      const bool in = m0 + r < rows && k0 + k < inner;
-      la[r][k] = !in ? 0 : OP == DW ? pa[(first + k0 + k) * a.O + m0 + r] : pa[(first + m0 + r) * depth + k0 + k];
+  const int depth = OP == FORWARD ? a.K : OP == DX ? a.O : at.count;
+  const int m0 = at.tm * BM, c0 = at.tc * BC;
+  const int ncols = OP == FORWARD ? a.O : a.K;
+  const int rows = min(BM, (OP == DW ? a.O : at.count) - m0), cols = min(BC, ncols - c0);
+  const int stages = (depth + 63) / 64;
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)&lds[0];
+
+  // operands: first byte, bytes of a row; direct ones with a descriptor of this tile's rows, transposed ones with one of a stage's
+  const int mrow = (OP == FORWARD ? a.K : a.O) * 2, crow = a.K * 2;
+  const char* const mp = (const char*)a.m + (OP == DW ? at.first * mrow + m0 * 2 : (at.first + m0) * mrow);
+  const char* const cp = (const char*)a.c + (OP == FORWARD ? ((i64)at.g * a.O + c0) * crow : OP == DX ? (i64)at.g * a.O * crow + c0 * 2 : at.first * crow + c0 * 2);
+  const i32x4 rm = rsrc4(mp, (uint32_t)(rows * mrow)), rc = rsrc4(cp, (uint32_t)(cols * crow));
+
+  // the channel of the first operand's row p (direct) or of its columns' piece q of tile t
+  auto channel = [&](int p) __attribute__((always_inline)) {
+    const int t = p / 16 % TC, r = p % 16;
+    return p / (16 * TC) * (16 * TC) + t / RUN * (16 * RUN) + r / 4 * (4 * RUN) + t % RUN * 4 + r % 4;
+  };
+  auto swizzle = [](int row) __attribute__((always_inline)) { return (row & 3) << 2 | (row >> 3 & 1) << 1; };
+  uint32_t moff[MI], coff[CI];
+#pragma unroll
+  for (int k = 0; k < MI; k++) {
+    const int p = (wave * MI + k) * 64 + lane;
+    if constexpr (MT) {
+      const int q = p / (BM / 8), c = p % (BM / 8) ^ swizzle(q);
+      moff[k] = c * 8 < rows ? (uint32_t)(q * mrow + c * 16) : kOOR;
+    } else {
+      const int q = p / 8;
+      moff[k] = q < rows ? (uint32_t)(q * mrow + (p % 8 ^ (q & 7)) * 16) : kOOR;
     }
-    for (int i = tid; i < 64 * 32; i += 256) {
-      const int c = OP == FORWARD ? i / 32 : i % 64, k = OP == FORWARD ? i % 32 : i / 64;
-      const bool in = c0 + c < cols && k0 + k < inner;
-      lb[c][k] = !in ? 0 : OP == FORWARD ? pb[wbase + (i64)(c0 + c) * a.K + k0 + k] : OP == DX ? pb[wbase + (k0 + k) * a.K + c0 + c]
-                                                                                         : pb[(first + k0 + k) * a.K + c0 + c];
-    }
-    __syncthreads();
-    const mx_u32x4 fb = *(const mx_u32x4*)&lb[wave * 16 + lane % 16][lane / 16 * 8];
-    for (int t = 0; t < 4; t++) acc[t] = mfma<F16>(fb, *(const mx_u32x4*)&la[t * 16 + lane % 16][lane / 16 * 8], acc[t]);
-    if (OP == DW && tid < 64)
-      for (int k = 0; k < 32; k++) sum += mx_lo<F16>(la[tid][k]);
-    __syncthreads();
   }
-  for (int t = 0; t < 4; t++)
-    for (int i = 0; i < 4; i++) {
-      const i64 m = m0 + t * 16 + lane % 16;
-      const int c = c0 + wave * 16 + lane / 16 * 4 + i;
+#pragma unroll
+  for (int k = 0; k < CI; k++) {
+    const int p = (wave * CI + k) * 64 + lane;
+    if constexpr (CT) {
+      const int q = p / (BC / 8), c = p % (BC / 8) ^ swizzle(q);
+      coff[k] = c * 8 < cols ? (uint32_t)(q * crow + c * 16) : kOOR;
+    } else {
+      const int q = p / 8, ch = channel(q);
+      coff[k] = ch < cols ? (uint32_t)(ch * crow + (p % 8 ^ (q & 7)) * 16) : kOOR;
+    }
+  }
+  // fills stage t's slot; past the last one the DMAs still run (the waits count them) but read nothing
+  auto issue = [&](int t, int slot) __attribute__((always_inline)) {
+    const bool live = t < stages;
+    const uint32_t base = lds0 + slot * kSlot;
+    const int left = live ? min(64, depth - t * 64) : 0;  // of the depth
+    auto fill = [&](auto TC_, auto NC, const char* p, i32x4 r, int row, int width, const uint32_t* off, uint32_t to) __attribute__((always_inline)) {
+      constexpr int N = decltype(NC)::value;
+      if constexpr (decltype(TC_)::value) {  // rows t * 64 ..: `left` of them
+        const i32x4 rs = rsrc4(p + (i64)t * 64 * row, left ? (uint32_t)((left - 1) * row + width * 2) : 0);
+#pragma unroll
+        for (int k = 0; k < N; k++) dma16(rs, to + (wave * N + k) * 1024, off[k], 0);
+      } else {
+        r[2] = live ? r[2] : 0;
+        const int s = live ? t * 128 : 0;
+        if (live && left < 64) {  // pieces past the last column read as zeros
+          int l = lane;
+          asm volatile("" : "+v"(l));
+#pragma unroll
+          for (int k = 0; k < N; k++) {
+            const int u = (wave * N + k) * 64 + l;
+            dma16(r, to + (wave * N + k) * 1024, (u % 8 ^ (u / 8 & 7)) * 8 < left ? off[k] : kOOR, s);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; k++) dma16(r, to + (wave * N + k) * 1024, off[k], s);
+        }
+      }
+    };
+    fill(std::bool_constant<MT>{}, std::integral_constant<int, MI>{}, mp, rm, mrow, rows, moff, base);
+    fill(std::bool_constant<CT>{}, std::integral_constant<int, CI>{}, cp, rc, crow, cols, coff, base + kC);
+  };
+
+  f32x4 acc[TC][TM];
+#pragma unroll
+  for (int t = 0; t < TC; t++)
+#pragma unroll
+    for (int u = 0; u < TM; u++) acc[t][u] = f32x4{};
+  f32x4 accb[OP == DW ? TM : 1];
+#pragma unroll
+  for (int u = 0; u < (OP == DW ? TM : 1); u++) accb[u] = f32x4{};
+  const bool with_db = OP == DW && a.db && at.tc == 0 && wc == 0;
+
+  // LDS addresses. Direct: row (tile, r16), piece 4 j + g. Transposed: rows 32 j + 8 g + r16 / 4 and 4 further, the piece of 4 columns
+  // r16 % 4 of the tile, whose place the swizzle scatters: one address per tile (pair of tiles where a piece holds columns of both).
+  const int mq = wm * (16 * TM) + r16, cq = wc * (16 * TC) + r16;
+  uint32_t ma[MT ? TM : 2], ca[CT ? TC / RUN : 2];
+  auto transposed = [&](int width, int col) __attribute__((always_inline)) {  // col: the lane's first column in the operand's tile
+    const int row = 8 * g + r16 / 4;
+    return (uint32_t)(row * width * 2 + ((col / 8) ^ swizzle(row)) * 16 + col % 8 * 2);
+  };
+  if constexpr (MT) {
+#pragma unroll
+    for (int t = 0; t < TM; t++) ma[t] = lds0 + transposed(BM, wm * (16 * TM) + t * 16 + r16 % 4 * 4);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; j++) ma[j] = lds0 + (mq * 8 + ((4 * j + g) ^ (r16 & 7))) * 16;
+  }
+  if constexpr (CT) {
+#pragma unroll
+    for (int t = 0; t < TC / RUN; t++) ca[t] = lds0 + kC + transposed(BC, wc * (16 * TC) + t * (16 * RUN) + r16 % 4 * (4 * RUN));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; j++) ca[j] = lds0 + kC + (cq * 8 + ((4 * j + g) ^ (r16 & 7))) * 16;
+  }
+  auto read16 = [](uint32_t at) __attribute__((always_inline)) { return *(__attribute__((address_space(3))) mx_u32x4*)(size_t)at; };
+  auto read_tr = [](uint32_t at) __attribute__((always_inline)) {
+    return __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)at));
+  };
+  auto read_m = [&](mx_u32x4(&f)[HM], int slot, int j, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < HM; u++) {
+      const int t = half * HM + u;
+      if constexpr (MT) {
+        const uint32_t p = ma[t] + slot * kSlot + j * (32 * BM * 2);
+        const mx_u32x2 lo = read_tr(p), hi = read_tr(p + 4 * BM * 2);
+        f[u] = mx_u32x4{lo[0], lo[1], hi[0], hi[1]};
+      } else {
+        f[u] = read16(ma[j] + slot * kSlot + t * 2048);
+      }
+    }
+  };
+  auto read_c = [&](mx_u32x4(&f)[HC], int slot, int j, int half) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < HC; u++) {
+      const int t = half * HC + u;
+      if constexpr (CT) {
+        const uint32_t p = ca[t / RUN] + slot * kSlot + j * (32 * BC * 2) + t % RUN * 8;
+        const mx_u32x2 lo = read_tr(p), hi = read_tr(p + 4 * BC * 2);
+        f[u] = mx_u32x4{lo[0], lo[1], hi[0], hi[1]};
+      } else {
+        f[u] = read16(ca[j] + slot * kSlot + t * 2048);
+      }
+    }
+  };
+
+  mx_u32x4 fm[2][HM], fc[2][HC];
+  // which halves of this wavefront's part hold anything
+  const bool ml[2] = {wm * (16 * TM) < rows, wm * (16 * TM) + 16 * HM < rows};
+  const bool cl[2] = {wc * (16 * TC) < cols, wc * (16 * TC) + 16 * HC < cols};
+  const mx_u32x4 ones = F16 ? mx_u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : mx_u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  int cur = 0;
+  auto step = [&](auto JC, int s) __attribute__((always_inline)) {
+    constexpr int J = decltype(JC)::value, f = J;  // step J of stage s
+    auto quarter = [&](auto CC, auto MC) __attribute__((always_inline)) {
+      constexpr int hc = decltype(CC)::value, hm = decltype(MC)::value;
+      if (ml[hm] && cl[hc]) {
+#pragma unroll
+        for (int u = 0; u < HM; u++)
+#pragma unroll
+          for (int t = 0; t < HC; t++) {
+            f32x4& c = acc[hc * HC + t][hm * HM + u];
+            c = mfma<F16>(fc[hc][t], fm[hm][u], c);
+          }
+      }
+      if constexpr (OP == DW && hc == 0) {
+        if (with_db) {
+#pragma unroll
+          for (int u = 0; u < HM; u++) accb[hm * HM + u] = mfma<F16>(ones, fm[hm][u], accb[hm * HM + u]);
+        }
+      }
+    };
+    constexpr std::integral_constant<int, 0> first{};
+    constexpr std::integral_constant<int, 1> second{};
+    constexpr std::integral_constant<int, f> mf{};
+    constexpr std::integral_constant<int, 1 - f> mo{};
+    read_m(fm[1 - f], cur, J, 1 - f);
+    read_c(fc[1], cur, J, 1);
+    quarter(first, mf);
+    __builtin_amdgcn_sched_barrier(0);
+    quarter(first, mo);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (J == 1) {  // the next stage has landed, and this one is in registers
+      wait_vm<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      bare_barrier();
+      issue(s + 2, cur);
+      cur ^= 1;
+    }
+    read_c(fc[0], cur, 1 - J, 0);
+    quarter(second, mo);
+    __builtin_amdgcn_sched_barrier(0);
+    read_m(fm[1 - f], cur, 1 - J, 1 - f);
+    quarter(second, mf);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (stages) {
+    issue(0, 0);
+    issue(1, 1);
+    wait_vm<MI + CI>();
+    bare_barrier();
+    read_m(fm[0], 0, 0, 0);
+    read_c(fc[0], 0, 0, 0);
+    for (int s = 0; s < stages; s++) {
+      step(std::integral_constant<int, 0>{}, s);
+      step(std::integral_constant<int, 1>{}, s);
+    }
+    wait_vm<0>();  // nothing lands in LDS after the workgroup has gone
+  }
+
+  const i64 obase = OP == DW ? ((i64)at.g * a.O + m0) * a.K : (at.first + m0) * ncols;
+#pragma unroll
+  for (int run = 0; run < TC / RUN; run++) {
+    const int c = wc * (16 * TC) + run * (16 * RUN) + g * (4 * RUN);
+    float bias[4 * RUN];
+    mx_params<4 * RUN>(OP == FORWARD && c < cols ? a.bias : nullptr, a.bias_dt, (i64)at.g * a.O + c0 + c, 0.f, bias);
+#pragma unroll
+    for (int u = 0; u < TM; u++) {
+      const int m = mq + u * 16;
       if (m >= rows || c >= cols) continue;
-      float bias[1];
-      mx_params<1>(a.bias, a.bias_dt, (i64)g * a.O + c, 0.f, bias);
-      const float v = acc[t][i] + bias[0];
-      const i64 at = OP == DW ? wbase + m * a.K + c : (first + m) * cols + c;
-      if (a.out_f32) ((float*)a.out)[at] = v;
-      else ((uint16_t*)a.out)[at] = (uint16_t)mx_pack2<F16>(v, 0.f);
+      float v[4 * RUN];
+#pragma unroll
+      for (int j = 0; j < RUN; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[j * 4 + i] = acc[run * RUN + j][u][i] + bias[j * 4 + i];
+      const i64 to = obase + (i64)m * ncols + c0 + c;
+      if constexpr (OUT == OUT_F32) *(f32x4*)((float*)a.out + to) = f32x4{v[0], v[1], v[2], v[3]};
+      else *(mx_u32x4*)((uint16_t*)a.out + to) = mx_pack8<F16>(*(float(*)[8])v);
     }
-  if (OP == DW && a.db && blockIdx.x == 0 && tid < 64 && m0 + tid < rows) {
-    const i64 at = (i64)g * a.O + m0 + tid;
-    if (a.out_f32) ((float*)a.db)[at] = sum;
-    else ((uint16_t*)a.db)[at] = (uint16_t)mx_pack2<F16>(sum, 0.f);
+  }
+  if constexpr (OP == DW) {
+    if (with_db && g == 0) {
+#pragma unroll
+      for (int u = 0; u < TM; u++) {
+        const int m = mq + u * 16;
+        if (m >= rows) continue;
+        const i64 to = (i64)at.g * a.O + m0 + m;
+        if constexpr (OUT == OUT_F32) ((float*)a.db)[to] = accb[u][0];
+        else ((uint16_t*)a.db)[to] = (uint16_t)mx_pack2<F16>(accb[u][0], 0.f);
+      }
+    }
   }
 }
 
-template <int OP>
-void launch(const GroupArgs& a, DT dt) {
-  const int cols = OP == FORWARD ? a.O : a.K;
-  const i64 tiles = a.N / 64 + a.G;  // the sum over groups of ceil(rows / 64) is at most this
-  REQ(OP == DW || tiles <= 65535, "%lld rows", (long long)a.N);
-  const dim3 grid(cdiv(cols, 64), OP == DW ? cdiv(a.O, 64) : (unsigned)tiles, OP == DW ? a.G : 1);
-  if (dt == F16) k_group<OP, true><<<grid, 256, 0, stream()>>>(a);
-  else k_group<OP, false><<<grid, 256, 0, stream()>>>(a);
+template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM>
+void launch_tile(GroupArgs a) {
+  constexpr int BC = 16 * TC * WC, BM = 16 * TM * WM;
+  a.tiles_c = cdiv(OP == FORWARD ? a.O : a.K, BC);
+  a.band = 4;
+  i64 blocks;
+  if (OP == DW) {
+    a.tiles_m = cdiv(a.O, BM);
+    const i64 tiles = (i64)a.tiles_m * a.tiles_c;
+    a.per = tiles >= 64 ? (int)((tiles + 7) / 8) : 0;
+    blocks = a.per ? 8ll * a.per * a.G : tiles * a.G;
+  } else {  // the sum over groups of ceil(rows / BM) is at most this
+    blocks = ((a.N / BM + a.G) * a.tiles_c + 7) / 8 * 8;
+  }
+  REQ(blocks * 64 * WC * WM < (1ll << 32), "%lld tiles: too many for a launch", (long long)blocks);
+  k_group_tile<OP, F16, OUT, TC, TM, WC, WM><<<(unsigned)blocks, 64 * WC * WM, 0, stream()>>>(a);
   CK(hipGetLastError());
+}
+template <int OP>
+void launch(const GroupArgs& a, DT dt, bool f32 = false) {
+  auto by = [&](auto F, auto T) { launch_tile<OP, decltype(F)::value, decltype(T)::value, 8, 4, 2, 4>(a); };
+  constexpr std::integral_constant<int, OUT_16> o16{};
+  constexpr std::integral_constant<int, OUT_F32> o32{};
+  if constexpr (OP == DW) {
+    if (f32) return dt == F16 ? by(std::true_type{}, o32) : by(std::false_type{}, o32);
+  }
+  dt == F16 ? by(std::true_type{}, o16) : by(std::false_type{}, o16);
 }
 
 constexpr i64 kWidest = 1 << 20, kMostGroups = 1 << 16;
@@ -150,7 +440,7 @@ void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Te
     REQ(bias->numel() == G * O && bias->p && (bias->dt == F32 || bias->dt == F16 || bias->dt == BF16), "bias must have %lld elements", (long long)(G * O));
   for (const Tensor* t : {&x, &w, &ends, bias}) apart(y, t, "out");
   if (N == 0) return;
-  GroupArgs a{x.p, w.p, bias ? bias->p : nullptr, ends.ptr<int32_t>(), y.p, nullptr, N, (int)G, (int)K, (int)O, bias ? bias->dt : F32, 0};
+  GroupArgs a{x.p, w.p, bias ? bias->p : nullptr, ends.ptr<int32_t>(), y.p, nullptr, N, (int)G, (int)K, (int)O, bias ? bias->dt : F32};
   launch<FORWARD>(a, x.dt);
 }
 
@@ -165,7 +455,7 @@ void group_linear_dx(const Tensor& dy, const Tensor& w, const Tensor& ends, Tens
   check_ends(ends, G);
   for (const Tensor* t : {&dy, &w, &ends}) apart(dx, t, "out");
   if (N == 0) return;
-  GroupArgs a{dy.p, w.p, nullptr, ends.ptr<int32_t>(), dx.p, nullptr, N, (int)G, (int)K, (int)O, F32, 0};
+  GroupArgs a{dy.p, w.p, nullptr, ends.ptr<int32_t>(), dx.p, nullptr, N, (int)G, (int)K, (int)O, F32};
   launch<DX>(a, dy.dt);
 }
 
@@ -184,6 +474,6 @@ void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tens
         (long long)(G * O));
     for (const Tensor* t : std::initializer_list<const Tensor*>{&dy, &x, &ends, &dw}) apart(*db, t, "the bias' gradient");
   }
-  GroupArgs a{dy.p, x.p, nullptr, ends.ptr<int32_t>(), dw.p, db ? db->p : nullptr, N, (int)G, (int)K, (int)O, F32, dw.dt == F32};
-  launch<DW>(a, dy.dt);
+  GroupArgs a{dy.p, x.p, nullptr, ends.ptr<int32_t>(), dw.p, db ? db->p : nullptr, N, (int)G, (int)K, (int)O, F32};
+  launch<DW>(a, dy.dt, dw.dt == F32);
 }
