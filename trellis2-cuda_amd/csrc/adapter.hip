@@ -1,45 +1,167 @@
 // Low-rank adapters of many requests beside one shared projection: with s = slots[n], row n gets scale[s] B_s (A_s x[n]) added to its
 // projection; a slot outside [0, L) is no adapter.
-#include "mx.h"
+#include "group.h"
+
+#include <algorithm>
 
 namespace {
-struct AdapterArgs {
-  const void *x, *w, *a, *b, *y, *bias;
-  const int32_t* slots;
-  const float* scale;
-  void* out;
-  i64 N;
-  int L, R, K, O, bias_dt;
-};
-
-// One workgroup a row: h = A_s x[n] by wavefronts, then every thread its channels
-template <bool F16>
-__global__ void __launch_bounds__(256) k_adapter(AdapterArgs a) {
-  __shared__ float h[256];
-  const i64 n = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, s = a.slots[n];
-  const bool has = s >= 0 && s < a.L;
-  const uint16_t* x = (const uint16_t*)a.x + n * a.K;
-  if (has)
-    for (int r = wave; r < a.R; r += 4) {
-      const uint16_t* row = (const uint16_t*)a.a + ((i64)s * a.R + r) * a.K;
-      float v = 0.f;
-      for (int k = lane; k < a.K; k += 64) v += mx_lo<F16>(x[k]) * mx_lo<F16>(row[k]);
-      for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-      if (lane == 0) h[r] = v * (a.scale ? a.scale[s] : 1.f);
+// The first product, h = x a[s]^T per row (not scaled yet): 16 U rows per workgroup and one of `parts` parts of the depth, up to 16 RT ranks
+// (blockIdx.z: which). Its 8 wavefronts share the part out, and their sums meet in LDS in a fixed order. Every adapter that some of the
+// rows have takes its turn; a lane keeps what is its row's.
+template <bool F16, int U, int RT>
+__global__ void __launch_bounds__(512) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, float* h, i64 N, int L, int R, int K) {
+  constexpr int NW = 8;
+  __shared__ f32x4 sums[NW][U * RT][64];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const i64 n0 = (i64)blockIdx.x * (16 * U);
+  const int rows = (int)min((i64)(16 * U), N - n0), r0 = blockIdx.z * (16 * RT), ranks = min(16 * RT, R - r0);
+  int mine = lane < rows && lane < 16 * U ? slots[n0 + lane] : -1;
+  mine = mine < L ? mine : -1;
+  int slot[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) slot[u] = __shfl(mine, u * 16 + r16, 64);
+  const int S = (K + 31) / 32, pieces = gridDim.y * NW, piece = blockIdx.y * NW + wave;
+  const int s0 = (int)((i64)S * piece / pieces), s1 = (int)((i64)S * (piece + 1) / pieces);
+  const auto rx = buffer(x + n0 * K, (uint32_t)(rows * K * 2));
+  uint32_t xo[U], ao[RT];
+#pragma unroll
+  for (int u = 0; u < U; u++) xo[u] = slot[u] >= 0 ? (uint32_t)((u * 16 + r16) * K * 2 + g * 16) : kOOR;
+#pragma unroll
+  for (int t = 0; t < RT; t++) ao[t] = t * 16 + r16 < ranks ? (uint32_t)((t * 16 + r16) * K * 2 + g * 16) : kOOR;
+  f32x4 keep[U][RT];
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int t = 0; t < RT; t++) keep[u][t] = f32x4{};
+  struct Step {
+    mx_u32x4 a[RT], x[U];
+  };
+  for (uint64_t left = __ballot(mine >= 0); left;) {
+    const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    left &= ~__ballot(mine == s);
+    const auto ra = buffer(a + ((i64)s * R + r0) * K, (uint32_t)(ranks * K * 2));
+    f32x4 acc[U][RT];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int t = 0; t < RT; t++) acc[u][t] = f32x4{};
+    constexpr int AT = 4;  // steps on their way together
+    for (int k = s0; k < s1; k += AT) {
+      Step q[AT];
+#pragma unroll
+      for (int i = 0; i < AT; i++) {
+        const bool in = k + i < s1 && (k + i) * 32 + g * 8 < K;
+#pragma unroll
+        for (int t = 0; t < RT; t++) q[i].a[t] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? ao[t] : kOOR, (k + i) * 64, 0);
+#pragma unroll
+        for (int u = 0; u < U; u++) q[i].x[u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u] : kOOR, (k + i) * 64, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < AT; i++)
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+          for (int t = 0; t < RT; t++) acc[u][t] = mfma<F16>(q[i].a[t], q[i].x[u], acc[u][t]);
     }
-  __syncthreads();
-  for (int o = tid; o < a.O; o += 256) {
-    float v[1] = {0.f}, acc = 0.f;
-    mx_params<1>(a.bias, a.bias_dt, o, 0.f, v);
-    if (a.w)
-      for (int k = 0; k < a.K; k++) acc += mx_lo<F16>(x[k]) * mx_lo<F16>(((const uint16_t*)a.w)[(i64)o * a.K + k]);
-    else acc = mx_lo<F16>(((const uint16_t*)a.y)[n * a.O + o]);
-    acc += v[0];
-    if (has)
-      for (int r = 0; r < a.R; r++) acc += h[r] * mx_lo<F16>(((const uint16_t*)a.b)[((i64)s * a.O + o) * a.R + r]);
-    ((uint16_t*)a.out)[n * a.O + o] = (uint16_t)mx_pack2<F16>(acc, 0.f);
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int t = 0; t < RT; t++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) keep[u][t][i] = slot[u] == s ? acc[u][t][i] : keep[u][t][i];
   }
+#pragma unroll
+  for (int u = 0; u < U; u++)
+#pragma unroll
+    for (int t = 0; t < RT; t++) sums[wave][u * RT + t][lane] = keep[u][t];
+  __syncthreads();
+  for (int q = wave; q < U * RT; q += NW) {
+    f32x4 c = sums[0][q][lane];
+#pragma unroll
+    for (int w = 1; w < NW; w++) c += sums[w][q][lane];
+    const int n = q / RT * 16 + r16, r = q % RT * 16 + g * 4;
+    if (n < rows && r < ranks) *(f32x4*)(h + ((i64)blockIdx.y * N + n0 + n) * R + r0 + r) = c;
+  }
+}
+
+// out = y + scale b[s] h: 16 TM rows by 16 TC channels per wavefront, four wavefronts beside each other
+template <bool F16, int TC, int TM>
+__global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
+  const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const i64 n0 = (i64)(blockIdx.x / a.tiles_c) * (16 * TM);
+  const int rows = (int)min((i64)(16 * TM), a.N - n0), c0 = (blockIdx.x % a.tiles_c * 4 + wave) * (16 * TC), cols = min(16 * TC, a.O - c0);
+  if (cols <= 0) return;
+  const auto ry = buffer((const uint16_t*)a.m + n0 * a.O + c0, (uint32_t)(((rows - 1) * a.O + cols) * 2));
+  mx_u32x4 y[TC / 2][TM];
+#pragma unroll
+  for (int t = 0; t < TC / 2; t++)
+#pragma unroll
+    for (int u = 0; u < TM; u++) {
+      const int c = t * 32 + g * 8, m = u * 16 + r16;
+      y[t][u] = __builtin_amdgcn_raw_buffer_load_b128(ry, c < cols && m < rows ? (uint32_t)((m * a.O + c) * 2) : kOOR, 0, 0);
+    }
+  f32x4 acc[TC][TM];
+#pragma unroll
+  for (int t = 0; t < TC; t++)
+#pragma unroll
+    for (int u = 0; u < TM; u++) acc[t][u] = f32x4{};
+  add_adapters<F16>(a, acc, n0, rows, c0, cols, lane,
+                    [&](int t) __attribute__((always_inline)) { return t / 2 * 32 + r16 / 4 * 8 + t % 2 * 4 + r16 % 4; });
+#pragma unroll
+  for (int t = 0; t < TC / 2; t++)
+#pragma unroll
+    for (int u = 0; u < TM; u++) {
+      const int c = t * 32 + g * 8, m = u * 16 + r16;
+      if (c >= cols || m >= rows) continue;
+      float v[8];
+      mx_unpack8<F16>(y[t][u], v);
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] += acc[t * 2 + j / 4][u][j % 4];
+      *(mx_u32x4*)((uint16_t*)a.out + (n0 + m) * a.O + c0 + c) = mx_pack8<F16>(v);
+    }
+}
+
+template <bool F16>
+void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, float* h, int parts) {
+  const i64 N = x.size(0);
+  const int L = (int)a.size(0), R = (int)a.size(1), K = (int)a.size(2);
+  auto go = [&](auto UC, auto RC) {
+    constexpr int U = decltype(UC)::value, RT = decltype(RC)::value;
+    const dim3 grid((unsigned)((N + 16 * U - 1) / (16 * U)), parts, cdiv(R, 16 * RT));
+    REQ((i64)grid.x * grid.y * grid.z * 512 < (1ll << 32), "%lld rows: too many for a launch", (long long)N);
+    k_adapter_in<F16, U, RT><<<grid, 512, 0, stream()>>>(x.ptr<uint16_t>(), a.ptr<uint16_t>(), slots.ptr<int32_t>(), h, N, L, R, K);
+    CK(hipGetLastError());
+  };
+  auto by = [&](auto UC) {
+    if (R <= 16) go(UC, std::integral_constant<int, 1>{});
+    else if (R <= 32) go(UC, std::integral_constant<int, 2>{});
+    else go(UC, std::integral_constant<int, 4>{});
+  };
+  if (N <= 128) by(std::integral_constant<int, 1>{});
+  else by(std::integral_constant<int, 2>{});
+}
+template <bool F16>
+void launch_add(const GroupArgs& a) {
+  auto go = [&](auto TCC, auto TMC) {
+    constexpr int TC = decltype(TCC)::value, TM = decltype(TMC)::value;
+    const i64 tiles = (a.N + 16 * TM - 1) / (16 * TM);
+    GroupArgs p = a;
+    p.tiles_c = cdiv(a.O, 64 * TC);
+    const i64 blocks = tiles * p.tiles_c;
+    REQ(blocks * 256 < (1ll << 32), "%lld rows by %d channels: too many for a launch", (long long)a.N, a.O);
+    k_adapter_add<F16, TC, TM><<<(unsigned)blocks, 256, 0, stream()>>>(p);
+    CK(hipGetLastError());
+  };
+  if (a.N <= 1024) go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+  else go(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+}
+
+// Parts of the depth: enough workgroups for the CUs, each wavefront a step of 32 at least
+int adapter_parts(i64 N, i64 K) {
+  const i64 tiles = N <= 128 ? cdiv(N, 16) : cdiv(N, 32), most = N <= 128 ? 16 : 4;
+  return (int)std::max<i64>(1, std::min({most, 256 / std::max<i64>(tiles, 1), K / 256}));
 }
 
 constexpr int kHighestRank = 256;
@@ -77,15 +199,28 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
       if (t) mx_apart(t->p, t->bytes(), workspace, (size_t)need, "the workspace");
   }
   MxWorkspace ws(workspace, workspace_bytes, need);
-  AdapterArgs g{x.p, w ? w->p : nullptr, a.p, b.p, y ? y->p : nullptr, bias ? bias->p : nullptr, slots.ptr<int32_t>(),
-                scale ? scale->ptr<float>() : nullptr, out.p, N, (int)L, (int)R, (int)K, (int)O, bias ? bias->dt : F32};
-  if (x.dt == F16) k_adapter<true><<<(unsigned)N, 256, 0, stream()>>>(g);
-  else k_adapter<false><<<(unsigned)N, 256, 0, stream()>>>(g);
-  CK(hipGetLastError());
+  const int parts = adapter_parts(N, K);
+  float* h = (float*)ws.p;
+  GroupArgs g{};
+  g.m = w ? x.p : y->p;
+  g.c = w ? w->p : nullptr;
+  g.bias = bias ? bias->p : nullptr;
+  g.bias_dt = bias ? bias->dt : F32;
+  g.out = out.p;
+  g.N = N;
+  g.G = 1;
+  g.K = (int)K;
+  g.O = (int)O;
+  g.ad = AdapterPart{b.p, h, slots.ptr<int32_t>(), scale ? scale->ptr<float>() : nullptr, (int)L, (int)R, parts};
+  if (x.dt == F16) launch_in<true>(x, a, slots, h, parts);
+  else launch_in<false>(x, a, slots, h, parts);
+  if (w) adapter_product(g, x.dt);
+  else if (x.dt == F16) launch_add<true>(g);
+  else launch_add<false>(g);
 }
 }  // namespace
 
-i64 adapter_workspace(i64 N, i64 K, i64 R) { return 0; }
+i64 adapter_workspace(i64 N, i64 K, i64 R) { return N * R * 4 * adapter_parts(N, K); }
 
 void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
                     const Tensor* bias, Tensor& out, void* workspace, i64 workspace_bytes) {

@@ -1,0 +1,127 @@
+// What the kernels of linear layers with many weights share: the products of groups of rows (group.hip) and the low-rank
+// adapters beside one projection (adapter.hip).
+//
+// v_mfma_f32_16x16x32 multiplies 16 x 32 by 32 x 16 values: lane l supplies row l % 16 of either operand, depths 8 (l / 16) .. + 7, and gets
+// column l % 16 and rows 4 (l / 16) + i of the result. The channels' operand (w) is the first and the rows' (x) the second, so a lane has
+// 4 channels of one row per product.
+#pragma once
+#include "ldsdma.h"
+#include "mx.h"
+
+namespace {
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+constexpr uint32_t kOOR = 0x80000000u;  // past every buffer of these kernels, also with a step's offset added: reads as zeros
+
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma(mx_u32x4 a, mx_u32x4 b, f32x4 c) {
+  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
+}
+}  // namespace
+
+// Adapters of a product's rows: the second of their two products is added to the result
+struct AdapterPart {
+  const void* b;         // [L,O,R]
+  const float* h;        // the first product's sums in `parts` parts of the depth: [parts,N,R]
+  const int32_t* slots;  // [N]
+  const float* scale;    // [L] or null
+  int L, R, parts;
+};
+struct GroupArgs {
+  const void *m, *c, *bias;  // operands of the result's rows and columns: x, w (forward); dy, w (dx); dy, x (dw)
+  const int32_t* ends;
+  void *out, *db;
+  i64 N;
+  int G, K, O, bias_dt;
+  int tiles_m, tiles_c, per, band;
+  AdapterPart ad;
+};
+
+namespace {
+// The adapters' second product for up to 64 rows of one wavefront (16 TM rows, the first of them row n0, `rows` of which exist):
+// acc[t][u] += scale b h over tiles t of 16 channels and u of 16 rows. Every adapter that some row has takes its turn, of whose products a
+// lane takes its row's (rows of zeros for the others would let an infinity in b reach them), so rows come in any order; those that share
+// an adapter share its reading. h is held in 16 bits. chan(t): the channel of
+// the first operand's row lane % 16 in tile t, counted from c0, `cols` of which exist. Turns first, first + every, ...
+template <bool F16, int TC, int TM, class Chan>
+__device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC][TM], i64 n0, int rows, int c0, int cols, int lane, Chan&& chan,
+                                             int first = 0, int every = 1) {
+  static_assert(TM <= 4, "a lane a row");
+  const AdapterPart& p = a.ad;
+  const int r16 = lane & 15, g = lane >> 4;
+  int mine = lane < 16 * TM && lane < rows ? p.slots[n0 + lane] : -1;
+  mine = mine < p.L ? mine : -1;
+  int slot[TM];
+  float scale[TM];
+#pragma unroll
+  for (int u = 0; u < TM; u++) {
+    slot[u] = __shfl(mine, u * 16 + r16, 64);
+    scale[u] = slot[u] < 0 ? 0.f : p.scale ? p.scale[slot[u]] : 1.f;
+  }
+  const uint64_t all = __ballot(mine >= 0);
+  constexpr int RC = 2;  // 64 ranks at a time
+  for (int r0 = 0; r0 < p.R; r0 += 32 * RC) {
+    mx_u32x4 h[RC][TM];
+#pragma unroll
+    for (int c = 0; c < RC; c++)
+#pragma unroll
+      for (int u = 0; u < TM; u++) {
+        const int r = r0 + c * 32 + g * 8;
+        float v[8] = {};
+        if (r < p.R && slot[u] >= 0) {
+          const float* at = p.h + (n0 + u * 16 + r16) * p.R + r;
+          for (int q = 0; q < p.parts; q++, at += a.N * p.R) {
+            const f32x4 lo = *(const f32x4*)at, hi = *(const f32x4*)(at + 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              v[j] += lo[j];
+              v[4 + j] += hi[j];
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] *= scale[u];
+        }
+        h[c][u] = mx_pack8<F16>(v);
+      }
+    int turn = 0;
+    for (uint64_t left = all; left; turn++) {
+      const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+      const uint64_t same = __ballot(mine == s);
+      left &= ~same;
+      if (turn % every != first) continue;
+      const auto rb = buffer((const char*)p.b + ((i64)s * a.O + c0) * p.R * 2, (uint32_t)(cols * p.R * 2));
+      mx_u32x4 b[RC][TC];
+#pragma unroll
+      for (int c = 0; c < RC; c++) {
+        const int r = r0 + c * 32 + g * 8;
+#pragma unroll
+        for (int t = 0; t < TC; t++) {
+          const int ch = chan(t);
+          b[c][t] = __builtin_amdgcn_raw_buffer_load_b128(rb, ch < cols && r < p.R ? (uint32_t)((ch * p.R + r) * 2) : kOOR, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < TM; u++) {
+        if (!(same >> (16 * u) & 0xffff)) continue;
+#pragma unroll
+        for (int t = 0; t < TC; t++) {
+          f32x4 d = mfma<F16>(b[0][t], h[0][u], f32x4{});
+#pragma unroll
+          for (int c = 1; c < RC; c++) d = mfma<F16>(b[c][t], h[c][u], d);
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[t][u][i] += slot[u] == s ? d[i] : 0.f;
+        }
+      }
+    }
+  }
+}
+}  // namespace
+
+// out = x w^T + bias + adapters over all N rows (group.hip), without checks
+void adapter_product(const GroupArgs& a, DT dt);

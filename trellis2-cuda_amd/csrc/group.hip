@@ -1,40 +1,18 @@
 // Products of groups of rows with a weight matrix each, and their gradients. Rows ends[g-1] .. ends[g] - 1 are group g's.
 //   forward  y[n] = W_g x[n] + b_g        dx[n] = W_g^T dy[n]        dW_g = sum over g's rows of dy[n] x[n]^T, db_g = sum of dy[n]
-#include "ldsdma.h"
-#include "mx.h"
+#include "group.h"
 
 #include <type_traits>
 
 namespace {
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 enum { FORWARD = 0, DX = 1, DW = 2 };
 enum { OUT_16 = 0, OUT_F32 = 1 };
-struct GroupArgs {
-  const void *m, *c, *bias;  // operands of the result's rows and columns: x, w (forward); dy, w (dx); dy, x (dw)
-  const int32_t* ends;
-  void *out, *db;
-  i64 N;
-  int G, K, O, bias_dt;
-  int tiles_m, tiles_c, per, band;
-};
-
-template <bool F16>
-__device__ __forceinline__ f32x4 mfma(mx_u32x4 a, mx_u32x4 b, f32x4 c) {
-  if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 // Group g's rows: [first, first + count), inside [0, N) whatever ends holds
 __device__ __forceinline__ void rows_of(const GroupArgs& a, int g, i64& first, i64& count) {
   const i64 s = g ? min((i64)max(a.ends[g - 1], 0), a.N) : 0, e = min((i64)max(a.ends[g], 0), a.N);
   first = s;
   count = max(e - s, (i64)0);
 }
-
-constexpr uint32_t kOOR = 0x80000000u;  // past every buffer below, also with a step's offset added: reads as zeros
 
 // This workgroup's tile of the rows' products: group, row tile and column tile. The tiles of all groups stand in one list, a group's in
 // bands of `band` columns, row by row within a band; each XCD takes a contiguous eighth of it, so that the tiles that run
@@ -43,10 +21,15 @@ struct TilePlace {
   i64 first;  // the group's first row
   int count, g, tm, tc;
 };
-template <int BM>
+template <int BM, bool ONE>
 __device__ __forceinline__ bool find_tile(const GroupArgs& a, int lane, TilePlace& at) {
   auto chunk = [&](int g0, int& first, int& count) __attribute__((always_inline)) {  // lane's group, and the tiles up to its end
     const int g = g0 + lane, N = (int)a.N;
+    if constexpr (ONE) {  // one group, of all rows
+      first = 0;
+      count = lane ? 0 : N;
+      return (int)(((i64)N + BM - 1) / BM);
+    }
     const int s = g > 0 && g < a.G ? min(max(a.ends[g - 1], 0), N) : 0, e = g < a.G ? min(max(a.ends[g], 0), N) : 0;
     first = s;
     count = max(e - s, 0);
@@ -103,7 +86,7 @@ __device__ __forceinline__ bool find_tile(const GroupArgs& a, int lane, TilePlac
 // (0, 1 - f), (1, 1 - f), (1, f) with f = 0, 1 in turn: each quarter changes one operand's half, whose registers were free a quarter
 // earlier, so every LDS read is issued one quarter before its use and a wavefront holds one step's operands only. In the
 // middle of a stage's second step all wavefronts meet: by then each has read the whole slot, so it is filled again at once.
-template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM>
+template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT>
 __global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
   constexpr bool MT = OP == DW, CT = OP != FORWARD;  // transposed: the rows' operand, the columns'
   constexpr int NW = WC * WM, BC = 16 * TC * WC, BM = 16 * TM * WM, HC = TC / 2, HM = TM / 2;
@@ -133,7 +116,7 @@ __global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
     rows_of(a, at.g, at.first, count);
     at.count = (int)count;
   } else {
-    if (!find_tile<BM>(a, lane, at)) return;
+    if (!find_tile<BM, ADAPT>(a, lane, at)) return;
   }
   const int depth = OP == FORWARD ? a.K : OP == DX ? a.O : at.count;
   const int m0 = at.tm * BM, c0 = at.tc * BC;
@@ -336,6 +319,10 @@ __global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
     wait_vm<0>();  // nothing lands in LDS after the workgroup has gone
   }
 
+  if constexpr (ADAPT)
+    add_adapters<F16>(a, acc, at.first + m0 + wm * (16 * TM), rows - wm * (16 * TM), c0, cols, lane,
+                      [&](int t) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r16); });
+
   const i64 obase = OP == DW ? ((i64)at.g * a.O + m0) * a.K : (at.first + m0) * ncols;
 #pragma unroll
   for (int run = 0; run < TC / RUN; run++) {
@@ -370,7 +357,7 @@ __global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
   }
 }
 
-template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM>
+template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT = false>
 void launch_tile(GroupArgs a) {
   constexpr int BC = 16 * TC * WC, BM = 16 * TM * WM;
   a.tiles_c = cdiv(OP == FORWARD ? a.O : a.K, BC);
@@ -385,14 +372,138 @@ void launch_tile(GroupArgs a) {
     blocks = ((a.N / BM + a.G) * a.tiles_c + 7) / 8 * 8;
   }
   REQ(blocks * 64 * WC * WM < (1ll << 32), "%lld tiles: too many for a launch", (long long)blocks);
-  k_group_tile<OP, F16, OUT, TC, TM, WC, WM><<<(unsigned)blocks, 64 * WC * WM, 0, stream()>>>(a);
+  k_group_tile<OP, F16, OUT, TC, TM, WC, WM, ADAPT><<<(unsigned)blocks, 64 * WC * WM, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
+// Few rows: the weights' bytes count, and that many of them are on their way at once. A workgroup has 16 OT channels by up to 16 NT rows of a
+// group; each of its 8 wavefronts takes a contiguous eighth of the depth, both operands straight into registers, and the sums meet in
+// LDS in a fixed order. With adapters, 4 wavefronts more add them meanwhile.
+template <bool F16, int OT, int NT, bool ADAPT>
+__global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
+  constexpr int NW = 8, NA = ADAPT ? 4 : 0, RUN = OT;
+  static_assert(OT == 1 || OT == 2, "4 or 8 channels a lane");
+  __shared__ f32x4 part[NW + NA][OT * NT][64];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  TilePlace at;
+  if (!find_tile<16 * NT, ADAPT>(a, lane, at)) return;
+  const i64 n0 = at.first + at.tm * (16 * NT);
+  const int rows = min(16 * NT, at.count - at.tm * (16 * NT)), c0 = at.tc * (16 * OT), cols = min(16 * OT, a.O - c0);
+  auto chan = [&](int t) __attribute__((always_inline)) { return r16 / 4 * (4 * RUN) + t * 4 + r16 % 4; };
+  f32x4 acc[OT][NT];
+#pragma unroll
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int u = 0; u < NT; u++) acc[t][u] = f32x4{};
+  if (!ADAPT || wave < NW) {
+    // every load is a buffer load whose offset is past the end where there is nothing (a row or a channel past the last, depths past K)
+    const auto rw = buffer((const char*)a.c + ((i64)at.g * a.O + c0) * a.K * 2, (uint32_t)(cols * a.K * 2));
+    const auto rx = buffer((const char*)a.m + n0 * a.K * 2, (uint32_t)(rows * a.K * 2));
+    uint32_t wo[OT], xo[NT];
+#pragma unroll
+    for (int t = 0; t < OT; t++) wo[t] = chan(t) < cols ? (uint32_t)(chan(t) * a.K * 2 + g * 16) : kOOR;
+#pragma unroll
+    for (int u = 0; u < NT; u++) xo[u] = u * 16 + r16 < rows ? (uint32_t)((u * 16 + r16) * a.K * 2 + g * 16) : kOOR;
+    const int S = (a.K + 31) / 32, per = (S + NW - 1) / NW, s0 = wave * per, s1 = min(s0 + per, S);
+    struct Step {
+      mx_u32x4 w[OT], x[NT];
+    };
+    auto load = [&](Step& q, int s) __attribute__((always_inline)) {
+      const bool in = s * 32 + g * 8 < a.K;
+#pragma unroll
+      for (int t = 0; t < OT; t++) q.w[t] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? wo[t] : kOOR, s * 64, 0);
+#pragma unroll
+      for (int u = 0; u < NT; u++) q.x[u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u] : kOOR, s * 64, 0);
+    };
+    auto multiply = [&](const Step& q) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < NT; u++)
+#pragma unroll
+        for (int t = 0; t < OT; t++) acc[t][u] = mfma<F16>(q.w[t], q.x[u], acc[t][u]);
+    };
+    constexpr int U = 8;  // steps on their way together
+    int s = s0;
+    for (; s + U <= s1; s += U) {
+      Step q[U];
+#pragma unroll
+      for (int k = 0; k < U; k++) load(q[k], s + k);
+#pragma unroll
+      for (int k = 0; k < U; k++) multiply(q[k]);
+    }
+    if (s < s1) {
+      Step q[U];
+#pragma unroll
+      for (int k = 0; k < U; k++)
+        if (s + k < s1) load(q[k], s + k);
+#pragma unroll
+      for (int k = 0; k < U; k++)
+        if (s + k < s1) multiply(q[k]);
+    }
+  } else {
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, wave - NW, NA);
+  }
+#pragma unroll
+  for (int t = 0; t < OT; t++)
+#pragma unroll
+    for (int u = 0; u < NT; u++) part[wave][t * NT + u][lane] = acc[t][u];
+  __syncthreads();
+  for (int u = wave; u < NT; u += NW + NA) {
+    float v[4 * OT], bias[4 * OT];
+#pragma unroll
+    for (int t = 0; t < OT; t++) {
+      f32x4 c = part[0][t * NT + u][lane];
+#pragma unroll
+      for (int w = 1; w < NW + NA; w++) c += part[w][t * NT + u][lane];
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[t * 4 + i] = c[i];
+    }
+    const int m = u * 16 + r16, c = g * (4 * RUN);
+    if (m >= rows || c >= cols) continue;
+    mx_params<4 * OT>(a.bias, a.bias_dt, (i64)at.g * a.O + c0 + c, 0.f, bias);
+#pragma unroll
+    for (int j = 0; j < 4 * OT; j++) v[j] += bias[j];
+    uint16_t* to = (uint16_t*)a.out + (n0 + m) * a.O + c0 + c;
+    if constexpr (OT == 2) *(mx_u32x4*)to = mx_pack8<F16>(*(float(*)[8])v);
+    else *(mx_u32x2*)to = mx_u32x2{mx_pack2<F16>(v[0], v[1]), mx_pack2<F16>(v[2], v[3])};
+  }
+}
+template <bool F16, int OT, int NT, bool ADAPT>
+void launch_rows(GroupArgs a) {
+  a.tiles_c = cdiv(a.O, 16 * OT);
+  a.band = 8;
+  const i64 blocks = ((a.N / (16 * NT) + a.G) * a.tiles_c + 7) / 8 * 8;
+  REQ(blocks * (ADAPT ? 768 : 512) < (1ll << 32), "%lld tiles: too many for a launch", (long long)blocks);
+  k_group_rows<F16, OT, NT, ADAPT><<<(unsigned)blocks, ADAPT ? 768 : 512, 0, stream()>>>(a);
+  CK(hipGetLastError());
+}
+
+template <bool ADAPT>
+bool few_rows(const GroupArgs& a, DT dt) {
+  const i64 mean = (a.N + a.G - 1) / a.G;
+  if (mean > 64) return false;
+  auto by = [&](auto F) {
+    constexpr bool f = decltype(F)::value;
+    if (mean <= 16) {
+      if (a.O * (a.N < a.G ? a.N : a.G) <= 16 * 1024) launch_rows<f, 1, 1, ADAPT>(a);
+      else launch_rows<f, 2, 1, ADAPT>(a);
+    } else if (mean <= 32) {
+      launch_rows<f, 2, 2, ADAPT>(a);
+    } else {
+      launch_rows<f, 2, 4, ADAPT>(a);
+    }
+  };
+  dt == F16 ? by(std::true_type{}) : by(std::false_type{});
+  return true;
+}
+
 template <int OP>
 void launch(const GroupArgs& a, DT dt, bool f32 = false) {
   auto by = [&](auto F, auto T) { launch_tile<OP, decltype(F)::value, decltype(T)::value, 8, 4, 2, 4>(a); };
   constexpr std::integral_constant<int, OUT_16> o16{};
   constexpr std::integral_constant<int, OUT_F32> o32{};
+  if constexpr (OP == FORWARD) {
+    if (few_rows<false>(a, dt)) return;
+  }
   if constexpr (OP == DW) {
     if (f32) return dt == F16 ? by(std::true_type{}, o32) : by(std::false_type{}, o32);
   }
@@ -426,6 +537,12 @@ void apart(const Tensor& out, const Tensor* t, const char* what) {
   if (t) mx_apart(out.p, out.bytes(), t->p, t->bytes(), what);
 }
 }  // namespace
+
+void adapter_product(const GroupArgs& a, DT dt) {
+  if (few_rows<true>(a, dt)) return;
+  if (dt == F16) launch_tile<FORWARD, true, OUT_16, 8, 4, 2, 4, true>(a);
+  else launch_tile<FORWARD, false, OUT_16, 8, 4, 2, 4, true>(a);
+}
 
 void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Tensor* bias, Tensor& y) {
   i64 G, O, K;
