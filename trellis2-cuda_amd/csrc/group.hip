@@ -87,7 +87,7 @@ __device__ __forceinline__ bool find_tile(const GroupArgs& a, int lane, TilePlac
 // earlier, so every LDS read is issued one quarter before its use and a wavefront holds one step's operands only. In the
 // middle of a stage's second step all wavefronts meet: by then each has read the whole slot, so it is filled again at once.
 template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT>
-__global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
+__global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupArgs a) {
   constexpr bool MT = OP == DW, CT = OP != FORWARD;  // transposed: the rows' operand, the columns'
   constexpr int NW = WC * WM, BC = 16 * TC * WC, BM = 16 * TM * WM, HC = TC / 2, HM = TM / 2;
   constexpr int RUN = OUT == OUT_F32 ? 1 : 2;
@@ -160,36 +160,39 @@ __global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
       coff[k] = ch < cols ? (uint32_t)(ch * crow + (p % 8 ^ (q & 7)) * 16) : kOOR;
     }
   }
-  // fills stage t's slot; past the last one the DMAs still run (the waits count them) but read nothing
-  auto issue = [&](int t, int slot) __attribute__((always_inline)) {
+  // What is asked for next: a stage's descriptors and offsets. Past the last stage the DMAs still run (the waits count them) but read
+  // nothing.
+  i32x4 nm = rm, nc = rc;
+  int msoff = 0, csoff = 0;
+  uint32_t fill = lds0 + wave * (MI * 1024);  // the slot that is filled, where this wavefront's part of the rows' operand goes
+  auto ask = [&](int t) __attribute__((always_inline)) {
     const bool live = t < stages;
-    const uint32_t base = lds0 + slot * kSlot;
     const int left = live ? min(64, depth - t * 64) : 0;  // of the depth
-    auto fill = [&](auto TC_, auto NC, const char* p, i32x4 r, int row, int width, const uint32_t* off, uint32_t to) __attribute__((always_inline)) {
+    auto aim = [&](auto TC_, auto NC, const char* p, i32x4 whole, int row, int width, uint32_t* off, i32x4& r, int& soff) __attribute__((always_inline)) {
       constexpr int N = decltype(NC)::value;
       if constexpr (decltype(TC_)::value) {  // rows t * 64 ..: `left` of them
-        const i32x4 rs = rsrc4(p + (i64)t * 64 * row, left ? (uint32_t)((left - 1) * row + width * 2) : 0);
-#pragma unroll
-        for (int k = 0; k < N; k++) dma16(rs, to + (wave * N + k) * 1024, off[k], 0);
+        r = rsrc4(p + (i64)t * 64 * row, left ? (uint32_t)((left - 1) * row + width * 2) : 0);
       } else {
-        r[2] = live ? r[2] : 0;
-        const int s = live ? t * 128 : 0;
-        if (live && left < 64) {  // pieces past the last column read as zeros
-          int l = lane;
-          asm volatile("" : "+v"(l));
+        r[2] = live ? whole[2] : 0;
+        soff = live ? t * 128 : 0;
+        if (live && left < 64) {  // the last stage: pieces past the last column read as zeros
 #pragma unroll
           for (int k = 0; k < N; k++) {
-            const int u = (wave * N + k) * 64 + l;
-            dma16(r, to + (wave * N + k) * 1024, (u % 8 ^ (u / 8 & 7)) * 8 < left ? off[k] : kOOR, s);
+            const int u = (wave * N + k) * 64 + lane;
+            off[k] = (u % 8 ^ (u / 8 & 7)) * 8 < left ? off[k] : kOOR;
           }
-        } else {
-#pragma unroll
-          for (int k = 0; k < N; k++) dma16(r, to + (wave * N + k) * 1024, off[k], s);
         }
       }
     };
-    fill(std::bool_constant<MT>{}, std::integral_constant<int, MI>{}, mp, rm, mrow, rows, moff, base);
-    fill(std::bool_constant<CT>{}, std::integral_constant<int, CI>{}, cp, rc, crow, cols, coff, base + kC);
+    aim(std::bool_constant<MT>{}, std::integral_constant<int, MI>{}, mp, rm, mrow, rows, moff, nm, msoff);
+    aim(std::bool_constant<CT>{}, std::integral_constant<int, CI>{}, cp, rc, crow, cols, coff, nc, csoff);
+  };
+  constexpr int DI = MI + CI;  // DMAs of a stage
+  static_assert(MI == CI, "one LDS address for both operands");
+  auto issue = [&](auto KC) __attribute__((always_inline)) {  // number k of the stage asked for
+    constexpr int K = decltype(KC)::value;
+    if constexpr (K < MI) dma16_at<K * 1024>(nm, fill, moff[K], msoff);
+    else dma16_at<kC + (K - MI) * 1024>(nc, fill, coff[K - MI], csoff);
   };
 
   f32x4 acc[TC][TM];
@@ -228,100 +231,125 @@ __global__ void __launch_bounds__(64 * WC * WM, 2) k_group_tile(GroupArgs a) {
   auto read_tr = [](uint32_t at) __attribute__((always_inline)) {
     return __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(size_t)at));
   };
-  auto read_m = [&](mx_u32x4(&f)[HM], int slot, int j, int half) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < HM; u++) {
-      const int t = half * HM + u;
-      if constexpr (MT) {
-        const uint32_t p = ma[t] + slot * kSlot + j * (32 * BM * 2);
-        const mx_u32x2 lo = read_tr(p), hi = read_tr(p + 4 * BM * 2);
-        f[u] = mx_u32x4{lo[0], lo[1], hi[0], hi[1]};
-      } else {
-        f[u] = read16(ma[j] + slot * kSlot + t * 2048);
-      }
+  auto read_m = [&](mx_u32x4& f, int j, int t) __attribute__((always_inline)) {
+    if constexpr (MT) {
+      const uint32_t p = ma[t] + j * (32 * BM * 2);
+      const mx_u32x2 lo = read_tr(p), hi = read_tr(p + 4 * BM * 2);
+      f = mx_u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      f = read16(ma[j] + t * 2048);
     }
   };
-  auto read_c = [&](mx_u32x4(&f)[HC], int slot, int j, int half) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < HC; u++) {
-      const int t = half * HC + u;
-      if constexpr (CT) {
-        const uint32_t p = ca[t / RUN] + slot * kSlot + j * (32 * BC * 2) + t % RUN * 8;
-        const mx_u32x2 lo = read_tr(p), hi = read_tr(p + 4 * BC * 2);
-        f[u] = mx_u32x4{lo[0], lo[1], hi[0], hi[1]};
-      } else {
-        f[u] = read16(ca[j] + slot * kSlot + t * 2048);
-      }
+  auto read_c = [&](mx_u32x4& f, int j, int t) __attribute__((always_inline)) {
+    if constexpr (CT) {
+      const uint32_t p = ca[t / RUN] + j * (32 * BC * 2) + t % RUN * 8;
+      const mx_u32x2 lo = read_tr(p), hi = read_tr(p + 4 * BC * 2);
+      f = mx_u32x4{lo[0], lo[1], hi[0], hi[1]};
+    } else {
+      f = read16(ca[j] + t * 2048);
     }
   };
 
   mx_u32x4 fm[2][HM], fc[2][HC];
-  // which halves of this wavefront's part hold anything
-  const bool ml[2] = {wm * (16 * TM) < rows, wm * (16 * TM) + 16 * HM < rows};
-  const bool cl[2] = {wc * (16 * TC) < cols, wc * (16 * TC) + 16 * HC < cols};
   const mx_u32x4 ones = F16 ? mx_u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : mx_u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-  int cur = 0;
-  auto step = [&](auto JC, int s) __attribute__((always_inline)) {
-    constexpr int J = decltype(JC)::value, f = J;  // step J of stage s
-    auto quarter = [&](auto CC, auto MC) __attribute__((always_inline)) {
-      constexpr int hc = decltype(CC)::value, hm = decltype(MC)::value;
-      if (ml[hm] && cl[hc]) {
+  // A quarter's products, with READS LDS reads and DMAS DMAs between them: a wavefront that has its SIMD to itself (or shares it with
+  // one at the same place) feeds the matrix unit only if few instructions stand between two products.
+  auto quarter = [&](auto BC_, auto CC, auto MC, auto RC, auto&& read, auto DC, auto&& dma) __attribute__((always_inline)) {
+    constexpr bool BUSY = decltype(BC_)::value;
+    constexpr int hc = decltype(CC)::value, hm = decltype(MC)::value, R = decltype(RC)::value, D = decltype(DC)::value, P = HC * HM;
+    if constexpr (BUSY) {
+      mx_unroll<P>([&](auto IC) __attribute__((always_inline)) {
+        constexpr int i = decltype(IC)::value, u = i / HC, t = i % HC;
+        mx_unroll<R>([&](auto KC) __attribute__((always_inline)) {
+          if constexpr (decltype(KC)::value * P / 2 / (R ? R : 1) == i) read(decltype(KC)::value);  // the first half: they land by the quarter's end
+        });
+        mx_unroll<D>([&](auto KC) __attribute__((always_inline)) {
+          if constexpr (decltype(KC)::value * P / (D ? D : 1) + P / (2 * (D ? D : 1)) == i) dma(KC);
+        });
+        f32x4& c = acc[hc * HC + t][hm * HM + u];
+        c = mfma<F16>(fc[hc][t], fm[hm][u], c);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+    } else {
+      mx_unroll<D>([&](auto KC) __attribute__((always_inline)) { dma(KC); });
+    }
+    if constexpr (BUSY && OP == DW && hc == 0) {
+      if (with_db) {
 #pragma unroll
-        for (int u = 0; u < HM; u++)
-#pragma unroll
-          for (int t = 0; t < HC; t++) {
-            f32x4& c = acc[hc * HC + t][hm * HM + u];
-            c = mfma<F16>(fc[hc][t], fm[hm][u], c);
-          }
+        for (int u = 0; u < HM; u++) accb[hm * HM + u] = mfma<F16>(ones, fm[hm][u], accb[hm * HM + u]);
       }
-      if constexpr (OP == DW && hc == 0) {
-        if (with_db) {
-#pragma unroll
-          for (int u = 0; u < HM; u++) accb[hm * HM + u] = mfma<F16>(ones, fm[hm][u], accb[hm * HM + u]);
-        }
-      }
-    };
-    constexpr std::integral_constant<int, 0> first{};
-    constexpr std::integral_constant<int, 1> second{};
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::integral_constant<int, 0> zero{};
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, HM> hm{};
+  constexpr std::integral_constant<int, HC> hc{};
+  int turn = kSlot;  // from this slot to the other one
+  auto step = [&](auto busy, auto JC, int s) __attribute__((always_inline)) {  // step J of stage s
+    constexpr int J = decltype(JC)::value, f = J, JN = 1 - J;
     constexpr std::integral_constant<int, f> mf{};
     constexpr std::integral_constant<int, 1 - f> mo{};
-    read_m(fm[1 - f], cur, J, 1 - f);
-    read_c(fc[1], cur, J, 1);
-    quarter(first, mf);
-    __builtin_amdgcn_sched_barrier(0);
-    quarter(first, mo);
-    __builtin_amdgcn_sched_barrier(0);
+    // DMAs into the other slot: the second half of the next stage, or the first half of the one after
+    constexpr std::integral_constant<int, J == 0 ? DI / 4 : 0> d12{};
+    constexpr std::integral_constant<int, J == 0 ? 0 : DI / 4> d34{};
+    auto dmas = [&](auto FROM) __attribute__((always_inline)) {
+      return [&](auto KC) __attribute__((always_inline)) { issue(std::integral_constant<int, decltype(FROM)::value + decltype(KC)::value>{}); };
+    };
+    quarter(busy, zero, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], J, (1 - f) * HM + u); }, d12,
+            dmas(std::integral_constant<int, DI / 2>{}));
+    quarter(busy, zero, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[1][t], J, HC + t); }, d12,
+            dmas(std::integral_constant<int, DI * 3 / 4>{}));
     if constexpr (J == 1) {  // the next stage has landed, and this one is in registers
       wait_vm<0>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       bare_barrier();
-      issue(s + 2, cur);
-      cur ^= 1;
+#pragma unroll
+      for (uint32_t& x : ma) x += turn;
+#pragma unroll
+      for (uint32_t& x : ca) x += turn;
+      turn = -turn;
+      fill += turn;
+      ask(s + 2);
     }
-    read_c(fc[0], cur, 1 - J, 0);
-    quarter(second, mo);
-    __builtin_amdgcn_sched_barrier(0);
-    read_m(fm[1 - f], cur, 1 - J, 1 - f);
-    quarter(second, mf);
-    __builtin_amdgcn_sched_barrier(0);
+    quarter(busy, one, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[0][t], JN, t); }, d34, dmas(zero));
+    quarter(busy, one, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], JN, (1 - f) * HM + u); }, d34,
+            dmas(std::integral_constant<int, DI / 4>{}));
   };
   if (stages) {
-    issue(0, 0);
-    issue(1, 1);
-    wait_vm<MI + CI>();
+    ask(0);
+    mx_unroll<DI>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
+    ask(1);
+    fill += kSlot;
+    mx_unroll<DI / 2>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
+    wait_vm<DI / 2>();
     bare_barrier();
-    read_m(fm[0], 0, 0, 0);
-    read_c(fc[0], 0, 0, 0);
-    for (int s = 0; s < stages; s++) {
-      step(std::integral_constant<int, 0>{}, s);
-      step(std::integral_constant<int, 1>{}, s);
+#pragma unroll
+    for (int u = 0; u < HM; u++) read_m(fm[0][u], 0, u);
+#pragma unroll
+    for (int t = 0; t < HC; t++) read_c(fc[0][t], 0, t);
+    auto loop = [&](auto busy) __attribute__((always_inline)) {
+      for (int s = 0; s < stages; s++) {
+        step(busy, zero, s);
+        step(busy, one, s);
+      }
+    };
+    if (wm * (16 * TM) >= rows || wc * (16 * TC) >= cols) {  // nothing of the result is this wavefront's: its share of the DMAs alone
+      loop(std::false_type{});
+      wait_vm<0>();
+      return;
     }
+    loop(std::true_type{});
     wait_vm<0>();  // nothing lands in LDS after the workgroup has gone
   }
 
   if constexpr (ADAPT)
-    add_adapters<F16>(a, acc, at.first + m0 + wm * (16 * TM), rows - wm * (16 * TM), c0, cols, lane,
-                      [&](int t) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r16); });
+    mx_unroll<(TM + 3) / 4>([&](auto HC_) __attribute__((always_inline)) {
+      constexpr int u0 = decltype(HC_)::value * 4, n = TM < 4 ? TM : 4;
+      const int r0 = wm * (16 * TM) + u0 * 16;
+      add_adapters<F16, n, u0>(a, acc, at.first + m0 + r0, rows - r0, c0, cols, lane,
+                               [&](int t) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r16); });
+    });
 
   const i64 obase = OP == DW ? ((i64)at.g * a.O + m0) * a.K : (at.first + m0) * ncols;
 #pragma unroll
@@ -440,7 +468,7 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
         if (s + k < s1) multiply(q[k]);
     }
   } else {
-    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, wave - NW, NA);
+    add_adapters<F16, NT, 0>(a, acc, n0, rows, c0, cols, lane, chan, wave - NW, NA);
   }
 #pragma unroll
   for (int t = 0; t < OT; t++)

@@ -18,6 +18,12 @@ __device__ __forceinline__ void dma16(i32x4 r, uint32_t lds, uint32_t off, int s
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                ::"s"(lds), "v"(off), "s"(r), "s"(soff) : "memory", "m0");
 }
+// The same to lds + AT
+template <int AT>
+__device__ __forceinline__ void dma16_at(i32x4 r, uint32_t lds, uint32_t off, int soff) {
+  asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+               ::"s"(lds), "v"(off), "s"(r), "s"(soff), "n"(AT) : "memory", "m0", "scc");
+}
 template <int N>
 __device__ __forceinline__ void wait_vm() {
   static_assert(N >= 0 && N < 64, "vmcnt range");
