@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
 #pragma unroll
     for (int u = 0; u < TM; u++) acc[t][u] = f32x4{};
   add_adapters<F16, TM, 0>(a, acc, n0, rows, c0, cols, lane,
-                    [&](int t) __attribute__((always_inline)) { return t / 2 * 32 + r16 / 4 * 8 + t % 2 * 4 + r16 % 4; });
+                    [](int t, int r) __attribute__((always_inline)) { return t / 2 * 32 + r / 4 * 8 + t % 2 * 4 + r % 4; });
 #pragma unroll
   for (int t = 0; t < TC / 2; t++)
 #pragma unroll

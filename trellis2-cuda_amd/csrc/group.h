@@ -47,8 +47,8 @@ namespace {
 // The adapters' second product for up to 64 rows of one wavefront (16 TM rows, the first of them row n0, `rows` of which exist):
 // acc[t][u] += scale b h over tiles t of 16 channels and u of 16 rows. Every adapter that some row has takes its turn, of whose products a
 // lane takes its row's (rows of zeros for the others would let an infinity in b reach them), so rows come in any order; those that share
-// an adapter share its reading. h is held in 16 bits. chan(t): the channel of
-// the first operand's row lane % 16 in tile t, counted from c0, `cols` of which exist. Turns first, first + every, ...
+// an adapter share its reading. h is held in 16 bits. chan(t, r): the channel of
+// the first operand's row r in tile t, counted from c0, `cols` of which exist. Turns first, first + every, ...
 // (TM row tiles of acc's TT, from U0 on.)
 template <bool F16, int TM, int U0, int TC, int TT, class Chan>
 __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC][TT], i64 n0, int rows, int c0, int cols, int lane, Chan&& chan,
@@ -97,26 +97,30 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
       left &= ~same;
       if (turn % every != first) continue;
       const auto rb = buffer((const char*)p.b + ((i64)s * a.O + c0) * p.R * 2, (uint32_t)(cols * p.R * 2));
-      mx_u32x4 b[RC][TC];
+      constexpr int TP = TC < 4 ? TC : 4;  // channel tiles at a time
 #pragma unroll
-      for (int c = 0; c < RC; c++) {
-        const int r = r0 + c * 32 + g * 8;
+      for (int t0 = 0; t0 < TC; t0 += TP) {
+        mx_u32x4 b[RC][TP];
 #pragma unroll
-        for (int t = 0; t < TC; t++) {
-          const int ch = chan(t);
-          b[c][t] = __builtin_amdgcn_raw_buffer_load_b128(rb, ch < cols && r < p.R ? (uint32_t)((ch * p.R + r) * 2) : kOOR, 0, 0);
+        for (int c = 0; c < RC; c++) {
+          const int r = r0 + c * 32 + g * 8;
+#pragma unroll
+          for (int t = 0; t < TP; t++) {
+            const int ch = chan(t0 + t, r16);
+            b[c][t] = __builtin_amdgcn_raw_buffer_load_b128(rb, ch < cols && r < p.R ? (uint32_t)((ch * p.R + r) * 2) : kOOR, 0, 0);
+          }
         }
-      }
 #pragma unroll
-      for (int u = 0; u < TM; u++) {
-        if (!(same >> (16 * u) & 0xffff)) continue;
+        for (int u = 0; u < TM; u++) {
+          if (!(same >> (16 * u) & 0xffff)) continue;
 #pragma unroll
-        for (int t = 0; t < TC; t++) {
-          f32x4 d = mfma<F16>(b[0][t], h[0][u], f32x4{});
+          for (int t = 0; t < TP; t++) {
+            f32x4 d = mfma<F16>(b[0][t], h[0][u], f32x4{});
 #pragma unroll
-          for (int c = 1; c < RC; c++) d = mfma<F16>(b[c][t], h[c][u], d);
+            for (int c = 1; c < RC; c++) d = mfma<F16>(b[c][t], h[c][u], d);
 #pragma unroll
-          for (int i = 0; i < 4; i++) acc[t][U0 + u][i] += slot[u] == s ? d[i] : 0.f;
+            for (int i = 0; i < 4; i++) acc[t0 + t][U0 + u][i] += slot[u] == s ? d[i] : 0.f;
+          }
         }
       }
     }

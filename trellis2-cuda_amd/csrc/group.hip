@@ -2,75 +2,129 @@
 //   forward  y[n] = W_g x[n] + b_g        dx[n] = W_g^T dy[n]        dW_g = sum over g's rows of dy[n] x[n]^T, db_g = sum of dy[n]
 #include "group.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace {
 enum { FORWARD = 0, DX = 1, DW = 2 };
 enum { OUT_16 = 0, OUT_F32 = 1 };
-// Group g's rows: [first, first + count), inside [0, N) whatever ends holds
-__device__ __forceinline__ void rows_of(const GroupArgs& a, int g, i64& first, i64& count) {
-  const i64 s = g ? min((i64)max(a.ends[g - 1], 0), a.N) : 0, e = min((i64)max(a.ends[g], 0), a.N);
-  first = s;
-  count = max(e - s, (i64)0);
-}
-
-// This workgroup's tile of the rows' products: group, row tile and column tile. The tiles of all groups stand in one list, a group's in
-// bands of `band` columns, row by row within a band; each XCD takes a contiguous eighth of it, so that the tiles that run
-// beside each other on it share operands in its L2. Every wavefront finds it for itself, 64 groups at a time.
+// A workgroup's tiles, one after another. Every wavefront finds them for itself, with a lane a group, 64 groups at a time.
+//
+// Rows' products: the tiles of all groups stand in one list, a group's in bands of `band` columns, row by row within a band. Each XCD
+// takes a contiguous eighth of it, its workgroups every W-th tile of that, so that the tiles that run beside each other on it share
+// operands in its L2.
+// dw: tiles are as deep as their group is long, so the longest groups come first (up to 64 groups; more are short), in rounds of W tiles
+// a XCD that run to and fro; each XCD takes a contiguous eighth of every group's tiles (where they are many).
 struct TilePlace {
   i64 first;  // the group's first row
   int count, g, tm, tc;
 };
-template <int BM, bool ONE>
-__device__ __forceinline__ bool find_tile(const GroupArgs& a, int lane, TilePlace& at) {
-  auto chunk = [&](int g0, int& first, int& count) __attribute__((always_inline)) {  // lane's group, and the tiles up to its end
+template <int OP, int BM, bool ONE>  // ONE: one group, of all rows
+struct Tiles {
+  const GroupArgs& a;
+  int lane, first, count, key;  // of the lane's group among the first 64; key: tiles up to its end, or (dw) its place in the order
+  int W, round = 0;
+  i64 begin, end;  // this XCD's part of the list
+
+  __device__ __forceinline__ Tiles(const GroupArgs& a_, int lane_) : a(a_), lane(lane_), W(gridDim.x / 8) {
+    key = chunk(0);
+    if constexpr (OP == DW) {
+      int place = 0;
+      for (int i = 0; i < min(a.G, 64); i++) {
+        const int c = __builtin_amdgcn_readlane(count, i);
+        place += c > count || (c == count && i < lane) ? 1 : 0;
+      }
+      key = lane < a.G ? place : -1;
+      const i64 per = (i64)a.tiles_m * a.tiles_c;
+      begin = 0;
+      end = a.per ? (i64)a.per * a.G : (per * a.G + 7) / 8;
+    } else {
+      i64 total = __builtin_amdgcn_readlane(key, 63);
+      if (a.G > 64) {
+        for (int g0 = 64; g0 < a.G; g0 += 64) total += __builtin_amdgcn_readlane(chunk(g0), 63);
+        key = chunk(0);
+      }
+      const i64 all = total * a.tiles_c, per = (all + 7) / 8;
+      begin = blockIdx.x % 8 * per;
+      end = min(begin + per, all);
+    }
+  }
+  // The lane's group of those from g0 on, its rows inside [0, N) whatever ends holds; the tiles of all up to it
+  __device__ __forceinline__ int chunk(int g0) {
     const int g = g0 + lane, N = (int)a.N;
-    if constexpr (ONE) {  // one group, of all rows
+    if constexpr (ONE) {
       first = 0;
       count = lane ? 0 : N;
       return (int)(((i64)N + BM - 1) / BM);
     }
-    const int s = g > 0 && g < a.G ? min(max(a.ends[g - 1], 0), N) : 0, e = g < a.G ? min(max(a.ends[g], 0), N) : 0;
-    first = s;
-    count = max(e - s, 0);
+    first = g > 0 && g < a.G ? min(max(a.ends[g - 1], 0), N) : 0;
+    count = max((g < a.G ? min(max(a.ends[g], 0), N) : 0) - first, 0);
     int sum = (int)(((i64)count + BM - 1) / BM);
+    if constexpr (OP == DW) return sum;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int below = __shfl_up(sum, d, 64);
       sum += lane >= d ? below : 0;
     }
     return sum;
-  };
-  int first, count, upto = chunk(0, first, count), total = __builtin_amdgcn_readlane(upto, 63);
-  if (a.G > 64) {
-    for (int g0 = 64; g0 < a.G; g0 += 64) total += __builtin_amdgcn_readlane(chunk(g0, first, count), 63);
-    upto = chunk(0, first, count);
   }
-  const int xcd = blockIdx.x % 8, k = blockIdx.x / 8;
-  const i64 all = (i64)total * a.tiles_c, per = (all + 7) / 8, l = xcd * per + k;
-  if (k >= per || l >= all) return false;
-  const int row_tile = (int)(l / a.tiles_c);
-  int before = 0;
-  for (int g0 = 0;; g0 += 64) {
-    if (g0) upto = chunk(g0, first, count);
-    const uint64_t past = __ballot(before + upto > row_tile);
-    if (past) {
-      const int who = __builtin_ctzll(past);
-      at.g = g0 + who;
-      at.first = __builtin_amdgcn_readlane(first, who);
-      at.count = __builtin_amdgcn_readlane(count, who);
-      if (who) before += __builtin_amdgcn_readlane(upto, who - 1);
-      break;
+  __device__ __forceinline__ void group(TilePlace& at, int g0, int who) {
+    at.g = g0 + who;
+    at.first = __builtin_amdgcn_readlane(first, who);
+    at.count = __builtin_amdgcn_readlane(count, who);
+  }
+  __device__ __forceinline__ bool next(TilePlace& at) {
+    const int k = blockIdx.x / 8;
+    if constexpr (OP == DW) {
+      const int tiles = a.tiles_m * a.tiles_c;
+      for (;; round++) {
+        const i64 start = (i64)round * W;
+        if (start >= end) return false;
+        const i64 q = start + (round & 1 ? W - 1 - k : k);
+        const i64 b = q * 8 + blockIdx.x % 8;
+        const int order = (int)(a.per ? q / a.per : b / tiles);
+        const int inside = (int)(a.per ? blockIdx.x % 8 * a.per + q % a.per : b % tiles);
+        if (q >= end || order >= a.G || inside >= tiles) continue;
+        at.tm = inside / a.tiles_c;
+        at.tc = inside % a.tiles_c;
+        if (a.G <= 64) {
+          group(at, 0, __builtin_ctzll(__ballot(key == order)));
+        } else {
+          at.g = order;
+          const int N = (int)a.N, s = order ? min(max(a.ends[order - 1], 0), N) : 0;
+          at.first = s;
+          at.count = max(min(max(a.ends[order], 0), N) - s, 0);
+        }
+        round++;
+        return true;
+      }
+    } else {
+      const i64 l = begin + (i64)round * W + k;
+      round++;
+      if (l >= end) return false;
+      const int row_tile = (int)(l / a.tiles_c);
+      int before = 0, upto = key;
+      for (int g0 = 0;; g0 += 64) {
+        if (g0) upto = chunk(g0);
+        const uint64_t past = __ballot(before + upto > row_tile);
+        if (past) {
+          const int who = __builtin_ctzll(past);
+          group(at, g0, who);
+          if (who) before += __builtin_amdgcn_readlane(upto, who - 1);
+          break;
+        }
+        if (g0 + 64 >= a.G) return false;
+        before += __builtin_amdgcn_readlane(upto, 63);
+      }
+      if (a.G > 64) chunk(0);  // back to the first groups
+      const int tiles = (int)(((i64)at.count + BM - 1) / BM), inside = (int)(l - (i64)before * a.tiles_c);
+      const int band = inside / (a.band * tiles) * a.band, width = min(a.band, a.tiles_c - band), rest = inside - band * tiles;
+      at.tm = rest / width;
+      at.tc = band + rest % width;
+      return inside >= 0 && at.tm < tiles;
     }
-    if (g0 + 64 >= a.G) return false;
-    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  const int tiles = (int)(((i64)at.count + BM - 1) / BM), inside = (int)(l - (i64)before * a.tiles_c);
-  const int band = inside / (a.band * tiles) * a.band, width = min(a.band, a.tiles_c - band), rest = inside - band * tiles;
-  at.tm = rest / width;
-  at.tc = band + rest % width;
-  return inside >= 0 && at.tm < tiles;
-}
+};
 
 // Tiled products of all three kinds. A workgroup of WC x WM wavefronts has BC = 16 TC WC columns of the result by BM = 16 TM WM rows;
 // the depth goes by stages of 64 through two slots of LDS, filled by DMA. An operand whose depth is contiguous (x and w of the
@@ -98,38 +152,22 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
 
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wc = wave % WC, wm = wave / WC;
-  TilePlace at;
-  if constexpr (OP == DW) {
-    const int b = blockIdx.x;
-    int inside;
-    if (a.per) {  // many tiles a group: each XCD takes a contiguous eighth of every group's
-      at.g = b / 8 / a.per;
-      inside = b % 8 * a.per + b / 8 % a.per;
-      if (inside >= a.tiles_m * a.tiles_c) return;
-    } else {
-      at.g = b / (a.tiles_m * a.tiles_c);
-      inside = b % (a.tiles_m * a.tiles_c);
-    }
-    at.tm = inside / a.tiles_c;
-    at.tc = inside % a.tiles_c;
-    i64 count;
-    rows_of(a, at.g, at.first, count);
-    at.count = (int)count;
-  } else {
-    if (!find_tile<BM, ADAPT>(a, lane, at)) return;
-  }
-  const int depth = OP == FORWARD ? a.K : OP == DX ? a.O : at.count;
-  const int m0 = at.tm * BM, c0 = at.tc * BC;
   const int ncols = OP == FORWARD ? a.O : a.K;
-  const int rows = min(BM, (OP == DW ? a.O : at.count) - m0), cols = min(BC, ncols - c0);
-  const int stages = (depth + 63) / 64;
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)&lds[0];
-
-  // operands: first byte, bytes of a row; direct ones with a descriptor of this tile's rows, transposed ones with one of a stage's
-  const int mrow = (OP == FORWARD ? a.K : a.O) * 2, crow = a.K * 2;
-  const char* const mp = (const char*)a.m + (OP == DW ? at.first * mrow + m0 * 2 : (at.first + m0) * mrow);
-  const char* const cp = (const char*)a.c + (OP == FORWARD ? ((i64)at.g * a.O + c0) * crow : OP == DX ? (i64)at.g * a.O * crow + c0 * 2 : at.first * crow + c0 * 2);
-  const i32x4 rm = rsrc4(mp, (uint32_t)(rows * mrow)), rc = rsrc4(cp, (uint32_t)(cols * crow));
+  struct Part {  // what of the result a tile is
+    int m0, c0, rows, cols, depth, stages;
+  };
+  auto part_of = [&](const TilePlace& at) __attribute__((always_inline)) {
+    Part p;
+    p.depth = OP == FORWARD ? a.K : OP == DX ? a.O : at.count;
+    p.stages = (int)(((i64)p.depth + 63) / 64);
+    p.m0 = at.tm * BM;
+    p.c0 = at.tc * BC;
+    p.rows = min(BM, (OP == DW ? a.O : at.count) - p.m0);
+    p.cols = min(BC, ncols - p.c0);
+    return p;
+  };
+  Tiles<OP, BM, ADAPT> tiles(a, lane), ahead = tiles;
 
   // the channel of the first operand's row p (direct) or of its columns' piece q of tile t
   auto channel = [&](int p) __attribute__((always_inline)) {
@@ -137,45 +175,72 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
     return p / (16 * TC) * (16 * TC) + t / RUN * (16 * RUN) + r / 4 * (4 * RUN) + t % RUN * 4 + r % 4;
   };
   auto swizzle = [](int row) __attribute__((always_inline)) { return (row & 3) << 2 | (row >> 3 & 1) << 1; };
+  // The stages of all tiles are asked for one after another, two ahead of the products, across the tiles' borders: descriptors and
+  // offsets of the one asked for. An operand's first byte, bytes of a row; direct operands have a descriptor of the tile's rows,
+  // transposed ones one of the stage's. Past the last tile the DMAs still run but read nothing.
+  const int mrow = (OP == FORWARD ? a.K : a.O) * 2, crow = a.K * 2;
+  Part asked{};
+  int stage = 0;  // of the tile `asked`, next
+  const char *mp = nullptr, *cp = nullptr;
   uint32_t moff[MI], coff[CI];
-#pragma unroll
-  for (int k = 0; k < MI; k++) {
-    const int p = (wave * MI + k) * 64 + lane;
-    if constexpr (MT) {
-      const int q = p / (BM / 8), c = p % (BM / 8) ^ swizzle(q);
-      moff[k] = c * 8 < rows ? (uint32_t)(q * mrow + c * 16) : kOOR;
-    } else {
-      const int q = p / 8;
-      moff[k] = q < rows ? (uint32_t)(q * mrow + (p % 8 ^ (q & 7)) * 16) : kOOR;
-    }
-  }
-#pragma unroll
-  for (int k = 0; k < CI; k++) {
-    const int p = (wave * CI + k) * 64 + lane;
-    if constexpr (CT) {
-      const int q = p / (BC / 8), c = p % (BC / 8) ^ swizzle(q);
-      coff[k] = c * 8 < cols ? (uint32_t)(q * crow + c * 16) : kOOR;
-    } else {
-      const int q = p / 8, ch = channel(q);
-      coff[k] = ch < cols ? (uint32_t)(ch * crow + (p % 8 ^ (q & 7)) * 16) : kOOR;
-    }
-  }
-  // What is asked for next: a stage's descriptors and offsets. Past the last stage the DMAs still run (the waits count them) but read
-  // nothing.
-  i32x4 nm = rm, nc = rc;
-  int msoff = 0, csoff = 0;
+  i32x4 nm{}, nc{};
+  int soff = 0;
   uint32_t fill = lds0 + wave * (MI * 1024);  // the slot that is filled, where this wavefront's part of the rows' operand goes
-  auto ask = [&](int t) __attribute__((always_inline)) {
-    const bool live = t < stages;
-    const int left = live ? min(64, depth - t * 64) : 0;  // of the depth
-    auto aim = [&](auto TC_, auto NC, const char* p, i32x4 whole, int row, int width, uint32_t* off, i32x4& r, int& soff) __attribute__((always_inline)) {
-      constexpr int N = decltype(NC)::value;
-      if constexpr (decltype(TC_)::value) {  // rows t * 64 ..: `left` of them
-        r = rsrc4(p + (i64)t * 64 * row, left ? (uint32_t)((left - 1) * row + width * 2) : 0);
+  auto enter = [&](const TilePlace& at) __attribute__((always_inline)) {
+    const Part& p = asked;
+    mp = (const char*)a.m + (OP == DW ? at.first * mrow + p.m0 * 2 : (at.first + p.m0) * mrow);
+    cp = (const char*)a.c + (OP == FORWARD ? ((i64)at.g * a.O + p.c0) * crow : OP == DX ? (i64)at.g * a.O * crow + p.c0 * 2 : at.first * crow + p.c0 * 2);
+    int l = lane;
+    asm volatile("" : "+v"(l));  // (computed here, not kept in registers over the loop)
+#pragma unroll
+    for (int k = 0; k < MI; k++) {
+      const int u = (wave * MI + k) * 64 + l;
+      if constexpr (MT) {
+        const int q = u / (BM / 8), c = u % (BM / 8) ^ swizzle(q);
+        moff[k] = c * 8 < p.rows ? (uint32_t)(q * mrow + c * 16) : kOOR;
       } else {
-        r[2] = live ? whole[2] : 0;
-        soff = live ? t * 128 : 0;
-        if (live && left < 64) {  // the last stage: pieces past the last column read as zeros
+        const int q = u / 8;
+        moff[k] = q < p.rows ? (uint32_t)(q * mrow + (u % 8 ^ (q & 7)) * 16) : kOOR;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < CI; k++) {
+      const int u = (wave * CI + k) * 64 + l;
+      if constexpr (CT) {
+        const int q = u / (BC / 8), c = u % (BC / 8) ^ swizzle(q);
+        coff[k] = c * 8 < p.cols ? (uint32_t)(q * crow + c * 16) : kOOR;
+      } else {
+        const int q = u / 8, ch = channel(q);
+        coff[k] = ch < p.cols ? (uint32_t)(ch * crow + (u % 8 ^ (q & 7)) * 16) : kOOR;
+      }
+    }
+    if constexpr (!MT) nm = rsrc4(mp, (uint32_t)(p.rows * mrow));
+    if constexpr (!CT) nc = rsrc4(cp, (uint32_t)(p.cols * crow));
+  };
+  auto ask = [&]() __attribute__((always_inline)) {
+    if (stage == asked.stages) {
+      stage = 0;
+      TilePlace at;
+      bool more;
+      do {
+        more = ahead.next(at);
+        if (more) asked = part_of(at);
+      } while (more && !asked.stages);  // an empty group's gradient has none
+      if (more) {
+        enter(at);
+      } else {
+        asked.depth = 0;
+        asked.stages = -1;  // never again
+        nm[2] = nc[2] = 0;
+      }
+    }
+    const int left = min(64, asked.depth - stage * 64);  // of the depth
+    auto aim = [&](auto TC_, auto NC, const char* p, int row, int width, uint32_t* off, i32x4& r) __attribute__((always_inline)) {
+      constexpr int N = decltype(NC)::value;
+      if constexpr (decltype(TC_)::value) {  // rows stage * 64 ..: `left` of them
+        r = rsrc4(p + (i64)stage * 64 * row, left > 0 ? (uint32_t)((left - 1) * row + width * 2) : 0);
+      } else {
+        if (left > 0 && left < 64) {  // the last stage: pieces past the last column read as zeros
 #pragma unroll
           for (int k = 0; k < N; k++) {
             const int u = (wave * N + k) * 64 + lane;
@@ -184,26 +249,21 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
         }
       }
     };
-    aim(std::bool_constant<MT>{}, std::integral_constant<int, MI>{}, mp, rm, mrow, rows, moff, nm, msoff);
-    aim(std::bool_constant<CT>{}, std::integral_constant<int, CI>{}, cp, rc, crow, cols, coff, nc, csoff);
+    aim(std::bool_constant<MT>{}, std::integral_constant<int, MI>{}, mp, mrow, asked.rows, moff, nm);
+    aim(std::bool_constant<CT>{}, std::integral_constant<int, CI>{}, cp, crow, asked.cols, coff, nc);
+    soff = left > 0 ? stage * 128 : 0;
+    if (asked.stages >= 0) stage++;
   };
   constexpr int DI = MI + CI;  // DMAs of a stage
   static_assert(MI == CI, "one LDS address for both operands");
   auto issue = [&](auto KC) __attribute__((always_inline)) {  // number k of the stage asked for
     constexpr int K = decltype(KC)::value;
-    if constexpr (K < MI) dma16_at<K * 1024>(nm, fill, moff[K], msoff);
-    else dma16_at<kC + (K - MI) * 1024>(nc, fill, coff[K - MI], csoff);
+    if constexpr (K < MI) dma16_at<K * 1024>(nm, fill, moff[K], MT ? 0 : soff);
+    else dma16_at<kC + (K - MI) * 1024>(nc, fill, coff[K - MI], CT ? 0 : soff);
   };
 
-  f32x4 acc[TC][TM];
-#pragma unroll
-  for (int t = 0; t < TC; t++)
-#pragma unroll
-    for (int u = 0; u < TM; u++) acc[t][u] = f32x4{};
-  f32x4 accb[OP == DW ? TM : 1];
-#pragma unroll
-  for (int u = 0; u < (OP == DW ? TM : 1); u++) accb[u] = f32x4{};
-  const bool with_db = OP == DW && a.db && at.tc == 0 && wc == 0;
+  f32x4 acc[TC][TM], accb[OP == DW ? TM : 1];
+  bool with_db = false;
 
   // LDS addresses. Direct: row (tile, r16), piece 4 j + g. Transposed: rows 32 j + 8 g + r16 / 4 and 4 further, the piece of 4 columns
   // r16 % 4 of the tile, whose place the swizzle scatters: one address per tile (pair of tiles where a piece holds columns of both).
@@ -286,7 +346,7 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
   constexpr std::integral_constant<int, HM> hm{};
   constexpr std::integral_constant<int, HC> hc{};
   int turn = kSlot;  // from this slot to the other one
-  auto step = [&](auto busy, auto JC, int s) __attribute__((always_inline)) {  // step J of stage s
+  auto step = [&](auto busy, auto JC) __attribute__((always_inline)) {  // step J of a stage
     constexpr int J = decltype(JC)::value, f = J, JN = 1 - J;
     constexpr std::integral_constant<int, f> mf{};
     constexpr std::integral_constant<int, 1 - f> mo{};
@@ -310,79 +370,121 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
       for (uint32_t& x : ca) x += turn;
       turn = -turn;
       fill += turn;
-      ask(s + 2);
+      ask();
     }
     quarter(busy, one, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[0][t], JN, t); }, d34, dmas(zero));
     quarter(busy, one, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], JN, (1 - f) * HM + u); }, d34,
             dmas(std::integral_constant<int, DI / 4>{}));
   };
-  if (stages) {
-    ask(0);
-    mx_unroll<DI>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
-    ask(1);
-    fill += kSlot;
-    mx_unroll<DI / 2>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
-    wait_vm<DI / 2>();
-    bare_barrier();
-#pragma unroll
-    for (int u = 0; u < HM; u++) read_m(fm[0][u], 0, u);
-#pragma unroll
-    for (int t = 0; t < HC; t++) read_c(fc[0][t], 0, t);
+  ask();
+  mx_unroll<DI>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
+  ask();
+  fill += kSlot;
+  mx_unroll<DI / 2>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
+  wait_vm<DI / 2>();
+  bare_barrier();
+
+  TilePlace at;
+  while (tiles.next(at)) {
+    const Part p = part_of(at);
     auto loop = [&](auto busy) __attribute__((always_inline)) {
-      for (int s = 0; s < stages; s++) {
-        step(busy, zero, s);
-        step(busy, one, s);
+      for (int s = 0; s < p.stages; s++) {
+        step(busy, zero);
+        step(busy, one);
       }
     };
-    if (wm * (16 * TM) >= rows || wc * (16 * TC) >= cols) {  // nothing of the result is this wavefront's: its share of the DMAs alone
+    if (wm * (16 * TM) >= p.rows || wc * (16 * TC) >= p.cols) {  // nothing of the result is this wavefront's: its share of the DMAs alone
       loop(std::false_type{});
-      wait_vm<0>();
-      return;
+      continue;
     }
-    loop(std::true_type{});
-    wait_vm<0>();  // nothing lands in LDS after the workgroup has gone
-  }
-
-  if constexpr (ADAPT)
-    mx_unroll<(TM + 3) / 4>([&](auto HC_) __attribute__((always_inline)) {
-      constexpr int u0 = decltype(HC_)::value * 4, n = TM < 4 ? TM : 4;
-      const int r0 = wm * (16 * TM) + u0 * 16;
-      add_adapters<F16, n, u0>(a, acc, at.first + m0 + r0, rows - r0, c0, cols, lane,
-                               [&](int t) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r16); });
-    });
-
-  const i64 obase = OP == DW ? ((i64)at.g * a.O + m0) * a.K : (at.first + m0) * ncols;
+    with_db = OP == DW && a.db && at.tc == 0 && wc == 0;
+    int bl = lane;
+    asm volatile("" : "+v"(bl));
+    // the sums begin with the bias
 #pragma unroll
-  for (int run = 0; run < TC / RUN; run++) {
-    const int c = wc * (16 * TC) + run * (16 * RUN) + g * (4 * RUN);
-    float bias[4 * RUN];
-    mx_params<4 * RUN>(OP == FORWARD && c < cols ? a.bias : nullptr, a.bias_dt, (i64)at.g * a.O + c0 + c, 0.f, bias);
-#pragma unroll
-    for (int u = 0; u < TM; u++) {
-      const int m = mq + u * 16;
-      if (m >= rows || c >= cols) continue;
-      float v[4 * RUN];
+    for (int run = 0; run < TC / RUN; run++) {
+      float bias[4 * RUN] = {};
+      const int c = wc * (16 * TC) + run * (16 * RUN) + (bl >> 4) * (4 * RUN);
+      if constexpr (OP == FORWARD) {
+        if (a.bias) mx_params<4 * RUN>(c < p.cols ? a.bias : nullptr, a.bias_dt, (i64)at.g * a.O + p.c0 + c, 0.f, bias);
+      }
 #pragma unroll
       for (int j = 0; j < RUN; j++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[j * 4 + i] = acc[run * RUN + j][u][i] + bias[j * 4 + i];
-      const i64 to = obase + (i64)m * ncols + c0 + c;
-      if constexpr (OUT == OUT_F32) *(f32x4*)((float*)a.out + to) = f32x4{v[0], v[1], v[2], v[3]};
-      else *(mx_u32x4*)((uint16_t*)a.out + to) = mx_pack8<F16>(*(float(*)[8])v);
+        for (int u = 0; u < TM; u++) acc[run * RUN + j][u] = f32x4{bias[j * 4], bias[j * 4 + 1], bias[j * 4 + 2], bias[j * 4 + 3]};
     }
-  }
-  if constexpr (OP == DW) {
-    if (with_db && g == 0) {
+#pragma unroll
+    for (int u = 0; u < (OP == DW ? TM : 1); u++) accb[u] = f32x4{};
+    if (p.stages) {
+#pragma unroll
+      for (int u = 0; u < HM; u++) read_m(fm[0][u], 0, u);
+#pragma unroll
+      for (int t = 0; t < HC; t++) read_c(fc[0][t], 0, t);
+    }
+    loop(std::true_type{});
+
+    int el = lane;  // what follows is computed here, not kept in registers over the loop
+    asm volatile("" : "+v"(el));
+    if constexpr (ADAPT)
+      mx_unroll<(TM + 3) / 4>([&](auto HC_) __attribute__((always_inline)) {
+        constexpr int u0 = decltype(HC_)::value * 4, n = TM < 4 ? TM : 4;
+        const int r0 = wm * (16 * TM) + u0 * 16;
+        add_adapters<F16, n, u0>(a, acc, at.first + p.m0 + r0, p.rows - r0, p.c0, p.cols, el,
+                                 [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); });
+      });
+
+    // Two runs' pieces change places between lanes 8 apart, so that a store writes whole 128-byte lines of 8 rows (a run alone is 64 bytes of
+    // 16), past the caches, which keep the operands.
+    const i64 obase = OP == DW ? ((i64)at.g * a.O + p.m0) * a.K : (at.first + p.m0) * ncols;
+    constexpr int OS = OUT == OUT_F32 ? 4 : 2;
+    const int er = el & 15, eg = el >> 4;
+    const bool upper = er >= 8;
+#pragma unroll
+    for (int run = 0; run < TC / RUN; run += 2) {
+      const int c = wc * (16 * TC) + (run + upper) * (16 * RUN) + eg * (4 * RUN);
 #pragma unroll
       for (int u = 0; u < TM; u++) {
-        const int m = mq + u * 16;
-        if (m >= rows) continue;
-        const i64 to = (i64)at.g * a.O + m0 + m;
-        if constexpr (OUT == OUT_F32) ((float*)a.db)[to] = accb[u][0];
-        else ((uint16_t*)a.db)[to] = (uint16_t)mx_pack2<F16>(accb[u][0], 0.f);
+        mx_u32x4 piece[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          if constexpr (OUT == OUT_F32) {
+            piece[k] = __builtin_bit_cast(mx_u32x4, acc[run + k][u]);
+          } else {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = acc[(run + k) * 2 + j / 4][u][j % 4];
+            piece[k] = mx_pack8<F16>(v);
+          }
+        }
+        mx_u32x4 low, high;  // of rows r16 % 8 and 8 further
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const uint32_t away = upper ? piece[0][j] : piece[1][j];
+          const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)away, 0x128, 0xf, 0xf, true);  // from 8 lanes on
+          low[j] = upper ? got : piece[0][j];
+          high[j] = upper ? piece[1][j] : got;
+        }
+        const int m = wm * (16 * TM) + u * 16 + (er & 7);
+        if (c >= p.cols) continue;
+        char* to = (char*)a.out + (obase + (i64)m * ncols + p.c0 + c) * OS;
+        if (m < p.rows) __builtin_nontemporal_store(low, (mx_u32x4*)to);
+        if (m + 8 < p.rows) __builtin_nontemporal_store(high, (mx_u32x4*)(to + (i64)8 * ncols * OS));
+      }
+    }
+    if constexpr (OP == DW) {
+      if (with_db && eg == 0) {
+#pragma unroll
+        for (int u = 0; u < TM; u++) {
+          const int m = wm * (16 * TM) + u * 16 + er;
+          if (m >= p.rows) continue;
+          const i64 to = (i64)at.g * a.O + p.m0 + m;
+          if constexpr (OUT == OUT_F32) ((float*)a.db)[to] = accb[u][0];
+          else ((uint16_t*)a.db)[to] = (uint16_t)mx_pack2<F16>(accb[u][0], 0.f);
+        }
       }
     }
   }
+  wait_vm<0>();  // nothing lands in LDS after the workgroup has gone
 }
 
 template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT = false>
@@ -390,16 +492,16 @@ void launch_tile(GroupArgs a) {
   constexpr int BC = 16 * TC * WC, BM = 16 * TM * WM;
   a.tiles_c = cdiv(OP == FORWARD ? a.O : a.K, BC);
   a.band = 4;
-  i64 blocks;
+  i64 tiles;
   if (OP == DW) {
     a.tiles_m = cdiv(a.O, BM);
-    const i64 tiles = (i64)a.tiles_m * a.tiles_c;
-    a.per = tiles >= 64 ? (int)((tiles + 7) / 8) : 0;
-    blocks = a.per ? 8ll * a.per * a.G : tiles * a.G;
-  } else {  // the sum over groups of ceil(rows / BM) is at most this
-    blocks = ((a.N / BM + a.G) * a.tiles_c + 7) / 8 * 8;
+    const i64 each = (i64)a.tiles_m * a.tiles_c;
+    a.per = each >= 64 ? (int)((each + 7) / 8) : 0;
+    tiles = each * a.G;
+  } else {
+    tiles = (a.N / BM + a.G) * a.tiles_c;  // the sum over groups of ceil(rows / BM) is at most N / BM + G
   }
-  REQ(blocks * 64 * WC * WM < (1ll << 32), "%lld tiles: too many for a launch", (long long)blocks);
+  const i64 blocks = std::min<i64>(mx_device_cus(), tiles + 7) / 8 * 8;  // one workgroup fits a CU
   k_group_tile<OP, F16, OUT, TC, TM, WC, WM, ADAPT><<<(unsigned)blocks, 64 * WC * WM, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
@@ -414,10 +516,10 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TilePlace at;
-  if (!find_tile<16 * NT, ADAPT>(a, lane, at)) return;
+  if (Tiles<FORWARD, 16 * NT, ADAPT> tiles(a, lane); !tiles.next(at)) return;
   const i64 n0 = at.first + at.tm * (16 * NT);
   const int rows = min(16 * NT, at.count - at.tm * (16 * NT)), c0 = at.tc * (16 * OT), cols = min(16 * OT, a.O - c0);
-  auto chan = [&](int t) __attribute__((always_inline)) { return r16 / 4 * (4 * RUN) + t * 4 + r16 % 4; };
+  auto chan = [](int t, int r) __attribute__((always_inline)) { return r / 4 * (4 * RUN) + t * 4 + r % 4; };
   f32x4 acc[OT][NT];
 #pragma unroll
   for (int t = 0; t < OT; t++)
@@ -429,7 +531,7 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
     const auto rx = buffer((const char*)a.m + n0 * a.K * 2, (uint32_t)(rows * a.K * 2));
     uint32_t wo[OT], xo[NT];
 #pragma unroll
-    for (int t = 0; t < OT; t++) wo[t] = chan(t) < cols ? (uint32_t)(chan(t) * a.K * 2 + g * 16) : kOOR;
+    for (int t = 0; t < OT; t++) wo[t] = chan(t, r16) < cols ? (uint32_t)(chan(t, r16) * a.K * 2 + g * 16) : kOOR;
 #pragma unroll
     for (int u = 0; u < NT; u++) xo[u] = u * 16 + r16 < rows ? (uint32_t)((u * 16 + r16) * a.K * 2 + g * 16) : kOOR;
     const int S = (a.K + 31) / 32, per = (S + NW - 1) / NW, s0 = wave * per, s1 = min(s0 + per, S);
