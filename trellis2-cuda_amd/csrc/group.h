@@ -39,7 +39,7 @@ struct GroupArgs {
   void *out, *db;
   i64 N;
   int G, K, O, bias_dt;
-  int tiles_m, tiles_c, per, band;
+  int tiles_m, tiles_c, per, band, width;
   AdapterPart ad;
 };
 

@@ -15,16 +15,20 @@ enum { OUT_16 = 0, OUT_F32 = 1 };
 // operands in its L2.
 // dw: tiles are as deep as their group is long, so the longest groups come first (up to 64 groups; more are short), in rounds of W tiles
 // a XCD that run to and fro; each XCD takes a contiguous eighth of every group's tiles (where they are many).
+//
+// The last round of an XCD's W workgroups may have few tiles left: where at most half of them would have one, these are taken in quarters
+// instead (PART = REST, after the whole ones), which take two fifths of a whole one's time.
+enum { WHOLE = 0, REST = 1, ALL = 2 };
 struct TilePlace {
-  i64 first;  // the group's first row
-  int count, g, tm, tc;
+  i64 first = 0;  // the group's first row
+  int count = 0, g = 0, tm = 0, tc = 0;
 };
-template <int OP, int BM, bool ONE>  // ONE: one group, of all rows
+template <int OP, int BM, bool ONE, int PART>  // ONE: one group, of all rows; BM: rows of a whole tile; of a REST, at counts quarters
 struct Tiles {
   const GroupArgs& a;
   int lane, first, count, key;  // of the lane's group among the first 64; key: tiles up to its end, or (dw) its place in the order
   int W, round = 0;
-  i64 begin, end;  // this XCD's part of the list
+  i64 begin, end, split;  // this XCD's part of the list, and where its quartered tiles begin
 
   __device__ __forceinline__ Tiles(const GroupArgs& a_, int lane_) : a(a_), lane(lane_), W(gridDim.x / 8) {
     key = chunk(0);
@@ -48,7 +52,11 @@ struct Tiles {
       begin = blockIdx.x % 8 * per;
       end = min(begin + per, all);
     }
+    const i64 rest = end > begin ? (end - begin) % W : 0;
+    split = end - (PART != ALL && rest * 2 <= W ? rest : 0);
+    if constexpr (PART == WHOLE) end = split;
   }
+  __device__ __forceinline__ bool any() const { return PART == REST ? split < end : begin < end; }
   // The lane's group of those from g0 on, its rows inside [0, N) whatever ends holds; the tiles of all up to it
   __device__ __forceinline__ int chunk(int g0) {
     const int g = g0 + lane, N = (int)a.N;
@@ -73,35 +81,58 @@ struct Tiles {
     at.first = __builtin_amdgcn_readlane(first, who);
     at.count = __builtin_amdgcn_readlane(count, who);
   }
-  __device__ __forceinline__ bool next(TilePlace& at) {
+  __device__ __forceinline__ bool next(TilePlace& at) {  // (the same in every lane, which the compiler does not see)
+    const bool more = __builtin_amdgcn_readfirstlane(find(at));
+    round = __builtin_amdgcn_readfirstlane(round);
+    at.first = __builtin_amdgcn_readfirstlane((int)at.first);
+    at.count = __builtin_amdgcn_readfirstlane(at.count);
+    at.g = __builtin_amdgcn_readfirstlane(at.g);
+    at.tm = __builtin_amdgcn_readfirstlane(at.tm);
+    at.tc = __builtin_amdgcn_readfirstlane(at.tc);
+    return more;
+  }
+  __device__ __forceinline__ bool find(TilePlace& at) {
     const int k = blockIdx.x / 8;
+    for (;;) {
+      i64 l = begin + (i64)round * W + k;
+      int quarter = 0;
+      if constexpr (PART == REST) {
+        const i64 i = (i64)round * W + k;
+        quarter = (int)(i & 3);
+        l = split + (i >> 2);
+      } else if constexpr (OP == DW) {
+        if (round & 1) l += W - 1 - 2 * k;
+      }
+      if (l - l % W * (OP == DW && PART != REST) >= end) return false;
+      round++;
+      if (l >= end || !place(at, l)) continue;
+      if constexpr (PART == REST) {
+        at.tm = at.tm * 2 + (quarter >> 1);
+        at.tc = at.tc * 2 + (quarter & 1);
+        if (at.tm * (BM / 2) >= (OP == DW ? a.O : at.count) || at.tc * (a.width / 2) >= (OP == FORWARD ? a.O : a.K)) continue;
+      }
+      return true;
+    }
+  }
+  __device__ __forceinline__ bool place(TilePlace& at, i64 l) {  // of tile l
     if constexpr (OP == DW) {
       const int tiles = a.tiles_m * a.tiles_c;
-      for (;; round++) {
-        const i64 start = (i64)round * W;
-        if (start >= end) return false;
-        const i64 q = start + (round & 1 ? W - 1 - k : k);
-        const i64 b = q * 8 + blockIdx.x % 8;
-        const int order = (int)(a.per ? q / a.per : b / tiles);
-        const int inside = (int)(a.per ? blockIdx.x % 8 * a.per + q % a.per : b % tiles);
-        if (q >= end || order >= a.G || inside >= tiles) continue;
-        at.tm = inside / a.tiles_c;
-        at.tc = inside % a.tiles_c;
-        if (a.G <= 64) {
-          group(at, 0, __builtin_ctzll(__ballot(key == order)));
-        } else {
-          at.g = order;
-          const int N = (int)a.N, s = order ? min(max(a.ends[order - 1], 0), N) : 0;
-          at.first = s;
-          at.count = max(min(max(a.ends[order], 0), N) - s, 0);
-        }
-        round++;
-        return true;
+      const i64 b = l * 8 + blockIdx.x % 8;
+      const int order = (int)(a.per ? l / a.per : b / tiles);
+      const int inside = (int)(a.per ? blockIdx.x % 8 * a.per + l % a.per : b % tiles);
+      if (order >= a.G || inside >= tiles) return false;
+      at.tm = inside / a.tiles_c;
+      at.tc = inside % a.tiles_c;
+      if (a.G <= 64) {
+        group(at, 0, __builtin_ctzll(__ballot(key == order)));
+      } else {
+        at.g = order;
+        const int N = (int)a.N, s = order ? min(max(a.ends[order - 1], 0), N) : 0;
+        at.first = s;
+        at.count = max(min(max(a.ends[order], 0), N) - s, 0);
       }
+      return true;
     } else {
-      const i64 l = begin + (i64)round * W + k;
-      round++;
-      if (l >= end) return false;
       const int row_tile = (int)(l / a.tiles_c);
       int before = 0, upto = key;
       for (int g0 = 0;; g0 += 64) {
@@ -127,7 +158,7 @@ struct Tiles {
 };
 
 // Tiled products of all three kinds. A workgroup of WC x WM wavefronts has BC = 16 TC WC columns of the result by BM = 16 TM WM rows;
-// the depth goes by stages of 64 through two slots of LDS, filled by DMA. An operand whose depth is contiguous (x and w of the
+// the depth goes by stages of 64 through two slots of LDS (four of a quarter's), filled by DMA. An operand whose depth is contiguous (x and w of the
 // forward product, dy of dx) lies there as rows of 64 values, its 16-byte pieces permuted (piece c of row q at c ^ q % 8), so that
 // eight lanes of neighbouring rows read from distinct banks; one whose depth runs over rows (w of dx, dy and x of dw) as 64 rows, and
 // is transposed on its way into registers (ds_read_b64_tr_b16: 16 lanes give the addresses of 4 rows by four pieces of 4 values, lane i gets
@@ -140,20 +171,20 @@ struct Tiles {
 // (0, 1 - f), (1, 1 - f), (1, f) with f = 0, 1 in turn: each quarter changes one operand's half, whose registers were free a quarter
 // earlier, so every LDS read is issued one quarter before its use and a wavefront holds one step's operands only. In the
 // middle of a stage's second step all wavefronts meet: by then each has read the whole slot, so it is filled again at once.
-template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT>
-__global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupArgs a) {
+template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT, int PART>
+__device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds) {
   constexpr bool MT = OP == DW, CT = OP != FORWARD;  // transposed: the rows' operand, the columns'
   constexpr int NW = WC * WM, BC = 16 * TC * WC, BM = 16 * TM * WM, HC = TC / 2, HM = TM / 2;
   constexpr int RUN = OUT == OUT_F32 ? 1 : 2;
   constexpr int MI = BM / 8 / NW, CI = BC / 8 / NW;  // DMAs per wavefront and stage
   static_assert(MI * 8 * NW == BM && CI * 8 * NW == BC && TC % 2 == 0 && TM % 2 == 0 && HC % RUN == 0, "whole DMAs, halves of whole runs");
   constexpr uint32_t kC = BM * 128, kSlot = (BM + BC) * 128;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kSlot];
+  constexpr int NS = 131072 / kSlot;  // slots
 
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wc = wave % WC, wm = wave / WC;
   const int ncols = OP == FORWARD ? a.O : a.K;
-  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)&lds[0];
+  const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)lds;
   struct Part {  // what of the result a tile is
     int m0, c0, rows, cols, depth, stages;
   };
@@ -167,7 +198,8 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
     p.cols = min(BC, ncols - p.c0);
     return p;
   };
-  Tiles<OP, BM, ADAPT> tiles(a, lane), ahead = tiles;
+  Tiles<OP, PART == REST ? 2 * BM : BM, ADAPT, PART> tiles(a, lane), ahead = tiles;
+  if (!tiles.any()) return;
 
   // the channel of the first operand's row p (direct) or of its columns' piece q of tile t
   auto channel = [&](int p) __attribute__((always_inline)) {
@@ -175,7 +207,7 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
     return p / (16 * TC) * (16 * TC) + t / RUN * (16 * RUN) + r / 4 * (4 * RUN) + t % RUN * 4 + r % 4;
   };
   auto swizzle = [](int row) __attribute__((always_inline)) { return (row & 3) << 2 | (row >> 3 & 1) << 1; };
-  // The stages of all tiles are asked for one after another, two ahead of the products, across the tiles' borders: descriptors and
+  // The stages of all tiles are asked for one after another, NS ahead of the products, across the tiles' borders: descriptors and
   // offsets of the one asked for. An operand's first byte, bytes of a row; direct operands have a descriptor of the tile's rows,
   // transposed ones one of the stage's. Past the last tile the DMAs still run but read nothing.
   const int mrow = (OP == FORWARD ? a.K : a.O) * 2, crow = a.K * 2;
@@ -240,6 +272,8 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
       if constexpr (decltype(TC_)::value) {  // rows stage * 64 ..: `left` of them
         r = rsrc4(p + (i64)stage * 64 * row, left > 0 ? (uint32_t)((left - 1) * row + width * 2) : 0);
       } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] = __builtin_amdgcn_readfirstlane(r[i]);  // (in SGPRs, whatever the compiler makes of the branches)
         if (left > 0 && left < 64) {  // the last stage: pieces past the last column read as zeros
 #pragma unroll
           for (int k = 0; k < N; k++) {
@@ -345,12 +379,12 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
   constexpr std::integral_constant<int, 1> one{};
   constexpr std::integral_constant<int, HM> hm{};
   constexpr std::integral_constant<int, HC> hc{};
-  int turn = kSlot;  // from this slot to the other one
+  uint32_t slot = 0;  // where the stage that is multiplied stands
   auto step = [&](auto busy, auto JC) __attribute__((always_inline)) {  // step J of a stage
     constexpr int J = decltype(JC)::value, f = J, JN = 1 - J;
     constexpr std::integral_constant<int, f> mf{};
     constexpr std::integral_constant<int, 1 - f> mo{};
-    // DMAs into the other slot: the second half of the next stage, or the first half of the one after
+    // DMAs into the slot that the last stage has left: the second half of the one asked for there, or the first half of a new one
     constexpr std::integral_constant<int, J == 0 ? DI / 4 : 0> d12{};
     constexpr std::integral_constant<int, J == 0 ? 0 : DI / 4> d34{};
     auto dmas = [&](auto FROM) __attribute__((always_inline)) {
@@ -361,27 +395,31 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
     quarter(busy, zero, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[1][t], J, HC + t); }, d12,
             dmas(std::integral_constant<int, DI * 3 / 4>{}));
     if constexpr (J == 1) {  // the next stage has landed, and this one is in registers
-      wait_vm<0>();
+      wait_vm<(NS - 2) * DI>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       bare_barrier();
+      fill = lds0 + slot + wave * (MI * 1024);
+      const uint32_t on = slot == (NS - 1) * kSlot ? -slot : kSlot;
+      slot += on;
 #pragma unroll
-      for (uint32_t& x : ma) x += turn;
+      for (uint32_t& x : ma) x += on;
 #pragma unroll
-      for (uint32_t& x : ca) x += turn;
-      turn = -turn;
-      fill += turn;
+      for (uint32_t& x : ca) x += on;
       ask();
     }
     quarter(busy, one, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[0][t], JN, t); }, d34, dmas(zero));
     quarter(busy, one, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], JN, (1 - f) * HM + u); }, d34,
             dmas(std::integral_constant<int, DI / 4>{}));
   };
+#pragma unroll
+  for (int t = 0; t < NS - 1; t++) {
+    ask();
+    mx_unroll<DI>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
+    fill += kSlot;
+  }
   ask();
-  mx_unroll<DI>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
-  ask();
-  fill += kSlot;
   mx_unroll<DI / 2>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
-  wait_vm<DI / 2>();
+  wait_vm<(NS - 2) * DI + DI / 2>();
   bare_barrier();
 
   TilePlace at;
@@ -484,12 +522,20 @@ __global__ void __launch_bounds__(64 * WC * WM, WC * WM / 4) k_group_tile(GroupA
       }
     }
   }
-  wait_vm<0>();  // nothing lands in LDS after the workgroup has gone
+  wait_vm<0>();  // nothing lands in LDS after this
+  bare_barrier();
+}
+template <int OP, bool F16, int OUT, bool ADAPT>
+__global__ void __launch_bounds__(512, 2) k_group_tile(GroupArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 512 * 128];
+  multiply_tiles<OP, F16, OUT, 8, 4, 2, 4, ADAPT, WHOLE>(a, lds);
+  multiply_tiles<OP, F16, OUT, 4, 2, 2, 4, ADAPT, REST>(a, lds);
 }
 
-template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT = false>
+template <int OP, bool F16, int OUT, bool ADAPT = false>
 void launch_tile(GroupArgs a) {
-  constexpr int BC = 16 * TC * WC, BM = 16 * TM * WM;
+  constexpr int BC = 256, BM = 256;
+  a.width = BC;
   a.tiles_c = cdiv(OP == FORWARD ? a.O : a.K, BC);
   a.band = 4;
   i64 tiles;
@@ -502,7 +548,7 @@ void launch_tile(GroupArgs a) {
     tiles = (a.N / BM + a.G) * a.tiles_c;  // the sum over groups of ceil(rows / BM) is at most N / BM + G
   }
   const i64 blocks = std::min<i64>(mx_device_cus(), tiles + 7) / 8 * 8;  // one workgroup fits a CU
-  k_group_tile<OP, F16, OUT, TC, TM, WC, WM, ADAPT><<<(unsigned)blocks, 64 * WC * WM, 0, stream()>>>(a);
+  k_group_tile<OP, F16, OUT, ADAPT><<<(unsigned)blocks, 512, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
 // Few rows: the weights' bytes count, and that many of them are on their way at once. A workgroup has 16 OT channels by up to 16 NT rows of a
@@ -516,7 +562,7 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TilePlace at;
-  if (Tiles<FORWARD, 16 * NT, ADAPT> tiles(a, lane); !tiles.next(at)) return;
+  if (Tiles<FORWARD, 16 * NT, ADAPT, ALL> tiles(a, lane); !tiles.next(at)) return;
   const i64 n0 = at.first + at.tm * (16 * NT);
   const int rows = min(16 * NT, at.count - at.tm * (16 * NT)), c0 = at.tc * (16 * OT), cols = min(16 * OT, a.O - c0);
   auto chan = [](int t, int r) __attribute__((always_inline)) { return r / 4 * (4 * RUN) + t * 4 + r % 4; };
@@ -628,7 +674,7 @@ bool few_rows(const GroupArgs& a, DT dt) {
 
 template <int OP>
 void launch(const GroupArgs& a, DT dt, bool f32 = false) {
-  auto by = [&](auto F, auto T) { launch_tile<OP, decltype(F)::value, decltype(T)::value, 8, 4, 2, 4>(a); };
+  auto by = [&](auto F, auto T) { launch_tile<OP, decltype(F)::value, decltype(T)::value>(a); };
   constexpr std::integral_constant<int, OUT_16> o16{};
   constexpr std::integral_constant<int, OUT_F32> o32{};
   if constexpr (OP == FORWARD) {
@@ -670,8 +716,8 @@ void apart(const Tensor& out, const Tensor* t, const char* what) {
 
 void adapter_product(const GroupArgs& a, DT dt) {
   if (few_rows<true>(a, dt)) return;
-  if (dt == F16) launch_tile<FORWARD, true, OUT_16, 8, 4, 2, 4, true>(a);
-  else launch_tile<FORWARD, false, OUT_16, 8, 4, 2, 4, true>(a);
+  if (dt == F16) launch_tile<FORWARD, true, OUT_16, true>(a);
+  else launch_tile<FORWARD, false, OUT_16, true>(a);
 }
 
 void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Tensor* bias, Tensor& y) {
