@@ -233,7 +233,7 @@ int spc_group_linear_dw(const void* dy, const void* x, const int32_t* ends, int 
  * NULL. a x is summed in fp32, scaled and held in `dtype`. workspace: device memory of spc_adapter_workspace's bytes, 16-byte
  * aligned, or NULL (the library's own; refused while the stream is captured, if any is needed).
  * No counterpart in the reference; beside spc_mx_linear, the shared projection in 4 bits. */
-int spc_adapter_workspace(int64_t N, int64_t K, int64_t R, int64_t* bytes);
+int spc_adapter_workspace(int64_t N, int64_t R, int64_t* bytes);
 int spc_adapter_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* slots, const float* scale,
                        const void* bias, int dtype, int b_dtype, int64_t N, int64_t L, int64_t R, int64_t K, int64_t Co,
                        void* out, void* workspace, int64_t workspace_bytes);

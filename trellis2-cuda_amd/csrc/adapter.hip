@@ -3,95 +3,159 @@
 #include "group.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
-// The first product, h = x a[s]^T per row (not scaled yet): 16 U rows per workgroup and one of `parts` parts of the depth, up to 16 RT ranks
-// (blockIdx.z: which). Its 8 wavefronts share the part out, and their sums meet in LDS in a fixed order. Every adapter that some of the
-// rows have takes its turn; a lane keeps what is its row's.
+// The first product, h = scale[s] x a[s]^T per row, summed in fp32 and held in 16 bits (a matrix instruction's operand; half an ulp of it
+// reaches the result through b), one row per workgroup: the reading of a is shared by nobody but the caches, and no row waits for
+// another's adapter. The 8 wavefronts share the depth out, and their sums meet in LDS in a fixed order. 16 RT ranks (blockIdx.y: which).
+template <bool F16, int RT>
+__global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, int L, int R, int K) {
+  constexpr int NW = 8;
+  __shared__ f32x4 sums[NW][RT][4];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const i64 n = blockIdx.x;
+  const int s = slots[n], r0 = blockIdx.y * (16 * RT), ranks = min(16 * RT, R - r0);
+  if (s < 0 || s >= L) return;
+  const int S = (K + 31) / 32, s0 = S * wave / NW, s1 = S * (wave + 1) / NW;
+  const auto rx = buffer(x + n * K, (uint32_t)(K * 2)), ra = buffer(a + ((i64)s * R + r0) * K, (uint32_t)(ranks * K * 2));
+  const uint32_t xo = r16 == 0 ? (uint32_t)(g * 16) : kOOR;
+  uint32_t ao[RT];
+#pragma unroll
+  for (int t = 0; t < RT; t++) ao[t] = t * 16 + r16 < ranks ? (uint32_t)((t * 16 + r16) * K * 2 + g * 16) : kOOR;
+  f32x4 acc[RT] = {};
+  constexpr int AT = RT == 4 ? 4 : 8;  // steps on their way together
+  for (int k = s0; k < s1; k += AT) {
+    mx_u32x4 qa[AT][RT], qx[AT];
+#pragma unroll
+    for (int i = 0; i < AT; i++) {
+      const bool in = k + i < s1 && (k + i) * 32 + g * 8 < K;
+#pragma unroll
+      for (int t = 0; t < RT; t++) qa[i][t] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? ao[t] : kOOR, (k + i) * 64, 0);
+      qx[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo : kOOR, (k + i) * 64, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // the loads stay together
+#pragma unroll
+    for (int i = 0; i < AT; i++)
+#pragma unroll
+      for (int t = 0; t < RT; t++) acc[t] = mfma<F16>(qa[i][t], qx[i], acc[t]);
+  }
+  if (r16 == 0) {
+#pragma unroll
+    for (int t = 0; t < RT; t++) sums[wave][t][g] = acc[t];
+  }
+  __syncthreads();
+  if (tid < RT * 4 && tid * 4 < ranks) {
+    f32x4 c = sums[0][tid / 4][tid % 4];
+#pragma unroll
+    for (int w = 1; w < NW; w++) c += sums[w][tid / 4][tid % 4];
+    c *= scale ? scale[s] : 1.f;
+    *(mx_u32x2*)(h + n * R + r0 + tid * 4) = mx_u32x2{mx_pack2<F16>(c[0], c[1]), mx_pack2<F16>(c[2], c[3])};
+  }
+}
+
+// The same for many rows: 16 U of them per workgroup. Each XCD takes neighbouring rows, whose adapters are the same ones. Every adapter that some of the rows have takes its turn, and the
+// lanes whose row has it keep the sums; `turns` workgroups share the adapters out, so that one with a request's border among its
+// rows takes no longer than the others (those without a turn end at once).
 template <bool F16, int U, int RT>
-__global__ void __launch_bounds__(512) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, float* h, i64 N, int L, int R, int K) {
+__global__ void __launch_bounds__(512, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, i64 N, int L, int R,
+                                                       int K, int turns) {
   constexpr int NW = 8;
   __shared__ f32x4 sums[NW][U * RT][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const i64 n0 = (i64)blockIdx.x * (16 * U);
-  const int rows = (int)min((i64)(16 * U), N - n0), r0 = blockIdx.z * (16 * RT), ranks = min(16 * RT, R - r0);
+  const i64 n0 = ((i64)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8) * (16 * U);
+  if (n0 >= N) return;
+  const int rows = (int)min((i64)(16 * U), N - n0), r0 = blockIdx.y / turns * (16 * RT), ranks = min(16 * RT, R - r0);
   int mine = lane < rows && lane < 16 * U ? slots[n0 + lane] : -1;
   mine = mine < L ? mine : -1;
   int slot[U];
 #pragma unroll
   for (int u = 0; u < U; u++) slot[u] = __shfl(mine, u * 16 + r16, 64);
-  const int S = (K + 31) / 32, pieces = gridDim.y * NW, piece = blockIdx.y * NW + wave;
-  const int s0 = (int)((i64)S * piece / pieces), s1 = (int)((i64)S * (piece + 1) / pieces);
+  const int S = (K + 31) / 32, s0 = S * wave / NW, s1 = S * (wave + 1) / NW;
   const auto rx = buffer(x + n0 * K, (uint32_t)(rows * K * 2));
   uint32_t xo[U], ao[RT];
 #pragma unroll
   for (int u = 0; u < U; u++) xo[u] = slot[u] >= 0 ? (uint32_t)((u * 16 + r16) * K * 2 + g * 16) : kOOR;
 #pragma unroll
   for (int t = 0; t < RT; t++) ao[t] = t * 16 + r16 < ranks ? (uint32_t)((t * 16 + r16) * K * 2 + g * 16) : kOOR;
-  f32x4 keep[U][RT];
-#pragma unroll
-  for (int u = 0; u < U; u++)
-#pragma unroll
-    for (int t = 0; t < RT; t++) keep[u][t] = f32x4{};
-  struct Step {
-    mx_u32x4 a[RT], x[U];
-  };
-  for (uint64_t left = __ballot(mine >= 0); left;) {
+  uint64_t done = 0;  // rows whose adapters this workgroup took
+  int turn = 0;
+  for (uint64_t left = __ballot(mine >= 0); left; turn++) {
     const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-    left &= ~__ballot(mine == s);
+    const uint64_t same = __ballot(mine == s);
+    left &= ~same;
+    if (turn % turns != blockIdx.y % turns) continue;
+    done |= same;
     const auto ra = buffer(a + ((i64)s * R + r0) * K, (uint32_t)(ranks * K * 2));
     f32x4 acc[U][RT];
 #pragma unroll
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int t = 0; t < RT; t++) acc[u][t] = f32x4{};
-    constexpr int AT = 4;  // steps on their way together
-    for (int k = s0; k < s1; k += AT) {
-      Step q[AT];
+    constexpr int AT = U * RT >= 8 ? 2 : 4;  // steps loaded together, while the last ones are multiplied
+    struct Steps {
+      mx_u32x4 a[AT][RT], x[AT][U];
+    } q[2];
+    auto load = [&](Steps& q, int k) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < AT; i++) {
         const bool in = k + i < s1 && (k + i) * 32 + g * 8 < K;
 #pragma unroll
-        for (int t = 0; t < RT; t++) q[i].a[t] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? ao[t] : kOOR, (k + i) * 64, 0);
+        for (int t = 0; t < RT; t++) q.a[i][t] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? ao[t] : kOOR, (k + i) * 64, 0);
 #pragma unroll
-        for (int u = 0; u < U; u++) q[i].x[u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u] : kOOR, (k + i) * 64, 0);
+        for (int u = 0; u < U; u++) q.x[i][u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u] : kOOR, (k + i) * 64, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);  // the loads stay together
+    };
+    auto multiply = [&](const Steps& q) __attribute__((always_inline)) {
 #pragma unroll
       for (int i = 0; i < AT; i++)
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-          for (int t = 0; t < RT; t++) acc[u][t] = mfma<F16>(q[i].a[t], q[i].x[u], acc[u][t]);
+          for (int t = 0; t < RT; t++) acc[u][t] = mfma<F16>(q.a[i][t], q.x[i][u], acc[u][t]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    load(q[0], s0);
+    for (int k = s0; k < s1; k += 2 * AT) {
+      load(q[1], k + AT);
+      multiply(q[0]);
+      load(q[0], k + 2 * AT);
+      multiply(q[1]);
     }
 #pragma unroll
-    for (int u = 0; u < U; u++)
+    for (int u = 0; u < U; u++) {
+      if (slot[u] != s) continue;
 #pragma unroll
-      for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) keep[u][t][i] = slot[u] == s ? acc[u][t][i] : keep[u][t][i];
+      for (int t = 0; t < RT; t++) sums[wave][u * RT + t][lane] = acc[u][t];
+    }
   }
-#pragma unroll
-  for (int u = 0; u < U; u++)
-#pragma unroll
-    for (int t = 0; t < RT; t++) sums[wave][u * RT + t][lane] = keep[u][t];
+  if (!done) return;
   __syncthreads();
   for (int q = wave; q < U * RT; q += NW) {
+    const int n = q / RT * 16 + r16, r = q % RT * 16 + g * 4;
+    if (!(done >> n & 1) || r >= ranks) continue;
     f32x4 c = sums[0][q][lane];
 #pragma unroll
     for (int w = 1; w < NW; w++) c += sums[w][q][lane];
-    const int n = q / RT * 16 + r16, r = q % RT * 16 + g * 4;
-    if (n < rows && r < ranks) *(f32x4*)(h + ((i64)blockIdx.y * N + n0 + n) * R + r0 + r) = c;
+    c *= scale ? scale[slots[n0 + n]] : 1.f;
+    *(mx_u32x2*)(h + (n0 + n) * R + r0 + r) = mx_u32x2{mx_pack2<F16>(c[0], c[1]), mx_pack2<F16>(c[2], c[3])};
   }
 }
 
-// out = y + scale b[s] h: 16 TM rows by 16 TC channels per wavefront, four wavefronts beside each other
-template <bool F16, int TC, int TM>
+// out = y + scale b[s] h: 16 TM rows by 16 TC channels per wavefront, four wavefronts beside each other; or (SHARE) all four at the same
+// place, sharing out the rows' adapters, for few rows that differ in theirs
+template <bool F16, int TC, int TM, bool SHARE>
 __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
+  constexpr int NW = 4;
+  __shared__ f32x4 part[SHARE ? NW : 1][SHARE ? TC * TM : 1][64];
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const i64 n0 = (i64)(blockIdx.x / a.tiles_c) * (16 * TM);
-  const int rows = (int)min((i64)(16 * TM), a.N - n0), c0 = (blockIdx.x % a.tiles_c * 4 + wave) * (16 * TC), cols = min(16 * TC, a.O - c0);
+  const int rows = (int)min((i64)(16 * TM), a.N - n0), tile = blockIdx.x % a.tiles_c * (SHARE ? 1 : NW) + (SHARE ? 0 : wave);
+  const int c0 = tile * (16 * TC), cols = min(16 * TC, a.O - c0);
   if (cols <= 0) return;
   const auto ry = buffer((const uint16_t*)a.m + n0 * a.O + c0, (uint32_t)(((rows - 1) * a.O + cols) * 2));
   mx_u32x4 y[TC / 2][TM];
@@ -108,11 +172,28 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
 #pragma unroll
     for (int u = 0; u < TM; u++) acc[t][u] = f32x4{};
   add_adapters<F16, TM, 0>(a, acc, n0, rows, c0, cols, lane,
-                    [](int t, int r) __attribute__((always_inline)) { return t / 2 * 32 + r / 4 * 8 + t % 2 * 4 + r % 4; });
+                           [](int t, int r) __attribute__((always_inline)) { return t / 2 * 32 + r / 4 * 8 + t % 2 * 4 + r % 4; }, SHARE ? wave : 0,
+                           SHARE ? NW : 1);
+  if constexpr (SHARE) {
+#pragma unroll
+    for (int t = 0; t < TC; t++)
+#pragma unroll
+      for (int u = 0; u < TM; u++) part[wave][t * TM + u][lane] = acc[t][u];
+    __syncthreads();
+  }
 #pragma unroll
   for (int t = 0; t < TC / 2; t++)
 #pragma unroll
     for (int u = 0; u < TM; u++) {
+      if (SHARE && (t * TM + u) % NW != wave) continue;
+      if constexpr (SHARE) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          acc[t * 2 + k][u] = part[0][(t * 2 + k) * TM + u][lane];
+#pragma unroll
+          for (int w = 1; w < NW; w++) acc[t * 2 + k][u] += part[w][(t * 2 + k) * TM + u][lane];
+        }
+      }
       const int c = t * 32 + g * 8, m = u * 16 + r16;
       if (c >= cols || m >= rows) continue;
       float v[8];
@@ -123,15 +204,22 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
     }
 }
 
+constexpr int kTurns = 2;
+// One workgroup a row reads 2 R K bytes of a for each; 16 U rows share them, but wait for every adapter among them in turn.
+bool by_row(i64 N, i64 R) { return N * R <= 8192; }
 template <bool F16>
-void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, float* h, int parts) {
+void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tensor* scale, uint16_t* h) {
   const i64 N = x.size(0);
   const int L = (int)a.size(0), R = (int)a.size(1), K = (int)a.size(2);
   auto go = [&](auto UC, auto RC) {
     constexpr int U = decltype(UC)::value, RT = decltype(RC)::value;
-    const dim3 grid((unsigned)((N + 16 * U - 1) / (16 * U)), parts, cdiv(R, 16 * RT));
-    REQ((i64)grid.x * grid.y * grid.z * 512 < (1ll << 32), "%lld rows: too many for a launch", (long long)N);
-    k_adapter_in<F16, U, RT><<<grid, 512, 0, stream()>>>(x.ptr<uint16_t>(), a.ptr<uint16_t>(), slots.ptr<int32_t>(), h, N, L, R, K);
+    const i64 tiles = U ? ((N + 16 * U - 1) / (16 * (U ? U : 1)) + 7) / 8 * 8 : N;
+    const dim3 grid((unsigned)tiles, cdiv(R, 16 * RT) * (U ? kTurns : 1));
+    REQ(tiles * grid.y * 512 < (1ll << 32), "%lld rows: too many for a launch", (long long)N);
+    const uint16_t *px = x.ptr<uint16_t>(), *pa = a.ptr<uint16_t>();
+    const float* ps = scale ? scale->ptr<float>() : nullptr;
+    if constexpr (U == 0) k_adapter_in_rows<F16, RT><<<grid, 512, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, L, R, K);
+    else k_adapter_in<F16, U, RT><<<grid, 512, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, N, L, R, K, kTurns);
     CK(hipGetLastError());
   };
   auto by = [&](auto UC) {
@@ -139,29 +227,24 @@ void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, float* h, 
     else if (R <= 32) go(UC, std::integral_constant<int, 2>{});
     else go(UC, std::integral_constant<int, 4>{});
   };
-  if (N <= 128) by(std::integral_constant<int, 1>{});
+  if (by_row(N, R)) by(std::integral_constant<int, 0>{});
   else by(std::integral_constant<int, 2>{});
 }
 template <bool F16>
 void launch_add(const GroupArgs& a) {
-  auto go = [&](auto TCC, auto TMC) {
+  auto go = [&](auto TCC, auto TMC, auto share) {
     constexpr int TC = decltype(TCC)::value, TM = decltype(TMC)::value;
+    constexpr bool SHARE = decltype(share)::value;
     const i64 tiles = (a.N + 16 * TM - 1) / (16 * TM);
     GroupArgs p = a;
-    p.tiles_c = cdiv(a.O, 64 * TC);
+    p.tiles_c = cdiv(a.O, (SHARE ? 16 : 64) * TC);
     const i64 blocks = tiles * p.tiles_c;
     REQ(blocks * 256 < (1ll << 32), "%lld rows by %d channels: too many for a launch", (long long)a.N, a.O);
-    k_adapter_add<F16, TC, TM><<<(unsigned)blocks, 256, 0, stream()>>>(p);
+    k_adapter_add<F16, TC, TM, SHARE><<<(unsigned)blocks, 256, 0, stream()>>>(p);
     CK(hipGetLastError());
   };
-  if (a.N <= 1024) go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
-  else go(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
-}
-
-// Parts of the depth: enough workgroups for the CUs, each wavefront a step of 32 at least
-int adapter_parts(i64 N, i64 K) {
-  const i64 tiles = N <= 128 ? cdiv(N, 16) : cdiv(N, 32), most = N <= 128 ? 16 : 4;
-  return (int)std::max<i64>(1, std::min({most, 256 / std::max<i64>(tiles, 1), K / 256}));
+  if (a.N <= 1024) go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{}, std::true_type{});
+  else go(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{}, std::false_type{});
 }
 
 constexpr int kHighestRank = 256;
@@ -193,14 +276,13 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
     if (t) mx_apart(out.p, out.bytes(), t->p, t->bytes(), "out");
   if (y) REQ(y->p == out.p || !mx_overlap(y->p, y->bytes(), out.p, out.bytes()), "out must be y or apart from it");
   if (N == 0) return;
-  const i64 need = adapter_workspace(N, K, R);
+  const i64 need = adapter_workspace(N, R);
   if (workspace) {
     for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &a, &b, &slots, w, y, scale, bias, &out})
       if (t) mx_apart(t->p, t->bytes(), workspace, (size_t)need, "the workspace");
   }
   MxWorkspace ws(workspace, workspace_bytes, need);
-  const int parts = adapter_parts(N, K);
-  float* h = (float*)ws.p;
+  uint16_t* h = (uint16_t*)ws.p;
   GroupArgs g{};
   g.m = w ? x.p : y->p;
   g.c = w ? w->p : nullptr;
@@ -211,16 +293,16 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
   g.G = 1;
   g.K = (int)K;
   g.O = (int)O;
-  g.ad = AdapterPart{b.p, h, slots.ptr<int32_t>(), scale ? scale->ptr<float>() : nullptr, (int)L, (int)R, parts};
-  if (x.dt == F16) launch_in<true>(x, a, slots, h, parts);
-  else launch_in<false>(x, a, slots, h, parts);
+  g.ad = AdapterPart{b.p, h, slots.ptr<int32_t>(), (int)L, (int)R};
+  if (x.dt == F16) launch_in<true>(x, a, slots, scale, h);
+  else launch_in<false>(x, a, slots, scale, h);
   if (w) adapter_product(g, x.dt);
   else if (x.dt == F16) launch_add<true>(g);
   else launch_add<false>(g);
 }
 }  // namespace
 
-i64 adapter_workspace(i64 N, i64 K, i64 R) { return N * R * 4 * adapter_parts(N, K); }
+i64 adapter_workspace(i64 N, i64 R) { return N * R * 2; }
 
 void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
                     const Tensor* bias, Tensor& out, void* workspace, i64 workspace_bytes) {

@@ -540,10 +540,10 @@ SPC_API int spc_group_linear_dw(const void* dy, const void* x, const int32_t* en
   });
 }
 
-SPC_API int spc_adapter_workspace(int64_t N, int64_t K, int64_t R, int64_t* bytes) {
+SPC_API int spc_adapter_workspace(int64_t N, int64_t R, int64_t* bytes) {
   return guarded([&] {
-    REQ(bytes && N >= 0 && N < (1ll << 31) && K > 0 && K <= (1 << 20) && R > 0 && R <= 256, "arguments");
-    *bytes = adapter_workspace(N, K, R);
+    REQ(bytes && N >= 0 && N < (1ll << 31) && R > 0 && R <= 256, "arguments");
+    *bytes = adapter_workspace(N, R);
   });
 }
 

@@ -28,10 +28,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t
 // Adapters of a product's rows: the second of their two products is added to the result
 struct AdapterPart {
   const void* b;         // [L,O,R]
-  const float* h;        // the first product's sums in `parts` parts of the depth: [parts,N,R]
+  const uint16_t* h;     // the first product, scaled: [N,R], in the operands' type (rows without an adapter: anything)
   const int32_t* slots;  // [N]
-  const float* scale;    // [L] or null
-  int L, R, parts;
+  int L, R;
 };
 struct GroupArgs {
   const void *m, *c, *bias;  // operands of the result's rows and columns: x, w (forward); dy, w (dx); dy, x (dw)
@@ -45,9 +44,9 @@ struct GroupArgs {
 
 namespace {
 // The adapters' second product for up to 64 rows of one wavefront (16 TM rows, the first of them row n0, `rows` of which exist):
-// acc[t][u] += scale b h over tiles t of 16 channels and u of 16 rows. Every adapter that some row has takes its turn, of whose products a
+// acc[t][u] += b h over tiles t of 16 channels and u of 16 rows. Every adapter that some row has takes its turn, of whose products a
 // lane takes its row's (rows of zeros for the others would let an infinity in b reach them), so rows come in any order; those that share
-// an adapter share its reading. h is held in 16 bits. chan(t, r): the channel of
+// an adapter share its reading. chan(t, r): the channel of
 // the first operand's row r in tile t, counted from c0, `cols` of which exist. Turns first, first + every, ...
 // (TM row tiles of acc's TT, from U0 on.)
 template <bool F16, int TM, int U0, int TC, int TT, class Chan>
@@ -59,12 +58,8 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
   int mine = lane < 16 * TM && lane < rows ? p.slots[n0 + lane] : -1;
   mine = mine < p.L ? mine : -1;
   int slot[TM];
-  float scale[TM];
 #pragma unroll
-  for (int u = 0; u < TM; u++) {
-    slot[u] = __shfl(mine, u * 16 + r16, 64);
-    scale[u] = slot[u] < 0 ? 0.f : p.scale ? p.scale[slot[u]] : 1.f;
-  }
+  for (int u = 0; u < TM; u++) slot[u] = __shfl(mine, u * 16 + r16, 64);
   const uint64_t all = __ballot(mine >= 0);
   constexpr int RC = 2;  // 64 ranks at a time
   for (int r0 = 0; r0 < p.R; r0 += 32 * RC) {
@@ -74,21 +69,7 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
 #pragma unroll
       for (int u = 0; u < TM; u++) {
         const int r = r0 + c * 32 + g * 8;
-        float v[8] = {};
-        if (r < p.R && slot[u] >= 0) {
-          const float* at = p.h + (n0 + u * 16 + r16) * p.R + r;
-          for (int q = 0; q < p.parts; q++, at += a.N * p.R) {
-            const f32x4 lo = *(const f32x4*)at, hi = *(const f32x4*)(at + 4);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              v[j] += lo[j];
-              v[4 + j] += hi[j];
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 8; j++) v[j] *= scale[u];
-        }
-        h[c][u] = mx_pack8<F16>(v);
+        h[c][u] = r < p.R && slot[u] >= 0 ? *(const mx_u32x4*)(p.h + (n0 + u * 16 + r16) * p.R + r) : mx_u32x4{};
       }
     int turn = 0;
     for (uint64_t left = all; left; turn++) {
@@ -104,6 +85,11 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
 #pragma unroll
         for (int c = 0; c < RC; c++) {
           const int r = r0 + c * 32 + g * 8;
+          if (c && r0 + c * 32 >= p.R) {
+#pragma unroll
+            for (int t = 0; t < TP; t++) b[c][t] = mx_u32x4{};
+            continue;
+          }
 #pragma unroll
           for (int t = 0; t < TP; t++) {
             const int ch = chan(t0 + t, r16);

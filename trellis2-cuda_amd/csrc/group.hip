@@ -464,19 +464,20 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     int el = lane;  // what follows is computed here, not kept in registers over the loop
     asm volatile("" : "+v"(el));
     if constexpr (ADAPT)
-      mx_unroll<(TM + 3) / 4>([&](auto HC_) __attribute__((always_inline)) {
-        constexpr int u0 = decltype(HC_)::value * 4, n = TM < 4 ? TM : 4;
+      mx_unroll<TM>([&](auto UC) __attribute__((always_inline)) {  // 16 rows at a time: more would not fit the registers
+        constexpr int u0 = decltype(UC)::value, n = 1;
         const int r0 = wm * (16 * TM) + u0 * 16;
         add_adapters<F16, n, u0>(a, acc, at.first + p.m0 + r0, p.rows - r0, p.c0, p.cols, el,
                                  [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); });
       });
 
     // Two runs' pieces change places between lanes 8 apart, so that a store writes whole 128-byte lines of 8 rows (a run alone is 64 bytes of
-    // 16), past the caches, which keep the operands.
+    // 16). Where rows are whole lines they go past the caches, which keep the operands ([8192, 1024] by [8192, 1024] 133 -> 116 us); parts of
+    // lines are put together there (dw of [1416, 1032] in 16 bits: 32 us, 46 past the caches).
     const i64 obase = OP == DW ? ((i64)at.g * a.O + p.m0) * a.K : (at.first + p.m0) * ncols;
     constexpr int OS = OUT == OUT_F32 ? 4 : 2;
     const int er = el & 15, eg = el >> 4;
-    const bool upper = er >= 8;
+    const bool upper = er >= 8, lines = ((uintptr_t)a.out | (uintptr_t)(ncols * OS)) % 128 == 0;
 #pragma unroll
     for (int run = 0; run < TC / RUN; run += 2) {
       const int c = wc * (16 * TC) + (run + upper) * (16 * RUN) + eg * (4 * RUN);
@@ -505,8 +506,14 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
         const int m = wm * (16 * TM) + u * 16 + (er & 7);
         if (c >= p.cols) continue;
         char* to = (char*)a.out + (obase + (i64)m * ncols + p.c0 + c) * OS;
-        if (m < p.rows) __builtin_nontemporal_store(low, (mx_u32x4*)to);
-        if (m + 8 < p.rows) __builtin_nontemporal_store(high, (mx_u32x4*)(to + (i64)8 * ncols * OS));
+        char* const on = to + (i64)8 * ncols * OS;
+        if (lines) {
+          if (m < p.rows) __builtin_nontemporal_store(low, (mx_u32x4*)to);
+          if (m + 8 < p.rows) __builtin_nontemporal_store(high, (mx_u32x4*)on);
+        } else {
+          if (m < p.rows) *(mx_u32x4*)to = low;
+          if (m + 8 < p.rows) *(mx_u32x4*)on = high;
+        }
       }
     }
     if constexpr (OP == DW) {
@@ -603,6 +610,7 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
       Step q[U];
 #pragma unroll
       for (int k = 0; k < U; k++) load(q[k], s + k);
+      __builtin_amdgcn_sched_barrier(0);  // the loads stay together
 #pragma unroll
       for (int k = 0; k < U; k++) multiply(q[k]);
     }
@@ -611,6 +619,7 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
 #pragma unroll
       for (int k = 0; k < U; k++)
         if (s + k < s1) load(q[k], s + k);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int k = 0; k < U; k++)
         if (s + k < s1) multiply(q[k]);

@@ -235,7 +235,7 @@ void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Ten
                     const Tensor* bias, Tensor& out, void* workspace = nullptr, i64 workspace_bytes = 0);
 void adapter_add(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale, Tensor& out,
                  void* workspace = nullptr, i64 workspace_bytes = 0);
-i64 adapter_workspace(i64 N, i64 K, i64 R);
+i64 adapter_workspace(i64 N, i64 R);
 
 // Conv plus the upsample block's skip connection in one pass: out = act(conv(x) + b) + skip, skip[i, c] =
 // x_skip[src[i] >> 3, (src[i] & 7) * Cin/8 + c / rep], rep = Co / (Cin/8) a power of two, one rounding (reference:

@@ -102,7 +102,7 @@ def load_library():
     L.spc_group_linear.argtypes = [P, P, P, P, I, I, I64, I64, I64, I64, P]
     L.spc_group_linear_dx.argtypes = [P, P, P, I, I64, I64, I64, I64, P]
     L.spc_group_linear_dw.argtypes = [P, P, P, I, I64, I64, I64, I64, I, P, P]
-    L.spc_adapter_workspace.argtypes = [I64, I64, I64, PI64]
+    L.spc_adapter_workspace.argtypes = [I64, I64, PI64]
     L.spc_adapter_linear.argtypes = [P, P, P, P, P, P, P, I, I, I64, I64, I64, I64, I64, P, P, I64]
     L.spc_adapter_add.argtypes = [P, P, P, P, P, P, I, I64, I64, I64, I64, I64, P, P, I64]
     for name in SYMBOLS:
@@ -705,7 +705,7 @@ def adapter_linear(x, w, a, b, slots, scale=None, bias=None, out=None):
         out = x.new_empty(N, Co)
     else:
         _matrix(out, "out", (N, Co), x.dtype)
-    nws = _workspace_bytes("spc_adapter_workspace", N, K, R)
+    nws = _workspace_bytes("spc_adapter_workspace", N, R)
     ws = _workspace(nws, x) if nws else None
     dev = torch.cuda.current_device()
     _check(load_library().spc_adapter_linear(
@@ -724,7 +724,7 @@ def adapter_add(y, x, a, b, slots, scale=None, out=None):
         out = torch.empty_like(y)
     else:
         _matrix(out, "out", (N, Co), x.dtype)
-    nws = _workspace_bytes("spc_adapter_workspace", N, K, R)
+    nws = _workspace_bytes("spc_adapter_workspace", N, R)
     ws = _workspace(nws, x) if nws else None
     dev = torch.cuda.current_device()
     _check(load_library().spc_adapter_add(
