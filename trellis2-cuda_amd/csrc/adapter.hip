@@ -18,28 +18,39 @@ __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, cons
   const i64 n = blockIdx.x;
   const int s = slots[n], r0 = blockIdx.y * (16 * RT), ranks = min(16 * RT, R - r0);
   if (s < 0 || s >= L) return;
-  const int S = (K + 31) / 32, s0 = S * wave / NW, s1 = S * (wave + 1) / NW;
+  const int S = (K + 63) / 64, s0 = S * wave / NW, s1 = S * (wave + 1) / NW;
   const auto rx = buffer(x + n * K, (uint32_t)(K * 2)), ra = buffer(a + ((i64)s * R + r0) * K, (uint32_t)(ranks * K * 2));
-  const uint32_t xo = r16 == 0 ? (uint32_t)(g * 16) : kOOR;
-  uint32_t ao[RT];
-#pragma unroll
-  for (int t = 0; t < RT; t++) ao[t] = t * 16 + r16 < ranks ? (uint32_t)((t * 16 + r16) * K * 2 + g * 16) : kOOR;
+  const uint32_t off = line_offset(lane, K * 2);
+  const int depth = line_depth(lane);
   f32x4 acc[RT] = {};
-  constexpr int AT = RT == 4 ? 4 : 8;  // steps on their way together
+  constexpr int AT = RT == 1 ? 4 : 2;  // steps on their way together
   for (int k = s0; k < s1; k += AT) {
-    mx_u32x4 qa[AT][RT], qx[AT];
+    Lines qa[AT][RT], qx[AT];
 #pragma unroll
     for (int i = 0; i < AT; i++) {
-      const bool in = k + i < s1 && (k + i) * 32 + g * 8 < K;
+      const bool in = k + i < s1 && (k + i) * 64 + depth < K;
 #pragma unroll
-      for (int t = 0; t < RT; t++) qa[i][t] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? ao[t] : kOOR, (k + i) * 64, 0);
-      qx[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo : kOOR, (k + i) * 64, 0);
+      for (int t = 0; t < RT; t++) {
+        const uint32_t at = off + t * 16 * K * 2;
+        const int r = t * 16 + (r16 & 14);
+        qa[i][t].even = __builtin_amdgcn_raw_buffer_load_b128(ra, in && r < ranks ? at : kOOR, (k + i) * 128, 0);
+        qa[i][t].odd = __builtin_amdgcn_raw_buffer_load_b128(ra, in && r + 1 < ranks ? at + K * 2 : kOOR, (k + i) * 128, 0);
+      }
+      qx[i].even = __builtin_amdgcn_raw_buffer_load_b128(rx, in && r16 < 2 ? off : kOOR, (k + i) * 128, 0);
+      qx[i].odd = mx_u32x4{};
     }
     __builtin_amdgcn_sched_barrier(0);  // the loads stay together
 #pragma unroll
-    for (int i = 0; i < AT; i++)
+    for (int i = 0; i < AT; i++) {
+      mx_u32x4 x0, x1, a0, a1;
+      operands(qx[i], lane, x0, x1);
 #pragma unroll
-      for (int t = 0; t < RT; t++) acc[t] = mfma<F16>(qa[i][t], qx[i], acc[t]);
+      for (int t = 0; t < RT; t++) {
+        operands(qa[i][t], lane, a0, a1);
+        acc[t] = mfma<F16>(a0, x0, acc[t]);
+        acc[t] = mfma<F16>(a1, x1, acc[t]);
+      }
+    }
   }
   if (r16 == 0) {
 #pragma unroll
@@ -59,9 +70,9 @@ __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, cons
 // lanes whose row has it keep the sums; `turns` workgroups share the adapters out, so that one with a request's border among its
 // rows takes no longer than the others (those without a turn end at once).
 template <bool F16, int U, int RT>
-__global__ void __launch_bounds__(512, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, i64 N, int L, int R,
+__global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, i64 N, int L, int R,
                                                        int K, int turns) {
-  constexpr int NW = 8;
+  constexpr int NW = 4;
   __shared__ f32x4 sums[NW][U * RT][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -73,13 +84,10 @@ __global__ void __launch_bounds__(512, 2) k_adapter_in(const uint16_t* x, const 
   int slot[U];
 #pragma unroll
   for (int u = 0; u < U; u++) slot[u] = __shfl(mine, u * 16 + r16, 64);
-  const int S = (K + 31) / 32, s0 = S * wave / NW, s1 = S * (wave + 1) / NW;
+  const int S = (K + 63) / 64, s0 = S * wave / NW, s1 = S * (wave + 1) / NW;
   const auto rx = buffer(x + n0 * K, (uint32_t)(rows * K * 2));
-  uint32_t xo[U], ao[RT];
-#pragma unroll
-  for (int u = 0; u < U; u++) xo[u] = slot[u] >= 0 ? (uint32_t)((u * 16 + r16) * K * 2 + g * 16) : kOOR;
-#pragma unroll
-  for (int t = 0; t < RT; t++) ao[t] = t * 16 + r16 < ranks ? (uint32_t)((t * 16 + r16) * K * 2 + g * 16) : kOOR;
+  const uint32_t off = line_offset(lane, K * 2);
+  const int depth = line_depth(lane);
   uint64_t done = 0;  // rows whose adapters this workgroup took
   int turn = 0;
   for (uint64_t left = __ballot(mine >= 0); left; turn++) {
@@ -94,35 +102,47 @@ __global__ void __launch_bounds__(512, 2) k_adapter_in(const uint16_t* x, const 
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int t = 0; t < RT; t++) acc[u][t] = f32x4{};
-    constexpr int AT = U * RT >= 8 ? 2 : 4;  // steps loaded together, while the last ones are multiplied
-    struct Steps {
-      mx_u32x4 a[AT][RT], x[AT][U];
-    } q[2];
-    auto load = [&](Steps& q, int k) __attribute__((always_inline)) {
+    struct Step {
+      Lines a[RT], x[U];
+    } q[2];  // one is loaded while the other is multiplied
+    auto load = [&](Step& q, int k) __attribute__((always_inline)) {
+      const bool in = k < s1 && k * 64 + depth < K;
 #pragma unroll
-      for (int i = 0; i < AT; i++) {
-        const bool in = k + i < s1 && (k + i) * 32 + g * 8 < K;
+      for (int t = 0; t < RT; t++) {
+        const uint32_t at = off + t * 16 * K * 2;
+        const int r = t * 16 + (r16 & 14);
+        q.a[t].even = __builtin_amdgcn_raw_buffer_load_b128(ra, in && r < ranks ? at : kOOR, k * 128, 0);
+        q.a[t].odd = __builtin_amdgcn_raw_buffer_load_b128(ra, in && r + 1 < ranks ? at + K * 2 : kOOR, k * 128, 0);
+      }
 #pragma unroll
-        for (int t = 0; t < RT; t++) q.a[i][t] = __builtin_amdgcn_raw_buffer_load_b128(ra, in ? ao[t] : kOOR, (k + i) * 64, 0);
-#pragma unroll
-        for (int u = 0; u < U; u++) q.x[i][u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u] : kOOR, (k + i) * 64, 0);
+      for (int u = 0; u < U; u++) {
+        const uint32_t at = off + u * 16 * K * 2;
+        const int n = u * 16 + (r16 & 14);
+        q.x[u].even = __builtin_amdgcn_raw_buffer_load_b128(rx, in && n < rows ? at : kOOR, k * 128, 0);
+        q.x[u].odd = __builtin_amdgcn_raw_buffer_load_b128(rx, in && n + 1 < rows ? at + K * 2 : kOOR, k * 128, 0);
       }
       __builtin_amdgcn_sched_barrier(0);  // the loads stay together
     };
-    auto multiply = [&](const Steps& q) __attribute__((always_inline)) {
+    auto multiply = [&](const Step& q) __attribute__((always_inline)) {
+      mx_u32x4 x[U][2];
 #pragma unroll
-      for (int i = 0; i < AT; i++)
+      for (int u = 0; u < U; u++) operands(q.x[u], lane, x[u][0], x[u][1]);
+#pragma unroll
+      for (int t = 0; t < RT; t++) {
+        mx_u32x4 a[2];
+        operands(q.a[t], lane, a[0], a[1]);
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-          for (int t = 0; t < RT; t++) acc[u][t] = mfma<F16>(q.a[i][t], q.x[i][u], acc[u][t]);
+          for (int j = 0; j < 2; j++) acc[u][t] = mfma<F16>(a[j], x[u][j], acc[u][t]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     };
     load(q[0], s0);
-    for (int k = s0; k < s1; k += 2 * AT) {
-      load(q[1], k + AT);
+    for (int k = s0; k < s1; k += 2) {
+      load(q[1], k + 1);
       multiply(q[0]);
-      load(q[0], k + 2 * AT);
+      load(q[0], k + 2);
       multiply(q[1]);
     }
 #pragma unroll
@@ -219,7 +239,7 @@ void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tens
     const uint16_t *px = x.ptr<uint16_t>(), *pa = a.ptr<uint16_t>();
     const float* ps = scale ? scale->ptr<float>() : nullptr;
     if constexpr (U == 0) k_adapter_in_rows<F16, RT><<<grid, 512, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, L, R, K);
-    else k_adapter_in<F16, U, RT><<<grid, 512, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, N, L, R, K, kTurns);
+    else k_adapter_in<F16, U, RT><<<grid, 256, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, N, L, R, K, kTurns);
     CK(hipGetLastError());
   };
   auto by = [&](auto UC) {
@@ -227,8 +247,19 @@ void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tens
     else if (R <= 32) go(UC, std::integral_constant<int, 2>{});
     else go(UC, std::integral_constant<int, 4>{});
   };
+  // Workgroups of 16 u rows. With more than 32 ranks one takes some u + 2 (its rows of x, and a) and fills a CU; a second one doubles the time ([8209, 4096],
+  // 64 ranks of 16 adapters: 41 us with 32 rows, whose 257 workgroups are one too many; [8192, 4096] 28)
+  const i64 cus = mx_device_cus();
+  int u = 2;
+  i64 least = 0;
+  for (int t = 2; t <= (R > 32 ? 4 : 2); t++) {
+    const i64 rounds = cdiv(cdiv(cdiv(N, 16 * t), 8) * 8, cus), cost = rounds * (t + 2);
+    if (t == 2 || cost < least) u = t, least = cost;
+  }
   if (by_row(N, R)) by(std::integral_constant<int, 0>{});
-  else by(std::integral_constant<int, 2>{});
+  else if (u == 2) by(std::integral_constant<int, 2>{});
+  else if (u == 3) by(std::integral_constant<int, 3>{});
+  else by(std::integral_constant<int, 4>{});
 }
 template <bool F16>
 void launch_add(const GroupArgs& a) {

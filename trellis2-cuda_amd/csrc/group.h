@@ -25,6 +25,31 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t
 }
 }  // namespace
 
+namespace {
+// 16 rows of 64 depths straight from memory into operands. A load instruction that takes 64 bytes of each of 16 rows gets half of what one that
+// takes 128 bytes of each of 8 gets (x and a of 8192 rows by 4096, 64 ranks: 28 us and 17), so one loads the even rows' lines and one the
+// odd ones', two lanes beside each other 64 bytes of either row, and change halves afterwards.
+struct Lines {
+  mx_u32x4 even, odd;
+};
+// Byte offset of this lane's 16 bytes of the even rows' lines, `row` bytes apart; the odd ones' are a row further
+__device__ __forceinline__ uint32_t line_offset(int lane, int row) {
+  return (uint32_t)((lane & 14) * row + ((lane & 1) * 4 + (lane >> 4)) * 16);
+}
+__device__ __forceinline__ int line_depth(int lane) { return ((lane & 1) * 4 + (lane >> 4)) * 8; }  // its first depth of the 64
+// Operands of the first and the last 32 depths: lane l has row l % 16, depths 8 (l / 16) .. + 7
+__device__ __forceinline__ void operands(const Lines& q, int lane, mx_u32x4& first, mx_u32x4& last) {
+  const bool odd = lane & 1;
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    const uint32_t away = odd ? q.even[j] : q.odd[j];
+    const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)away, 0xB1, 0xf, 0xf, true);  // of lanes 1, 0, 3, 2
+    first[j] = odd ? got : q.even[j];
+    last[j] = odd ? q.odd[j] : got;
+  }
+}
+}  // namespace
+
 // Adapters of a product's rows: the second of their two products is added to the result
 struct AdapterPart {
   const void* b;         // [L,O,R]

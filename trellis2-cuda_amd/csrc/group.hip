@@ -582,29 +582,47 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
     // every load is a buffer load whose offset is past the end where there is nothing (a row or a channel past the last, depths past K)
     const auto rw = buffer((const char*)a.c + ((i64)at.g * a.O + c0) * a.K * 2, (uint32_t)(cols * a.K * 2));
     const auto rx = buffer((const char*)a.m + n0 * a.K * 2, (uint32_t)(rows * a.K * 2));
-    uint32_t wo[OT], xo[NT];
+    // (the channels' operand as in Lines: row r of a tile is channel chan(t, r))
+    const int even = r16 & 14, S = (a.K + 63) / 64, per = (S + NW - 1) / NW, s0 = wave * per, s1 = min(s0 + per, S), depth = line_depth(lane);
+    const uint32_t off = depth * 2;
+    uint32_t wo[OT][2], xo[NT][2];
 #pragma unroll
-    for (int t = 0; t < OT; t++) wo[t] = chan(t, r16) < cols ? (uint32_t)(chan(t, r16) * a.K * 2 + g * 16) : kOOR;
+    for (int k = 0; k < 2; k++) {
 #pragma unroll
-    for (int u = 0; u < NT; u++) xo[u] = u * 16 + r16 < rows ? (uint32_t)((u * 16 + r16) * a.K * 2 + g * 16) : kOOR;
-    const int S = (a.K + 31) / 32, per = (S + NW - 1) / NW, s0 = wave * per, s1 = min(s0 + per, S);
+      for (int t = 0; t < OT; t++) wo[t][k] = chan(t, even + k) < cols ? (uint32_t)(chan(t, even + k) * a.K * 2) + off : kOOR;
+#pragma unroll
+      for (int u = 0; u < NT; u++) xo[u][k] = u * 16 + even + k < rows ? (uint32_t)((u * 16 + even + k) * a.K * 2) + off : kOOR;
+    }
     struct Step {
-      mx_u32x4 w[OT], x[NT];
+      Lines w[OT], x[NT];
     };
     auto load = [&](Step& q, int s) __attribute__((always_inline)) {
-      const bool in = s * 32 + g * 8 < a.K;
+      const bool in = s * 64 + depth < a.K;
 #pragma unroll
-      for (int t = 0; t < OT; t++) q.w[t] = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? wo[t] : kOOR, s * 64, 0);
+      for (int t = 0; t < OT; t++) {
+        q.w[t].even = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? wo[t][0] : kOOR, s * 128, 0);
+        q.w[t].odd = __builtin_amdgcn_raw_buffer_load_b128(rw, in ? wo[t][1] : kOOR, s * 128, 0);
+      }
 #pragma unroll
-      for (int u = 0; u < NT; u++) q.x[u] = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u] : kOOR, s * 64, 0);
+      for (int u = 0; u < NT; u++) {
+        q.x[u].even = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u][0] : kOOR, s * 128, 0);
+        q.x[u].odd = __builtin_amdgcn_raw_buffer_load_b128(rx, in ? xo[u][1] : kOOR, s * 128, 0);
+      }
     };
     auto multiply = [&](const Step& q) __attribute__((always_inline)) {
+      mx_u32x4 w[OT][2], x[2];
 #pragma unroll
-      for (int u = 0; u < NT; u++)
+      for (int t = 0; t < OT; t++) operands(q.w[t], lane, w[t][0], w[t][1]);
 #pragma unroll
-        for (int t = 0; t < OT; t++) acc[t][u] = mfma<F16>(q.w[t], q.x[u], acc[t][u]);
+      for (int u = 0; u < NT; u++) {
+        operands(q.x[u], lane, x[0], x[1]);
+#pragma unroll
+        for (int t = 0; t < OT; t++)
+#pragma unroll
+          for (int j = 0; j < 2; j++) acc[t][u] = mfma<F16>(w[t][j], x[j], acc[t][u]);
+      }
     };
-    constexpr int U = 8;  // steps on their way together
+    constexpr int U = 4;  // steps on their way together
     int s = s0;
     for (; s + U <= s1; s += U) {
       Step q[U];
