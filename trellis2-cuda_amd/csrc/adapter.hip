@@ -191,8 +191,8 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
   for (int t = 0; t < TC; t++)
 #pragma unroll
     for (int u = 0; u < TM; u++) acc[t][u] = f32x4{};
-  add_adapters<F16, TM, 0>(a, acc, n0, rows, c0, cols, lane,
-                           [](int t, int r) __attribute__((always_inline)) { return t / 2 * 32 + r / 4 * 8 + t % 2 * 4 + r % 4; }, SHARE ? wave : 0,
+  add_adapters<F16>(a, acc, n0, rows, c0, cols, lane,
+                    [](int t, int r) __attribute__((always_inline)) { return t / 2 * 32 + r / 4 * 8 + t % 2 * 4 + r % 4; }, SHARE ? wave : 0,
                            SHARE ? NW : 1);
   if constexpr (SHARE) {
 #pragma unroll

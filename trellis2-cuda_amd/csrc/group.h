@@ -73,11 +73,10 @@ namespace {
 // lane takes its row's (rows of zeros for the others would let an infinity in b reach them), so rows come in any order; those that share
 // an adapter share its reading. chan(t, r): the channel of
 // the first operand's row r in tile t, counted from c0, `cols` of which exist. Turns first, first + every, ...
-// (TM row tiles of acc's TT, from U0 on.)
-template <bool F16, int TM, int U0, int TC, int TT, class Chan>
-__device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC][TT], i64 n0, int rows, int c0, int cols, int lane, Chan&& chan,
+template <bool F16, int TC, int TM, class Chan>
+__device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC][TM], i64 n0, int rows, int c0, int cols, int lane, Chan&& chan,
                                              int first = 0, int every = 1) {
-  static_assert(TM <= 4 && U0 + TM <= TT, "a lane a row");
+  static_assert(TM <= 4, "a lane a row");
   const AdapterPart& p = a.ad;
   const int r16 = lane & 15, g = lane >> 4;
   int mine = lane < 16 * TM && lane < rows ? p.slots[n0 + lane] : -1;
@@ -130,7 +129,7 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
 #pragma unroll
             for (int c = 1; c < RC; c++) d = mfma<F16>(b[c][t], h[c][u], d);
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[t0 + t][U0 + u][i] += slot[u] == s ? d[i] : 0.f;
+            for (int i = 0; i < 4; i++) acc[t0 + t][u][i] += slot[u] == s ? d[i] : 0.f;
           }
         }
       }

@@ -464,12 +464,8 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     int el = lane;  // what follows is computed here, not kept in registers over the loop
     asm volatile("" : "+v"(el));
     if constexpr (ADAPT)
-      mx_unroll<TM>([&](auto UC) __attribute__((always_inline)) {  // 16 rows at a time: more would not fit the registers
-        constexpr int u0 = decltype(UC)::value, n = 1;
-        const int r0 = wm * (16 * TM) + u0 * 16;
-        add_adapters<F16, n, u0>(a, acc, at.first + p.m0 + r0, p.rows - r0, p.c0, p.cols, el,
-                                 [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); });
-      });
+      add_adapters<F16>(a, acc, at.first + p.m0 + wm * (16 * TM), p.rows - wm * (16 * TM), p.c0, p.cols, el,
+                        [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); });
 
     // Two runs' pieces change places between lanes 8 apart, so that a store writes whole 128-byte lines of 8 rows (a run alone is 64 bytes of
     // 16). Where rows are whole lines they go past the caches, which keep the operands ([8192, 1024] by [8192, 1024] 133 -> 116 us); parts of
@@ -643,7 +639,7 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
         if (s + k < s1) multiply(q[k]);
     }
   } else {
-    add_adapters<F16, NT, 0>(a, acc, n0, rows, c0, cols, lane, chan, wave - NW, NA);
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, wave - NW, NA);
   }
 #pragma unroll
   for (int t = 0; t < OT; t++)
