@@ -83,6 +83,7 @@ def test_adapters():
     refused(lib.spc_adapter_workspace(4, 8, None), "arguments")
     assert lib.spc_adapter_workspace(0, 8, ctypes.byref(n)) == 0 and n.value == 0
     assert lib.spc_adapter_workspace(7, 24, ctypes.byref(n)) == 0 and n.value == 2 * 7 * 24
+    assert lib.spc_adapter_workspace(1, 16, ctypes.byref(n)) == 0 and n.value == 0  # one kernel
 
     def linear(x=A, w=2 * A, a=3 * A, b=4 * A, slots=5 * A, scale=None, bias=None, dt=2, bdt=0, n=4, l=3, r=16, k=64, o=72, out=6 * A,
                work=None, nwork=0):

@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const 
 }
 
 // out = y + scale b[s] h: 16 TM rows by 16 TC channels per wavefront, four wavefronts beside each other; or (SHARE) all four at the same
-// place, sharing out the rows' adapters, for few rows that differ in theirs
-template <bool F16, int TC, int TM, bool SHARE>
+// place, sharing out the rows' adapters, for few rows that differ in theirs; FUSED, they make the first product, too
+template <bool F16, int TC, int TM, bool SHARE, bool FUSED>
 __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
   constexpr int NW = 4;
   __shared__ f32x4 part[SHARE ? NW : 1][SHARE ? TC * TM : 1][64];
@@ -191,9 +191,16 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
   for (int t = 0; t < TC; t++)
 #pragma unroll
     for (int u = 0; u < TM; u++) acc[t][u] = f32x4{};
-  add_adapters<F16>(a, acc, n0, rows, c0, cols, lane,
-                    [](int t, int r) __attribute__((always_inline)) { return t / 2 * 32 + r / 4 * 8 + t % 2 * 4 + r % 4; }, SHARE ? wave : 0,
-                           SHARE ? NW : 1);
+  auto chan = [](int t, int r) __attribute__((always_inline)) { return t / 2 * 32 + r / 4 * 8 + t % 2 * 4 + r % 4; };
+  if constexpr (FUSED) {
+    __shared__ __attribute__((aligned(16))) InnerSums inner[NW];
+    inner_products<F16, NW>(a, lane, wave, inner[wave]);
+    __syncthreads();
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan,
+                      [&](i64 n, int r, int s) __attribute__((always_inline)) { return inner_of<F16, NW>(a, inner, (int)n, r, s); }, wave, NW);
+  } else {
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, stored_inner(a), SHARE ? wave : 0, SHARE ? NW : 1);
+  }
   if constexpr (SHARE) {
 #pragma unroll
     for (int t = 0; t < TC; t++)
@@ -263,26 +270,37 @@ void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tens
 }
 template <bool F16>
 void launch_add(const GroupArgs& a) {
-  auto go = [&](auto TCC, auto TMC, auto share) {
+  auto go = [&](auto TCC, auto TMC, auto share, auto fused) {
     constexpr int TC = decltype(TCC)::value, TM = decltype(TMC)::value;
-    constexpr bool SHARE = decltype(share)::value;
+    constexpr bool SHARE = decltype(share)::value, FUSED = decltype(fused)::value;
     const i64 tiles = (a.N + 16 * TM - 1) / (16 * TM);
     GroupArgs p = a;
     p.tiles_c = cdiv(a.O, (SHARE ? 16 : 64) * TC);
     const i64 blocks = tiles * p.tiles_c;
     REQ(blocks * 256 < (1ll << 32), "%lld rows by %d channels: too many for a launch", (long long)a.N, a.O);
-    k_adapter_add<F16, TC, TM, SHARE><<<(unsigned)blocks, 256, 0, stream()>>>(p);
+    k_adapter_add<F16, TC, TM, SHARE, FUSED><<<(unsigned)blocks, 256, 0, stream()>>>(p);
     CK(hipGetLastError());
   };
-  if (a.N <= 1024) go(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{}, std::true_type{});
-  else go(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{}, std::false_type{});
+  constexpr std::integral_constant<int, 1> one{};
+  constexpr std::integral_constant<int, 2> two{};
+  constexpr std::integral_constant<int, 4> four{};
+  if (!a.ad.h) go(four, one, std::true_type{}, std::true_type{});
+  else if (a.N <= 1024) go(four, one, std::true_type{}, std::false_type{});
+  else go(two, four, std::false_type{}, std::false_type{});
 }
 
 constexpr int kHighestRank = 256;
-void check(const Tensor& t, const char* what, DT dt, std::vector<i64> sh) {
-  std::string s;
-  for (i64 v : sh) s += (s.empty() ? "" : ",") + std::to_string(v);
-  REQ(t.dt == dt && t.sh == sh, "%s must be %s [%s]", what, dname(dt), s.c_str());
+void check(const Tensor& t, const char* what, DT dt, std::initializer_list<i64> sh) {
+  bool same = t.dt == dt && t.dim() == (int)sh.size();
+  if (same) {
+    int i = 0;
+    for (i64 v : sh) same &= t.sh[i++] == v;
+  }
+  if (!same) {  // (the message is put together only now: a call takes some microseconds in all)
+    std::string s;
+    for (i64 v : sh) s += (s.empty() ? "" : ",") + std::to_string(v);
+    REQ(same, "%s must be %s [%s]", what, dname(dt), s.c_str());
+  }
   REQ((uintptr_t)t.p % 16 == 0 && (t.p || t.numel() == 0), "%s must be 16-byte aligned and not null", what);
 }
 void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
@@ -314,6 +332,7 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
   }
   MxWorkspace ws(workspace, workspace_bytes, need);
   uint16_t* h = (uint16_t*)ws.p;
+  const bool fused = adapter_fused(N, R);
   GroupArgs g{};
   g.m = w ? x.p : y->p;
   g.c = w ? w->p : nullptr;
@@ -324,16 +343,15 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
   g.G = 1;
   g.K = (int)K;
   g.O = (int)O;
-  g.ad = AdapterPart{b.p, h, slots.ptr<int32_t>(), (int)L, (int)R};
-  if (x.dt == F16) launch_in<true>(x, a, slots, scale, h);
-  else launch_in<false>(x, a, slots, scale, h);
+  g.ad = AdapterPart{b.p, fused ? nullptr : h, slots.ptr<int32_t>(), (int)L, (int)R, x.p, a.p, scale ? scale->ptr<float>() : nullptr};
+  if (!fused) x.dt == F16 ? launch_in<true>(x, a, slots, scale, h) : launch_in<false>(x, a, slots, scale, h);
   if (w) adapter_product(g, x.dt);
   else if (x.dt == F16) launch_add<true>(g);
   else launch_add<false>(g);
 }
 }  // namespace
 
-i64 adapter_workspace(i64 N, i64 R) { return N * R * 2; }
+i64 adapter_workspace(i64 N, i64 R) { return adapter_fused(N, R) ? 0 : N * R * 2; }
 
 void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
                     const Tensor* bias, Tensor& out, void* workspace, i64 workspace_bytes) {

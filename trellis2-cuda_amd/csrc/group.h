@@ -56,7 +56,13 @@ struct AdapterPart {
   const uint16_t* h;     // the first product, scaled: [N,R], in the operands' type (rows without an adapter: anything)
   const int32_t* slots;  // [N]
   int L, R;
+  const void *x, *a;     // what h is made of where the same kernel makes it (h null): [N,K], [L,R,K]
+  const float* scale;    // [L] or null
 };
+// Where that is: so few rows and ranks that every workgroup reads a for itself, in about the time that it waits for the weights, rather than
+// wait for a kernel of its own ([1, 4096] by [4096, 4096], 16 ranks: 16.7 -> 11.3 us)
+constexpr int kFusedRows = 4, kFusedRanks = 32;
+inline bool adapter_fused(i64 N, i64 R) { return N <= kFusedRows && N * R <= kFusedRanks; }
 struct GroupArgs {
   const void *m, *c, *bias;  // operands of the result's rows and columns: x, w (forward); dy, w (dx); dy, x (dw)
   const int32_t* ends;
@@ -68,14 +74,71 @@ struct GroupArgs {
 };
 
 namespace {
+__device__ __forceinline__ auto stored_inner(const GroupArgs& a) {
+  return [&a](i64 n, int r, int) __attribute__((always_inline)) { return *(const mx_u32x4*)(a.ad.h + n * a.ad.R + r); };
+}
+// The first product of up to kFusedRows rows, by NW wavefronts, of which this is number w: its part of the sums, to be added over w
+typedef float InnerSums[kFusedRows][kFusedRanks];
+template <bool F16, int NW>
+__device__ __forceinline__ void inner_products(const GroupArgs& a, int lane, int w, InnerSums& sums) {
+  const AdapterPart& p = a.ad;
+  const int r16 = lane & 15, g = lane >> 4, S = (a.K + 63) / 64, s0 = S * w / NW, s1 = S * (w + 1) / NW, depth = line_depth(lane), even = r16 & 14;
+  const uint32_t off = line_offset(lane, a.K * 2);
+  for (int n = 0; n < (int)a.N; n++) {
+    const int slot = p.slots[n];
+    if (slot < 0 || slot >= p.L) continue;
+    const auto rx = buffer((const char*)p.x + (i64)n * a.K * 2, (uint32_t)(a.K * 2)), ra = buffer((const char*)p.a + (i64)slot * p.R * a.K * 2, (uint32_t)(p.R * a.K * 2));
+    for (int r0 = 0; r0 < p.R; r0 += 16) {
+      f32x4 acc{};
+      constexpr int AT = 8;  // steps on their way together
+      for (int k = s0; k < s1; k += AT) {
+        Lines qa[AT], qx[AT];
+#pragma unroll
+        for (int i = 0; i < AT; i++) {
+          const bool in = k + i < s1 && (k + i) * 64 + depth < a.K;
+          const uint32_t at = off + r0 * a.K * 2;
+          qa[i].even = __builtin_amdgcn_raw_buffer_load_b128(ra, in && r0 + even < p.R ? at : kOOR, (k + i) * 128, 0);
+          qa[i].odd = __builtin_amdgcn_raw_buffer_load_b128(ra, in && r0 + even + 1 < p.R ? at + a.K * 2 : kOOR, (k + i) * 128, 0);
+          qx[i].even = __builtin_amdgcn_raw_buffer_load_b128(rx, in && r16 < 2 ? off : kOOR, (k + i) * 128, 0);
+          qx[i].odd = mx_u32x4{};
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the loads stay together
+#pragma unroll
+        for (int i = 0; i < AT; i++) {
+          mx_u32x4 a0, a1, x0, x1;
+          operands(qa[i], lane, a0, a1);
+          operands(qx[i], lane, x0, x1);
+          acc = mfma<F16>(a0, x0, acc);
+          acc = mfma<F16>(a1, x1, acc);
+        }
+      }
+      if (r16 == 0) *(f32x4*)&sums[n][r0 + g * 4] = acc;
+    }
+  }
+}
+// Ranks r .. r + 7 of row n of the first product, scaled and in 16 bits, from the sums of NW wavefronts
+template <bool F16, int NW>
+__device__ __forceinline__ mx_u32x4 inner_of(const GroupArgs& a, const InnerSums* sums, int n, int r, int slot) {
+  float v[8] = {};
+#pragma unroll
+  for (int w = 0; w < NW; w++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] += sums[w][n][r + j];
+  const float scale = a.ad.scale ? a.ad.scale[slot] : 1.f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) v[j] *= scale;
+  return mx_pack8<F16>(v);
+}
+
 // The adapters' second product for up to 64 rows of one wavefront (16 TM rows, the first of them row n0, `rows` of which exist):
 // acc[t][u] += b h over tiles t of 16 channels and u of 16 rows. Every adapter that some row has takes its turn, of whose products a
 // lane takes its row's (rows of zeros for the others would let an infinity in b reach them), so rows come in any order; those that share
 // an adapter share its reading. chan(t, r): the channel of
-// the first operand's row r in tile t, counted from c0, `cols` of which exist. Turns first, first + every, ...
-template <bool F16, int TC, int TM, class Chan>
+// the first operand's row r in tile t, counted from c0, `cols` of which exist. inner(n, r, s): ranks r .. r + 7 of h's row n (stored_inner: as
+// it lies in memory). Turns first, first + every, ...
+template <bool F16, int TC, int TM, class Chan, class Inner>
 __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC][TM], i64 n0, int rows, int c0, int cols, int lane, Chan&& chan,
-                                             int first = 0, int every = 1) {
+                                             Inner&& inner, int first = 0, int every = 1) {
   static_assert(TM <= 4, "a lane a row");
   const AdapterPart& p = a.ad;
   const int r16 = lane & 15, g = lane >> 4;
@@ -93,7 +156,7 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
 #pragma unroll
       for (int u = 0; u < TM; u++) {
         const int r = r0 + c * 32 + g * 8;
-        h[c][u] = r < p.R && slot[u] >= 0 ? *(const mx_u32x4*)(p.h + (n0 + u * 16 + r16) * p.R + r) : mx_u32x4{};
+        h[c][u] = r < p.R && slot[u] >= 0 ? inner(n0 + u * 16 + r16, r, slot[u]) : mx_u32x4{};
       }
     int turn = 0;
     for (uint64_t left = all; left; turn++) {

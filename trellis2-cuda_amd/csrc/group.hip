@@ -465,7 +465,7 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     asm volatile("" : "+v"(el));
     if constexpr (ADAPT)
       add_adapters<F16>(a, acc, at.first + p.m0 + wm * (16 * TM), p.rows - wm * (16 * TM), p.c0, p.cols, el,
-                        [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); });
+                        [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); }, stored_inner(a));
 
     // Two runs' pieces change places between lanes 8 apart, so that a store writes whole 128-byte lines of 8 rows (a run alone is 64 bytes of
     // 16). Where rows are whole lines they go past the caches, which keep the operands ([8192, 1024] by [8192, 1024] 133 -> 116 us); parts of
@@ -556,12 +556,13 @@ void launch_tile(GroupArgs a) {
 }
 // Few rows: the weights' bytes count, and that many of them are on their way at once. A workgroup has 16 OT channels by up to 16 NT rows of a
 // group; each of its 8 wavefronts takes a contiguous eighth of the depth, both operands straight into registers, and the sums meet in
-// LDS in a fixed order. With adapters, 4 wavefronts more add them meanwhile.
-template <bool F16, int OT, int NT, bool ADAPT>
+// LDS in a fixed order. With adapters, 4 wavefronts more add them meanwhile; FUSED, they also make the first product.
+template <bool F16, int OT, int NT, bool ADAPT, bool FUSED>
 __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
   constexpr int NW = 8, NA = ADAPT ? 4 : 0, RUN = OT;
   static_assert(OT == 1 || OT == 2, "4 or 8 channels a lane");
   __shared__ f32x4 part[NW + NA][OT * NT][64];
+  __shared__ __attribute__((aligned(16))) InnerSums inner[FUSED ? NA : 1];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   TilePlace at;
@@ -638,8 +639,16 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
       for (int k = 0; k < U; k++)
         if (s + k < s1) multiply(q[k]);
     }
+  } else if constexpr (FUSED) {
+    inner_products<F16, NA>(a, lane, wave - NW, inner[wave - NW]);
   } else {
-    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, wave - NW, NA);
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, stored_inner(a), wave - NW, NA);
+  }
+  if constexpr (FUSED) {
+    __syncthreads();
+    if (wave >= NW)
+      add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan,
+                        [&](i64 n, int r, int s) __attribute__((always_inline)) { return inner_of<F16, NA>(a, inner, (int)n, r, s); }, wave - NW, NA);
   }
 #pragma unroll
   for (int t = 0; t < OT; t++)
@@ -666,13 +675,13 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
     else *(mx_u32x2*)to = mx_u32x2{mx_pack2<F16>(v[0], v[1]), mx_pack2<F16>(v[2], v[3])};
   }
 }
-template <bool F16, int OT, int NT, bool ADAPT>
+template <bool F16, int OT, int NT, bool ADAPT, bool FUSED = false>
 void launch_rows(GroupArgs a) {
   a.tiles_c = cdiv(a.O, 16 * OT);
   a.band = 8;
   const i64 blocks = ((a.N / (16 * NT) + a.G) * a.tiles_c + 7) / 8 * 8;
   REQ(blocks * (ADAPT ? 768 : 512) < (1ll << 32), "%lld tiles: too many for a launch", (long long)blocks);
-  k_group_rows<F16, OT, NT, ADAPT><<<(unsigned)blocks, ADAPT ? 768 : 512, 0, stream()>>>(a);
+  k_group_rows<F16, OT, NT, ADAPT, FUSED><<<(unsigned)blocks, ADAPT ? 768 : 512, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
 
@@ -682,6 +691,9 @@ bool few_rows(const GroupArgs& a, DT dt) {
   if (mean > 64) return false;
   auto by = [&](auto F) {
     constexpr bool f = decltype(F)::value;
+    if constexpr (ADAPT) {
+      if (!a.ad.h) return launch_rows<f, 1, 1, true, true>(a);
+    }
     if (mean <= 16) {
       if (a.O * (a.N < a.G ? a.N : a.G) <= 16 * 1024) launch_rows<f, 1, 1, ADAPT>(a);
       else launch_rows<f, 2, 1, ADAPT>(a);

@@ -508,7 +508,7 @@ def _workspace(nbytes, like):
     torch hands it on only to work behind the call's, and never while earlier work on it is under way."""
     torch = _torch()
     lib = _library_stream()
-    if torch.cuda.current_stream().cuda_stream == lib:
+    if torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()) == lib:  # (an address; a Stream object takes 7 us)
         return like.new_empty(nbytes, dtype=torch.uint8)
     with torch.cuda.stream(torch.cuda.ExternalStream(lib, like.device) if lib else torch.cuda.default_stream(like.device)):
         return like.new_empty(nbytes, dtype=torch.uint8)
