@@ -541,17 +541,13 @@ void launch_tile(GroupArgs a) {
   a.width = BC;
   a.tiles_c = cdiv(OP == FORWARD ? a.O : a.K, BC);
   a.band = 4;
-  i64 tiles;
   if (OP == DW) {
     a.tiles_m = cdiv(a.O, BM);
     const i64 each = (i64)a.tiles_m * a.tiles_c;
     a.per = each >= 64 ? (int)((each + 7) / 8) : 0;
-    tiles = each * a.G;
-  } else {
-    tiles = (a.N / BM + a.G) * a.tiles_c;  // the sum over groups of ceil(rows / BM) is at most N / BM + G
   }
-  const i64 blocks = std::min<i64>(mx_device_cus(), tiles + 7) / 8 * 8;  // one workgroup fits a CU
-  k_group_tile<OP, F16, OUT, ADAPT><<<(unsigned)blocks, 512, 0, stream()>>>(a);
+  const int blocks = mx_device_cus() / 8 * 8;  // one workgroup fits a CU; what has no tile ends at once
+  k_group_tile<OP, F16, OUT, ADAPT><<<blocks, 512, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
 // Few rows: the weights' bytes count, and that many of them are on their way at once. A workgroup has 16 OT channels by up to 16 NT rows of a
