@@ -216,13 +216,17 @@ int spc_convnext_mlp_mx(const void* h, const void* x, const void* gamma, const v
  *   spc_group_linear_dx  dx = w[g]^T dy
  *   spc_group_linear_dw  dw[g] = sum of dy x^T over g's rows (zeros where there are none), db[g] = sum of dy unless db is NULL;
  *                        dw [G,Co,K], db [G,Co] of `out_dtype`: SPC_F32 or `dtype`
- * Results overlap no input. No counterpart in the reference; beside spc_mx_linear, whose weight all rows share. */
+ * Results overlap no input. workspace: device memory of spc_group_linear_workspace's bytes for the product (0 unless the result is
+ * small and the sums are long), 16-byte aligned, or NULL (the library's own; refused while the stream is captured, if any is needed).
+ * No counterpart in the reference; beside spc_mx_linear, whose weight all rows share. */
+enum { SPC_GROUP_FORWARD = 0, SPC_GROUP_DX = 1, SPC_GROUP_DW = 2 };
+int spc_group_linear_workspace(int product, int64_t N, int64_t G, int64_t K, int64_t Co, int64_t* bytes);
 int spc_group_linear(const void* x, const void* w, const int32_t* ends, const void* bias, int dtype, int b_dtype, int64_t N,
-                     int64_t G, int64_t K, int64_t Co, void* y);
+                     int64_t G, int64_t K, int64_t Co, void* y, void* workspace, int64_t workspace_bytes);
 int spc_group_linear_dx(const void* dy, const void* w, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
-                        int64_t Co, void* dx);
+                        int64_t Co, void* dx, void* workspace, int64_t workspace_bytes);
 int spc_group_linear_dw(const void* dy, const void* x, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
-                        int64_t Co, int out_dtype, void* dw, void* db);
+                        int64_t Co, int out_dtype, void* dw, void* db, void* workspace, int64_t workspace_bytes);
 
 /* Low-rank adapters of many requests beside one shared projection. Row n's adapter is s = slots[n] (int32 [N] on the device;
  * outside [0, L): none), and it gets scale[s] b[s] (a[s] x[n]) added:
@@ -230,10 +234,10 @@ int spc_group_linear_dw(const void* dy, const void* x, const int32_t* ends, int 
  *   spc_adapter_add      out = y + that, for a projection y made elsewhere (spc_mx_linear's); out may be y
  * x [N,K], w [Co,K], a [L,R,K], b [L,Co,R], y, out [N,Co] of one `dtype` (SPC_F16/SPC_BF16), 16-byte aligned; R a multiple of 8,
  * at most 256; K and Co multiples of 8, at most 2^20; L at most 2^16; scale float [L] or NULL (1); bias [Co] of `b_dtype` or
- * NULL. a x is summed in fp32, scaled and held in `dtype`. workspace: device memory of spc_adapter_workspace's bytes, 16-byte
- * aligned, or NULL (the library's own; refused while the stream is captured, if any is needed).
+ * NULL. a x is summed in fp32, scaled and held in `dtype`. workspace: device memory of spc_adapter_workspace's bytes (K = 0 for
+ * spc_adapter_add), 16-byte aligned, or NULL (the library's own; refused while the stream is captured, if any is needed).
  * No counterpart in the reference; beside spc_mx_linear, the shared projection in 4 bits. */
-int spc_adapter_workspace(int64_t N, int64_t R, int64_t* bytes);
+int spc_adapter_workspace(int64_t N, int64_t R, int64_t K, int64_t Co, int64_t* bytes);
 int spc_adapter_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* slots, const float* scale,
                        const void* bias, int dtype, int b_dtype, int64_t N, int64_t L, int64_t R, int64_t K, int64_t Co,
                        void* out, void* workspace, int64_t workspace_bytes);

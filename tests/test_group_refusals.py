@@ -22,8 +22,8 @@ def refused(rc, word):
 def test_forward():
     lib = sp.load_library()
 
-    def call(x=A, w=2 * A, ends=3 * A, bias=None, dt=2, bdt=0, n=4, g=3, k=64, o=72, y=4 * A):
-        return lib.spc_group_linear(p(x), p(w), p(ends), p(bias), dt, bdt, n, g, k, o, p(y))
+    def call(x=A, w=2 * A, ends=3 * A, bias=None, dt=2, bdt=0, n=4, g=3, k=64, o=72, y=4 * A, work=None, nwork=0):
+        return lib.spc_group_linear(p(x), p(w), p(ends), p(bias), dt, bdt, n, g, k, o, p(y), p(work), nwork)
 
     refused(call(k=60), "multiple of 8")
     refused(call(o=70), "multiple of 8")
@@ -46,16 +46,22 @@ def test_forward():
     refused(call(bias=4 * A + 64), "overlap")
     refused(call(bias=5 * A, bdt=3), "dtype code 3")
     assert call(n=0, x=None, y=None) == 0
+    # 500 rows of one group: few tiles, deep
+    deep = dict(n=500, g=1, k=4096, o=128, x=0x10000000, w=0x20000000, y=0x30000000)
+    refused(call(**deep, work=0x40000000, nwork=16), "workspace of 16 bytes")
+    refused(call(**deep, work=0x40000008, nwork=1 << 30), "16-byte aligned")
+    for over in ("x", "w", "y"):
+        refused(call(**deep, work=deep[over], nwork=1 << 30), "overlap the workspace")
 
 
 def test_gradients():
     lib = sp.load_library()
 
-    def dx(dy=A, w=2 * A, ends=3 * A, dt=2, n=4, g=3, k=64, o=72, out=4 * A):
-        return lib.spc_group_linear_dx(p(dy), p(w), p(ends), dt, n, g, k, o, p(out))
+    def dx(dy=A, w=2 * A, ends=3 * A, dt=2, n=4, g=3, k=64, o=72, out=4 * A, work=None, nwork=0):
+        return lib.spc_group_linear_dx(p(dy), p(w), p(ends), dt, n, g, k, o, p(out), p(work), nwork)
 
-    def dw(dy=A, x=2 * A, ends=3 * A, dt=2, n=4, g=3, k=64, o=72, odt=0, out=4 * A, db=5 * A):
-        return lib.spc_group_linear_dw(p(dy), p(x), p(ends), dt, n, g, k, o, odt, p(out), p(db))
+    def dw(dy=A, x=2 * A, ends=3 * A, dt=2, n=4, g=3, k=64, o=72, odt=0, out=4 * A, db=5 * A, work=None, nwork=0):
+        return lib.spc_group_linear_dw(p(dy), p(x), p(ends), dt, n, g, k, o, odt, p(out), p(db), p(work), nwork)
 
     refused(dx(k=4), "multiple of 8")
     refused(dx(dt=0), "bf16/fp16")
@@ -64,6 +70,11 @@ def test_gradients():
     refused(dx(w=None), "null")
     refused(dx(ends=None), "null")
     assert dx(n=0, dy=None, out=None) == 0
+    refused(dx(n=500, g=1, k=128, o=4096, dy=0x10000000, w=0x20000000, out=0x30000000, work=0x40000000, nwork=16), "workspace of 16 bytes")
+    refused(dx(n=500, g=1, k=128, o=4096, dy=0x10000000, w=0x20000000, out=0x30000000, work=0x10000000, nwork=1 << 30), "overlap the workspace")
+    deep = dict(n=9000, g=1, k=128, o=128, dy=0x10000000, x=0x20000000, out=0x30000000)
+    refused(dw(**deep, work=0x40000000, nwork=16), "workspace of 16 bytes")
+    refused(dw(**deep, work=5 * A, nwork=1 << 30), "overlap the workspace")
     refused(dw(o=12), "multiple of 8")
     refused(dw(odt=1), "fp32 or of dy's type")
     refused(dw(out=None), "null")
@@ -76,14 +87,37 @@ def test_gradients():
     refused(dw(n=1 << 31), "rows")
 
 
-def test_adapters():
+def test_workspaces():
+    """Zero unless a few tiles are deep; the adapters' also holds the first product, except a single row's."""
     lib, n = sp.load_library(), ctypes.c_int64()
-    refused(lib.spc_adapter_workspace(4, 0, ctypes.byref(n)), "arguments")
-    refused(lib.spc_adapter_workspace(1 << 31, 8, ctypes.byref(n)), "arguments")
-    refused(lib.spc_adapter_workspace(4, 8, None), "arguments")
-    assert lib.spc_adapter_workspace(0, 8, ctypes.byref(n)) == 0 and n.value == 0
-    assert lib.spc_adapter_workspace(7, 24, ctypes.byref(n)) == 0 and n.value == 2 * 7 * 24
-    assert lib.spc_adapter_workspace(1, 16, ctypes.byref(n)) == 0 and n.value == 0  # one kernel
+
+    def group(*sizes):
+        assert lib.spc_group_linear_workspace(*sizes, ctypes.byref(n)) == 0
+        return n.value
+
+    def adapter(*sizes):
+        assert lib.spc_adapter_workspace(*sizes, ctypes.byref(n)) == 0
+        return n.value
+
+    assert group(sp.GROUP_FORWARD, 0, 1, 4096, 128) == group(sp.GROUP_FORWARD, 64, 1, 4096, 128) == group(sp.GROUP_FORWARD, 500, 1, 1024, 128) == 0
+    assert group(sp.GROUP_FORWARD, 16000, 8, 4096, 4096) == 0
+    assert group(sp.GROUP_FORWARD, 500, 1, 4096, 128) % (500 * 128 * 4) == 0 < n.value < 1 << 26
+    assert group(sp.GROUP_DX, 500, 1, 128, 4096) % (500 * 128 * 4) == 0 < n.value < 1 << 26
+    assert group(sp.GROUP_DW, 9000, 1, 128, 136) % (129 * 136 * 4) == 0 < n.value < 1 << 26
+    assert group(sp.GROUP_DW, 1000, 1, 128, 128) == group(sp.GROUP_DW, 0, 1, 128, 128) == 0
+    assert adapter(0, 8, 64, 64) == adapter(1, 16, 4096, 4096) == adapter(1, 16, 0, 4096) == 0
+    assert adapter(7, 24, 0, 64) == 512 and adapter(500, 8, 64, 64) == 500 * 16 // 256 * 256 + 256
+    assert adapter(500, 8, 4096, 128) > adapter(500, 8, 0, 128) > 0
+    for bad in ((3, 4, 1, 64, 64), (-1, 4, 1, 64, 64), (0, 1 << 31, 1, 64, 64), (0, 4, 0, 64, 64), (0, 4, 1, 0, 64), (0, 4, 1, 64, 1 << 21)):
+        refused(lib.spc_group_linear_workspace(*bad, ctypes.byref(n)), "arguments")
+    refused(lib.spc_group_linear_workspace(0, 4, 1, 64, 64, None), "arguments")
+    for bad in ((4, 0, 64, 64), (1 << 31, 8, 64, 64), (4, 264, 64, 64), (4, 8, -1, 64), (4, 8, 64, 0)):
+        refused(lib.spc_adapter_workspace(*bad, ctypes.byref(n)), "arguments")
+    refused(lib.spc_adapter_workspace(4, 8, 64, 64, None), "arguments")
+
+
+def test_adapters():
+    lib = sp.load_library()
 
     def linear(x=A, w=2 * A, a=3 * A, b=4 * A, slots=5 * A, scale=None, bias=None, dt=2, bdt=0, n=4, l=3, r=16, k=64, o=72, out=6 * A,
                work=None, nwork=0):

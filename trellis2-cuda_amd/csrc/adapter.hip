@@ -289,6 +289,7 @@ void launch_add(const GroupArgs& a) {
   else go(two, four, std::false_type{}, std::false_type{});
 }
 
+i64 inner_bytes(i64 N, i64 R) { return adapter_fused(N, R) ? 0 : (N * R * 2 + 255) / 256 * 256; }
 constexpr int kHighestRank = 256;
 void check(const Tensor& t, const char* what, DT dt, std::initializer_list<i64> sh) {
   bool same = t.dt == dt && t.dim() == (int)sh.size();
@@ -325,13 +326,14 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
     if (t) mx_apart(out.p, out.bytes(), t->p, t->bytes(), "out");
   if (y) REQ(y->p == out.p || !mx_overlap(y->p, y->bytes(), out.p, out.bytes()), "out must be y or apart from it");
   if (N == 0) return;
-  const i64 need = adapter_workspace(N, R);
+  const i64 need = adapter_workspace(N, R, w ? K : 0, O);
   if (workspace) {
     for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &a, &b, &slots, w, y, scale, bias, &out})
       if (t) mx_apart(t->p, t->bytes(), workspace, (size_t)need, "the workspace");
   }
   MxWorkspace ws(workspace, workspace_bytes, need);
   uint16_t* h = (uint16_t*)ws.p;
+  const i64 inner = inner_bytes(N, R);
   const bool fused = adapter_fused(N, R);
   GroupArgs g{};
   g.m = w ? x.p : y->p;
@@ -345,13 +347,13 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
   g.O = (int)O;
   g.ad = AdapterPart{b.p, fused ? nullptr : h, slots.ptr<int32_t>(), (int)L, (int)R, x.p, a.p, scale ? scale->ptr<float>() : nullptr};
   if (!fused) x.dt == F16 ? launch_in<true>(x, a, slots, scale, h) : launch_in<false>(x, a, slots, scale, h);
-  if (w) adapter_product(g, x.dt);
+  if (w) adapter_product(g, x.dt, inner < need ? ws.p + inner : nullptr);
   else if (x.dt == F16) launch_add<true>(g);
   else launch_add<false>(g);
 }
 }  // namespace
 
-i64 adapter_workspace(i64 N, i64 R) { return adapter_fused(N, R) ? 0 : N * R * 2; }
+i64 adapter_workspace(i64 N, i64 R, i64 K, i64 O) { return inner_bytes(N, R) + (K ? adapter_product_bytes(N, K, O) : 0); }
 
 void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
                     const Tensor* bias, Tensor& out, void* workspace, i64 workspace_bytes) {

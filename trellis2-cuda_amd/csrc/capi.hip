@@ -509,41 +509,49 @@ SPC_API int spc_convnext_mlp_mx(const void* h, const void* x, const void* gamma,
   });
 }
 
+SPC_API int spc_group_linear_workspace(int product, int64_t N, int64_t G, int64_t K, int64_t Co, int64_t* bytes) {
+  return guarded([&] {
+    REQ(bytes && product >= SPC_GROUP_FORWARD && product <= SPC_GROUP_DW && N >= 0 && N < (1ll << 31) && G > 0 && G <= (1 << 16) && K > 0 &&
+            K <= (1 << 20) && Co > 0 && Co <= (1 << 20), "arguments");
+    *bytes = group_linear_workspace(product, N, G, K, Co);
+  });
+}
+
 SPC_API int spc_group_linear(const void* x, const void* w, const int32_t* ends, const void* bias, int dtype, int b_dtype, int64_t N,
-                             int64_t G, int64_t K, int64_t Co, void* y) {
+                             int64_t G, int64_t K, int64_t Co, void* y, void* workspace, int64_t workspace_bytes) {
   return guarded([&] {
     REQ(N >= 0 && G > 0 && K > 0 && Co > 0, "N=%lld G=%lld K=%lld Co=%lld", (long long)N, (long long)G, (long long)K, (long long)Co);
     const DT dt = float_dt(dtype, "x/w");
     Tensor tb, ty = borrow(y, {N, Co}, dt);
     if (bias) tb = borrow(bias, {G, Co}, float_dt(b_dtype, "bias"));
-    group_linear(borrow(x, {N, K}, dt), borrow(w, {G, Co, K}, dt), borrow(ends, {G}, I32), bias ? &tb : nullptr, ty);
+    group_linear(borrow(x, {N, K}, dt), borrow(w, {G, Co, K}, dt), borrow(ends, {G}, I32), bias ? &tb : nullptr, ty, workspace, workspace_bytes);
   });
 }
 
 SPC_API int spc_group_linear_dx(const void* dy, const void* w, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
-                                int64_t Co, void* dx) {
+                                int64_t Co, void* dx, void* workspace, int64_t workspace_bytes) {
   return guarded([&] {
     REQ(N >= 0 && G > 0 && K > 0 && Co > 0, "N=%lld G=%lld K=%lld Co=%lld", (long long)N, (long long)G, (long long)K, (long long)Co);
     const DT dt = float_dt(dtype, "dy/w");
     Tensor tx = borrow(dx, {N, K}, dt);
-    group_linear_dx(borrow(dy, {N, Co}, dt), borrow(w, {G, Co, K}, dt), borrow(ends, {G}, I32), tx);
+    group_linear_dx(borrow(dy, {N, Co}, dt), borrow(w, {G, Co, K}, dt), borrow(ends, {G}, I32), tx, workspace, workspace_bytes);
   });
 }
 
 SPC_API int spc_group_linear_dw(const void* dy, const void* x, const int32_t* ends, int dtype, int64_t N, int64_t G, int64_t K,
-                                int64_t Co, int out_dtype, void* dw, void* db) {
+                                int64_t Co, int out_dtype, void* dw, void* db, void* workspace, int64_t workspace_bytes) {
   return guarded([&] {
     REQ(N >= 0 && G > 0 && K > 0 && Co > 0, "N=%lld G=%lld K=%lld Co=%lld", (long long)N, (long long)G, (long long)K, (long long)Co);
     const DT dt = float_dt(dtype, "dy/x"), odt = float_dt(out_dtype, "out");
     Tensor tw = borrow(dw, {G, Co, K}, odt), tb = borrow(db, {G, Co}, odt);
-    group_linear_dw(borrow(dy, {N, Co}, dt), borrow(x, {N, K}, dt), borrow(ends, {G}, I32), tw, db ? &tb : nullptr);
+    group_linear_dw(borrow(dy, {N, Co}, dt), borrow(x, {N, K}, dt), borrow(ends, {G}, I32), tw, db ? &tb : nullptr, workspace, workspace_bytes);
   });
 }
 
-SPC_API int spc_adapter_workspace(int64_t N, int64_t R, int64_t* bytes) {
+SPC_API int spc_adapter_workspace(int64_t N, int64_t R, int64_t K, int64_t Co, int64_t* bytes) {
   return guarded([&] {
-    REQ(bytes && N >= 0 && N < (1ll << 31) && R > 0 && R <= 256, "arguments");
-    *bytes = adapter_workspace(N, R);
+    REQ(bytes && N >= 0 && N < (1ll << 31) && R > 0 && R <= 256 && K >= 0 && K <= (1 << 20) && Co > 0 && Co <= (1 << 20), "arguments");
+    *bytes = adapter_workspace(N, R, K, Co);
   });
 }
 

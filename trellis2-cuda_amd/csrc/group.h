@@ -71,6 +71,8 @@ struct GroupArgs {
   int G, K, O, bias_dt;
   int tiles_m, tiles_c, per, band, width;
   AdapterPart ad;
+  int split;  // parts of the depth, of `elems` results each
+  i64 elems;
 };
 
 namespace {
@@ -201,5 +203,6 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
 }
 }  // namespace
 
-// out = x w^T + bias + adapters over all N rows (group.hip), without checks
-void adapter_product(const GroupArgs& a, DT dt);
+// out = x w^T + bias + adapters over all N rows (group.hip), without checks; workspace: of that many bytes
+void adapter_product(const GroupArgs& a, DT dt, void* workspace);
+i64 adapter_product_bytes(i64 N, i64 K, i64 O);

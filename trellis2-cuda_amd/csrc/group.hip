@@ -6,7 +6,7 @@
 #include <type_traits>
 
 namespace {
-enum { FORWARD = 0, DX = 1, DW = 2 };
+enum { FORWARD = GROUP_FORWARD, DX = GROUP_DX, DW = GROUP_DW };
 enum { OUT_16 = 0, OUT_F32 = 1 };
 // A workgroup's tiles, one after another. Every wavefront finds them for itself, with a lane a group, 64 groups at a time.
 //
@@ -18,17 +18,21 @@ enum { OUT_16 = 0, OUT_F32 = 1 };
 //
 // The last round of an XCD's W workgroups may have few tiles left: where at most half of them would have one, these are taken in quarters
 // instead (PART = REST, after the whole ones), which take two fifths of a whole one's time.
+//
+// A few deep tiles are each taken in `split` parts of the depth, whose fp32 sums a second kernel adds (split_of says when).
 enum { WHOLE = 0, REST = 1, ALL = 2 };
 struct TilePlace {
   i64 first = 0;  // the group's first row
   int count = 0, g = 0, tm = 0, tc = 0;
+  int part = 0;  // of the depth
 };
 template <int OP, int BM, bool ONE, int PART>  // ONE: one group, of all rows; BM: rows of a whole tile; of a REST, at counts quarters
 struct Tiles {
   const GroupArgs& a;
   int lane, first, count, key;  // of the lane's group among the first 64; key: tiles up to its end, or (dw) its place in the order
   int W, round = 0;
-  i64 begin, end, split;  // this XCD's part of the list, and where its quartered tiles begin
+  i64 begin;         // this XCD's first part of a tile
+  i64 end, quarter;  // how many it has, and where the quartered ones begin
 
   __device__ __forceinline__ Tiles(const GroupArgs& a_, int lane_) : a(a_), lane(lane_), W(gridDim.x / 8) {
     key = chunk(0);
@@ -41,22 +45,22 @@ struct Tiles {
       key = lane < a.G ? place : -1;
       const i64 per = (i64)a.tiles_m * a.tiles_c;
       begin = 0;
-      end = a.per ? (i64)a.per * a.G : (per * a.G + 7) / 8;
+      end = a.per ? (i64)a.per * a.G : (per * a.G * a.split + 7) / 8;
     } else {
       i64 total = __builtin_amdgcn_readlane(key, 63);
       if (a.G > 64) {
         for (int g0 = 64; g0 < a.G; g0 += 64) total += __builtin_amdgcn_readlane(chunk(g0), 63);
         key = chunk(0);
       }
-      const i64 all = total * a.tiles_c, per = (all + 7) / 8;
+      const i64 all = total * a.tiles_c * a.split, per = (all + 7) / 8;
       begin = blockIdx.x % 8 * per;
-      end = min(begin + per, all);
+      end = max(min(per, all - begin), (i64)0);
     }
-    const i64 rest = end > begin ? (end - begin) % W : 0;
-    split = end - (PART != ALL && rest * 2 <= W ? rest : 0);
-    if constexpr (PART == WHOLE) end = split;
+    const i64 rest = end % W;
+    quarter = end - (PART != ALL && rest * 2 <= W ? rest : 0);
+    if constexpr (PART == WHOLE) end = quarter;
   }
-  __device__ __forceinline__ bool any() const { return PART == REST ? split < end : begin < end; }
+  __device__ __forceinline__ bool any() const { return PART == REST ? quarter < end : end > 0; }
   // The lane's group of those from g0 on, its rows inside [0, N) whatever ends holds; the tiles of all up to it
   __device__ __forceinline__ int chunk(int g0) {
     const int g = g0 + lane, N = (int)a.N;
@@ -89,35 +93,41 @@ struct Tiles {
     at.g = __builtin_amdgcn_readfirstlane(at.g);
     at.tm = __builtin_amdgcn_readfirstlane(at.tm);
     at.tc = __builtin_amdgcn_readfirstlane(at.tc);
+    at.part = __builtin_amdgcn_readfirstlane(at.part);
     return more;
   }
   __device__ __forceinline__ bool find(TilePlace& at) {
     const int k = blockIdx.x / 8;
     for (;;) {
-      i64 l = begin + (i64)round * W + k;
-      int quarter = 0;
+      const i64 start = (i64)round * W;
+      i64 l = start + k;
+      int which = 0;
       if constexpr (PART == REST) {
-        const i64 i = (i64)round * W + k;
-        quarter = (int)(i & 3);
-        l = split + (i >> 2);
-      } else if constexpr (OP == DW) {
-        if (round & 1) l += W - 1 - 2 * k;
+        const int across = (OP == FORWARD ? a.O : a.K) <= a.width / 2 ? 1 : 2;  // (a narrow result has none to the right)
+        which = (int)(l % (2 * across));
+        l = quarter + l / (2 * across);
+        if (quarter + start / (2 * across) >= end) return false;
+        which = across == 1 ? which * 2 : which;
+      } else {
+        if (OP == DW && (round & 1)) l = start + W - 1 - k;
+        if (start >= end) return false;
       }
-      if (l - l % W * (OP == DW && PART != REST) >= end) return false;
       round++;
-      if (l >= end || !place(at, l)) continue;
+      if (l >= end) continue;
+      if (!place(at, begin + l)) continue;
       if constexpr (PART == REST) {
-        at.tm = at.tm * 2 + (quarter >> 1);
-        at.tc = at.tc * 2 + (quarter & 1);
+        at.tm = at.tm * 2 + (which >> 1);
+        at.tc = at.tc * 2 + (which & 1);
         if (at.tm * (BM / 2) >= (OP == DW ? a.O : at.count) || at.tc * (a.width / 2) >= (OP == FORWARD ? a.O : a.K)) continue;
       }
       return true;
     }
   }
-  __device__ __forceinline__ bool place(TilePlace& at, i64 l) {  // of tile l
+  __device__ __forceinline__ bool place(TilePlace& at, i64 l) {
     if constexpr (OP == DW) {
       const int tiles = a.tiles_m * a.tiles_c;
-      const i64 b = l * 8 + blockIdx.x % 8;
+      const i64 u = l * 8 + blockIdx.x % 8, b = u / a.split;
+      at.part = a.per ? 0 : (int)(u % a.split);  // (many tiles are not split)
       const int order = (int)(a.per ? l / a.per : b / tiles);
       const int inside = (int)(a.per ? blockIdx.x % 8 * a.per + l % a.per : b % tiles);
       if (order >= a.G || inside >= tiles) return false;
@@ -133,6 +143,8 @@ struct Tiles {
       }
       return true;
     } else {
+      at.part = (int)(l % a.split);
+      l /= a.split;
       const int row_tile = (int)(l / a.tiles_c);
       int before = 0, upto = key;
       for (int g0 = 0;; g0 += 64) {
@@ -186,12 +198,16 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
   const int ncols = OP == FORWARD ? a.O : a.K;
   const uint32_t lds0 = (uint32_t)(size_t)(__attribute__((address_space(3))) uint8_t*)lds;
   struct Part {  // what of the result a tile is
-    int m0, c0, rows, cols, depth, stages;
+    int m0, c0, rows, cols, from, depth, stages;  // from: its first depth
   };
   auto part_of = [&](const TilePlace& at) __attribute__((always_inline)) {
     Part p;
     p.depth = OP == FORWARD ? a.K : OP == DX ? a.O : at.count;
     p.stages = (int)(((i64)p.depth + 63) / 64);
+    const int s0 = (int)((i64)p.stages * at.part / a.split), s1 = (int)((i64)p.stages * (at.part + 1) / a.split);
+    p.from = s0 * 64;
+    p.depth = max(min(p.depth, s1 * 64) - p.from, 0);
+    p.stages = s1 - s0;
     p.m0 = at.tm * BM;
     p.c0 = at.tc * BC;
     p.rows = min(BM, (OP == DW ? a.O : at.count) - p.m0);
@@ -220,8 +236,10 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
   uint32_t fill = lds0 + wave * (MI * 1024);  // the slot that is filled, where this wavefront's part of the rows' operand goes
   auto enter = [&](const TilePlace& at) __attribute__((always_inline)) {
     const Part& p = asked;
-    mp = (const char*)a.m + (OP == DW ? at.first * mrow + p.m0 * 2 : (at.first + p.m0) * mrow);
-    cp = (const char*)a.c + (OP == FORWARD ? ((i64)at.g * a.O + p.c0) * crow : OP == DX ? (i64)at.g * a.O * crow + p.c0 * 2 : at.first * crow + p.c0 * 2);
+    mp = (const char*)a.m + (OP == DW ? (at.first + p.from) * mrow + p.m0 * 2 : (at.first + p.m0) * mrow + p.from * 2);
+    cp = (const char*)a.c + (OP == FORWARD ? ((i64)at.g * a.O + p.c0) * crow + p.from * 2
+                             : OP == DX    ? ((i64)at.g * a.O + p.from) * crow + p.c0 * 2
+                                           : (at.first + p.from) * crow + p.c0 * 2);
     int l = lane;
     asm volatile("" : "+v"(l));  // (computed here, not kept in registers over the loop)
 #pragma unroll
@@ -246,8 +264,8 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
         coff[k] = ch < p.cols ? (uint32_t)(ch * crow + (u % 8 ^ (q & 7)) * 16) : kOOR;
       }
     }
-    if constexpr (!MT) nm = rsrc4(mp, (uint32_t)(p.rows * mrow));
-    if constexpr (!CT) nc = rsrc4(cp, (uint32_t)(p.cols * crow));
+    if constexpr (!MT) nm = rsrc4(mp, (uint32_t)(p.rows * mrow - p.from * 2));
+    if constexpr (!CT) nc = rsrc4(cp, (uint32_t)(p.cols * crow - p.from * 2));
   };
   auto ask = [&]() __attribute__((always_inline)) {
     if (stage == asked.stages) {
@@ -444,7 +462,7 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
       float bias[4 * RUN] = {};
       const int c = wc * (16 * TC) + run * (16 * RUN) + (bl >> 4) * (4 * RUN);
       if constexpr (OP == FORWARD) {
-        if (a.bias) mx_params<4 * RUN>(c < p.cols ? a.bias : nullptr, a.bias_dt, (i64)at.g * a.O + p.c0 + c, 0.f, bias);
+        if (a.bias && at.part == 0) mx_params<4 * RUN>(c < p.cols ? a.bias : nullptr, a.bias_dt, (i64)at.g * a.O + p.c0 + c, 0.f, bias);
       }
 #pragma unroll
       for (int j = 0; j < RUN; j++)
@@ -463,14 +481,14 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
 
     int el = lane;  // what follows is computed here, not kept in registers over the loop
     asm volatile("" : "+v"(el));
-    if constexpr (ADAPT)
+    if (ADAPT && at.part == 0)
       add_adapters<F16>(a, acc, at.first + p.m0 + wm * (16 * TM), p.rows - wm * (16 * TM), p.c0, p.cols, el,
                         [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); }, stored_inner(a));
 
     // Two runs' pieces change places between lanes 8 apart, so that a store writes whole 128-byte lines of 8 rows (a run alone is 64 bytes of
     // 16). Where rows are whole lines they go past the caches, which keep the operands ([8192, 1024] by [8192, 1024] 133 -> 116 us); parts of
     // lines are put together there (dw of [1416, 1032] in 16 bits: 32 us, 46 past the caches).
-    const i64 obase = OP == DW ? ((i64)at.g * a.O + p.m0) * a.K : (at.first + p.m0) * ncols;
+    const i64 obase = at.part * a.elems + (OP == DW ? ((i64)at.g * a.O + p.m0) * a.K : (at.first + p.m0) * ncols);
     constexpr int OS = OUT == OUT_F32 ? 4 : 2;
     const int er = el & 15, eg = el >> 4;
     const bool upper = er >= 8, lines = ((uintptr_t)a.out | (uintptr_t)(ncols * OS)) % 128 == 0;
@@ -518,7 +536,7 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
         for (int u = 0; u < TM; u++) {
           const int m = wm * (16 * TM) + u * 16 + er;
           if (m >= p.rows) continue;
-          const i64 to = (i64)at.g * a.O + p.m0 + m;
+          const i64 to = ((i64)at.part * a.G + at.g) * a.O + p.m0 + m;
           if constexpr (OUT == OUT_F32) ((float*)a.db)[to] = accb[u][0];
           else ((uint16_t*)a.db)[to] = (uint16_t)mx_pack2<F16>(accb[u][0], 0.f);
         }
@@ -533,6 +551,54 @@ __global__ void __launch_bounds__(512, 2) k_group_tile(GroupArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 512 * 128];
   multiply_tiles<OP, F16, OUT, 8, 4, 2, 4, ADAPT, WHOLE>(a, lds);
   multiply_tiles<OP, F16, OUT, 4, 2, 2, 4, ADAPT, REST>(a, lds);
+}
+
+// Adds the parts of the depth, in order, eight values a thread: the result's first `elems`, then the bias' gradient. Rows of no group stay.
+template <bool F16, bool F32OUT>
+__global__ void __launch_bounds__(64) k_group_sum(const float* parts, const float* db_parts, const int32_t* ends, void* out, void* db, i64 elems, i64 db_elems,
+                                                   int split, int ncols, int G, i64 N) {
+  i64 i = ((i64)blockIdx.x * 64 + threadIdx.x) * 8, each = elems;
+  const float* from = parts;
+  void* to = out;
+  if (i >= elems) {
+    i -= elems;
+    each = db_elems;
+    from = db_parts;
+    to = db;
+    if (i >= db_elems) return;
+  } else if (ends && i / ncols >= min((i64)max(ends[G - 1], 0), N)) {
+    return;
+  }
+  float v[8] = {};
+  constexpr int AT = 8;  // parts loaded together
+  for (int s = 0; s < split; s += AT) {
+    f32x4 q[AT][2];
+#pragma unroll
+    for (int k = 0; k < AT; k++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) q[k][h] = s + k < split ? *(const f32x4*)(from + (s + k) * each + i + h * 4) : f32x4{};
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int k = 0; k < AT; k++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] += q[k][j / 4][j % 4];
+  }
+  if constexpr (F32OUT) {
+    *(f32x4*)((float*)to + i) = f32x4{v[0], v[1], v[2], v[3]};
+    *(f32x4*)((float*)to + i + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    *(mx_u32x4*)((uint16_t*)to + i) = mx_pack8<F16>(v);
+  }
+}
+
+constexpr int kSplitStages = 32;
+// Parts of the depth for a product that is a few quartered tiles only, so that they fill the CUs: a stage of 64 of a quarter takes some 0.5 us,
+// the second kernel 7 us and more.
+int split_of(int op, i64 N, i64 G, i64 K, i64 O) {
+  const i64 across = op == DW ? G * cdiv(O, 128) : N / 128 + (G + 1) / 2, quarters = std::max<i64>(across, 1) * cdiv(op == FORWARD ? O : K, 128);
+  const i64 stages = op == DW ? cdiv(N, 64 * G) : cdiv(op == FORWARD ? K : O, 64);
+  if (quarters > 128 || stages < kSplitStages) return 1;
+  return (int)std::min(256 / quarters, stages / 8);
 }
 
 template <int OP, bool F16, int OUT, bool ADAPT = false>
@@ -673,6 +739,7 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
 }
 template <bool F16, int OT, int NT, bool ADAPT, bool FUSED = false>
 void launch_rows(GroupArgs a) {
+  a.split = 1;
   a.tiles_c = cdiv(a.O, 16 * OT);
   a.band = 8;
   const i64 blocks = ((a.N / (16 * NT) + a.G) * a.tiles_c + 7) / 8 * 8;
@@ -681,10 +748,12 @@ void launch_rows(GroupArgs a) {
   CK(hipGetLastError());
 }
 
+// Up to 64 rows a group, on average, go straight into registers
+bool goes_by_rows(i64 N, i64 G) { return (N + G - 1) / G <= 64; }
 template <bool ADAPT>
 bool few_rows(const GroupArgs& a, DT dt) {
   const i64 mean = (a.N + a.G - 1) / a.G;
-  if (mean > 64) return false;
+  if (!goes_by_rows(a.N, a.G)) return false;
   auto by = [&](auto F) {
     constexpr bool f = decltype(F)::value;
     if constexpr (ADAPT) {
@@ -703,13 +772,37 @@ bool few_rows(const GroupArgs& a, DT dt) {
   return true;
 }
 
-template <int OP>
-void launch(const GroupArgs& a, DT dt, bool f32 = false) {
-  auto by = [&](auto F, auto T) { launch_tile<OP, decltype(F)::value, decltype(T)::value>(a); };
+i64 out_elems(int op, i64 N, i64 G, i64 K, i64 O) { return op == DW ? G * O * K : N * (op == FORWARD ? O : K); }
+// What a tiled product takes of a workspace: the fp32 sums of each part of the depth
+i64 split_bytes(int op, i64 N, i64 G, i64 K, i64 O) {
+  if (N == 0 || (op == FORWARD && goes_by_rows(N, G))) return 0;
+  const i64 s = split_of(op, N, G, K, O);
+  return s > 1 ? s * 4 * (out_elems(op, N, G, K, O) + (op == DW ? G * O : 0)) : 0;
+}
+template <int OP, bool ADAPT = false>
+void launch(GroupArgs a, DT dt, bool f32, void* workspace) {
+  const i64 elems = out_elems(OP, a.N, a.G, a.K, a.O), db_elems = OP == DW && a.db ? (i64)a.G * a.O : 0;
+  auto by = [&](auto F, auto T) { launch_tile<OP, decltype(F)::value, decltype(T)::value, ADAPT>(a); };
   constexpr std::integral_constant<int, OUT_16> o16{};
   constexpr std::integral_constant<int, OUT_F32> o32{};
-  if constexpr (OP == FORWARD) {
-    if (few_rows<false>(a, dt)) return;
+  a.split = 1;
+  if (workspace) {
+    void *out = a.out, *db = a.db;
+    a.split = split_of(OP, a.N, a.G, a.K, a.O);
+    a.elems = elems;
+    a.out = workspace;
+    a.db = db ? (float*)workspace + a.split * elems : nullptr;
+    dt == F16 ? by(std::true_type{}, o32) : by(std::false_type{}, o32);
+    const unsigned blocks = (unsigned)((elems + db_elems + 511) / 512);
+    auto sum = [&](auto F, auto T) {
+      k_group_sum<decltype(F)::value, decltype(T)::value><<<blocks, 64, 0, stream()>>>((const float*)a.out, (const float*)a.db, OP == DW || ADAPT ? nullptr : a.ends, out, db,
+                                                                                       elems, db_elems, a.split, OP == FORWARD ? a.O : a.K, a.G, a.N);
+    };
+    if (f32) sum(std::false_type{}, std::true_type{});
+    else if (dt == F16) sum(std::true_type{}, std::false_type{});
+    else sum(std::false_type{}, std::false_type{});
+    CK(hipGetLastError());
+    return;
   }
   if constexpr (OP == DW) {
     if (f32) return dt == F16 ? by(std::true_type{}, o32) : by(std::false_type{}, o32);
@@ -743,15 +836,27 @@ i64 rows_in(const Tensor& t, const char* what) {
 void apart(const Tensor& out, const Tensor* t, const char* what) {
   if (t) mx_apart(out.p, out.bytes(), t->p, t->bytes(), what);
 }
+// The workspace of a call with the given tensors, its result (and the bias' gradient) last
+struct GroupRoom {
+  MxWorkspace ws;
+  GroupRoom(void* workspace, i64 bytes, i64 need, std::initializer_list<const Tensor*> all) : ws(check(workspace, need, all), bytes, need) {}
+  static void* check(void* workspace, i64 need, std::initializer_list<const Tensor*> all) {
+    if (workspace)
+      for (const Tensor* t : all)
+        if (t) mx_apart(t->p, t->bytes(), workspace, (size_t)need, "the workspace");
+    return need ? workspace : nullptr;
+  }
+};
 }  // namespace
 
-void adapter_product(const GroupArgs& a, DT dt) {
-  if (few_rows<true>(a, dt)) return;
-  if (dt == F16) launch_tile<FORWARD, true, OUT_16, true>(a);
-  else launch_tile<FORWARD, false, OUT_16, true>(a);
+i64 adapter_product_bytes(i64 N, i64 K, i64 O) { return split_bytes(FORWARD, N, 1, K, O); }
+void adapter_product(const GroupArgs& a, DT dt, void* workspace) {
+  if (!few_rows<true>(a, dt)) launch<FORWARD, true>(a, dt, false, workspace);
 }
 
-void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Tensor* bias, Tensor& y) {
+i64 group_linear_workspace(int product, i64 N, i64 G, i64 K, i64 O) { return split_bytes(product, N, G, K, O); }
+
+void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Tensor* bias, Tensor& y, void* workspace, i64 workspace_bytes) {
   i64 G, O, K;
   check_16(x, "x");
   const i64 N = rows_in(x, "x");
@@ -764,11 +869,12 @@ void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Te
     REQ(bias->numel() == G * O && bias->p && (bias->dt == F32 || bias->dt == F16 || bias->dt == BF16), "bias must have %lld elements", (long long)(G * O));
   for (const Tensor* t : {&x, &w, &ends, bias}) apart(y, t, "out");
   if (N == 0) return;
+  GroupRoom room(workspace, workspace_bytes, group_linear_workspace(FORWARD, N, G, K, O), {&x, &w, &ends, bias, &y});
   GroupArgs a{x.p, w.p, bias ? bias->p : nullptr, ends.ptr<int32_t>(), y.p, nullptr, N, (int)G, (int)K, (int)O, bias ? bias->dt : F32};
-  launch<FORWARD>(a, x.dt);
+  if (!few_rows<false>(a, x.dt)) launch<FORWARD>(a, x.dt, false, room.ws.p);
 }
 
-void group_linear_dx(const Tensor& dy, const Tensor& w, const Tensor& ends, Tensor& dx) {
+void group_linear_dx(const Tensor& dy, const Tensor& w, const Tensor& ends, Tensor& dx, void* workspace, i64 workspace_bytes) {
   i64 G, O, K;
   check_16(dy, "dy");
   const i64 N = rows_in(dy, "dy");
@@ -779,11 +885,12 @@ void group_linear_dx(const Tensor& dy, const Tensor& w, const Tensor& ends, Tens
   check_ends(ends, G);
   for (const Tensor* t : {&dy, &w, &ends}) apart(dx, t, "out");
   if (N == 0) return;
+  GroupRoom room(workspace, workspace_bytes, group_linear_workspace(DX, N, G, K, O), {&dy, &w, &ends, &dx});
   GroupArgs a{dy.p, w.p, nullptr, ends.ptr<int32_t>(), dx.p, nullptr, N, (int)G, (int)K, (int)O, F32};
-  launch<DX>(a, dy.dt);
+  launch<DX>(a, dy.dt, false, room.ws.p);
 }
 
-void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tensor& dw, Tensor* db) {
+void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tensor& dw, Tensor* db, void* workspace, i64 workspace_bytes) {
   i64 G, O, K;
   check_16(dy, "dy");
   const i64 N = rows_in(dy, "dy");
@@ -798,6 +905,7 @@ void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tens
         (long long)(G * O));
     for (const Tensor* t : std::initializer_list<const Tensor*>{&dy, &x, &ends, &dw}) apart(*db, t, "the bias' gradient");
   }
+  GroupRoom room(workspace, workspace_bytes, group_linear_workspace(DW, N, G, K, O), {&dy, &x, &ends, &dw, db});
   GroupArgs a{dy.p, x.p, nullptr, ends.ptr<int32_t>(), dw.p, db ? db->p : nullptr, N, (int)G, (int)K, (int)O, F32};
-  launch<DW>(a, dy.dt, dw.dt == F32);
+  launch<DW>(a, dy.dt, dw.dt == F32, room.ws.p);
 }

@@ -222,9 +222,14 @@ i64 convnext_mlp_mx_workspace(i64 N, i64 C, int fmt);
 // K and O multiples of 8 up to 2^20; fp32 sums, one rounding.
 // y = w[g] x + bias[g] (bias [G,O] of any float type or null); dx = w[g]^T dy; dw[g] = sum of dy x^T over g's rows (zeros for
 // an empty group) and, with db, db[g] = sum of dy; dw [G,O,K] and db [G,O] fp32 or of the inputs' type.
-void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Tensor* bias, Tensor& y);
-void group_linear_dx(const Tensor& dy, const Tensor& w, const Tensor& ends, Tensor& dx);
-void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tensor& dw, Tensor* db);
+// workspace as for mx_linear, of group_linear_workspace() bytes (0 unless the result is small and the sums are long).
+enum GroupProduct : int { GROUP_FORWARD = 0, GROUP_DX = 1, GROUP_DW = 2 };
+void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Tensor* bias, Tensor& y, void* workspace = nullptr,
+                  i64 workspace_bytes = 0);
+void group_linear_dx(const Tensor& dy, const Tensor& w, const Tensor& ends, Tensor& dx, void* workspace = nullptr, i64 workspace_bytes = 0);
+void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tensor& dw, Tensor* db, void* workspace = nullptr,
+                     i64 workspace_bytes = 0);
+i64 group_linear_workspace(int product, i64 N, i64 G, i64 K, i64 O);
 
 // Low-rank adapters of many requests beside one shared projection: out = x w^T + bias + scale[s] b[s] (a[s] x) per row, s = slots[n]
 // (int32 [N]; outside [0, L): no adapter), or the same added to a projection y made elsewhere (out may be y). x [N,K], w [O,K],
@@ -235,7 +240,7 @@ void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Ten
                     const Tensor* bias, Tensor& out, void* workspace = nullptr, i64 workspace_bytes = 0);
 void adapter_add(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale, Tensor& out,
                  void* workspace = nullptr, i64 workspace_bytes = 0);
-i64 adapter_workspace(i64 N, i64 R);
+i64 adapter_workspace(i64 N, i64 R, i64 K, i64 O);  // K = 0: adapter_add's
 
 // Conv plus the upsample block's skip connection in one pass: out = act(conv(x) + b) + skip, skip[i, c] =
 // x_skip[src[i] >> 3, (src[i] & 7) * Cin/8 + c / rep], rep = Co / (Cin/8) a power of two, one rounding (reference:

@@ -26,6 +26,7 @@ EPI_F16_COMPAT = 256  # or'ed into act: the reference's fp16 epilogue rounding s
 EMPTY = 0xFFFFFFFF
 MX_E4M3, MX_E2M1 = 1, 2  # element formats of microscaled rows (MxTensor)
 NORM_RMS, NORM_LAYER = 0, 1
+GROUP_FORWARD, GROUP_DX, GROUP_DW = 0, 1, 2
 
 # the C ABI's exported symbols (every declaration of include/spconv_amd.h)
 SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_get_stream", "spc_build_neighbors", "spc_build_neighbors_ex", "spc_cache_lookup",
@@ -37,7 +38,7 @@ SYMBOLS = ("spc_last_error", "spc_set_stream", "spc_get_stream", "spc_build_neig
            "spc_kernel_times", "spc_release_cached_memory", "spc_mx_sizes", "spc_mx_quantize", "spc_mx_dequantize",
            "spc_add_norm_mx", "spc_mx_linear_workspace", "spc_mx_linear_tile",
            "spc_mx_linear", "spc_convnext_mlp_mx_workspace",
-           "spc_convnext_mlp_mx", "spc_group_linear", "spc_group_linear_dx", "spc_group_linear_dw", "spc_adapter_workspace",
+           "spc_convnext_mlp_mx", "spc_group_linear_workspace", "spc_group_linear", "spc_group_linear_dx", "spc_group_linear_dw", "spc_adapter_workspace",
            "spc_adapter_linear", "spc_adapter_add")
 
 _lib = None
@@ -99,10 +100,11 @@ def load_library():
     L.spc_mx_linear.argtypes = [P, P, I, I, P, P, P, I, P, I, I64, I64, I64, I, P, P, P, I64]
     L.spc_convnext_mlp_mx_workspace.argtypes = [I64, I64, I, PI64]
     L.spc_convnext_mlp_mx.argtypes = [P, P, P, P, ctypes.c_float, P, P, P, P, P, P, I, I, I, I64, I64, P, P, I64]
-    L.spc_group_linear.argtypes = [P, P, P, P, I, I, I64, I64, I64, I64, P]
-    L.spc_group_linear_dx.argtypes = [P, P, P, I, I64, I64, I64, I64, P]
-    L.spc_group_linear_dw.argtypes = [P, P, P, I, I64, I64, I64, I64, I, P, P]
-    L.spc_adapter_workspace.argtypes = [I64, I64, PI64]
+    L.spc_group_linear_workspace.argtypes = [I, I64, I64, I64, I64, PI64]
+    L.spc_group_linear.argtypes = [P, P, P, P, I, I, I64, I64, I64, I64, P, P, I64]
+    L.spc_group_linear_dx.argtypes = [P, P, P, I, I64, I64, I64, I64, P, P, I64]
+    L.spc_group_linear_dw.argtypes = [P, P, P, I, I64, I64, I64, I64, I, P, P, P, I64]
+    L.spc_adapter_workspace.argtypes = [I64, I64, I64, I64, PI64]
     L.spc_adapter_linear.argtypes = [P, P, P, P, P, P, P, I, I, I64, I64, I64, I64, I64, P, P, I64]
     L.spc_adapter_add.argtypes = [P, P, P, P, P, P, I, I64, I64, I64, I64, I64, P, P, I64]
     for name in SYMBOLS:
@@ -625,9 +627,11 @@ def group_linear(x, w, ends, bias=None, out=None):
         out = x.new_empty(N, Co)
     else:
         _matrix(out, "out", (N, Co), x.dtype)
+    nws = _workspace_bytes("spc_group_linear_workspace", GROUP_FORWARD, N, G, K, Co)
+    ws = _workspace(nws, x) if nws else None
     dev = torch.cuda.current_device()
     _check(load_library().spc_group_linear(_adr(x, dev), _adr(w, dev), _adr(ends, dev), _adr(bias, dev), _dt(x),
-                                           _dt(bias) if bias is not None else F32, N, G, K, Co, _adr(out, dev)))
+                                           _dt(bias) if bias is not None else F32, N, G, K, Co, _adr(out, dev), _adr(ws, dev), nws))
     return out
 
 
@@ -644,8 +648,11 @@ def group_linear_dx(dy, w, ends, out=None):
         out = dy.new_empty(N, K)
     else:
         _matrix(out, "out", (N, K), dy.dtype)
+    nws = _workspace_bytes("spc_group_linear_workspace", GROUP_DX, N, G, K, Co)
+    ws = _workspace(nws, dy) if nws else None
     dev = torch.cuda.current_device()
-    _check(load_library().spc_group_linear_dx(_adr(dy, dev), _adr(w, dev), _adr(ends, dev), _dt(dy), N, G, K, Co, _adr(out, dev)))
+    _check(load_library().spc_group_linear_dx(_adr(dy, dev), _adr(w, dev), _adr(ends, dev), _dt(dy), N, G, K, Co, _adr(out, dev), _adr(ws, dev),
+                                              nws))
     return out
 
 
@@ -668,9 +675,11 @@ def group_linear_dw(dy, x, ends, out=None, out_dtype=None, bias: bool = False):
     elif out.shape != (G, Co, K) or out_dtype not in (None, out.dtype):
         raise ValueError(f"out must be [{G}, {Co}, {K}] of {out_dtype or out.dtype}, got {list(out.shape)} {out.dtype}")
     db = out.new_empty(G, Co) if bias else None
+    nws = _workspace_bytes("spc_group_linear_workspace", GROUP_DW, N, G, K, Co)
+    ws = _workspace(nws, dy) if nws else None
     dev = torch.cuda.current_device()
     _check(load_library().spc_group_linear_dw(_adr(dy, dev), _adr(x, dev), _adr(ends, dev), _dt(dy), N, G, K, Co, _dt(out), _adr(out, dev),
-                                              _adr(db, dev)))
+                                              _adr(db, dev), _adr(ws, dev), nws))
     return (out, db) if bias else out
 
 
@@ -705,7 +714,7 @@ def adapter_linear(x, w, a, b, slots, scale=None, bias=None, out=None):
         out = x.new_empty(N, Co)
     else:
         _matrix(out, "out", (N, Co), x.dtype)
-    nws = _workspace_bytes("spc_adapter_workspace", N, R)
+    nws = _workspace_bytes("spc_adapter_workspace", N, R, K, Co)
     ws = _workspace(nws, x) if nws else None
     dev = torch.cuda.current_device()
     _check(load_library().spc_adapter_linear(
@@ -724,7 +733,7 @@ def adapter_add(y, x, a, b, slots, scale=None, out=None):
         out = torch.empty_like(y)
     else:
         _matrix(out, "out", (N, Co), x.dtype)
-    nws = _workspace_bytes("spc_adapter_workspace", N, R)
+    nws = _workspace_bytes("spc_adapter_workspace", N, R, 0, Co)
     ws = _workspace(nws, x) if nws else None
     dev = torch.cuda.current_device()
     _check(load_library().spc_adapter_add(
