@@ -74,7 +74,7 @@ SHAPES = [
     ([2000, 700, 1500, 300], 5, 136, 8200), ([1300, 700, 1500, 300], 5, 8200, 136), ([900, 300, 0, 2000], 7, 2056, 2104), ([300] * 130, 3, 72, 520),
     ([20] * 70, 0, 520, 776), ([6000], 0, 8, 4104), ([700] * 40, 0, 264, 1032), ([9000, 4000], 0, 520, 1544),
     # few tiles of long sums, in parts
-    ([500, 0, 130], 9, 2056, 136), ([500, 0, 130], 9, 136, 2056), ([300], 0, 4104, 40), ([3000, 0, 2500, 7000], 20, 72, 200),
+    ([1500, 0, 530], 9, 2056, 136), ([500, 0, 130], 9, 136, 2056), ([600], 0, 4104, 40), ([300], 0, 4104, 40), ([3000, 0, 2500, 7000], 20, 72, 200),
     ([3] * 130, 0, 200, 328), ([40] * 70, 9, 72, 72), ([4100], 0, 72, 1096), ([40, 25, 60, 33], 0, 4096, 1024), ([700] * 9, 0, 512, 512),
 ]
 
@@ -230,7 +230,7 @@ ADAPTERS = [  # n, adapters, rank, k, o, order
     (128, 128, 8, 72, 72, "mixed"), (129, 3, 256, 136, 392, "mixed"), (300, 7, 40, 520, 264, "runs"), (1000, 2, 16, 1416, 1032, "runs"),
     (2600, 9, 64, 320, 1096, "runs"), (700, 70, 16, 512, 512, "mixed"), (50, 4, 16, 128, 64, "none"), (600, 4, 16, 128, 256, "none"),
     (4099, 6, 24, 136, 8200, "runs"), (2000, 40, 72, 72, 8200, "mixed"), (3, 5, 8, 520, 264, "mixed"), (2, 2, 16, 4104, 72, "mixed"),
-    (1, 2, 32, 1416, 200, "one"), (40, 3, 256, 264, 136, "mixed"), (500, 4, 16, 4104, 136, "runs"), (20000, 5, 48, 72, 136, "runs"), (4099, 1, 24, 136, 264, "one"), (513, 6, 200, 64, 40, "runs"), (9, 4, 16, 16384, 64, "mixed"), (300, 4, 16, 16384, 64, "runs"),
+    (1, 2, 32, 1416, 200, "one"), (40, 3, 256, 264, 136, "mixed"), (600, 4, 16, 4104, 136, "runs"), (500, 4, 16, 136, 136, "mixed"), (20000, 5, 48, 72, 136, "runs"), (4099, 1, 24, 136, 264, "one"), (513, 6, 200, 64, 40, "runs"), (9, 4, 16, 16384, 64, "mixed"), (300, 4, 16, 16384, 64, "runs"),
 ]
 
 

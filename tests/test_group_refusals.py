@@ -46,8 +46,8 @@ def test_forward():
     refused(call(bias=4 * A + 64), "overlap")
     refused(call(bias=5 * A, bdt=3), "dtype code 3")
     assert call(n=0, x=None, y=None) == 0
-    # 500 rows of one group: few tiles, deep
-    deep = dict(n=500, g=1, k=4096, o=128, x=0x10000000, w=0x20000000, y=0x30000000)
+    # 600 rows of one group: few tiles, deep
+    deep = dict(n=600, g=1, k=4096, o=128, x=0x10000000, w=0x20000000, y=0x30000000)
     refused(call(**deep, work=0x40000000, nwork=16), "workspace of 16 bytes")
     refused(call(**deep, work=0x40000008, nwork=1 << 30), "16-byte aligned")
     for over in ("x", "w", "y"):
@@ -101,13 +101,13 @@ def test_workspaces():
 
     assert group(sp.GROUP_FORWARD, 0, 1, 4096, 128) == group(sp.GROUP_FORWARD, 64, 1, 4096, 128) == group(sp.GROUP_FORWARD, 500, 1, 1024, 128) == 0
     assert group(sp.GROUP_FORWARD, 16000, 8, 4096, 4096) == 0
-    assert group(sp.GROUP_FORWARD, 500, 1, 4096, 128) % (500 * 128 * 4) == 0 < n.value < 1 << 26
+    assert group(sp.GROUP_FORWARD, 600, 1, 4096, 128) % (600 * 128 * 4) == 0 < n.value < 1 << 26
     assert group(sp.GROUP_DX, 500, 1, 128, 4096) % (500 * 128 * 4) == 0 < n.value < 1 << 26
     assert group(sp.GROUP_DW, 9000, 1, 128, 136) % (129 * 136 * 4) == 0 < n.value < 1 << 26
     assert group(sp.GROUP_DW, 1000, 1, 128, 128) == group(sp.GROUP_DW, 0, 1, 128, 128) == 0
     assert adapter(0, 8, 64, 64) == adapter(1, 16, 4096, 4096) == adapter(1, 16, 0, 4096) == 0
     assert adapter(7, 24, 0, 64) == 512 and adapter(500, 8, 64, 64) == 500 * 16 // 256 * 256 + 256
-    assert adapter(500, 8, 4096, 128) > adapter(500, 8, 0, 128) > 0
+    assert adapter(600, 8, 4096, 128) > adapter(600, 8, 0, 128) > 0
     for bad in ((3, 4, 1, 64, 64), (-1, 4, 1, 64, 64), (0, 1 << 31, 1, 64, 64), (0, 4, 0, 64, 64), (0, 4, 1, 0, 64), (0, 4, 1, 64, 1 << 21)):
         refused(lib.spc_group_linear_workspace(*bad, ctypes.byref(n)), "arguments")
     refused(lib.spc_group_linear_workspace(0, 4, 1, 64, 64, None), "arguments")

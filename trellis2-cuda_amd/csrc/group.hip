@@ -591,16 +591,6 @@ __global__ void __launch_bounds__(64) k_group_sum(const float* parts, const floa
   }
 }
 
-constexpr int kSplitStages = 32;
-// Parts of the depth for a product that is a few quartered tiles only, so that they fill the CUs: a stage of 64 of a quarter takes some 0.5 us,
-// the second kernel 7 us and more.
-int split_of(int op, i64 N, i64 G, i64 K, i64 O) {
-  const i64 across = op == DW ? G * cdiv(O, 128) : N / 128 + (G + 1) / 2, quarters = std::max<i64>(across, 1) * cdiv(op == FORWARD ? O : K, 128);
-  const i64 stages = op == DW ? cdiv(N, 64 * G) : cdiv(op == FORWARD ? K : O, 64);
-  if (quarters > 128 || stages < kSplitStages) return 1;
-  return (int)std::min(256 / quarters, stages / 8);
-}
-
 template <int OP, bool F16, int OUT, bool ADAPT = false>
 void launch_tile(GroupArgs a) {
   constexpr int BC = 256, BM = 256;
@@ -748,21 +738,41 @@ void launch_rows(GroupArgs a) {
   CK(hipGetLastError());
 }
 
-// Up to 64 rows a group, on average, go straight into registers
-bool goes_by_rows(i64 N, i64 G) { return (N + G - 1) / G <= 64; }
+// Whether a forward product's rows go straight into registers: up to 16 a group on average, or as many as make no more workgroups (of 32
+// channels by 32 or 64 rows) than there are CUs. us by rows / in tiles, bf16, [rows, K] by groups of [O, K]: [640, 1024] 32 of 1024
+// 21.8 / 21.1 (1280 rows 26.0 / 21.5), [60, 4096] one of 4096 17.4 / 21.2, [100, 4096] 17.9 / 25.3, [200, 4096] 32.1 / 21.6, [100, 1024] one of
+// 1024 7.8 / 14.4, [500, 4096] one of 512 17.9 / 18.3.
+constexpr i64 kCus = 256;  // (a workspace's size follows from it, also where no device is)
+int row_tiles(i64 N, i64 G) { return N <= 16 * G ? 1 : N <= 32 * G ? 2 : 4; }  // of 16 rows
+bool goes_by_rows(i64 N, i64 G, i64 O) {
+  if (N <= 16 * G) return true;
+  return N <= 512 * G && (N / (16 * row_tiles(N, G)) + G) * cdiv(O, 32) <= kCus;
+}
+// Parts of the depth for a product that is a few quartered tiles only, so that they fill the CUs: a stage of 64 of a quarter takes some 0.5 us,
+// the second kernel 7 us and more. us whole / in parts of 4, 8 and 16 stages at least: forward [500, 4096] by [512, 4096] 34 / 21 / 18 / 20,
+// [300, 2048] by [256, 2048] 21 / 14 / 16 / 19; dw of [512, 512] from 16000 rows 140 / 25 / 25 / 26, 2000 rows 26 / 16 / 17 / 20; with 16
+// stages in all ([500, 1024] by [512, 1024]) 14.8 / 15.3.
+constexpr int kSplitStages = 32;
+int split_of(int op, i64 N, i64 G, i64 K, i64 O) {
+  const i64 across = op == DW ? G * cdiv(O, 128) : N / 128 + (G + 1) / 2, quarters = std::max<i64>(across, 1) * cdiv(op == FORWARD ? O : K, 128);
+  const i64 stages = op == DW ? cdiv(N, 64 * G) : cdiv(op == FORWARD ? K : O, 64);
+  if (quarters > kCus / 2 || stages < kSplitStages) return 1;
+  return (int)std::min(kCus / quarters, stages / 8);
+}
+
 template <bool ADAPT>
 bool few_rows(const GroupArgs& a, DT dt) {
-  const i64 mean = (a.N + a.G - 1) / a.G;
-  if (!goes_by_rows(a.N, a.G)) return false;
+  if (!goes_by_rows(a.N, a.G, a.O)) return false;
+  const int tiles = row_tiles(a.N, a.G);
   auto by = [&](auto F) {
     constexpr bool f = decltype(F)::value;
     if constexpr (ADAPT) {
       if (!a.ad.h) return launch_rows<f, 1, 1, true, true>(a);
     }
-    if (mean <= 16) {
+    if (tiles == 1) {
       if (a.O * (a.N < a.G ? a.N : a.G) <= 16 * 1024) launch_rows<f, 1, 1, ADAPT>(a);
       else launch_rows<f, 2, 1, ADAPT>(a);
-    } else if (mean <= 32) {
+    } else if (tiles == 2) {
       launch_rows<f, 2, 2, ADAPT>(a);
     } else {
       launch_rows<f, 2, 4, ADAPT>(a);
@@ -775,7 +785,7 @@ bool few_rows(const GroupArgs& a, DT dt) {
 i64 out_elems(int op, i64 N, i64 G, i64 K, i64 O) { return op == DW ? G * O * K : N * (op == FORWARD ? O : K); }
 // What a tiled product takes of a workspace: the fp32 sums of each part of the depth
 i64 split_bytes(int op, i64 N, i64 G, i64 K, i64 O) {
-  if (N == 0 || (op == FORWARD && goes_by_rows(N, G))) return 0;
+  if (N == 0 || (op == FORWARD && goes_by_rows(N, G, O))) return 0;
   const i64 s = split_of(op, N, G, K, O);
   return s > 1 ? s * 4 * (out_elems(op, N, G, K, O) + (op == DW ? G * O : 0)) : 0;
 }
