@@ -16,23 +16,25 @@ enum { OUT_16 = 0, OUT_F32 = 1 };
 // dw: tiles are as deep as their group is long, so the longest groups come first (up to 64 groups; more are short), in rounds of W tiles
 // a XCD that run to and fro; each XCD takes a contiguous eighth of every group's tiles (where they are many).
 //
-// The last round of an XCD's W workgroups may have few tiles left: where at most half of them would have one, these are taken in quarters
-// instead (PART = REST, after the whole ones), which take two fifths of a whole one's time.
+// The last round of an XCD's W workgroups may have few tiles left: where at most a quarter of them would have one, these are taken in
+// QUARTERS (of half the rows and columns) after the whole ones, which take two fifths of a whole one's time, and where at most half of them
+// would, in HALVES (of the rows), which take three fifths ([2560, 2048] by [2048, 2048]: 32 us,
+// 40 in quarters; [4099, 1416] by 16 groups of [1416, 1032], dx: 28 and 37).
 //
 // A few deep tiles are each taken in `split` parts of the depth, whose fp32 sums a second kernel adds (split_of says when).
-enum { WHOLE = 0, REST = 1, ALL = 2 };
+enum { WHOLE = 0, HALVES = 1, QUARTERS = 2, ALL = 3 };
 struct TilePlace {
   i64 first = 0;  // the group's first row
   int count = 0, g = 0, tm = 0, tc = 0;
   int part = 0;  // of the depth
 };
-template <int OP, int BM, bool ONE, int PART>  // ONE: one group, of all rows; BM: rows of a whole tile; of a REST, at counts quarters
+template <int OP, int BM, bool ONE, int PART>  // ONE: one group, of all rows; BM: rows of a whole tile (at counts pieces)
 struct Tiles {
   const GroupArgs& a;
   int lane, first, count, key;  // of the lane's group among the first 64; key: tiles up to its end, or (dw) its place in the order
   int W, round = 0;
-  i64 begin;         // this XCD's first part of a tile
-  i64 end, quarter;  // how many it has, and where the quartered ones begin
+  i64 begin;     // this XCD's first part of a tile
+  i64 end, cut;  // how many it has, and where those begin that are taken in pieces
 
   __device__ __forceinline__ Tiles(const GroupArgs& a_, int lane_) : a(a_), lane(lane_), W(gridDim.x / 8) {
     key = chunk(0);
@@ -57,10 +59,11 @@ struct Tiles {
       end = max(min(per, all - begin), (i64)0);
     }
     const i64 rest = end % W;
-    quarter = end - (PART != ALL && rest * 2 <= W ? rest : 0);
-    if constexpr (PART == WHOLE) end = quarter;
+    cut = end;
+    if (PART == WHOLE ? rest * 2 <= W : PART == HALVES ? rest * 4 > W && rest * 2 <= W : PART == QUARTERS && rest * 4 <= W) cut -= rest;
+    if constexpr (PART == WHOLE) end = cut;
   }
-  __device__ __forceinline__ bool any() const { return PART == REST ? quarter < end : end > 0; }
+  __device__ __forceinline__ bool any() const { return PART == WHOLE || PART == ALL ? end > 0 : cut < end; }
   // The lane's group of those from g0 on, its rows inside [0, N) whatever ends holds; the tiles of all up to it
   __device__ __forceinline__ int chunk(int g0) {
     const int g = g0 + lane, N = (int)a.N;
@@ -102,11 +105,11 @@ struct Tiles {
       const i64 start = (i64)round * W;
       i64 l = start + k;
       int which = 0;
-      if constexpr (PART == REST) {
-        const int across = (OP == FORWARD ? a.O : a.K) <= a.width / 2 ? 1 : 2;  // (a narrow result has none to the right)
+      if constexpr (PART == HALVES || PART == QUARTERS) {
+        const int across = PART == HALVES || (OP == FORWARD ? a.O : a.K) <= a.width / 2 ? 1 : 2;  // (a narrow result has none to the right)
         which = (int)(l % (2 * across));
-        l = quarter + l / (2 * across);
-        if (quarter + start / (2 * across) >= end) return false;
+        l = cut + l / (2 * across);
+        if (cut + start / (2 * across) >= end) return false;
         which = across == 1 ? which * 2 : which;
       } else {
         if (OP == DW && (round & 1)) l = start + W - 1 - k;
@@ -115,10 +118,12 @@ struct Tiles {
       round++;
       if (l >= end) continue;
       if (!place(at, begin + l)) continue;
-      if constexpr (PART == REST) {
+      if constexpr (PART == HALVES || PART == QUARTERS) {
         at.tm = at.tm * 2 + (which >> 1);
-        at.tc = at.tc * 2 + (which & 1);
-        if (at.tm * (BM / 2) >= (OP == DW ? a.O : at.count) || at.tc * (a.width / 2) >= (OP == FORWARD ? a.O : a.K)) continue;
+        if constexpr (PART == QUARTERS) at.tc = at.tc * 2 + (which & 1);
+        if (at.tm * (BM / 2) >= (OP == DW ? a.O : at.count) ||
+            (PART == QUARTERS && at.tc * (a.width / 2) >= (OP == FORWARD ? a.O : a.K)))
+          continue;
       }
       return true;
     }
@@ -170,7 +175,7 @@ struct Tiles {
 };
 
 // Tiled products of all three kinds. A workgroup of WC x WM wavefronts has BC = 16 TC WC columns of the result by BM = 16 TM WM rows;
-// the depth goes by stages of 64 through two slots of LDS (four of a quarter's), filled by DMA. An operand whose depth is contiguous (x and w of the
+// the depth goes by stages of 64 through slots of LDS (two; three of a half's, five of a quarter's), filled by DMA. An operand whose depth is contiguous (x and w of the
 // forward product, dy of dx) lies there as rows of 64 values, its 16-byte pieces permuted (piece c of row q at c ^ q % 8), so that
 // eight lanes of neighbouring rows read from distinct banks; one whose depth runs over rows (w of dx, dy and x of dw) as 64 rows, and
 // is transposed on its way into registers (ds_read_b64_tr_b16: 16 lanes give the addresses of 4 rows by four pieces of 4 values, lane i gets
@@ -183,6 +188,7 @@ struct Tiles {
 // (0, 1 - f), (1, 1 - f), (1, f) with f = 0, 1 in turn: each quarter changes one operand's half, whose registers were free a quarter
 // earlier, so every LDS read is issued one quarter before its use and a wavefront holds one step's operands only. In the
 // middle of a stage's second step all wavefronts meet: by then each has read the whole slot, so it is filled again at once.
+constexpr int kTileLds = 163840;
 template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT, int PART>
 __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds) {
   constexpr bool MT = OP == DW, CT = OP != FORWARD;  // transposed: the rows' operand, the columns'
@@ -191,7 +197,7 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
   constexpr int MI = BM / 8 / NW, CI = BC / 8 / NW;  // DMAs per wavefront and stage
   static_assert(MI * 8 * NW == BM && CI * 8 * NW == BC && TC % 2 == 0 && TM % 2 == 0 && HC % RUN == 0, "whole DMAs, halves of whole runs");
   constexpr uint32_t kC = BM * 128, kSlot = (BM + BC) * 128;
-  constexpr int NS = 131072 / kSlot;  // slots
+  constexpr int NS = kTileLds / kSlot;  // slots
 
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wc = wave % WC, wm = wave / WC;
@@ -214,7 +220,7 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     p.cols = min(BC, ncols - p.c0);
     return p;
   };
-  Tiles<OP, PART == REST ? 2 * BM : BM, ADAPT, PART> tiles(a, lane), ahead = tiles;
+  Tiles<OP, PART == WHOLE ? BM : 2 * BM, ADAPT, PART> tiles(a, lane), ahead = tiles;
   if (!tiles.any()) return;
 
   // the channel of the first operand's row p (direct) or of its columns' piece q of tile t
@@ -233,7 +239,7 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
   uint32_t moff[MI], coff[CI];
   i32x4 nm{}, nc{};
   int soff = 0;
-  uint32_t fill = lds0 + wave * (MI * 1024);  // the slot that is filled, where this wavefront's part of the rows' operand goes
+  uint32_t fill_m = lds0 + wave * (MI * 1024), fill_c = lds0 + kC + wave * (CI * 1024);  // the slot that is filled, where this wavefront's parts go
   auto enter = [&](const TilePlace& at) __attribute__((always_inline)) {
     const Part& p = asked;
     mp = (const char*)a.m + (OP == DW ? (at.first + p.from) * mrow + p.m0 * 2 : (at.first + p.m0) * mrow + p.from * 2);
@@ -303,15 +309,14 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     };
     aim(std::bool_constant<MT>{}, std::integral_constant<int, MI>{}, mp, mrow, asked.rows, moff, nm);
     aim(std::bool_constant<CT>{}, std::integral_constant<int, CI>{}, cp, crow, asked.cols, coff, nc);
-    soff = left > 0 ? stage * 128 : 0;
+    soff = __builtin_amdgcn_readfirstlane(left > 0 ? stage * 128 : 0);
     if (asked.stages >= 0) stage++;
   };
   constexpr int DI = MI + CI;  // DMAs of a stage
-  static_assert(MI == CI, "one LDS address for both operands");
   auto issue = [&](auto KC) __attribute__((always_inline)) {  // number k of the stage asked for
     constexpr int K = decltype(KC)::value;
-    if constexpr (K < MI) dma16_at<K * 1024>(nm, fill, moff[K], MT ? 0 : soff);
-    else dma16_at<kC + (K - MI) * 1024>(nc, fill, coff[K - MI], CT ? 0 : soff);
+    if constexpr (K < MI) dma16_at<K * 1024>(nm, fill_m, moff[K], MT ? 0 : soff);
+    else dma16_at<(K - MI) * 1024>(nc, fill_c, coff[K - MI], CT ? 0 : soff);
   };
 
   f32x4 acc[TC][TM], accb[OP == DW ? TM : 1];
@@ -403,20 +408,23 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     constexpr std::integral_constant<int, f> mf{};
     constexpr std::integral_constant<int, 1 - f> mo{};
     // DMAs into the slot that the last stage has left: the second half of the one asked for there, or the first half of a new one
-    constexpr std::integral_constant<int, J == 0 ? DI / 4 : 0> d12{};
-    constexpr std::integral_constant<int, J == 0 ? 0 : DI / 4> d34{};
-    auto dmas = [&](auto FROM) __attribute__((always_inline)) {
-      return [&](auto KC) __attribute__((always_inline)) { issue(std::integral_constant<int, decltype(FROM)::value + decltype(KC)::value>{}); };
+    auto count = [](auto PC) { return std::integral_constant<int, decltype(PC)::value < 0 ? 0 : DI * (decltype(PC)::value + 1) / 4 - DI * decltype(PC)::value / 4>{}; };
+    auto dmas = [&](auto PC) __attribute__((always_inline)) {  // fourth P of a stage's
+      return [&](auto KC) __attribute__((always_inline)) { issue(std::integral_constant<int, DI * decltype(PC)::value / 4 + decltype(KC)::value>{}); };
     };
-    quarter(busy, zero, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], J, (1 - f) * HM + u); }, d12,
-            dmas(std::integral_constant<int, DI / 2>{}));
-    quarter(busy, zero, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[1][t], J, HC + t); }, d12,
-            dmas(std::integral_constant<int, DI * 3 / 4>{}));
+    constexpr std::integral_constant<int, J == 0 ? 2 : -1> p1{};
+    constexpr std::integral_constant<int, J == 0 ? 3 : -1> p2{};
+    constexpr std::integral_constant<int, J == 0 ? -1 : 0> p3{};
+    constexpr std::integral_constant<int, J == 0 ? -1 : 1> p4{};
+    quarter(busy, zero, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], J, (1 - f) * HM + u); }, count(p1),
+            dmas(p1));
+    quarter(busy, zero, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[1][t], J, HC + t); }, count(p2), dmas(p2));
     if constexpr (J == 1) {  // the next stage has landed, and this one is in registers
       wait_vm<(NS - 2) * DI>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       bare_barrier();
-      fill = lds0 + slot + wave * (MI * 1024);
+      fill_m = lds0 + slot + wave * (MI * 1024);
+      fill_c = lds0 + slot + kC + wave * (CI * 1024);
       const uint32_t on = slot == (NS - 1) * kSlot ? -slot : kSlot;
       slot += on;
 #pragma unroll
@@ -425,19 +433,20 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
       for (uint32_t& x : ca) x += on;
       ask();
     }
-    quarter(busy, one, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[0][t], JN, t); }, d34, dmas(zero));
-    quarter(busy, one, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], JN, (1 - f) * HM + u); }, d34,
-            dmas(std::integral_constant<int, DI / 4>{}));
+    quarter(busy, one, mo, hc, [&](int t) __attribute__((always_inline)) { read_c(fc[0][t], JN, t); }, count(p3), dmas(p3));
+    quarter(busy, one, mf, hm, [&](int u) __attribute__((always_inline)) { read_m(fm[1 - f][u], JN, (1 - f) * HM + u); }, count(p4),
+            dmas(p4));
   };
 #pragma unroll
   for (int t = 0; t < NS - 1; t++) {
     ask();
     mx_unroll<DI>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
-    fill += kSlot;
+    fill_m += kSlot;
+    fill_c += kSlot;
   }
   ask();
   mx_unroll<DI / 2>([&](auto KC) __attribute__((always_inline)) { issue(KC); });
-  wait_vm<(NS - 2) * DI + DI / 2>();
+  wait_vm<(NS - 2) * DI + DI / 2>();  // (of the last stage only the first half is asked for)
   bare_barrier();
 
   TilePlace at;
@@ -548,9 +557,10 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
 }
 template <int OP, bool F16, int OUT, bool ADAPT>
 __global__ void __launch_bounds__(512, 2) k_group_tile(GroupArgs a) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 512 * 128];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds];
   multiply_tiles<OP, F16, OUT, 8, 4, 2, 4, ADAPT, WHOLE>(a, lds);
-  multiply_tiles<OP, F16, OUT, 4, 2, 2, 4, ADAPT, REST>(a, lds);
+  multiply_tiles<OP, F16, OUT, 4, 4, 4, 2, ADAPT, HALVES>(a, lds);
+  multiply_tiles<OP, F16, OUT, 4, 2, 2, 4, ADAPT, QUARTERS>(a, lds);
 }
 
 // Adds the parts of the depth, in order, eight values a thread: the result's first `elems`, then the bias' gradient. Rows of no group stay.
