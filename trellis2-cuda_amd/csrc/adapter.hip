@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, cons
   const uint32_t off = line_offset(lane, K * 2);
   const int depth = line_depth(lane);
   f32x4 acc[RT] = {};
-  constexpr int AT = RT == 1 ? 4 : 2;  // steps on their way together
+  constexpr int AT = RT == 1 ? 8 : RT == 2 ? 4 : 2;  // steps on their way together
   for (int k = s0; k < s1; k += AT) {
     Lines qa[AT][RT], qx[AT];
 #pragma unroll
