@@ -298,6 +298,17 @@ def test_adapter_not_finite(gpu):
         assert torch.isfinite(got[0]).all()  # adapter_add's y of a row without an adapter does not read x
 
 
+def test_more_tiles_than_a_launch_holds(gpu):
+    """So many groups of a row each by so many channels that a workgroup for each would be past 2^32 threads."""
+    g, dt, n, k, o = gen(12), torch.bfloat16, 8192, 8, 32776
+    x, w = ints(g, n, k, dt=dt, most=1), torch.zeros((n, o, k), dtype=dt, device=gpu)
+    w[:, -40:], w[:, :40] = ints(g, n, 40, k, dt=dt, most=1), ints(g, n, 40, k, dt=dt, most=1)
+    y = sp.group_linear(x, w, torch.arange(1, n + 1, dtype=torch.int32, device=gpu))
+    for part in (slice(0, 40), slice(o - 40, o)):
+        assert torch.equal(y[:, part], (w[:, part].float() * x[:, None].float()).sum(-1).to(dt))
+    assert not y[:, 40:-40].any()
+
+
 def test_adapter_past_four_gigabytes(gpu):
     """Offsets past 32 bits: in the rows, the result and the adapters."""
     g, dt = gen(4), torch.bfloat16

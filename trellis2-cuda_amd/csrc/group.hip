@@ -742,8 +742,7 @@ void launch_rows(GroupArgs a) {
   a.split = 1;
   a.tiles_c = cdiv(a.O, 16 * OT);
   a.band = 8;
-  const i64 blocks = ((a.N / (16 * NT) + a.G) * a.tiles_c + 7) / 8 * 8;
-  REQ(blocks * (ADAPT ? 768 : 512) < (1ll << 32), "%lld tiles: too many for a launch", (long long)blocks);
+  const i64 blocks = ((a.N / (16 * NT) + std::min<i64>(a.G, a.N)) * a.tiles_c + 7) / 8 * 8;  // (no more groups than rows have any)
   k_group_rows<F16, OT, NT, ADAPT, FUSED><<<(unsigned)blocks, ADAPT ? 768 : 512, 0, stream()>>>(a);
   CK(hipGetLastError());
 }
@@ -755,7 +754,7 @@ void launch_rows(GroupArgs a) {
 constexpr i64 kCus = 256;  // (a workspace's size follows from it, also where no device is)
 int row_tiles(i64 N, i64 G) { return N <= 16 * G ? 1 : N <= 32 * G ? 2 : 4; }  // of 16 rows
 bool goes_by_rows(i64 N, i64 G, i64 O) {
-  if (N <= 16 * G) return true;
+  if (N <= 16 * G) return (N / 16 + std::min(G, N)) * cdiv(O, 16) < (1ll << 32) / 768;  // (a launch holds 2^32 threads)
   return N <= 512 * G && (N / (16 * row_tiles(N, G)) + G) * cdiv(O, 32) <= kCus;
 }
 // Parts of the depth for a product that is a few quartered tiles only, so that they fill the CUs: a stage of 64 of a quarter takes some 0.5 us,
