@@ -309,6 +309,26 @@ def test_more_tiles_than_a_launch_holds(gpu):
     assert not y[:, 40:-40].any()
 
 
+def test_as_many_rows_as_there_may_be(gpu):
+    """Row numbers up to the largest of 31 bits, in the last stage of the longest sum among them."""
+    dt, n, last = torch.float16, 2 ** 31 - 1, 70
+    g = gen(13)
+    x, dy = (torch.zeros((n, 8), dtype=dt, device=gpu) for _ in range(2))  # 34 GB each
+    x[-last:], dy[-last:] = ints(g, last, 8, dt=dt), ints(g, last, 8, dt=dt)
+    w, ends = ints(g, 2, 8, 8, dt=dt), torch.tensor([n - 3, n], dtype=torch.int32, device=gpu)
+    for e, which in ((ends, w), (ends[1:], w[:1])):
+        tail = (e - (n - last)).clamp(min=0)
+        assert torch.equal(sp.group_linear_dw(dy, x, e), dw64(dy[-last:], x[-last:], tail)[0].to(dt))
+        y = sp.group_linear(x, which, e)
+        assert torch.equal(y[-last:], forward64(x[-last:], which, tail, None, y[-last:]).to(dt))
+        del y
+        dx = sp.group_linear_dx(dy, which, e)
+        assert torch.equal(dx[-last:], dx64(dy[-last:], which, tail, x[-last:]).to(dt))
+        del dx
+    del x, dy
+    torch.cuda.empty_cache()
+
+
 def test_adapter_past_four_gigabytes(gpu):
     """Offsets past 32 bits: in the rows, the result and the adapters."""
     g, dt = gen(4), torch.bfloat16

@@ -212,7 +212,7 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     p.stages = (int)(((i64)p.depth + 63) / 64);
     const int s0 = (int)((i64)p.stages * at.part / a.split), s1 = (int)((i64)p.stages * (at.part + 1) / a.split);
     p.from = s0 * 64;
-    p.depth = max(min(p.depth, s1 * 64) - p.from, 0);
+    p.depth = max((int)min((i64)p.depth, (i64)s1 * 64) - p.from, 0);
     p.stages = s1 - s0;
     p.m0 = at.tm * BM;
     p.c0 = at.tc * BC;
