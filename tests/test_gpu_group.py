@@ -170,6 +170,17 @@ def test_ends_outside_the_rows(gpu):
         assert torch.equal(sp.group_linear_dw(dy, x, e), dw64(dy, x, same)[0].to(dt))
 
 
+def test_falling_ends(gpu):
+    """Not allowed, and what the rows get is anything; but the call ends as soon as others, and what lies behind the rows stays."""
+    g, dt, n, groups = gen(14), torch.bfloat16, 1 << 20, 4096
+    ends = torch.tensor([n, 0] * (groups // 2), dtype=torch.int32, device=gpu)  # 2^31 rows, were they all taken
+    x, w = ints(g, n, 8, dt=dt), ints(g, groups, 8, 8, dt=dt)
+    for call in (sp.group_linear, sp.group_linear_dx):
+        whole = torch.full((n + 300, 8), 7.0, dtype=dt, device=gpu)
+        call(x, w, ends, out=whole[:n])
+        assert (whole[n:] == 7).all()
+
+
 def test_group_past_four_gigabytes(gpu):
     """Rows and weights whose offsets pass 32 bits: the last ones, beside their neighbours."""
     dt, n, k = torch.bfloat16, (1 << 20) + 300, 2112

@@ -54,6 +54,7 @@ struct Tiles {
         for (int g0 = 64; g0 < a.G; g0 += 64) total += __builtin_amdgcn_readlane(chunk(g0), 63);
         key = chunk(0);
       }
+      total = min(total, a.N / BM + a.G);  // (only ends that fall, which is not allowed, have groups of more)
       const i64 all = total * a.tiles_c * a.split, per = (all + 7) / 8;
       begin = blockIdx.x % 8 * per;
       end = max(min(per, all - begin), (i64)0);
