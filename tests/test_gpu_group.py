@@ -340,6 +340,21 @@ def test_as_many_rows_as_there_may_be(gpu):
     torch.cuda.empty_cache()
 
 
+def test_adapters_of_as_many_rows_as_there_may_be(gpu):
+    dt, n, last = torch.float16, 1 << 27, 70
+    g = gen(15)
+    x = torch.zeros((n, 8), dtype=dt, device=gpu)
+    x[-last:] = ints(g, last, 8, dt=dt, most=1)
+    slots = torch.zeros(n, dtype=torch.int32, device=gpu)
+    for rank in (8, 72):
+        a, b, w = ints(g, 2, rank, 8, dt=dt, most=1), ints(g, 2, 8, rank, dt=dt, most=1), ints(g, 8, 8, dt=dt, most=1)
+        low = x[-last:].double() @ a[0].double().T @ b[0].double().T
+        y = sp.adapter_add(x, x, a, b, slots)
+        assert torch.equal(y[-last:], (x[-last:].double() + low).to(dt)) and not y[-n:-last].any()
+        y = sp.adapter_linear(x, w, a, b, slots)
+        assert torch.equal(y[-last:], (x[-last:].double() @ w.double().T + low).to(dt)) and not y[-n:-last].any()
+
+
 def test_adapter_past_four_gigabytes(gpu):
     """Offsets past 32 bits: in the rows, the result and the adapters."""
     g, dt = gen(4), torch.bfloat16

@@ -144,6 +144,7 @@ def test_adapters():
         refused(call(out=5 * A), "overlap")
         refused(call(scale=6 * A), "overlap")
         refused(call(n=1 << 31), "rows")
+        refused(call(n=(1 << 27) + 1, x=A, a=1 << 60, b=1 << 61), "2^27")
         assert call(n=0, x=None, slots=None, out=None, **({"y": None} if call is add else {})) == 0
     refused(linear(out=2 * A), "overlap")
     refused(linear(bias=6 * A), "overlap")

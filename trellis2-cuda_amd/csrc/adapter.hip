@@ -242,7 +242,6 @@ void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tens
     constexpr int U = decltype(UC)::value, RT = decltype(RC)::value;
     const i64 tiles = U ? ((N + 16 * U - 1) / (16 * (U ? U : 1)) + 7) / 8 * 8 : N;
     const dim3 grid((unsigned)tiles, cdiv(R, 16 * RT) * (U ? kTurns : 1));
-    REQ(tiles * grid.y * 512 < (1ll << 32), "%lld rows: too many for a launch", (long long)N);
     const uint16_t *px = x.ptr<uint16_t>(), *pa = a.ptr<uint16_t>();
     const float* ps = scale ? scale->ptr<float>() : nullptr;
     if constexpr (U == 0) k_adapter_in_rows<F16, RT><<<grid, 512, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, L, R, K);
@@ -291,6 +290,7 @@ void launch_add(const GroupArgs& a) {
 
 i64 inner_bytes(i64 N, i64 R) { return adapter_fused(N, R) ? 0 : (N * R * 2 + 255) / 256 * 256; }
 constexpr int kHighestRank = 256;
+constexpr i64 kMostRows = 1 << 27;  // whose launches hold fewer than 2^32 threads in any direction
 void check(const Tensor& t, const char* what, DT dt, std::initializer_list<i64> sh) {
   bool same = t.dt == dt && t.dim() == (int)sh.size();
   if (same) {
@@ -309,7 +309,7 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
   REQ(x.dt == F16 || x.dt == BF16, "x must be bf16/fp16, not %s", dname(x.dt));
   REQ(x.dim() == 2 && a.dim() == 3 && b.dim() == 3, "x must be [N,K], a [L,R,K], b [L,O,R]");
   const i64 N = x.size(0), K = x.size(1), L = a.size(0), R = a.size(1), O = b.size(1);
-  REQ(N < (1ll << 31), "%lld rows", (long long)N);
+  REQ(N <= kMostRows, "%lld rows: at most 2^27", (long long)N);
   REQ(L > 0 && L <= (1 << 16), "%lld adapters: 1 to 2^16", (long long)L);
   REQ(R > 0 && R % 8 == 0 && R <= kHighestRank, "rank %lld: a positive multiple of 8, at most %d", (long long)R, kHighestRank);
   for (i64 c : {O, K}) REQ(c > 0 && c % 8 == 0 && c <= (1 << 20), "%lld channels: a positive multiple of 8, at most 2^20", (long long)c);

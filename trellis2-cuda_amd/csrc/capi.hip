@@ -550,7 +550,7 @@ SPC_API int spc_group_linear_dw(const void* dy, const void* x, const int32_t* en
 
 SPC_API int spc_adapter_workspace(int64_t N, int64_t R, int64_t K, int64_t Co, int64_t* bytes) {
   return guarded([&] {
-    REQ(bytes && N >= 0 && N < (1ll << 31) && R > 0 && R <= 256 && K >= 0 && K <= (1 << 20) && Co > 0 && Co <= (1 << 20), "arguments");
+    REQ(bytes && N >= 0 && N <= (1 << 27) && R > 0 && R <= 256 && K >= 0 && K <= (1 << 20) && Co > 0 && Co <= (1 << 20), "arguments");
     *bytes = adapter_workspace(N, R, K, Co);
   });
 }
