@@ -241,7 +241,7 @@ ADAPTERS = [  # n, adapters, rank, k, o, order
     (128, 128, 8, 72, 72, "mixed"), (129, 3, 256, 136, 392, "mixed"), (300, 7, 40, 520, 264, "runs"), (1000, 2, 16, 1416, 1032, "runs"),
     (2600, 9, 64, 320, 1096, "runs"), (700, 70, 16, 512, 512, "mixed"), (50, 4, 16, 128, 64, "none"), (600, 4, 16, 128, 256, "none"),
     (4099, 6, 24, 136, 8200, "runs"), (2000, 40, 72, 72, 8200, "mixed"), (3, 5, 8, 520, 264, "mixed"), (2, 2, 16, 4104, 72, "mixed"),
-    (1, 2, 32, 1416, 200, "one"), (40, 3, 256, 264, 136, "mixed"), (600, 4, 16, 4104, 136, "runs"), (500, 4, 16, 136, 136, "mixed"), (20000, 5, 48, 72, 136, "runs"), (4099, 1, 24, 136, 264, "one"), (513, 6, 200, 64, 40, "runs"), (9, 4, 16, 16384, 64, "mixed"), (300, 4, 16, 16384, 64, "runs"),
+    (1, 2, 32, 1416, 200, "one"), (40, 3, 256, 264, 136, "mixed"), (600, 4, 16, 4104, 136, "runs"), (500, 4, 16, 136, 136, "mixed"), (20000, 5, 48, 72, 136, "runs"), (4099, 1, 24, 136, 264, "one"), (513, 6, 200, 64, 40, "runs"), (9, 4, 16, 16384, 64, "mixed"), (300, 4, 16, 16384, 64, "runs"), (2500, 5, 16, 136, 264, "mixed"),
 ]
 
 

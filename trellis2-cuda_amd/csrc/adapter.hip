@@ -9,6 +9,7 @@ namespace {
 // The first product, h = scale[s] x a[s]^T per row, summed in fp32 and held in 16 bits (a matrix instruction's operand; half an ulp of it
 // reaches the result through b), one row per workgroup: the reading of a is shared by nobody but the caches, and no row waits for
 // another's adapter. The 8 wavefronts share the depth out, and their sums meet in LDS in a fixed order. 16 RT ranks (blockIdx.y: which).
+// Bound by latency: [77, 4096], 16 ranks of 32 adapters 5.2 us, slots and then one load of all that a wavefront needs.
 template <bool F16, int RT>
 __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, int L, int R, int K) {
   constexpr int NW = 8;
@@ -68,7 +69,8 @@ __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, cons
 
 // The same for many rows: 16 U of them per workgroup. Each XCD takes neighbouring rows, whose adapters are the same ones. Every adapter that some of the rows have takes its turn, and the
 // lanes whose row has it keep the sums; `turns` workgroups share the adapters out, so that one with a request's border among its
-// rows takes no longer than the others (those without a turn end at once).
+// rows takes no longer than the others (those without a turn end at once). Bound by how many loads a CU has on their way: [8209, 4096], 64 ranks, 30 - 35 us
+// (x alone 13 at a copy's rate); [8209, 2080], 24 ranks, 15 us.
 template <bool F16, int U, int RT>
 __global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, i64 N, int L, int R,
                                                        int K, int turns) {
@@ -166,7 +168,8 @@ __global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const 
 }
 
 // out = y + scale b[s] h: 16 TM rows by 16 TC channels per wavefront, four wavefronts beside each other; or (SHARE) all four at the same
-// place, sharing out the rows' adapters, for few rows that differ in theirs; FUSED, they make the first product, too
+// place, sharing out the rows' adapters, for few rows that differ in theirs; FUSED, they make the first product, too. Bound by y's reading and
+// writing: [8209, 4128] fp16, 24 ranks, 29.5 us, 4.6 TB/s; few rows by latency ([77, 4096], 16 ranks of 32 adapters, 4.8 us).
 template <bool F16, int TC, int TM, bool SHARE, bool FUSED>
 __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
   constexpr int NW = 4;
@@ -232,8 +235,10 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
 }
 
 constexpr int kTurns = 2;
-// One workgroup a row reads 2 R K bytes of a for each; 16 U rows share them, but wait for every adapter among them in turn.
-bool by_row(i64 N, i64 R) { return N * R <= 8192; }
+// One workgroup a row reads 2 R K bytes of a for each; 16 U rows share them, but wait for every adapter among them in turn
+// us of adapter_add, by row / in tiles, [N, 4096] to 64 channels, four adapters in runs; every row another than its neighbour: 256 rows of 64 ranks 16 / 24; 23 / 127,
+// 512 of 64 24 / 21; 34 / 134, 1024 of 16 15 / 15; 19 / 68, of 64 39 / 18; 59 / 135, 2048 of 16 25 / 15; 36 / 80. (The order is not known here.)
+bool by_row(i64 N, i64 R) { return N <= 2048 && N * R <= 32768; }
 template <bool F16>
 void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tensor* scale, uint16_t* h) {
   const i64 N = x.size(0);
@@ -267,6 +272,9 @@ void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tens
   else if (u == 3) by(std::integral_constant<int, 3>{});
   else by(std::integral_constant<int, 4>{});
 }
+// Up to as many rows four wavefronts share a place's adapters out. us of adapter_add, so / not, [N, 64] to 4096 channels, every row another of 32 adapters than
+// its neighbour (the first product in tiles for 1024 rows and more): 512 rows 15.8 / 16.3, 1024 29 / 27, 2048 42 / 38
+constexpr i64 kSharedRows = 512;
 template <bool F16>
 void launch_add(const GroupArgs& a) {
   auto go = [&](auto TCC, auto TMC, auto share, auto fused) {
@@ -284,7 +292,7 @@ void launch_add(const GroupArgs& a) {
   constexpr std::integral_constant<int, 2> two{};
   constexpr std::integral_constant<int, 4> four{};
   if (!a.ad.h) go(four, one, std::true_type{}, std::true_type{});
-  else if (a.N <= 1024) go(four, one, std::true_type{}, std::false_type{});
+  else if (a.N <= kSharedRows) go(four, one, std::true_type{}, std::false_type{});
   else go(two, four, std::false_type{}, std::false_type{});
 }
 
