@@ -557,3 +557,15 @@ def test_refusals_on_the_device(gpu):
         sp.group_linear(room[1:513].view(8, 64), w, ends)
     with pytest.raises(RuntimeError, match="apart"):
         sp.adapter_add(room[:576].view(8, 72), x, a, b, slots, out=room[64:640].view(8, 72))
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n,k,o", [(2100, 16384, 128), (1990, 16136, 8), (4100, 128, 16384), (2500, 104, 16264), (2100, 16640, 128), (2100, 16128, 128)])
+def test_gradient_of_64_tiles_in_parts(gpu, n, k, o, dt):
+    """A result of one tile across and some 64 along, which is as many as are shared out by XCD and few enough for parts of the depth."""
+    g = gen(n + k)
+    x, dy, ends = ints(g, n, k, most=2, dt=dt), ints(g, n, o, most=2, dt=dt), ends_of([n])
+    dw, db = dw64(dy, x, ends)
+    for odt in (None, torch.float32):
+        got, gb = sp.group_linear_dw(dy, x, ends, out_dtype=odt, bias=True)
+        assert torch.equal(got, dw.to(got.dtype)) and torch.equal(gb, db.to(got.dtype))

@@ -14,7 +14,7 @@ enum { OUT_16 = 0, OUT_F32 = 1 };
 // takes a contiguous eighth of it, its workgroups every W-th tile of that, so that the tiles that run beside each other on it share
 // operands in its L2.
 // dw: tiles are as deep as their group is long, so the longest groups come first (up to 64 groups; more are short), in rounds of W tiles
-// a XCD that run to and fro; each XCD takes a contiguous eighth of every group's tiles (where they are many).
+// a XCD that run to and fro; each XCD takes a contiguous eighth of every group's tiles (where they are many, and whole in depth).
 //
 // The last round of an XCD's W workgroups may have few tiles left: where at most a quarter of them would have one, these are taken in
 // QUARTERS (of half the rows and columns) after the whole ones, which take two fifths of a whole one's time, and where at most half of them
@@ -133,7 +133,7 @@ struct Tiles {
     if constexpr (OP == DW) {
       const int tiles = a.tiles_m * a.tiles_c;
       const i64 u = l * 8 + blockIdx.x % 8, b = u / a.split;
-      at.part = a.per ? 0 : (int)(u % a.split);  // (many tiles are not split)
+      at.part = (int)(u % a.split);
       const int order = (int)(a.per ? l / a.per : b / tiles);
       const int inside = (int)(a.per ? blockIdx.x % 8 * a.per + l % a.per : b % tiles);
       if (order >= a.G || inside >= tiles) return false;
@@ -617,7 +617,7 @@ void launch_tile(GroupArgs a) {
   if (OP == DW) {
     a.tiles_m = cdiv(a.O, BM);
     const i64 each = (i64)a.tiles_m * a.tiles_c;
-    a.per = each >= 64 ? (int)((each + 7) / 8) : 0;
+    a.per = a.split == 1 && each >= 64 ? (int)((each + 7) / 8) : 0;  // (the list of eighths has no parts of the depth)
   }
   const int blocks = mx_device_cus() / 8 * 8;  // one workgroup fits a CU; what has no tile ends at once
   k_group_tile<OP, F16, OUT, ADAPT><<<blocks, 512, 0, stream()>>>(a);
