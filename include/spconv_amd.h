@@ -234,8 +234,10 @@ int spc_group_linear_dw(const void* dy, const void* x, const int32_t* ends, int 
  *   spc_adapter_add      out = y + that, for a projection y made elsewhere (spc_mx_linear's); out may be y
  * x [N,K], w [Co,K], a [L,R,K], b [L,Co,R], y, out [N,Co] of one `dtype` (SPC_F16/SPC_BF16), 16-byte aligned; R a multiple of 8,
  * at most 256; K and Co multiples of 8, at most 2^20; L at most 2^16, N at most 2^27; scale float [L] or NULL (1); bias [Co] of
- * `b_dtype` or NULL. a x is summed in fp32, scaled and held in `dtype`. workspace: device memory of spc_adapter_workspace's bytes (K = 0 for
- * spc_adapter_add), 16-byte aligned, or NULL (the library's own; refused while the stream is captured, if any is needed).
+ * `b_dtype` or NULL. a x is summed and scaled in fp32 and held in two halves of `dtype`, to 2^-15 of each value (SPC_BF16), or 2^-22 of
+ * each and 2^-39 of the row's largest (SPC_F16), whose power of two is kept apart. workspace: device memory of spc_adapter_workspace's bytes (K = 0 for spc_adapter_add), 16-byte
+ * aligned, or NULL (the library's own; refused while the stream is captured, if any is needed). That many bytes hold a x of about half
+ * of the rows, which then go in two parts or three; with 3 N R bytes more they go in one.
  * No counterpart in the reference; beside spc_mx_linear, the shared projection in 4 bits. */
 int spc_adapter_workspace(int64_t N, int64_t R, int64_t K, int64_t Co, int64_t* bytes);
 int spc_adapter_linear(const void* x, const void* w, const void* a, const void* b, const int32_t* slots, const float* scale,

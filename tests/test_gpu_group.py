@@ -569,3 +569,75 @@ def test_gradient_of_64_tiles_in_parts(gpu, n, k, o, dt):
     for odt in (None, torch.float32):
         got, gb = sp.group_linear_dw(dy, x, ends, out_dtype=odt, bias=True)
         assert torch.equal(got, dw.to(got.dtype)) and torch.equal(gb, db.to(got.dtype))
+
+
+# x, a, b, w, y and scale times these: as they come; A x past fp16's largest value, B small; scaled A x below fp16's least normal one, B large;
+# a scale past fp16's largest value
+RANGES = {"one": (1, 2.0 ** -6, 1, 1, 1, 1), "large": (256, 64, 2.0 ** -16, 2.0 ** -13, 1, 1), "small": (1, 2.0 ** -6, 2.0 ** 12, 2.0 ** -16, 2.0 ** -10, 2.0 ** -22),
+          "scale": (1, 2.0 ** -6, 2.0 ** -18, 1, 1, 2.0 ** 18)}
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("kind", list(RANGES))
+@pytest.mark.parametrize("n,count,rank,k,o,order", [ADAPTERS[i] for i in (1, 3, 4, 7, 9, 10, 11, 12, 17, 22)])
+def test_adapter_inner_product(gpu, n, count, rank, k, o, order, kind, dt):
+    """The inner product, a sum in fp32, keeps fp32's range, and the second product takes it to 2^-15 of each value (bf16), 2^-22 of
+    each and 2^-39 of the row's largest (fp16): its high half is cut to 8 (rounded to 11) bits, its low half rounded to as many, in fp16
+    both of values whose largest is in [2^14, 2^15) and whose least step is 2^-24."""
+    g = gen(n + rank)
+    px, pa, pb, pw, py, ps = RANGES[kind]
+    slots = slots_of(g, n, count, order)
+
+    def drawn(factor, *shape):
+        return (torch.randn(shape, generator=g, device=gpu) * factor).to(dt)
+
+    x, w, a, b, y = drawn(px, n, k), drawn(pw, o, k), drawn(pa, count, rank, k), drawn(pb, count, o, rank), drawn(py, n, o)
+    scale = (torch.rand(count, generator=g, device=gpu) + 0.5) * ps
+    zero = torch.zeros((n, o), dtype=torch.float64, device=gpu)
+    part = adapter64(zero, x, a, b, slots, scale, dt)[0]
+    size = adapter64(zero, x.abs(), a.abs(), b.abs(), slots, scale, dt)[0]
+    inner, most = zero.clone(), zero.clone()
+    for s in range(count):
+        r = (slots == s).nonzero().squeeze(1)
+        h = (x[r].double() @ a[s].double().T * float(scale[s])).abs()
+        inner[r] = h @ b[s].double().abs().T
+        most[r] = h.amax(1, keepdim=True) * b[s].double().abs().sum(1)
+    held = 2.0 ** -15 * inner if dt == torch.bfloat16 else 2.0 ** -22 * inner + 2.0 ** -39 * most
+    t = torch.finfo(dt)
+    for got, base, bs in ((sp.adapter_linear(x, w, a, b, slots, scale=scale), x.double() @ w.double().T, x.double().abs() @ w.double().abs().T),
+                          (sp.adapter_add(y, x, a, b, slots, scale=scale), y.double(), y.double().abs())):
+        want = base + part
+        assert want.abs().max() < t.max / 2
+        tol = (k + 2 * rank + 4) * 2.0 ** -23 * (bs + size) + 1.01 * held
+        tol = tol + t.eps / 2 * (want.abs() + tol) + t.tiny * t.eps / 2
+        assert ((got.double() - want).abs() <= tol).all(), float(((got.double() - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n,count,rank,k,o,order", [(1, 2, 256, 136, 72, "one"), (2, 2, 40, 520, 264, "mixed"), (5, 3, 8, 72, 136, "mixed"), (7, 3, 24, 136, 72, "mixed")]
+                         + [ADAPTERS[i] for i in (7, 9, 11, 12, 17, 22)])
+def test_adapter_workspaces(gpu, n, count, rank, k, o, order, dt):
+    """The least workspace, in which the rows go in parts, ones between, and one that holds them all: the exact result each time, and
+    nothing written behind it."""
+    import ctypes
+
+    g = gen(n + k + rank)
+    slots = slots_of(g, n, count, order)
+    x = ints(g, n, k, most=1, dt=dt) * (torch.rand((n, k), generator=g, device=gpu) < 20.0 / k).to(dt)
+    w, a, b, y = ints(g, o, k, most=2, dt=dt), ints(g, count, rank, k, most=2, dt=dt), ints(g, count, o, rank, most=1, dt=dt), ints(g, n, o, most=20, dt=dt)
+    part = adapter64(torch.zeros((n, o), dtype=torch.float64, device=gpu), x, a, b, slots, None, dt)[0]
+    lib, least, code = sp.load_library(), ctypes.c_int64(), 2 if dt == torch.bfloat16 else 1
+
+    def p(t):
+        return ctypes.c_void_p(t.data_ptr())
+
+    for depth, want in ((k, x.double() @ w.double().T + part), (0, y.double() + part)):
+        assert lib.spc_adapter_workspace(n, rank, depth, o, ctypes.byref(least)) == 0
+        for size in (least.value, least.value + 8, least.value + n * rank, least.value + 3 * n * rank):
+            out, ws = torch.full_like(y, 7.0), torch.full((size + 256,), 99, dtype=torch.uint8, device=gpu)
+            if depth:
+                rc = lib.spc_adapter_linear(p(x), p(w), p(a), p(b), p(slots), None, None, code, 0, n, count, rank, k, o, p(out), p(ws), size)
+            else:
+                rc = lib.spc_adapter_add(p(y), p(x), p(a), p(b), p(slots), None, code, n, count, rank, k, o, p(out), p(ws), size)
+            assert rc == 0, lib.spc_last_error()
+            assert torch.equal(out, want.to(dt)) and (ws[size:] == 99).all()

@@ -6,12 +6,35 @@
 #include <type_traits>
 
 namespace {
-// The first product, h = scale[s] x a[s]^T per row, summed in fp32 and held in 16 bits (a matrix instruction's operand; half an ulp of it
-// reaches the result through b), one row per workgroup: the reading of a is shared by nobody but the caches, and no row waits for
+// Four ranks of a row's first product, the first of them rank r of row n of N, into memory in halves (group.h)
+template <bool F16>
+__device__ __forceinline__ void store_inner(uint16_t* h, i64 n, i64 N, int R, int r, f32x4 c, float to) {
+  mx_u32x2 high, low;
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    uint32_t hi, lo;
+    halves<F16>(c[2 * j] * to, c[2 * j + 1] * to, hi, lo);
+    high[j] = hi;
+    low[j] = lo;
+  }
+  const i64 n0 = n / 16 * 16;
+  const int m = (int)min((i64)16, N - n0);
+  uint16_t* p = h + n0 * R * 2 + inner_tile_place((int)(n - n0), m, r);
+  *(mx_u32x2*)p = high;
+  *(mx_u32x2*)(p + inner_to_low(m, r, R)) = low;
+}
+__device__ __forceinline__ uint32_t top4(f32x4 c) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(c[j]) & 0x7fffffffu);
+  return m;
+}
+
+// The first product, h = scale[s] x a[s]^T per row, one row per workgroup: the reading of a is shared by nobody but the caches, and no row waits for
 // another's adapter. The 8 wavefronts share the depth out, and their sums meet in LDS in a fixed order. 16 RT ranks (blockIdx.y: which).
 // Bound by latency: [77, 4096], 16 ranks of 32 adapters 5.2 us, slots and then one load of all that a wavefront needs.
 template <bool F16, int RT>
-__global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, int L, int R, int K) {
+__global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, float* back, int L, int R, int K) {
   constexpr int NW = 8;
   __shared__ f32x4 sums[NW][RT][4];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
@@ -58,12 +81,24 @@ __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, cons
     for (int t = 0; t < RT; t++) sums[wave][t][g] = acc[t];
   }
   __syncthreads();
-  if (tid < RT * 4 && tid * 4 < ranks) {
-    f32x4 c = sums[0][tid / 4][tid % 4];
+  if (wave == 0) {  // the first 16 lanes have 4 ranks each
+    const bool in = lane < RT * 4 && lane * 4 < ranks;
+    f32x4 c{};
+    if (in) {
 #pragma unroll
-    for (int w = 1; w < NW; w++) c += sums[w][tid / 4][tid % 4];
-    c *= scale ? scale[s] : 1.f;
-    *(mx_u32x2*)(h + n * R + r0 + tid * 4) = mx_u32x2{mx_pack2<F16>(c[0], c[1]), mx_pack2<F16>(c[2], c[3])};
+      for (int w = 0; w < NW; w++) c += sums[w][lane / 4][lane % 4];
+      c *= scale ? scale[s] : 1.f;
+    }
+    float to = 1.f;
+    if constexpr (F16) {
+      uint32_t top = mx_quad_max(top4(c));
+      top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x124, 0xf, 0xf, true));  // of 4 lanes on, of the 16
+      top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x128, 0xf, 0xf, true));
+      float from;
+      inner_factors(top, to, from);
+      if (lane == 0) back[n * ((R + 63) / 64) + r0 / 64] = from;
+    }
+    if (in) store_inner<F16>(h, n, gridDim.x, R, r0 + lane * 4, c, to);
   }
 }
 
@@ -72,7 +107,7 @@ __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, cons
 // rows takes no longer than the others (those without a turn end at once). Bound by how many loads a CU has on their way: [8209, 4096], 64 ranks, 30 - 35 us
 // (x alone 13 at a copy's rate); [8209, 2080], 24 ranks, 15 us.
 template <bool F16, int U, int RT>
-__global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, i64 N, int L, int R,
+__global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, float* back, i64 N, int L, int R,
                                                        int K, int turns) {
   constexpr int NW = 4;
   __shared__ f32x4 sums[NW][U * RT][64];
@@ -156,14 +191,30 @@ __global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const 
   }
   if (!done) return;
   __syncthreads();
-  for (int q = wave; q < U * RT; q += NW) {
-    const int n = q / RT * 16 + r16, r = q % RT * 16 + g * 4;
-    if (!(done >> n & 1) || r >= ranks) continue;
-    f32x4 c = sums[0][q][lane];
+  for (int u = wave; u < U; u += NW) {
+    const int n = u * 16 + r16;
+    const bool mine_too = done >> n & 1;
+    const float by = mine_too && scale ? scale[slots[n0 + n]] : 1.f;
+    f32x4 c[RT];
+    uint32_t top = 0;
 #pragma unroll
-    for (int w = 1; w < NW; w++) c += sums[w][q][lane];
-    c *= scale ? scale[slots[n0 + n]] : 1.f;
-    *(mx_u32x2*)(h + (n0 + n) * R + r0 + r) = mx_u32x2{mx_pack2<F16>(c[0], c[1]), mx_pack2<F16>(c[2], c[3])};
+    for (int t = 0; t < RT; t++) {
+      c[t] = f32x4{};
+      if (!mine_too || t * 16 + g * 4 >= ranks) continue;
+#pragma unroll
+      for (int w = 0; w < NW; w++) c[t] += sums[w][u * RT + t][lane];
+      c[t] *= by;
+      top = max(top, top4(c[t]));
+    }
+    float to = 1.f;
+    if constexpr (F16) {
+      float from;
+      inner_factors(mx_max_across32(mx_max_across16(top)), to, from);
+      if (mine_too && g == 0) back[(n0 + n) * ((R + 63) / 64) + r0 / 64] = from;
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t++)
+      if (mine_too && t * 16 + g * 4 < ranks) store_inner<F16>(h, n0 + n, N, R, r0 + t * 16 + g * 4, c[t], to);
   }
 }
 
@@ -199,10 +250,9 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
     __shared__ __attribute__((aligned(16))) InnerSums inner[NW];
     inner_products<F16, NW>(a, lane, wave, inner[wave]);
     __syncthreads();
-    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan,
-                      [&](i64 n, int r, int s) __attribute__((always_inline)) { return inner_of<F16, NW>(a, inner, (int)n, r, s); }, wave, NW);
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, summed_inner<F16, NW>(a, inner, lane), wave, NW);
   } else {
-    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, stored_inner(a), SHARE ? wave : 0, SHARE ? NW : 1);
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, stored_inner<F16>(a, n0, rows, lane), SHARE ? wave : 0, SHARE ? NW : 1);
   }
   if constexpr (SHARE) {
 #pragma unroll
@@ -240,17 +290,15 @@ constexpr int kTurns = 2;
 // 512 of 64 24 / 21; 34 / 134, 1024 of 16 15 / 15; 19 / 68, of 64 39 / 18; 59 / 135, 2048 of 16 25 / 15; 36 / 80. (The order is not known here.)
 bool by_row(i64 N, i64 R) { return N <= 2048 && N * R <= 32768; }
 template <bool F16>
-void launch_in(const Tensor& x, const Tensor& a, const Tensor& slots, const Tensor* scale, uint16_t* h) {
-  const i64 N = x.size(0);
-  const int L = (int)a.size(0), R = (int)a.size(1), K = (int)a.size(2);
+void launch_in(const AdapterPart& p, i64 N, int K, uint16_t* h, float* back) {
+  const int L = p.L, R = p.R;
   auto go = [&](auto UC, auto RC) {
     constexpr int U = decltype(UC)::value, RT = decltype(RC)::value;
     const i64 tiles = U ? ((N + 16 * U - 1) / (16 * (U ? U : 1)) + 7) / 8 * 8 : N;
     const dim3 grid((unsigned)tiles, cdiv(R, 16 * RT) * (U ? kTurns : 1));
-    const uint16_t *px = x.ptr<uint16_t>(), *pa = a.ptr<uint16_t>();
-    const float* ps = scale ? scale->ptr<float>() : nullptr;
-    if constexpr (U == 0) k_adapter_in_rows<F16, RT><<<grid, 512, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, L, R, K);
-    else k_adapter_in<F16, U, RT><<<grid, 256, 0, stream()>>>(px, pa, slots.ptr<int32_t>(), ps, h, N, L, R, K, kTurns);
+    const uint16_t *px = (const uint16_t*)p.x, *pa = (const uint16_t*)p.a;
+    if constexpr (U == 0) k_adapter_in_rows<F16, RT><<<grid, 512, 0, stream()>>>(px, pa, p.slots, p.scale, h, back, L, R, K);
+    else k_adapter_in<F16, U, RT><<<grid, 256, 0, stream()>>>(px, pa, p.slots, p.scale, h, back, N, L, R, K, kTurns);
     CK(hipGetLastError());
   };
   auto by = [&](auto UC) {
@@ -296,7 +344,9 @@ void launch_add(const GroupArgs& a) {
   else go(two, four, std::false_type{}, std::false_type{});
 }
 
-i64 inner_bytes(i64 N, i64 R) { return adapter_fused(N, R) ? 0 : (N * R * 2 + 255) / 256 * 256; }
+// Of a row's first product: its halves and its factors
+i64 inner_row_bytes(i64 R) { return R * 4 + (R + 63) / 64 * 4; }
+i64 inner_bytes(i64 N, i64 R) { return adapter_fused(N, R) ? 0 : (N * inner_row_bytes(R) + 15) / 16 * 16; }
 constexpr int kHighestRank = 256;
 constexpr i64 kMostRows = 1 << 27;  // whose launches hold fewer than 2^32 threads in any direction
 void check(const Tensor& t, const char* what, DT dt, std::initializer_list<i64> sh) {
@@ -334,34 +384,48 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
     if (t) mx_apart(out.p, out.bytes(), t->p, t->bytes(), "out");
   if (y) REQ(y->p == out.p || !mx_overlap(y->p, y->bytes(), out.p, out.bytes()), "out must be y or apart from it");
   if (N == 0) return;
-  const i64 need = adapter_workspace(N, R, w ? K : 0, O);
+  // Rows go in as many parts as it takes for the workspace to hold a part's first product
+  const i64 product = w ? adapter_product_bytes(N, K, O) : 0, all = inner_bytes(N, R) + product;
+  const i64 need = workspace && workspace_bytes < all ? std::max(adapter_workspace(N, R, w ? K : 0, O), workspace_bytes) : all;
   if (workspace) {
     for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &a, &b, &slots, w, y, scale, bias, &out})
       if (t) mx_apart(t->p, t->bytes(), workspace, (size_t)need, "the workspace");
   }
   MxWorkspace ws(workspace, workspace_bytes, need);
-  uint16_t* h = (uint16_t*)ws.p;
-  const i64 inner = inner_bytes(N, R);
-  const bool fused = adapter_fused(N, R);
-  GroupArgs g{};
-  g.m = w ? x.p : y->p;
-  g.c = w ? w->p : nullptr;
-  g.bias = bias ? bias->p : nullptr;
-  g.bias_dt = bias ? bias->dt : F32;
-  g.out = out.p;
-  g.N = N;
-  g.G = 1;
-  g.K = (int)K;
-  g.O = (int)O;
-  g.ad = AdapterPart{b.p, fused ? nullptr : h, slots.ptr<int32_t>(), (int)L, (int)R, x.p, a.p, scale ? scale->ptr<float>() : nullptr};
-  if (!fused) x.dt == F16 ? launch_in<true>(x, a, slots, scale, h) : launch_in<false>(x, a, slots, scale, h);
-  if (w) adapter_product(g, x.dt, inner < need ? ws.p + inner : nullptr);
-  else if (x.dt == F16) launch_add<true>(g);
-  else launch_add<false>(g);
+  const i64 part = need < all ? (need - product) / 16 * 16 / inner_row_bytes(R) : N;
+  for (i64 n = 0; n < N; n += part) {
+    const i64 rows = std::min(part, N - n), inner = inner_bytes(rows, R);
+    GroupArgs g{};
+    g.m = w ? x.ptr<uint16_t>() + n * K : y->ptr<uint16_t>() + n * O;
+    g.c = w ? w->p : nullptr;
+    g.bias = bias ? bias->p : nullptr;
+    g.bias_dt = bias ? bias->dt : F32;
+    g.out = out.ptr<uint16_t>() + n * O;
+    g.N = rows;
+    g.G = 1;
+    g.K = (int)K;
+    g.O = (int)O;
+    uint16_t* h = inner ? (uint16_t*)ws.p : nullptr;
+    float* back = inner ? (float*)(h + rows * R * 2) : nullptr;
+    g.ad = AdapterPart{b.p, h, back, slots.ptr<int32_t>() + n, (int)L, (int)R, x.ptr<uint16_t>() + n * K, a.p, scale ? scale->ptr<float>() : nullptr};
+    if (h) x.dt == F16 ? launch_in<true>(g.ad, rows, (int)K, h, back) : launch_in<false>(g.ad, rows, (int)K, h, back);
+    if (w) {
+      const i64 deep = adapter_product_bytes(rows, K, O);  // (that of a part may be more than all rows': undivided then)
+      adapter_product(g, x.dt, deep && deep <= product ? ws.p + inner : nullptr);
+    } else if (x.dt == F16) {
+      launch_add<true>(g);
+    } else {
+      launch_add<false>(g);
+    }
+  }
 }
 }  // namespace
 
-i64 adapter_workspace(i64 N, i64 R, i64 K, i64 O) { return inner_bytes(N, R) + (K ? adapter_product_bytes(N, K, O) : 0); }
+i64 adapter_workspace(i64 N, i64 R, i64 K, i64 O) {
+  // half of the rows, and at least one
+  const i64 some = adapter_fused(N, R) ? 0 : (std::max((N + 1) / 2 * R * 4, inner_row_bytes(R)) + 255) / 256 * 256;
+  return some + (K ? adapter_product_bytes(N, K, O) : 0);
+}
 
 void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
                     const Tensor* bias, Tensor& out, void* workspace, i64 workspace_bytes) {

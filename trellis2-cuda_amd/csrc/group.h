@@ -53,7 +53,8 @@ __device__ __forceinline__ void operands(const Lines& q, int lane, mx_u32x4& fir
 // Adapters of a product's rows: the second of their two products is added to the result
 struct AdapterPart {
   const void* b;         // [L,O,R]
-  const uint16_t* h;     // the first product, scaled: [N,R], in the operands' type (rows without an adapter: anything)
+  const uint16_t* h;     // the first product, scaled, in halves (inner_tile_place says where; rows without an adapter: anything)
+  const float* back;     // what their products are multiplied by: [N,ceil(R/64)] (fp16 only)
   const int32_t* slots;  // [N]
   int L, R;
   const void *x, *a;     // what h is made of where the same kernel makes it (h null): [N,K], [L,R,K]
@@ -76,8 +77,58 @@ struct GroupArgs {
 };
 
 namespace {
-__device__ __forceinline__ auto stored_inner(const GroupArgs& a) {
-  return [&a](i64 n, int r, int) __attribute__((always_inline)) { return *(const mx_u32x4*)(a.ad.h + n * a.ad.R + r); };
+// The first product is a sum in fp32 and a factor of the second, whose instructions take 16-bit operands: it goes there as two, a high and a
+// low half, whose sum it is to 2^-15 of itself (bf16; one operand alone 2^-8) or 2^-22 (fp16; one alone 2^-11, up to 65504 only).
+//
+// In fp16 the 64 ranks of a row that share a factor are brought to below 2^15 by a power of two, which their products are multiplied back
+// with; their low halves end at 2^-39 of the largest. `largest`: the bits of its magnitude, an infinity's or a NaN's too.
+__device__ __forceinline__ void inner_factors(uint32_t largest, float& to, float& back) {
+  const uint32_t e = max(largest >> 23, 15u);
+  to = __uint_as_float((268 - e) << 23);  // 2^14 / the largest's power of two; both are normal
+  back = __uint_as_float((e - 14) << 23);
+}
+// Two values. The high half is cut in bf16, where rounding would make infinities of the largest. An infinity or NaN is the high half's alone.
+template <bool F16>
+__device__ __forceinline__ void halves(float x, float y, uint32_t& high, uint32_t& low) {
+  high = F16 ? mx_pack2<F16>(x, y) : __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+  const float dx = x - mx_lo<F16>(high), dy = y - mx_hi<F16>(high);
+  low = mx_pack2<F16>(dx == dx ? dx : 0.f, dy == dy ? dy : 0.f);
+}
+// 16-bit values with zeros for infinities and NaN: what the low half is multiplied by, so that the high half's product alone decides
+// what comes of an infinity
+template <bool F16>
+__device__ __forceinline__ mx_u32x4 finite_only(mx_u32x4 q) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  constexpr uint32_t kExponent = F16 ? 0x7c007c00u : 0x7f807f80u, kStep = F16 ? 0x04000400u : 0x00800080u;
+#pragma unroll
+  for (int j = 0; j < 4; j++) q[j] &= ~__builtin_bit_cast(uint32_t, __builtin_bit_cast(s16x2, (q[j] & kExponent) + kStep) >> (short)15);
+  return q;
+}
+// Where the high half of rank r of row n stands among the 2 R of all N rows: as the operands are loaded, 16 rows at a time (m where fewer
+// are left) and of these 32 ranks' high halves, then their low ones, eight ranks of each row together (64 bytes of 16 rows a load: adapter_add
+// [8209, 4096] to 4096 channels, 64 ranks, 92 -> 77 us)
+__device__ __forceinline__ int inner_tile_place(int i, int m, int r) { return r / 32 * 64 * m + (r % 32 / 8 * m + i) * 8 + r % 8; }
+__device__ __forceinline__ int inner_to_low(int m, int r, int R) { return m * min(32, R - r / 32 * 32); }
+// The first product of a wavefront's rows, from row n0 on, from memory: row i's high[c], low[c] are ranks r0 + 32 c + 8 (lane / 16) .. + 7,
+// anything where the row has no adapter, so that the loads do not wait for the slots. (Loads past a buffer's end, not branches: around the
+// lanes' branches the compiler, short of registers in the tiles' kernel, has copied a value of all lanes for some of them only.)
+template <bool F16>
+__device__ __forceinline__ auto stored_inner(const GroupArgs& a, i64 n0, int rows, int lane) {
+  const int R = a.ad.R, blocks = (R + 63) / 64, n = max(min(rows, 64), 0);
+  const auto rh = buffer(a.ad.h + n0 * R * 2, (uint32_t)(n * R * 4)), rf = buffer(F16 ? a.ad.back + n0 * blocks : nullptr, F16 ? (uint32_t)(n * blocks * 4) : 0u);
+  return [=](int i, int r0, int, auto& high, auto& low, float& back) __attribute__((always_inline)) {
+    constexpr int RC = sizeof(high) / sizeof(high[0]);
+#pragma unroll
+    for (int c = 0; c < RC; c++) {
+      const int r = r0 + c * 32 + (lane >> 4) * 8;
+      const bool in = r < R;
+      const int m = min(16, n - i / 16 * 16);
+      const uint32_t at = (uint32_t)((i / 16 * 16 * R * 2 + inner_tile_place(i % 16, m, r)) * 2);
+      high[c] = __builtin_amdgcn_raw_buffer_load_b128(rh, in ? at : kOOR, 0, 0);
+      low[c] = __builtin_amdgcn_raw_buffer_load_b128(rh, in ? at + inner_to_low(m, r, R) * 2 : kOOR, 0, 0);
+    }
+    if constexpr (F16) back = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rf, (uint32_t)((i * blocks + r0 / 64) * 4), 0, 0));
+  };
 }
 // The first product of up to kFusedRows rows, by NW wavefronts, of which this is number w: its part of the sums, to be added over w
 typedef float InnerSums[kFusedRows][kFusedRanks];
@@ -118,48 +169,69 @@ __device__ __forceinline__ void inner_products(const GroupArgs& a, int lane, int
     }
   }
 }
-// Ranks r .. r + 7 of row n of the first product, scaled and in 16 bits, from the sums of NW wavefronts
+// The same of rows 0 .. kFusedRows - 1 from the sums of NW wavefronts
 template <bool F16, int NW>
-__device__ __forceinline__ mx_u32x4 inner_of(const GroupArgs& a, const InnerSums* sums, int n, int r, int slot) {
-  float v[8] = {};
+__device__ __forceinline__ auto summed_inner(const GroupArgs& a, const InnerSums* sums, int lane) {
+  return [&a, sums, lane](int i, int, int slot, auto& high, auto& low, float& back) __attribute__((always_inline)) {
+    constexpr int RC = sizeof(high) / sizeof(high[0]), FC = kFusedRanks / 32;  // (there are no ranks past these)
+    const float scale = a.ad.scale ? a.ad.scale[max(slot, 0)] : 1.f;
+    float v[FC][8];
+    uint32_t top = 0;
 #pragma unroll
-  for (int w = 0; w < NW; w++)
+    for (int c = 0; c < FC; c++) {
+      const int r = c * 32 + (lane >> 4) * 8;
+      const bool in = r < a.ad.R && slot >= 0;
+      const int n = in ? i : 0, from = in ? r : 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] += sums[w][n][r + j];
-  const float scale = a.ad.scale ? a.ad.scale[slot] : 1.f;
+      for (int j = 0; j < 8; j++) {
+        float t = 0.f;
 #pragma unroll
-  for (int j = 0; j < 8; j++) v[j] *= scale;
-  return mx_pack8<F16>(v);
+        for (int w = 0; w < NW; w++) t += sums[w][n][from + j];
+        v[c][j] = in ? t * scale : 0.f;
+      }
+      top = max(top, mx_top8(v[c]));
+    }
+    float to = 1.f;
+    if constexpr (F16) inner_factors(mx_max_across32(mx_max_across16(top)), to, back);
+#pragma unroll
+    for (int c = 0; c < RC; c++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        uint32_t hi = 0, lo = 0;
+        if (c < FC) halves<F16>(v[c][2 * j] * to, v[c][2 * j + 1] * to, hi, lo);
+        high[c][j] = hi;
+        low[c][j] = lo;
+      }
+  };
 }
 
 // The adapters' second product for up to 64 rows of one wavefront (16 TM rows, the first of them row n0, `rows` of which exist):
 // acc[t][u] += b h over tiles t of 16 channels and u of 16 rows. Every adapter that some row has takes its turn, of whose products a
 // lane takes its row's (rows of zeros for the others would let an infinity in b reach them), so rows come in any order; those that share
 // an adapter share its reading. chan(t, r): the channel of
-// the first operand's row r in tile t, counted from c0, `cols` of which exist. inner(n, r, s): ranks r .. r + 7 of h's row n (stored_inner: as
-// it lies in memory). Turns first, first + every, ...
+// the first operand's row r in tile t, counted from c0, `cols` of which exist. inner: a row's first product (stored_inner, summed_inner).
+// Turns first, first + every, ...
 template <bool F16, int TC, int TM, class Chan, class Inner>
 __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC][TM], i64 n0, int rows, int c0, int cols, int lane, Chan&& chan,
                                              Inner&& inner, int first = 0, int every = 1) {
   static_assert(TM <= 4, "a lane a row");
   const AdapterPart& p = a.ad;
   const int r16 = lane & 15, g = lane >> 4;
-  int mine = lane < 16 * TM && lane < rows ? p.slots[n0 + lane] : -1;
-  mine = mine < p.L ? mine : -1;
+  const bool here = lane < 16 * TM && lane < rows;
+  int mine = (int)__builtin_amdgcn_raw_buffer_load_b32(buffer(p.slots + n0, (uint32_t)(max(min(rows, 64), 0) * 4)), here ? (uint32_t)(lane * 4) : kOOR, 0, 0);
+  mine = here && mine < p.L ? mine : -1;
   int slot[TM];
 #pragma unroll
   for (int u = 0; u < TM; u++) slot[u] = __shfl(mine, u * 16 + r16, 64);
   const uint64_t all = __ballot(mine >= 0);
-  constexpr int RC = 2;  // 64 ranks at a time
-  for (int r0 = 0; r0 < p.R; r0 += 32 * RC) {
-    mx_u32x4 h[RC][TM];
+  // 64 ranks and 4 channel tiles at a time; for 64 rows half of either, as registers allow ([8209, 4096] by [4096, 4096], 64 ranks, fp16 306 us;
+  // with 4 tiles 310, with 64 ranks 1060)
+  constexpr int RC = TM <= 2 ? 2 : 1, TP = TC < 4 ? TC : TM > 2 ? 2 : 4;
+  mx_u32x4 high[TM][RC], low[TM][RC];
+  float back[TM];
 #pragma unroll
-    for (int c = 0; c < RC; c++)
-#pragma unroll
-      for (int u = 0; u < TM; u++) {
-        const int r = r0 + c * 32 + g * 8;
-        h[c][u] = r < p.R && slot[u] >= 0 ? inner(n0 + u * 16 + r16, r, slot[u]) : mx_u32x4{};
-      }
+  for (int u = 0; u < TM; u++) inner(u * 16 + r16, 0, slot[u], high[u], low[u], back[u]);
+  for (int r0 = 0;;) {
     int turn = 0;
     for (uint64_t left = all; left; turn++) {
       const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
@@ -167,16 +239,15 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
       left &= ~same;
       if (turn % every != first) continue;
       const auto rb = buffer((const char*)p.b + ((i64)s * a.O + c0) * p.R * 2, (uint32_t)(cols * p.R * 2));
-      constexpr int TP = TC < 4 ? TC : 4;  // channel tiles at a time
 #pragma unroll
       for (int t0 = 0; t0 < TC; t0 += TP) {
-        mx_u32x4 b[RC][TP];
+        mx_u32x4 b[RC][TP], bf[RC][TP];
 #pragma unroll
         for (int c = 0; c < RC; c++) {
           const int r = r0 + c * 32 + g * 8;
           if (c && r0 + c * 32 >= p.R) {
 #pragma unroll
-            for (int t = 0; t < TP; t++) b[c][t] = mx_u32x4{};
+            for (int t = 0; t < TP; t++) b[c][t] = bf[c][t] = mx_u32x4{};
             continue;
           }
 #pragma unroll
@@ -186,19 +257,33 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
           }
         }
 #pragma unroll
+        for (int c = 0; c < RC; c++)
+          if (c == 0 || r0 + c * 32 < p.R) {
+#pragma unroll
+            for (int t = 0; t < TP; t++) bf[c][t] = finite_only<F16>(b[c][t]);
+          }
+#pragma unroll
         for (int u = 0; u < TM; u++) {
           if (!(same >> (16 * u) & 0xffff)) continue;
 #pragma unroll
           for (int t = 0; t < TP; t++) {
-            f32x4 d = mfma<F16>(b[0][t], h[0][u], f32x4{});
+            f32x4 d{};
 #pragma unroll
-            for (int c = 1; c < RC; c++) d = mfma<F16>(b[c][t], h[c][u], d);
+            for (int c = 0; c < RC; c++) {
+              if (c && r0 + c * 32 >= p.R) continue;
+              d = mfma<F16>(bf[c][t], low[u][c], d);
+              d = mfma<F16>(b[c][t], high[u][c], d);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[t0 + t][u][i] += slot[u] == s ? d[i] : 0.f;
+            for (int i = 0; i < 4; i++) acc[t0 + t][u][i] += slot[u] == s ? (F16 ? d[i] * back[u] : d[i]) : 0.f;
           }
         }
       }
     }
+    r0 += 32 * RC;
+    if (r0 >= p.R) break;
+#pragma unroll
+    for (int u = 0; u < TM; u++) inner(u * 16 + r16, r0, slot[u], high[u], low[u], back[u]);
   }
 }
 }  // namespace

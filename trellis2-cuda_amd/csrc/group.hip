@@ -498,7 +498,8 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     asm volatile("" : "+v"(el));
     if (ADAPT && at.part == 0)
       add_adapters<F16>(a, acc, at.first + p.m0 + wm * (16 * TM), p.rows - wm * (16 * TM), p.c0, p.cols, el,
-                        [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); }, stored_inner(a));
+                        [&](int t, int r) __attribute__((always_inline)) { return channel(wc * (16 * TC) + t * 16 + r); },
+                        stored_inner<F16>(a, at.first + p.m0 + wm * (16 * TM), p.rows - wm * (16 * TM), el));
 
     // Two runs' pieces change places between lanes 8 apart, so that a store writes whole 128-byte lines of 8 rows (a run alone is 64 bytes of
     // 16). Where rows are whole lines they go past the caches, which keep the operands ([8192, 1024] by [8192, 1024] 133 -> 116 us); parts of
@@ -713,13 +714,11 @@ __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
   } else if constexpr (FUSED) {
     inner_products<F16, NA>(a, lane, wave - NW, inner[wave - NW]);
   } else {
-    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, stored_inner(a), wave - NW, NA);
+    add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, stored_inner<F16>(a, n0, rows, lane), wave - NW, NA);
   }
   if constexpr (FUSED) {
     __syncthreads();
-    if (wave >= NW)
-      add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan,
-                        [&](i64 n, int r, int s) __attribute__((always_inline)) { return inner_of<F16, NA>(a, inner, (int)n, r, s); }, wave - NW, NA);
+    if (wave >= NW) add_adapters<F16>(a, acc, n0, rows, c0, cols, lane, chan, summed_inner<F16, NA>(a, inner, lane), wave - NW, NA);
   }
 #pragma unroll
   for (int t = 0; t < OT; t++)

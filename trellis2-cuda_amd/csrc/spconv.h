@@ -234,8 +234,8 @@ i64 group_linear_workspace(int product, i64 N, i64 G, i64 K, i64 O);
 // Low-rank adapters of many requests beside one shared projection: out = x w^T + bias + scale[s] b[s] (a[s] x) per row, s = slots[n]
 // (int32 [N]; outside [0, L): no adapter), or the same added to a projection y made elsewhere (out may be y). x [N,K], w [O,K],
 // a [L,R,K], b [L,O,R], y, out [N,O] of one 16-bit type, R a multiple of 8 up to 256, K and O multiples of 8 up to 2^20, N up to 2^27;
-// scale fp32 [L] or null (1); bias [O] of any float type or null. a x is summed in fp32 and held in 16 bits. workspace as for mx_linear, of
-// adapter_workspace() bytes.
+// scale fp32 [L] or null (1); bias [O] of any float type or null. a x is summed in fp32 and held in two 16-bit halves, of fp32's range.
+// workspace as for mx_linear, of adapter_workspace() bytes, where the rows go in two or three parts, or 3 N R more, where they go in one.
 void adapter_linear(const Tensor& x, const Tensor& w, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale,
                     const Tensor* bias, Tensor& out, void* workspace = nullptr, i64 workspace_bytes = 0);
 void adapter_add(const Tensor& y, const Tensor& x, const Tensor& a, const Tensor& b, const Tensor& slots, const Tensor* scale, Tensor& out,

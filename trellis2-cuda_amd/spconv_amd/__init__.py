@@ -701,11 +701,20 @@ def _adapters(x, a, b, slots, scale):
     return N, L, R, K, Co
 
 
+def _adapter_workspace(x, N, R, K, Co):
+    """(workspace, its bytes): with 3 N R more than the least, so that the rows go in one part."""
+    nws = _workspace_bytes("spc_adapter_workspace", N, R, K, Co)
+    if not nws:
+        return None, 0
+    nws += 3 * N * R
+    return _workspace(nws, x), nws
+
+
 def adapter_linear(x, w, a, b, slots, scale=None, bias=None, out=None):
     """x w^T + bias + scale[s] b[s] (a[s] x) per row with fp32 sums, s = slots[n] the row's adapter (int32 [N]; outside [0, L):
     none): the projection w [Co, K] that all rows share and low-rank adapters a [L, R, K], b [L, Co, R] of many requests, in
     any order, all of x's 16-bit type. scale float32 [L] (default 1), bias [Co] of any float type. K and Co multiples of 8, R one
-    up to 256. a[s] x, scaled, is held in x's type between its two products."""
+    up to 256. a[s] x, a float32 sum, is scaled and held in two halves of x's type between its two products."""
     torch = _torch()
     N, L, R, K, Co = _adapters(x, a, b, slots, scale)
     _matrix(w, "w", (Co, K), x.dtype)
@@ -714,8 +723,7 @@ def adapter_linear(x, w, a, b, slots, scale=None, bias=None, out=None):
         out = x.new_empty(N, Co)
     else:
         _matrix(out, "out", (N, Co), x.dtype)
-    nws = _workspace_bytes("spc_adapter_workspace", N, R, K, Co)
-    ws = _workspace(nws, x) if nws else None
+    ws, nws = _adapter_workspace(x, N, R, K, Co)
     dev = torch.cuda.current_device()
     _check(load_library().spc_adapter_linear(
         _adr(x, dev), _adr(w, dev), _adr(a, dev), _adr(b, dev), _adr(slots, dev), _adr(scale, dev), _adr(bias, dev), _dt(x),
@@ -733,8 +741,7 @@ def adapter_add(y, x, a, b, slots, scale=None, out=None):
         out = torch.empty_like(y)
     else:
         _matrix(out, "out", (N, Co), x.dtype)
-    nws = _workspace_bytes("spc_adapter_workspace", N, R, 0, Co)
-    ws = _workspace(nws, x) if nws else None
+    ws, nws = _adapter_workspace(x, N, R, 0, Co)
     dev = torch.cuda.current_device()
     _check(load_library().spc_adapter_add(
         _adr(y, dev), _adr(x, dev), _adr(a, dev), _adr(b, dev), _adr(slots, dev), _adr(scale, dev), _dt(x), N, L, R, K, Co, _adr(out, dev),
