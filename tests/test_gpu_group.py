@@ -641,3 +641,117 @@ def test_adapter_workspaces(gpu, n, count, rank, k, o, order, dt):
                 rc = lib.spc_adapter_add(p(y), p(x), p(a), p(b), p(slots), None, code, n, count, rank, k, o, p(out), p(ws), size)
             assert rc == 0, lib.spc_last_error()
             assert torch.equal(out, want.to(dt)) and (ws[size:] == 99).all()
+
+
+# ---- sums in parts: a second kernel adds them from a workspace -----------------------------------------------------
+
+
+def in_parts(product, n, groups, k, o):
+    return sp._workspace_bytes("spc_group_linear_workspace", product, n, groups, k, o) > 0
+
+
+def calls_in_parts(g, dt=torch.bfloat16):
+    def v(*shape):
+        return values(g, *shape, dt=dt)
+
+    one, two, some, long, deep = ends_of([600]), ends_of([370, 0, 230]), ends_of([700, 0, 900]), ends_of([4100]), ends_of([3000, 0, 3300])
+    assert in_parts(sp.GROUP_FORWARD, 600, 1, 4104, 40) and in_parts(sp.GROUP_FORWARD, 1600, 3, 4104, 40) and in_parts(sp.GROUP_DX, 600, 3, 136, 2056)
+    assert in_parts(sp.GROUP_DW, 4100, 1, 72, 136) and in_parts(sp.GROUP_DW, 6300, 3, 72, 136) and in_parts(sp.GROUP_FORWARD, 600, 1, 4104, 136)
+    x, w1, w3, b1 = v(1600, 4104), v(1, 40, 4104), v(3, 40, 4104), v(1, 40)
+    dy, w, xl, dyl = v(600, 2056), v(3, 2056, 136), v(6300, 72), v(6300, 136)
+    wa, a, b, slots = v(136, 4104), v(3, 16, 4104), v(3, 136, 16), slots_of(g, 600, 3, "mixed")
+    return [lambda: sp.group_linear(x[:600], w1, one, bias=b1), lambda: sp.group_linear(x, w3, some), lambda: sp.group_linear_dx(dy, w, two),
+            lambda: sp.group_linear_dw(dyl[:4100], xl[:4100], long, out_dtype=torch.float32, bias=True), lambda: sp.group_linear_dw(dyl, xl, deep),
+            lambda: sp.adapter_linear(x[:600], wa, a, b, slots)]
+
+
+def same(got, want):
+    return all(torch.equal(a, b) for a, b in zip(got, want)) if isinstance(got, tuple) else torch.equal(got, want)
+
+
+def test_parts_same_bits_every_time(gpu):
+    todo = calls_in_parts(gen(41))
+    first = [c() for c in todo]
+    for _ in range(3):
+        junk = torch.full((1 << 25,), 255, dtype=torch.uint8, device=gpu)  # NaN in what the next workspaces may hold
+        del junk
+        assert all(same(c(), want) for c, want in zip(todo, first))
+
+
+def captured(todo):
+    """Each call in a graph of its own, and its result."""
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs, outs = [], []
+    try:
+        for c in todo:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                sp.set_stream(torch.cuda.current_stream())
+                outs.append(c())
+            graphs.append(graph)
+    finally:
+        torch.cuda.synchronize()
+        sp.set_stream(torch.cuda.current_stream())
+    return graphs, outs
+
+
+def test_parts_in_graphs(gpu):
+    """Two graphs of each call, replayed in turn with the call itself between."""
+    todo = calls_in_parts(gen(42))
+    want = [c() for c in todo]
+    graphs, outs = captured(todo + todo)
+    for _ in range(4):
+        for out in outs:
+            for t in out if isinstance(out, tuple) else (out,):
+                t.fill_(3.0)
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(same(out, ref) for out, ref in zip(outs, want + want))
+        assert all(same(c(), ref) for c, ref in zip(todo, want))
+
+
+def test_parts_on_other_streams(gpu):
+    todo = calls_in_parts(gen(43))
+    want = [c() for c in todo]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    try:
+        sp.set_stream(s)
+        for _ in range(2):
+            got = [c() for c in todo]
+            torch.cuda.synchronize()
+            assert all(same(a, b) for a, b in zip(got, want))
+        with torch.cuda.stream(s):
+            got = [c() for c in todo]
+        torch.cuda.synchronize()
+        assert all(same(a, b) for a, b in zip(got, want))
+    finally:
+        torch.cuda.synchronize()
+        sp.set_stream(torch.cuda.current_stream())
+
+
+@pytest.mark.parametrize("dt", TYPES)
+def test_parts_follow_ends(gpu, dt):
+    """Captured calls in parts with other ends in the buffer at their replay, also ones outside the rows: the results of those; rows of no
+    group stay."""
+    g, n = gen(44), 1600
+    x, w = ints(g, n, 4104, dt=dt, most=1), ints(g, 3, 40, 4104, dt=dt, most=1)
+    dy, v = ints(g, 600, 2056, dt=dt, most=1), ints(g, 3, 2056, 136, dt=dt, most=1)
+    xl, dyl = ints(g, 6300, 72, dt=dt, most=1), ints(g, 6300, 136, dt=dt, most=1)
+    ends = [ends_of([t // 3] * 3) for t in (n, 600, 6300)]
+    y, dx, dw = torch.zeros((n, 40), dtype=dt, device=gpu), torch.zeros((600, 136), dtype=dt, device=gpu), torch.zeros((3, 136, 72), device=gpu)
+    todo = [lambda: sp.group_linear(x, w, ends[0], out=y), lambda: sp.group_linear_dx(dy, v, ends[1], out=dx), lambda: sp.group_linear_dw(dyl, xl, ends[2], out=dw)]
+    graphs, _ = captured(todo)
+    for now in ([1.0, 1.0, 1.0], [0, 0, 0.99], [0.03, 0.4, 0.5], [-0.5, 0.1, 9.0], [0, 0, 0], [-2.0, -1.0, -0.1], [0.4, 0.5, 1e9]):
+        for e, t in zip(ends, (n, 600, 6300)):
+            e.copy_(torch.tensor([min(int(f * t), 2 ** 31 - 1) for f in now], dtype=torch.int32))
+        for run in ([graph.replay for graph in graphs], todo):
+            for t, old in ((y, 5.0), (dx, 6.0), (dw, 7.0)):
+                t.fill_(old)
+            want = forward64(x, w, ends[0], None, y).to(dt), dx64(dy, v, ends[1], dx).to(dt), dw64(dyl, xl, ends[2])[0].float()
+            for r in run:
+                r()
+            torch.cuda.synchronize()
+            assert same((y, dx, dw), want)
