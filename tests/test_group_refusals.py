@@ -163,3 +163,23 @@ def test_binding():
                  lambda: sp.adapter_linear(x, w[0], a, b, slots, scale=torch.ones(3)), lambda: sp.adapter_add(x, x, a, b, slots)):
         with pytest.raises((ValueError, RuntimeError)):
             call()
+
+
+def test_adapter_workspace_borders():
+    """Nothing for up to 4 rows and 32 products of rows and ranks, which are one kernel; else half of the rows' inner products, and at least one row's."""
+    lib, n = sp.load_library(), ctypes.c_int64()
+
+    def adapter(rows, rank, k=0, o=64):
+        assert lib.spc_adapter_workspace(rows, rank, k, o, ctypes.byref(n)) == 0
+        return n.value
+
+    for rows, rank in ((1, 8), (1, 32), (2, 16), (4, 8), (1, 24)):
+        assert adapter(rows, rank) == adapter(rows, rank, 4096, 4096) == 0
+    for rows, rank in ((5, 8), (1, 40), (3, 16), (2, 24), (1, 256), (2, 256), (1000, 64), (1 << 27, 256)):
+        assert adapter(rows, rank) % 256 == 0 and adapter(rows, rank) >= max((rows + 1) // 2 * rank * 4, rank * 4 + (rank + 63) // 64 * 4)
+        assert adapter(rows, rank, 64) == adapter(rows, rank)
+    # with 3 N R bytes more there is room for every row's ranks and factors
+    for rows in (1, 3, 5, 17, 1001):
+        for rank in range(8, 264, 8):
+            least = adapter(rows, rank)
+            assert least == 0 or least + 3 * rows * rank >= (rows * (rank * 4 + (rank + 63) // 64 * 4) + 15) // 16 * 16
