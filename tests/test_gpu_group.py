@@ -634,13 +634,13 @@ def test_adapter_workspaces(gpu, n, count, rank, k, o, order, dt):
     for depth, want in ((k, x.double() @ w.double().T + part), (0, y.double() + part)):
         assert lib.spc_adapter_workspace(n, rank, depth, o, ctypes.byref(least)) == 0
         for size in (least.value, least.value + 8, least.value + n * rank, least.value + 3 * n * rank):
-            out, ws = torch.full_like(y, 7.0), torch.full((size + 256,), 99, dtype=torch.uint8, device=gpu)
+            out, ws = torch.full_like(y, 7.0), torch.full((size + 256,), 255, dtype=torch.uint8, device=gpu)
             if depth:
                 rc = lib.spc_adapter_linear(p(x), p(w), p(a), p(b), p(slots), None, None, code, 0, n, count, rank, k, o, p(out), p(ws), size)
             else:
                 rc = lib.spc_adapter_add(p(y), p(x), p(a), p(b), p(slots), None, code, n, count, rank, k, o, p(out), p(ws), size)
             assert rc == 0, lib.spc_last_error()
-            assert torch.equal(out, want.to(dt)) and (ws[size:] == 99).all()
+            assert torch.equal(out, want.to(dt)) and (ws[size:] == 255).all()
 
 
 # ---- sums in parts: a second kernel adds them from a workspace -----------------------------------------------------

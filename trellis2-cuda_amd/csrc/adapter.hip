@@ -302,9 +302,11 @@ void launch_in(const AdapterPart& p, i64 N, int K, uint16_t* h, float* back) {
     CK(hipGetLastError());
   };
   auto by = [&](auto UC) {
-    if (R <= 16) go(UC, std::integral_constant<int, 1>{});
-    else if (R <= 32) go(UC, std::integral_constant<int, 2>{});
-    else go(UC, std::integral_constant<int, 4>{});
+    if constexpr (decltype(UC)::value <= 2) {  // (more rows a workgroup only where it has 64 ranks)
+      if (R <= 16) return go(UC, std::integral_constant<int, 1>{});
+      if (R <= 32) return go(UC, std::integral_constant<int, 2>{});
+    }
+    go(UC, std::integral_constant<int, 4>{});
   };
   // Workgroups of 16 u rows. With more than 32 ranks one takes some u + 2 (its rows of x, and a) and fills a CU; a second one doubles the time ([8209, 4096],
   // 64 ranks of 16 adapters: 41 us with 32 rows, whose 257 workgroups are one too many; [8192, 4096] 28)
