@@ -755,3 +755,21 @@ def test_parts_follow_ends(gpu, dt):
                 r()
             torch.cuda.synchronize()
             assert same((y, dx, dw), want)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("n,rank", [(3, 8), (1, 32), (12, 40), (40, 256), (300, 72), (700, 16), (2600, 64)])
+def test_adapter_infinities(gpu, n, rank, dt):
+    """Infinities and NaN in x, a and b come out as the definition has them: infinities of the right sign, NaN where they meet a zero or each
+    other, and finite values elsewhere."""
+    g, k, o = gen(50 + n), 64, 200
+    x, w, y = ints(g, n, k, dt=dt, most=1), ints(g, o, k, dt=dt, most=1), ints(g, n, o, dt=dt)
+    a, b, slots = ints(g, 3, rank, k, dt=dt, most=1), ints(g, 3, o, rank, dt=dt, most=1), slots_of(g, n, 3, "mixed")
+    slots[0] = 1
+    x = x * (torch.rand((n, k), generator=g, device=gpu) < 0.3).to(dt)
+    a[1, 3, 5], b[1, 7, 2], b[1, 9, :2] = float("inf"), float("-inf"), torch.tensor([float("inf"), float("nan")])
+    b[2, 11, :2] = float("inf")
+    x[n // 2, 4] = float("-inf")
+    for got, base in ((sp.adapter_add(y, x, a, b, slots), y.double()), (sp.adapter_linear(x, w, a, b, slots), x.double() @ w.double().T)):
+        want = adapter64(base, x, a, b, slots, None, dt)[0].to(dt)
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))

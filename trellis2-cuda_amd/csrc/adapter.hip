@@ -26,7 +26,7 @@ __device__ __forceinline__ void store_inner(uint16_t* h, i64 n, i64 N, int R, in
 __device__ __forceinline__ uint32_t top4(f32x4 c) {
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 4; j++) m = max(m, __float_as_uint(c[j]) & 0x7fffffffu);
+  for (int j = 0; j < 4; j++) m = max(m, finite_bits(c[j]));
   return m;
 }
 

@@ -81,11 +81,16 @@ namespace {
 // low half, whose sum it is to 2^-15 of itself (bf16; one operand alone 2^-8) or 2^-22 (fp16; one alone 2^-11, up to 65504 only).
 //
 // In fp16 the 64 ranks of a row that share a factor are brought to below 2^15 by a power of two, which their products are multiplied back
-// with; their low halves end at 2^-39 of the largest. `largest`: the bits of its magnitude, an infinity's or a NaN's too.
+// with; their low halves end at 2^-39 of the largest. `largest`: the bits of the largest finite magnitude (an infinity stays one, and must not
+// make zeros of the others, which may meet an infinity of the second product).
 __device__ __forceinline__ void inner_factors(uint32_t largest, float& to, float& back) {
   const uint32_t e = max(largest >> 23, 15u);
   to = __uint_as_float((268 - e) << 23);  // 2^14 / the largest's power of two; both are normal
   back = __uint_as_float((e - 14) << 23);
+}
+__device__ __forceinline__ uint32_t finite_bits(float v) {  // of its magnitude; zero for an infinity or NaN
+  const uint32_t u = __float_as_uint(v) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
 }
 // Two values. The high half is cut in bf16, where rounding would make infinities of the largest. An infinity or NaN is the high half's alone.
 template <bool F16>
@@ -189,7 +194,8 @@ __device__ __forceinline__ auto summed_inner(const GroupArgs& a, const InnerSums
         for (int w = 0; w < NW; w++) t += sums[w][n][from + j];
         v[c][j] = in ? t * scale : 0.f;
       }
-      top = max(top, mx_top8(v[c]));
+#pragma unroll
+      for (int j = 0; j < 8; j++) top = max(top, finite_bits(v[c][j]));
     }
     float to = 1.f;
     if constexpr (F16) inner_factors(mx_max_across32(mx_max_across16(top)), to, back);
