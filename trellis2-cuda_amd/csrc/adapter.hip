@@ -34,7 +34,8 @@ __device__ __forceinline__ uint32_t top4(f32x4 c) {
 // another's adapter. The 8 wavefronts share the depth out, and their sums meet in LDS in a fixed order. 16 RT ranks (blockIdx.y: which).
 // Bound by latency: [77, 4096], 16 ranks of 32 adapters 5.2 us, slots and then one load of all that a wavefront needs.
 template <bool F16, int RT>
-__global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, float* back, int L, int R, int K) {
+__global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h,
+                                                         float* back, int L, int R, int K) {
   constexpr int NW = 8;
   __shared__ f32x4 sums[NW][RT][4];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
@@ -102,13 +103,13 @@ __global__ void __launch_bounds__(512) k_adapter_in_rows(const uint16_t* x, cons
   }
 }
 
-// The same for many rows: 16 U of them per workgroup. Each XCD takes neighbouring rows, whose adapters are the same ones. Every adapter that some of the rows have takes its turn, and the
-// lanes whose row has it keep the sums; `turns` workgroups share the adapters out, so that one with a request's border among its
-// rows takes no longer than the others (those without a turn end at once). Bound by how many loads a CU has on their way: [8209, 4096], 64 ranks, 30 - 35 us
-// (x alone 13 at a copy's rate); [8209, 2080], 24 ranks, 15 us.
+// The same for many rows: 16 U of them per workgroup. Each XCD takes neighbouring rows, whose adapters are the same ones. Every adapter that
+// some of the rows have takes its turn, and the lanes whose row has it keep the sums; `turns` workgroups share the adapters out, so that one
+// with a request's border among its rows takes no longer than the others (those without a turn end at once). Bound by how many loads a CU has
+// on their way: [8209, 4096], 64 ranks, 30 - 37 us (x alone 13 at a copy's rate); [8209, 2080], 24 ranks, 16 us.
 template <bool F16, int U, int RT>
-__global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h, float* back, i64 N, int L, int R,
-                                                       int K, int turns) {
+__global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const uint16_t* a, const int32_t* slots, const float* scale, uint16_t* h,
+                                                       float* back, i64 N, int L, int R, int K, int turns) {
   constexpr int NW = 4;
   __shared__ f32x4 sums[NW][U * RT][64];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(256, 2) k_adapter_in(const uint16_t* x, const 
 
 // out = y + scale b[s] h: 16 TM rows by 16 TC channels per wavefront, four wavefronts beside each other; or (SHARE) all four at the same
 // place, sharing out the rows' adapters, for few rows that differ in theirs; FUSED, they make the first product, too. Bound by y's reading and
-// writing: [8209, 4128] fp16, 24 ranks, 29.5 us, 4.6 TB/s; few rows by latency ([77, 4096], 16 ranks of 32 adapters, 4.8 us).
+// writing: [8209, 4128] fp16, 24 ranks, 31.4 us, 4.3 TB/s; few rows by latency ([77, 4096], 16 ranks of 32 adapters, 5.8 us).
 template <bool F16, int TC, int TM, bool SHARE, bool FUSED>
 __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
   constexpr int NW = 4;
@@ -284,10 +285,13 @@ __global__ void __launch_bounds__(256) k_adapter_add(GroupArgs a) {
     }
 }
 
+// us with one, two and four workgroups, [8209, 4096] to 64 channels, 64 ranks: 64 requests of 16 adapters 57, 40 and 37, 24 requests 44, 40 and
+// 36, one 23 each; of 16 ranks, 64 requests, 29, 25 and 25; adapter_linear to 4096 channels, 24 requests, 299, 290 and 290
 constexpr int kTurns = 2;
-// One workgroup a row reads 2 R K bytes of a for each; 16 U rows share them, but wait for every adapter among them in turn
-// us of adapter_add, by row / in tiles, [N, 4096] to 64 channels, four adapters in runs; every row another than its neighbour: 256 rows of 64 ranks 16 / 24; 23 / 127,
-// 512 of 64 24 / 21; 34 / 134, 1024 of 16 15 / 15; 19 / 68, of 64 39 / 18; 59 / 135, 2048 of 16 25 / 15; 36 / 80. (The order is not known here.)
+// One workgroup a row reads 2 R K bytes of a for each; 16 U rows share them, but wait for every adapter among them in turn. us of adapter_add,
+// by row / in tiles, [N, 4096] to 64 channels, four adapters in runs; every row another than its neighbour: 256 rows of 64 ranks 16 / 24;
+// 23 / 127, 512 of 64 24 / 21; 34 / 134, 1024 of 16 15 / 15; 19 / 68, of 64 39 / 18; 59 / 135, 2048 of 16 25 / 15; 36 / 80. The order is not
+// known here, so rows in runs pay up to 10 us for what others save.
 bool by_row(i64 N, i64 R) { return N <= 2048 && N * R <= 32768; }
 template <bool F16>
 void launch_in(const AdapterPart& p, i64 N, int K, uint16_t* h, float* back) {
@@ -308,8 +312,8 @@ void launch_in(const AdapterPart& p, i64 N, int K, uint16_t* h, float* back) {
     }
     go(UC, std::integral_constant<int, 4>{});
   };
-  // Workgroups of 16 u rows. With more than 32 ranks one takes some u + 2 (its rows of x, and a) and fills a CU; a second one doubles the time ([8209, 4096],
-  // 64 ranks of 16 adapters: 41 us with 32 rows, whose 257 workgroups are one too many; [8192, 4096] 28)
+  // Workgroups of 16 u rows. With more than 32 ranks one takes some u + 2 (its rows of x, and a) and fills a CU; a second one doubles the time
+  // ([8209, 4096], 64 ranks of 16 adapters: 41 us with 32 rows, whose 257 workgroups are one too many; [8192, 4096] 28)
   const i64 cus = mx_device_cus();
   int u = 2;
   i64 least = 0;
@@ -322,8 +326,8 @@ void launch_in(const AdapterPart& p, i64 N, int K, uint16_t* h, float* back) {
   else if (u == 3) by(std::integral_constant<int, 3>{});
   else by(std::integral_constant<int, 4>{});
 }
-// Up to as many rows four wavefronts share a place's adapters out. us of adapter_add, so / not, [N, 64] to 4096 channels, every row another of 32 adapters than
-// its neighbour (the first product in tiles for 1024 rows and more): 512 rows 15.8 / 16.3, 1024 29 / 27, 2048 42 / 38
+// Up to as many rows four wavefronts share a place's adapters out. us of adapter_add, so / not, [N, 64] to 4096 channels, every row another of
+// 32 adapters than its neighbour (the first product in tiles for 1024 rows and more): 512 rows 15.8 / 16.3, 1024 29 / 27, 2048 42 / 38
 constexpr i64 kSharedRows = 512;
 template <bool F16>
 void launch_add(const GroupArgs& a) {
@@ -379,9 +383,11 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
   if (w) check(*w, "w", x.dt, {O, K});
   if (y) check(*y, "y", x.dt, {N, O});
   check(out, "out", x.dt, {N, O});
-  REQ(slots.dt == I32 && slots.numel() == N && (slots.p || N == 0) && (uintptr_t)slots.p % 4 == 0, "slots must be int32 [%lld] and not null", (long long)N);
+  REQ(slots.dt == I32 && slots.numel() == N && (slots.p || N == 0) && (uintptr_t)slots.p % 4 == 0, "slots must be int32 [%lld] and not null",
+      (long long)N);
   if (scale) REQ(scale->dt == F32 && scale->numel() == L && scale->p, "scale must be F32 [%lld]", (long long)L);
-  if (bias) REQ(bias->numel() == O && bias->p && (bias->dt == F32 || bias->dt == F16 || bias->dt == BF16), "bias must have %lld elements", (long long)O);
+  if (bias)
+    REQ(bias->numel() == O && bias->p && (bias->dt == F32 || bias->dt == F16 || bias->dt == BF16), "bias must have %lld elements", (long long)O);
   for (const Tensor* t : {&x, &a, &b, &slots, w, scale, bias})
     if (t) mx_apart(out.p, out.bytes(), t->p, t->bytes(), "out");
   if (y) REQ(y->p == out.p || !mx_overlap(y->p, y->bytes(), out.p, out.bytes()), "out must be y or apart from it");

@@ -23,9 +23,7 @@ __device__ __forceinline__ f32x4 mfma(mx_u32x4 a, mx_u32x4 b, f32x4 c) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00020000);
 }
-}  // namespace
 
-namespace {
 // 16 rows of 64 depths straight from memory into operands. A load instruction that takes 64 bytes of each of 16 rows gets half of what one that
 // takes 128 bytes of each of 8 gets (x and a of 8192 rows by 4096, 64 ranks: 28 us and 17), so one loads the even rows' lines and one the
 // odd ones', two lanes beside each other 64 bytes of either row, and change halves afterwards.
@@ -61,7 +59,8 @@ struct AdapterPart {
   const float* scale;    // [L] or null
 };
 // Where that is: so few rows and ranks that every workgroup reads a for itself, in about the time that it waits for the weights, rather than
-// wait for a kernel of its own ([1, 4096] by [4096, 4096], 16 ranks: 16.7 -> 11.3 us)
+// wait for a kernel of its own. us so / in two kernels, 4096 to 4096 channels, bf16: adapter_linear 1 row of 16 ranks 12.2 / 16.6, 1 of 32
+// 14.2 / 16.8, 2 of 16 12.9 / 16.2, 4 of 8 16.1 / 15.8; adapter_add 10.2 - 10.3 / 15.8, 4 of 8 11.5 / 15.8. InnerSums holds no more.
 constexpr int kFusedRows = 4, kFusedRanks = 32;
 inline bool adapter_fused(i64 N, i64 R) { return N <= kFusedRows && N * R <= kFusedRanks; }
 struct GroupArgs {
@@ -120,7 +119,8 @@ __device__ __forceinline__ int inner_to_low(int m, int r, int R) { return m * mi
 template <bool F16>
 __device__ __forceinline__ auto stored_inner(const GroupArgs& a, i64 n0, int rows, int lane) {
   const int R = a.ad.R, blocks = (R + 63) / 64, n = max(min(rows, 64), 0);
-  const auto rh = buffer(a.ad.h + n0 * R * 2, (uint32_t)(n * R * 4)), rf = buffer(F16 ? a.ad.back + n0 * blocks : nullptr, F16 ? (uint32_t)(n * blocks * 4) : 0u);
+  const auto rh = buffer(a.ad.h + n0 * R * 2, (uint32_t)(n * R * 4));
+  const auto rf = buffer(F16 ? a.ad.back + n0 * blocks : nullptr, F16 ? (uint32_t)(n * blocks * 4) : 0u);
   return [=](int i, int r0, int, auto& high, auto& low, float& back) __attribute__((always_inline)) {
     constexpr int RC = sizeof(high) / sizeof(high[0]);
 #pragma unroll
@@ -145,7 +145,8 @@ __device__ __forceinline__ void inner_products(const GroupArgs& a, int lane, int
   for (int n = 0; n < (int)a.N; n++) {
     const int slot = p.slots[n];
     if (slot < 0 || slot >= p.L) continue;
-    const auto rx = buffer((const char*)p.x + (i64)n * a.K * 2, (uint32_t)(a.K * 2)), ra = buffer((const char*)p.a + (i64)slot * p.R * a.K * 2, (uint32_t)(p.R * a.K * 2));
+    const auto rx = buffer((const char*)p.x + (i64)n * a.K * 2, (uint32_t)(a.K * 2));
+    const auto ra = buffer((const char*)p.a + (i64)slot * p.R * a.K * 2, (uint32_t)(p.R * a.K * 2));
     for (int r0 = 0; r0 < p.R; r0 += 16) {
       f32x4 acc{};
       constexpr int AT = 8;  // steps on their way together
@@ -214,9 +215,8 @@ __device__ __forceinline__ auto summed_inner(const GroupArgs& a, const InnerSums
 // The adapters' second product for up to 64 rows of one wavefront (16 TM rows, the first of them row n0, `rows` of which exist):
 // acc[t][u] += b h over tiles t of 16 channels and u of 16 rows. Every adapter that some row has takes its turn, of whose products a
 // lane takes its row's (rows of zeros for the others would let an infinity in b reach them), so rows come in any order; those that share
-// an adapter share its reading. chan(t, r): the channel of
-// the first operand's row r in tile t, counted from c0, `cols` of which exist. inner: a row's first product (stored_inner, summed_inner).
-// Turns first, first + every, ...
+// an adapter share its reading. chan(t, r): the channel of the first operand's row r in tile t, counted from c0, `cols` of which exist.
+// inner: a row's first product (stored_inner, summed_inner). Turns first, first + every, ...
 template <bool F16, int TC, int TM, class Chan, class Inner>
 __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC][TM], i64 n0, int rows, int c0, int cols, int lane, Chan&& chan,
                                              Inner&& inner, int first = 0, int every = 1) {
@@ -224,7 +224,8 @@ __device__ __forceinline__ void add_adapters(const GroupArgs& a, f32x4 (&acc)[TC
   const AdapterPart& p = a.ad;
   const int r16 = lane & 15, g = lane >> 4;
   const bool here = lane < 16 * TM && lane < rows;
-  int mine = (int)__builtin_amdgcn_raw_buffer_load_b32(buffer(p.slots + n0, (uint32_t)(max(min(rows, 64), 0) * 4)), here ? (uint32_t)(lane * 4) : kOOR, 0, 0);
+  const auto rs = buffer(p.slots + n0, (uint32_t)(max(min(rows, 64), 0) * 4));
+  int mine = (int)__builtin_amdgcn_raw_buffer_load_b32(rs, here ? (uint32_t)(lane * 4) : kOOR, 0, 0);
   mine = here && mine < p.L ? mine : -1;
   int slot[TM];
 #pragma unroll

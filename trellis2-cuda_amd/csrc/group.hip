@@ -176,9 +176,9 @@ struct Tiles {
 };
 
 // Tiled products of all three kinds. A workgroup of WC x WM wavefronts has BC = 16 TC WC columns of the result by BM = 16 TM WM rows;
-// the depth goes by stages of 64 through slots of LDS (two; three of a half's, five of a quarter's), filled by DMA. An operand whose depth is contiguous (x and w of the
-// forward product, dy of dx) lies there as rows of 64 values, its 16-byte pieces permuted (piece c of row q at c ^ q % 8), so that
-// eight lanes of neighbouring rows read from distinct banks; one whose depth runs over rows (w of dx, dy and x of dw) as 64 rows, and
+// the depth goes by stages of 64 through slots of LDS (two; three of a half's, five of a quarter's), filled by DMA. An operand whose depth
+// is contiguous (x and w of the forward product, dy of dx) lies there as rows of 64 values, its 16-byte pieces permuted (piece c of row q at
+// c ^ q % 8), so that eight lanes of neighbouring rows read from distinct banks; one whose depth runs over rows (w of dx, dy and x of dw) as 64 rows, and
 // is transposed on its way into registers (ds_read_b64_tr_b16: 16 lanes give the addresses of 4 rows by four pieces of 4 values, lane i gets
 // column i of the four rows); piece c of row q is at c ^ (4 (q % 4) + 2 (q / 8 % 2)) there.
 //
@@ -190,9 +190,9 @@ struct Tiles {
 // earlier, so every LDS read is issued one quarter before its use and a wavefront holds one step's operands only. In the
 // middle of a stage's second step all wavefronts meet: by then each has read the whole slot, so it is filled again at once.
 //
-// Bound by the matrix unit at the clock that the card's power leaves (1.7 - 2.0 GHz under this load), and between tiles by the stores, which come from
-// all CUs at once and stand before the next tile's DMAs in the counter that both wait for. Measured, bf16: [8192, 8192] by [8192, 8192] 0.80 ms,
-// 1.37 PFLOP/s forward and dx, 1.24 dw into fp32, matrix unit busy 70 - 74%; 16411 rows by 8 groups of [4096, 2048] 267 us (1.03 PFLOP/s,
+// Bound by the matrix unit at the clock that the card's power leaves (1.7 - 2.0 GHz under this load), and between tiles by the stores, which
+// come from all CUs at once and stand before the next tile's DMAs in the counter that both wait for. Measured, bf16: [8192, 8192] by
+// [8192, 8192] 0.80 ms, 1.37 PFLOP/s forward and dx, 1.24 dw into fp32, matrix unit busy 70 - 74%; 16411 rows by 8 groups of [4096, 2048] 267 us (1.03 PFLOP/s,
 // busy 53%), dx 266, dw into fp32 278.
 constexpr int kTileLds = 163840;
 template <int OP, bool F16, int OUT, int TC, int TM, int WC, int WM, bool ADAPT, int PART>
@@ -374,7 +374,8 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
   };
 
   mx_u32x4 fm[2][HM], fc[2][HC];
-  const mx_u32x4 ones = F16 ? mx_u32x4{0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u} : mx_u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  constexpr uint32_t kOnes = F16 ? 0x3c003c00u : 0x3f803f80u;
+  const mx_u32x4 ones = {kOnes, kOnes, kOnes, kOnes};
   // A quarter's products, with READS LDS reads and DMAS DMAs between them: a wavefront that has its SIMD to itself (or shares it with
   // one at the same place) feeds the matrix unit only if few instructions stand between two products.
   auto quarter = [&](auto BC_, auto CC, auto MC, auto RC, auto&& read, auto DC, auto&& dma) __attribute__((always_inline)) {
@@ -414,9 +415,14 @@ __device__ __forceinline__ void multiply_tiles(const GroupArgs& a, uint8_t* lds)
     constexpr std::integral_constant<int, f> mf{};
     constexpr std::integral_constant<int, 1 - f> mo{};
     // DMAs into the slot that the last stage has left: the second half of the one asked for there, or the first half of a new one
-    auto count = [](auto PC) { return std::integral_constant<int, decltype(PC)::value < 0 ? 0 : DI * (decltype(PC)::value + 1) / 4 - DI * decltype(PC)::value / 4>{}; };
+    auto count = [](auto PC) {
+      constexpr int P = decltype(PC)::value;
+      return std::integral_constant<int, P < 0 ? 0 : DI * (P + 1) / 4 - DI * P / 4>{};
+    };
     auto dmas = [&](auto PC) __attribute__((always_inline)) {  // fourth P of a stage's
-      return [&](auto KC) __attribute__((always_inline)) { issue(std::integral_constant<int, DI * decltype(PC)::value / 4 + decltype(KC)::value>{}); };
+      return [&](auto KC) __attribute__((always_inline)) {
+        issue(std::integral_constant<int, DI * decltype(PC)::value / 4 + decltype(KC)::value>{});
+      };
     };
     constexpr std::integral_constant<int, J == 0 ? 2 : -1> p1{};
     constexpr std::integral_constant<int, J == 0 ? 3 : -1> p2{};
@@ -571,10 +577,11 @@ __global__ void __launch_bounds__(512, 2) k_group_tile(GroupArgs a) {
 }
 
 // Adds the parts of the depth, in order, eight values a thread: the result's first `elems`, then the bias' gradient. Rows of no group stay.
-// A kernel of its own, some 7 us behind the first with its reading of what that has just written: the order of the sums is fixed, as one of atomics is not.
+// A kernel of its own, some 7 us behind the first with its reading of what that has just written: the order of the sums is fixed, as one
+// of atomics is not.
 template <bool F16, bool F32OUT>
-__global__ void __launch_bounds__(64) k_group_sum(const float* parts, const float* db_parts, const int32_t* ends, void* out, void* db, i64 elems, i64 db_elems,
-                                                   int split, int ncols, int G, i64 N) {
+__global__ void __launch_bounds__(64) k_group_sum(const float* parts, const float* db_parts, const int32_t* ends, void* out, void* db, i64 elems,
+                                                   i64 db_elems, int split, int ncols, int G, i64 N) {
   i64 i = ((i64)blockIdx.x * 64 + threadIdx.x) * 8, each = elems;
   const float* from = parts;
   void* to = out;
@@ -627,8 +634,10 @@ void launch_tile(GroupArgs a) {
 // Few rows: the weights' bytes count, and that many of them are on their way at once. A workgroup has 16 OT channels by up to 16 NT rows of a
 // group; each of its 8 wavefronts takes a contiguous eighth of the depth, both operands straight into registers, and the sums meet in
 // LDS in a fixed order. With adapters, 4 wavefronts more add them meanwhile; FUSED, they also make the first product.
-// Measured: 384 rows by 64 groups of [1416, 2048] fp16 70 us (5.3 TB/s, a large copy's rate: bound by HBM); 2 rows by 16 groups of [1024, 1024] 4.9 us and 1
-// row by [4096, 4096] with an adapter of 16 ranks 10.8 us in the kernel, one trip to memory after another (the slots or ends, a, b).
+// Measured: 384 rows by 64 groups of [1416, 2048] fp16 70 us (5.3 TB/s, a large copy's rate: bound by HBM); 2 rows by 16 groups of
+// [1024, 1024] 4.9 us and 1 row by [4096, 4096] with an adapter of 16 ranks 11.4 us in the kernel, one trip to memory after another (the
+// slots or ends, a, b). The form of 64 rows with adapters is short of registers: 12 wavefronts have 168 each, and it keeps 222 in scratch
+// memory (no other of these forms keeps any).
 template <bool F16, int OT, int NT, bool ADAPT, bool FUSED>
 __global__ void __launch_bounds__(ADAPT ? 768 : 512) k_group_rows(GroupArgs a) {
   constexpr int NW = 8, NA = ADAPT ? 4 : 0, RUN = OT;
@@ -758,7 +767,9 @@ void launch_rows(GroupArgs a) {
 // Whether a forward product's rows go straight into registers: up to 16 a group on average, or as many as make no more workgroups (of 32
 // channels by 32 or 64 rows) than there are CUs. us by rows / in tiles, bf16, [rows, K] by groups of [O, K]: [640, 1024] 32 of 1024
 // 21.8 / 21.1 (1280 rows 26.0 / 21.5), [60, 4096] one of 4096 17.4 / 21.2, [100, 4096] 17.9 / 25.3, [200, 4096] 32.1 / 21.6, [100, 1024] one of
-// 1024 7.8 / 14.4, [500, 4096] one of 512 17.9 / 18.3.
+// 1024 7.8 / 14.4, [500, 4096] one of 512 17.9 / 18.3. With adapters in any order, 16 ranks, and in four runs, 64 ranks: [32, 4096] one of
+// 4096 19 / 38 and 24 / 36, [64, 4096] 39 / 50 and 46 / 38, [100, 4096] 44 / 51 and 51 / 40; [64, 1024] one of 1024 20 / 27 and 19 / 21, [500, 1024]
+// 23 / 35 and 23 / 25.
 constexpr i64 kCus = 256;  // (a workspace's size follows from it, also where no device is)
 int row_tiles(i64 N, i64 G) { return N <= 16 * G ? 1 : N <= 32 * G ? 2 : 4; }  // of 16 rows
 bool goes_by_rows(i64 N, i64 G, i64 O) {
@@ -786,6 +797,8 @@ bool few_rows(const GroupArgs& a, DT dt) {
     if constexpr (ADAPT) {
       if (!a.ad.h) return launch_rows<f, 1, 1, true, true>(a);
     }
+    // 4 channels a lane for up to 16384 over the groups that have rows, 8 for more. us with 4 / with 8, bf16: one row by [16384, 4096] 27.6 / 29.8, 8 rows by 16
+    // groups of [1024, 1024] 8.3 / 8.3, 16 by 16 8.8 / 8.4; beyond, 32 rows by 32 groups of [1024, 1024] 14.2 / 11.7, 64 by 64 of [1416, 1024] 36 / 27
     if (tiles == 1) {
       if (a.O * (a.N < a.G ? a.N : a.G) <= 16 * 1024) launch_rows<f, 1, 1, ADAPT>(a);
       else launch_rows<f, 2, 1, ADAPT>(a);
@@ -822,8 +835,9 @@ void launch(GroupArgs a, DT dt, bool f32, void* workspace) {
     dt == F16 ? by(std::true_type{}, o32) : by(std::false_type{}, o32);
     const unsigned blocks = (unsigned)((elems + db_elems + 511) / 512);
     auto sum = [&](auto F, auto T) {
-      k_group_sum<decltype(F)::value, decltype(T)::value><<<blocks, 64, 0, stream()>>>((const float*)a.out, (const float*)a.db, OP == DW || ADAPT ? nullptr : a.ends, out, db,
-                                                                                       elems, db_elems, a.split, OP == FORWARD ? a.O : a.K, a.G, a.N);
+      k_group_sum<decltype(F)::value, decltype(T)::value><<<blocks, 64, 0, stream()>>>(
+          (const float*)a.out, (const float*)a.db, OP == DW || ADAPT ? nullptr : a.ends, out, db, elems, db_elems, a.split,
+          OP == FORWARD ? a.O : a.K, a.G, a.N);
     };
     if (f32) sum(std::false_type{}, std::true_type{});
     else if (dt == F16) sum(std::true_type{}, std::false_type{});
@@ -893,7 +907,8 @@ void group_linear(const Tensor& x, const Tensor& w, const Tensor& ends, const Te
   check_rows(y, "out", x.dt, N, O);
   check_ends(ends, G);
   if (bias)
-    REQ(bias->numel() == G * O && bias->p && (bias->dt == F32 || bias->dt == F16 || bias->dt == BF16), "bias must have %lld elements", (long long)(G * O));
+    REQ(bias->numel() == G * O && bias->p && (bias->dt == F32 || bias->dt == F16 || bias->dt == BF16), "bias must have %lld elements",
+        (long long)(G * O));
   for (const Tensor* t : {&x, &w, &ends, bias}) apart(y, t, "out");
   if (N == 0) return;
   GroupRoom room(workspace, workspace_bytes, group_linear_workspace(FORWARD, N, G, K, O), {&x, &w, &ends, bias, &y});
@@ -928,8 +943,8 @@ void group_linear_dw(const Tensor& dy, const Tensor& x, const Tensor& ends, Tens
   check_ends(ends, G);
   for (const Tensor* t : {&dy, &x, &ends}) apart(dw, t, "out");
   if (db) {
-    REQ(db->dt == dw.dt && db->numel() == G * O && db->p && (uintptr_t)db->p % 16 == 0, "the bias' gradient must have %lld elements of out's type, 16-byte aligned",
-        (long long)(G * O));
+    REQ(db->dt == dw.dt && db->numel() == G * O && db->p && (uintptr_t)db->p % 16 == 0,
+        "the bias' gradient must have %lld elements of out's type, 16-byte aligned", (long long)(G * O));
     for (const Tensor* t : std::initializer_list<const Tensor*>{&dy, &x, &ends, &dw}) apart(*db, t, "the bias' gradient");
   }
   GroupRoom room(workspace, workspace_bytes, group_linear_workspace(DW, N, G, K, O), {&dy, &x, &ends, &dw, db});
