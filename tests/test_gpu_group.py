@@ -773,3 +773,19 @@ def test_adapter_infinities(gpu, n, rank, dt):
     for got, base in ((sp.adapter_add(y, x, a, b, slots), y.double()), (sp.adapter_linear(x, w, a, b, slots), x.double() @ w.double().T)):
         want = adapter64(base, x, a, b, slots, None, dt)[0].to(dt)
         assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+def test_adapters_in_parts_of_many_rows(gpu):
+    """So many inner products that room for all of them is not taken: the rows go in parts."""
+    g, dt, n, rank = gen(60), torch.float16, 360011, 256
+    x, w = ints(g, n, 16, dt=dt, most=1), ints(g, 24, 16, dt=dt, most=1)
+    a, b, slots, y = ints(g, 3, rank, 16, dt=dt, most=1), ints(g, 3, 24, rank, dt=dt, most=1), slots_of(g, n, 3, "runs"), ints(g, n, 24, dt=dt)
+    assert 3 * n * rank > 1 << 28
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    z = sp.adapter_add(y, x, a, b, slots)
+    assert torch.cuda.max_memory_allocated() - before <= 2 * n * rank + z.nbytes + (1 << 20)
+    v = sp.adapter_linear(x, w, a, b, slots)
+    part = adapter64(torch.zeros((n, 24), dtype=torch.float64, device=gpu), x, a, b, slots, None, dt)[0]
+    assert torch.equal(z, (y.double() + part).to(dt)) and torch.equal(v, (x.double() @ w.double().T + part).to(dt))

@@ -353,6 +353,7 @@ void launch_add(const GroupArgs& a) {
 // Of a row's first product: its halves and its factors
 i64 inner_row_bytes(i64 R) { return R * 4 + (R + 63) / 64 * 4; }
 i64 inner_bytes(i64 N, i64 R) { return adapter_fused(N, R) ? 0 : (N * inner_row_bytes(R) + 15) / 16 * 16; }
+constexpr i64 kWhole = 1 << 28;  // of a workspace of the library's own: more than 256 MB, and rows go in parts of some 10^5 and more
 constexpr int kHighestRank = 256;
 constexpr i64 kMostRows = 1 << 27;  // whose launches hold fewer than 2^32 threads in any direction
 void check(const Tensor& t, const char* what, DT dt, std::initializer_list<i64> sh) {
@@ -392,9 +393,9 @@ void adapter(const Tensor& x, const Tensor* w, const Tensor* y, const Tensor& a,
     if (t) mx_apart(out.p, out.bytes(), t->p, t->bytes(), "out");
   if (y) REQ(y->p == out.p || !mx_overlap(y->p, y->bytes(), out.p, out.bytes()), "out must be y or apart from it");
   if (N == 0) return;
-  // Rows go in as many parts as it takes for the workspace to hold a part's first product
-  const i64 product = w ? adapter_product_bytes(N, K, O) : 0, all = inner_bytes(N, R) + product;
-  const i64 need = workspace && workspace_bytes < all ? std::max(adapter_workspace(N, R, w ? K : 0, O), workspace_bytes) : all;
+  // Rows go in as many parts as it takes for the workspace to hold a part's first product; where all of it would be large, parts lose nothing
+  const i64 product = w ? adapter_product_bytes(N, K, O) : 0, all = inner_bytes(N, R) + product, least = adapter_workspace(N, R, w ? K : 0, O);
+  const i64 given = workspace ? workspace_bytes : all <= kWhole ? all : least, need = given < all ? std::max(least, given) : all;
   if (workspace) {
     for (const Tensor* t : std::initializer_list<const Tensor*>{&x, &a, &b, &slots, w, y, scale, bias, &out})
       if (t) mx_apart(t->p, t->bytes(), workspace, (size_t)need, "the workspace");

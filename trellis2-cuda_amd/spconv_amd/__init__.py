@@ -702,11 +702,12 @@ def _adapters(x, a, b, slots, scale):
 
 
 def _adapter_workspace(x, N, R, K, Co):
-    """(workspace, its bytes): with 3 N R more than the least, so that the rows go in one part."""
+    """(workspace, its bytes): the least, or 3 N R more, so that the rows go in one part, where that is up to 256 MB."""
     nws = _workspace_bytes("spc_adapter_workspace", N, R, K, Co)
     if not nws:
         return None, 0
-    nws += 3 * N * R
+    if 3 * N * R <= 1 << 28:
+        nws += 3 * N * R
     return _workspace(nws, x), nws
 
 
