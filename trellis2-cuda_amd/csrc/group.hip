@@ -133,7 +133,7 @@ struct Tiles {
     if constexpr (OP == DW) {
       const int tiles = a.tiles_m * a.tiles_c;
       const i64 u = l * 8 + blockIdx.x % 8, b = u / a.split;
-      at.part = (int)(u % a.split);
+      at.part = a.per ? 0 : (int)(u % a.split);  // (a list of eighths has whole depths)
       const int order = (int)(a.per ? l / a.per : b / tiles);
       const int inside = (int)(a.per ? blockIdx.x % 8 * a.per + l % a.per : b % tiles);
       if (order >= a.G || inside >= tiles) return false;
